@@ -163,7 +163,7 @@ def prepare(case, seed):
     total = [x + y for x, y in zip(new, past)]
     shared = -(-c.get("shared", 0) // b)
     need = [-(-t // b) for t in total]
-    blocks = shared + sum(need) + 2
+    blocks = shared + sum(total) // b + n + 2  # as many for every order of the lengths
     order = torch.randperm(blocks, generator=torch.Generator().manual_seed(int(seed) + 1)).to(torch.int32)
     wide = max(need)
     tables = torch.zeros(n, wide, dtype=torch.int32)
@@ -185,6 +185,7 @@ def prepare(case, seed):
         st["v"] = _randn(g, cu[-1], c["kv_heads"], c["dim"], dtype=dt)
         st["rope"] = _rotation_table(max(total), c["rot"])
         return st
+    st["max_new"] = max(new)  # the program that made the batch knows it
     st["slopes"] = None
     if c["slopes"]:
         st["slopes"] = (2.0 ** (-8.0 * torch.arange(1, c["heads"] + 1, dtype=torch.float64) / c["heads"])).float().cuda()
@@ -213,8 +214,8 @@ def run(state):
     if c["kind"] == "attend":
         from kernels.paged_attention import paged_attention
         return paged_attention(state["q"], state["k_pool"], state["v_pool"], state["tables"], state["lens"], state["cu"],
-                               softcap=c["cap"], slopes=state["slopes"], window=c["window"],
-                               prefix_lens=state["prefix_lens"])
+                               max_new=state["max_new"], softcap=c["cap"], slopes=state["slopes"],
+                               window=c["window"], prefix_lens=state["prefix_lens"])
     from kernels.paged_attention import shared_prefix_attention
     return shared_prefix_attention(state["q"], state["k_pool"], state["v_pool"], state["shared"], c["shared"],
                                    state["tables"], state["lens"], softcap=c["cap"], slopes=state["slopes"],
