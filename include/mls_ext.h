@@ -46,6 +46,49 @@ int mlsx_paged_attention_decode(const void* q, int q_dt, int64_t q_ss, int64_t q
                                 int64_t H, int64_t D, int64_t block_size, float scale, float* workspace,
                                 int64_t workspace_floats, mls_stream_t stream);
 
+/* Attention of new tokens over a paged cache with grouped heads (no reference counterpart; the
+ * one-token, one-head-a-K/V-head form is kernels/paged_attention.py:93-118). Every field has 8
+ * bytes. q and out: [tokens][kv_heads * group][head_dim], inner stride 1; pools [num_blocks]
+ * [kv_heads][block_size][head_dim], inner stride 1, K and V with one set of strides; all of
+ * type dt. Sequence s has the rows cu_seqlens[s] .. cu_seqlens[s + 1] (null: row s), its
+ * last context_lens[s] - 1 the position of its last row. Rows of no sequence get zeros. A block
+ * id outside the pool holds no keys. With prefix_blocks, the prefix_len keys in those
+ * prefix_count blocks come before every sequence's own (one row each), whose positions
+ * count from there. max_new: the longest sequence's rows if known (0: not), which only chooses
+ * kernels. The 16-byte aligned workspace holds mlsx_paged_attention_ws floats (0: none). */
+typedef struct mlsx_paged_attention_args {
+  const void *q, *k_pool, *v_pool;
+  const int32_t *block_tables, *context_lens, *cu_seqlens, *prefix_lens, *prefix_blocks;
+  const float* slopes;
+  void* out;
+  int64_t dt;
+  int64_t q_st, q_sh, o_st, o_sh, kv_sb, kv_sh, kv_st, bt_ss;
+  int64_t num_blocks, n_seqs, tokens, kv_heads, group, head_dim, block_size, max_blocks;
+  int64_t window, prefix_len, prefix_count, max_new;
+  double scale, softcap;
+} mlsx_paged_attention_args;
+int64_t mlsx_paged_attention_ws(const mlsx_paged_attention_args* args);
+int mlsx_paged_attention(const mlsx_paged_attention_args* args, float* workspace, int64_t workspace_floats,
+                         mls_stream_t stream);
+
+/* New keys and values into the cache that the above reads, with the position rotation on the
+ * way. q (null: none) [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim], inner stride 1, type
+ * dt, as the pools; rows, tables and lengths as above, context_lens with the new tokens.
+ * Row t at position p goes to slot p % block_size of block p / block_size of its sequence's
+ * table; a block id outside the pool, or a position outside the table, stores nothing. rope (null: none):
+ * fp32 [rope_rows][rope_ld], the cosines of a position's rot / 2 angles, then their sines; pairs
+ * are x[j], x[j + rot / 2], or, interleaved, x[2 j], x[2 j + 1]. A position outside rope gives NaN.
+ * q_out [tokens][heads][head_dim] dense: q rotated (0 for rows of no sequence); only with rope. */
+typedef struct mlsx_paged_append_args {
+  const void *q, *k, *v;
+  void *k_pool, *v_pool, *q_out;
+  const int32_t *block_tables, *context_lens, *cu_seqlens;
+  const float* rope;
+  int64_t dt, q_st, q_sh, k_st, k_sh, v_st, v_sh, kv_sb, kv_sh, kv_st, bt_ss, rope_ld;
+  int64_t num_blocks, n_seqs, tokens, heads, kv_heads, head_dim, block_size, max_blocks, rope_rows, rot, interleaved;
+} mlsx_paged_append_args;
+int mlsx_paged_append(const mlsx_paged_append_args* args, mls_stream_t stream);
+
 /* ---------------------------------------------------------------- grouped INT4 GEMMs */
 
 /* 1 where the grouped INT4 entry points of mls.h take a call of M_total rows on the kernel for

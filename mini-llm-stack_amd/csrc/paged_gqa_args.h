@@ -1,0 +1,198 @@
+// Arguments of the paged grouped-head attention kernels, and which rows, keys and pieces of a
+// context a block takes (found on the device: the host knows neither lengths nor offsets).
+#pragma once
+
+#include "common.h"
+
+namespace mls {
+
+struct GqaArgs {
+  const void* q;  // [T][Hkv * group][D], strides (q_st, q_sh, 1)
+  int64_t q_st, q_sh;
+  const void* kp;  // [num_blocks][Hkv][BS][D], strides (kv_sb, kv_sh, kv_st, 1), as vp
+  const void* vp;
+  int64_t kv_sb, kv_sh, kv_st;
+  const int32_t* bt;  // [n][max_blocks]; shared: [max_blocks]
+  int64_t bt_ss;
+  const int32_t* lens;    // [n] keys of each sequence, its new tokens among them
+  const int32_t* cu;      // [n + 1] first row of each sequence; null: one row each
+  const int32_t* prefix;  // [n] or null: keys that every row sees, also before it
+  const float* slopes;    // [Hkv * group] or null
+  void* out;
+  int64_t o_st, o_sh;
+  float* ws;     // [T][Hkv * group][pieces][DW]: O of each piece, not divided by its sum
+  float* ws_ml;  // [T][Hkv * group][pieces][2]: its reference and sum
+  int64_t num_blocks;
+  int n, T, Hkv, group, D, DW, BS;
+  uint32_t bs_magic;  // ceil(2^32 / BS)
+  int max_blocks;
+  int window;
+  int front;   // shared: keys of the prefix
+  int shared;  // the rows of all sequences (one each) over the one table's `front` keys
+  float c, cap, to_cap;  // scale log2(e); cap log2(e) (0: none), scale / cap
+  int simple;            // scores are positive multiples of the products: no cap, no slopes
+  int bm_log, bn;        // rows of a tile (log2) and keys of a step
+  int slots;             // row tiles that the grid has room for
+  int pieces;            // records a row has in the workspace
+  int piece0;            // first record of this launch's pieces (before it: the shared prefix's)
+  int splits, least, cap_tiles;  // pieces a context may have, least steps of one; n > 1024: steps of one
+  float target;                  // blocks to aim at
+  int q_vec, o_vec;
+};
+
+struct GqaShape {
+  bool keys, vec;
+  int nt, dp, bn;
+};
+
+struct GqaPlan {
+  const int32_t* table;
+  int tok0, rows, row0;  // the sequence's first row of q, its packed rows, the tile's first of them
+  int pos0, len, pfx;    // position of its first new token; its keys; keys seen both ways
+  int klo, khi;          // keys that any row of the tile sees
+  int lo, tiles;         // the tile's first step, steps
+  int live, per;         // pieces, steps of a piece
+  bool direct;           // the only piece writes the output itself
+};
+
+// key / BS
+__device__ __forceinline__ int gqa_block_of(const GqaArgs& a, int key) {
+  int b = a.BS == 1 ? key : (int)__umulhi((uint32_t)key, a.bs_magic);  // (one too many at most)
+  return b - (b * (int64_t)a.BS > key ? 1 : 0);
+}
+
+// The last s of [0, n] whose start(s) is at most `at`, -1: none; by 64 probes a round.
+template <typename F>
+__device__ __forceinline__ int last_start(int n, int at, int lane, F start) {
+  int lo = 0, hi = n + 1;
+  while (true) {
+    const int step = (hi - lo + 63) / 64, s = lo + lane * step;
+    const bool le = s < hi && start(s) <= at;
+    const int cnt = __builtin_popcountll(__ballot(le));
+    if (cnt == 0) return lo - 1;  // (only in the first round, where starts rise)
+    lo += (cnt - 1) * step;
+    if (step == 1) return lo;
+    hi = min(lo + step, hi);
+  }
+}
+
+__device__ __forceinline__ int gqa_cu(const GqaArgs& a, int s) { return min(max(a.cu[s], 0), a.T); }
+
+// First slot of sequence s's row tiles (s = n: the rows past the last sequence's): room for any
+// lengths without a prefix sum, since floor(x) + 1 >= ceil(x).
+__device__ __forceinline__ int gqa_slot_of(const GqaArgs& a, int s) {
+  return (int)(((int64_t)gqa_cu(a, s) * a.group) >> a.bm_log) + s + 1;
+}
+
+// The sequence of a slot, or of a row of q.
+template <bool SLOT>
+__device__ __forceinline__ int gqa_find(const GqaArgs& a, int at, int lane) {
+  return last_start(a.n, at, lane, [&](int s) { return SLOT ? gqa_slot_of(a, s) : gqa_cu(a, s); });
+}
+
+__device__ __forceinline__ int gqa_keys_of(const GqaArgs& a, int s) {
+  return (int)min((int64_t)max(a.lens[s], 0), (int64_t)a.max_blocks * a.BS);
+}
+
+// Steps of a piece: what makes about `target` blocks of the batch's own lengths, and at most
+// `splits` pieces of the longest. Every wavefront of both kernels finds the same.
+__device__ __forceinline__ int gqa_piece(const GqaArgs& a, int lane) {
+  if (a.n > 1024) return a.cap_tiles;
+  float sum = 0.0f;
+  int most = 0;
+  for (int s = lane; s < a.n; s += 64) {
+    const int nt = a.cu ? max(gqa_cu(a, s + 1) - gqa_cu(a, s), 0) : 1;
+    int64_t keys = gqa_keys_of(a, s);
+    if (a.window > 0) keys = min(keys, (int64_t)a.window + nt);
+    const int t = (int)((keys + a.bn - 1) / a.bn);
+    sum += (float)((((int64_t)nt * a.group + (1 << a.bm_log) - 1) >> a.bm_log) * t);
+    if (nt > 0) most = max(most, t);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    sum += __shfl_xor(sum, off, 64);
+    most = max(most, __shfl_xor(most, off, 64));
+  }
+  const int want = (int)fminf(ceilf(sum * a.Hkv / a.target), 1e9f);
+  return __builtin_amdgcn_readfirstlane(max(max(want, (most + a.splits - 1) / a.splits), a.least));
+}
+
+// Row tile rt of sequence seq (-1 and n: rows that no sequence holds, which see nothing).
+__device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int rt, int lane) {
+  GqaPlan p;
+  const bool real = seq >= 0 && seq < a.n;
+  int ntok;
+  if (a.shared) {
+    p.tok0 = 0;
+    ntok = a.n;
+    p.pos0 = 0;
+    p.len = a.front;
+  } else {
+    p.tok0 = a.cu ? (seq < 0 ? 0 : gqa_cu(a, seq)) : seq;
+    ntok = a.cu ? max((seq >= a.n ? a.T : gqa_cu(a, seq + 1)) - p.tok0, 0) : 1;
+    p.pos0 = real ? a.lens[seq] - ntok : 0;
+    p.len = real ? gqa_keys_of(a, seq) : 0;
+  }
+  p.pfx = real && a.prefix ? a.prefix[seq] : 0;
+  p.table = a.bt + (a.shared || !real ? 0 : seq * a.bt_ss);
+  p.rows = ntok * a.group;
+  p.row0 = rt << a.bm_log;
+  p.live = p.tiles = p.per = 0;
+  p.klo = p.khi = p.lo = 0;
+  p.direct = false;
+  if (p.row0 >= p.rows) return p;
+  const int first = p.row0 / a.group, last = (min(p.row0 + (1 << a.bm_log), p.rows) - 1) / a.group;
+  int pmin, pmax;
+  if (a.shared) {
+    pmin = 0x7FFFFFFF;
+    pmax = a.front - 1;
+    for (int t = first + lane; t <= last; t += 64) pmin = min(pmin, a.front + max(a.lens[t], 0) - 1);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) pmin = min(pmin, __shfl_xor(pmin, off, 64));
+  } else {
+    pmin = p.pos0 + first;
+    pmax = p.pos0 + last;
+  }
+  p.khi = __builtin_amdgcn_readfirstlane(min(max(pmax + 1, p.pfx), p.len));
+  p.klo = __builtin_amdgcn_readfirstlane(a.window > 0 ? max(0, pmin - a.window + 1) : 0);
+  p.lo = p.klo - p.klo % a.bn;
+  p.tiles = p.khi > p.klo ? (p.khi - p.lo + a.bn - 1) / a.bn : 0;
+  if (a.shared) {
+    p.live = a.splits;
+  } else if (a.splits > 1) {
+    const int piece = gqa_piece(a, lane);
+    p.live = min(max((p.tiles + piece - 1) / piece, 1), a.splits);
+  } else {
+    p.live = 1;
+  }
+  p.per = (p.tiles + p.live - 1) / p.live;
+  p.direct = p.live == 1 && a.pieces == 1;
+  if (!a.shared && a.piece0 == 0 && p.live == 1) p.direct = true;
+  return p;
+}
+
+// Block -> (K/V head, piece, row tile). Heads run fastest: with 8 of them, blocks go round the 8
+// XCDs in order, so that an XCD's L2 holds one head's keys. The later row tiles, which see more
+// keys, come first; the pieces that few sequences reach last.
+__device__ __forceinline__ GqaPlan gqa_block_plan(const GqaArgs& a, int block, int lane, int& kvh, int& split) {
+  kvh = block % a.Hkv;
+  const int rest = block / a.Hkv;
+  split = rest / a.slots;
+  const int slot = a.slots - 1 - rest % a.slots;
+  if (a.shared) return gqa_tile_plan(a, 0, slot, lane);
+  if (!a.cu) {
+    const int per = (a.group + (1 << a.bm_log) - 1) >> a.bm_log;
+    return gqa_tile_plan(a, slot / per, slot % per, lane);
+  }
+  const int seq = __builtin_amdgcn_readfirstlane(gqa_find<true>(a, slot, lane));
+  return gqa_tile_plan(a, seq, seq < 0 ? slot : slot - __builtin_amdgcn_readfirstlane(gqa_slot_of(a, seq)), lane);
+}
+
+// The keys [lo, hi) that the row of token `tok` sees, and its position.
+__device__ __forceinline__ void gqa_row_range(const GqaArgs& a, const GqaPlan& p, int tok, int& lo, int& hi, int& pos) {
+  pos = a.shared ? a.front + max(a.lens[tok], 0) - 1 : p.pos0 + (tok - p.tok0);
+  hi = min(max(pos + 1, p.pfx), p.len);
+  lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+}
+
+}  // namespace mls

@@ -11,14 +11,23 @@ online softmax, one wavefront per (sequence, head, piece of the context); contex
 cut into pieces of one length (128 tokens or more) and merged by a second kernel through a
 workspace this wrapper allocates (its size comes from mlsx_paged_attention_workspace). Tokens at or past a sequence's context
 length weigh 0; a zero context gives a zero output.
+
+paged_attention and shared_prefix_attention (csrc/paged_gqa.h, csrc/paged_gqa.hip; no reference
+counterpart) take any number of new tokens a sequence, several query heads a K/V head, capped
+scores, a bias by distance, windows, prefix masks, and batches behind one shared prefix.
 """
 
 from __future__ import annotations
+
+import struct
 
 import torch
 
 import kernels
 from kernels._hip import dt_code, require_hip, stream
+from kernels.paged_kv import int32, no_grad_of, pools
+
+_ARGS = struct.Struct("=10Q21q2d")  # mlsx_paged_attention_args
 
 
 def paged_attention_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -62,3 +71,90 @@ def paged_attention_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
         out.data_ptr(), out.stride(0), out.stride(1), n_seqs, H, D, block_size, float(scale),
         ws.data_ptr(), ws_n, stream(dev)), "paged_attention_decode")
     return out
+
+
+def _attend(fn, q, k_pool, v_pool, block_tables, context_lens, cu_seqlens, max_new, scale, softcap, slopes, window, prefix_lens,
+            prefix_blocks, prefix_len):
+    if q.dim() != 3:
+        raise ValueError(f"{fn}: q {tuple(q.shape)}, expected [tokens, heads, head_dim]")
+    T, Hq, D = q.shape
+    kv_sb, kv_sh, kv_st, _ = pools(k_pool, v_pool, fn)
+    num_blocks, Hkv, block_size, Dk = k_pool.shape
+    if Dk != D or Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"{fn}: q {tuple(q.shape)}, pools {tuple(k_pool.shape)}: head dims differ, or query heads are no "
+                         f"multiple of K/V heads")
+    if q.dtype != k_pool.dtype:
+        raise TypeError(f"{fn}: q {q.dtype} and pools {k_pool.dtype} must have one dtype")
+    n = context_lens.shape[0] if context_lens.dim() == 1 else -1
+    lens = int32(context_lens, "context_lens", fn, (None,))
+    tables = int32(block_tables, "block_tables", fn, (n, None))
+    cu = prefix = shared = None
+    if cu_seqlens is not None:
+        cu = int32(cu_seqlens, "cu_seqlens", fn, (n + 1,))
+    elif n != T:
+        raise ValueError(f"{fn}: {T} rows for {n} sequences: without cu_seqlens, each has one")
+    if prefix_lens is not None:
+        prefix = int32(prefix_lens, "prefix_lens", fn, (n,))
+    if prefix_blocks is not None:
+        shared = int32(prefix_blocks, "prefix_blocks", fn, (None,))
+        if not 0 <= prefix_len <= shared.shape[0] * block_size:
+            raise ValueError(f"{fn}: a prefix of {prefix_len} tokens in {shared.shape[0]} blocks of {block_size}")
+    if slopes is not None:
+        if slopes.shape != (Hq,) or slopes.dtype != torch.float32:
+            raise ValueError(f"{fn}: slopes must be float32 [{Hq}], got {slopes.dtype} {tuple(slopes.shape)}")
+        slopes = slopes.contiguous()
+    if not 0.0 <= softcap < 3e38:
+        raise ValueError(f"{fn}: softcap {softcap}: a positive cap, or 0 for none")
+    if window < 0 or max_new is not None and max_new < 0:
+        raise ValueError(f"{fn}: window {window}, max_new {max_new}: not negative")
+    no_grad_of(fn, q, k_pool, v_pool, slopes)
+    dev = require_hip(fn, *(t for t in (q, k_pool, v_pool, tables, lens, cu, prefix, shared, slopes) if t is not None))
+    if q.stride(2) != 1 and D > 1 or q.stride(1) < D and Hq > 1:
+        q = q.contiguous()
+    out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    args = _ARGS.pack(
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+        0 if cu is None else cu.data_ptr(), 0 if prefix is None else prefix.data_ptr(),
+        0 if not prefix_len else shared.data_ptr(), 0 if slopes is None else slopes.data_ptr(), out.data_ptr(),
+        dt_code(q.dtype, fn), q.stride(0), max(q.stride(1), D), Hq * D, D, kv_sb, max(kv_sh, D), max(kv_st, D),
+        tables.stride(0), num_blocks, n, T, Hkv, Hq // Hkv, D, block_size, tables.shape[1], min(window, 0x7FFFFFFF),
+        prefix_len, 0 if shared is None else shared.shape[0], max_new or 0, D ** -0.5 if scale is None else scale, softcap)
+    L = kernels.lib()
+    need = L.mlsx_paged_attention_ws(args)
+    ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
+    kernels.check(L.mlsx_paged_attention(args, ws.data_ptr() if need else None, need, stream(dev)), fn)
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,
+                    context_lens: torch.Tensor, cu_seqlens: torch.Tensor | None = None, *, max_new: int | None = None,
+                    scale: float | None = None, softcap: float = 0.0, slopes: torch.Tensor | None = None, window: int = 0,
+                    prefix_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of q [T, Hq, D] over the cached keys and values of each row's sequence; [T, Hq, D].
+
+    k_pool / v_pool [num_blocks, Hkv, block_size, D] of q's type, Hq a multiple of Hkv (query head h reads
+    K/V head h // (Hq / Hkv)), any strides with 1 for the last dimension. Sequence s holds rows
+    cu_seqlens[s] .. cu_seqlens[s + 1] (int32 [n + 1]; None: row s), the newest tokens of its
+    context_lens[s] cached ones (written before, as by kernels.paged_kv.paged_kv_append); token j of it is
+    slot j % block_size of block block_tables[s, j // block_size]. max_new: the longest sequence's rows where the
+    caller knows them; it only chooses between kernels.
+
+    The row at position p sees token j when j <= p or j < prefix_lens[s] (int32 [n]), and, with a window, when
+    p - j < window. A score is scale q.k (scale: D^-0.5), capped softcap tanh(score / softcap), less
+    slopes[h] |p - j| (float32 [Hq]). A row that sees nothing gives zeros, as do rows of no sequence; block ids
+    outside the pool hold no tokens, a context longer than its table is cut at the table's end."""
+    return _attend("paged_attention", q, k_pool, v_pool, block_tables, context_lens, cu_seqlens, max_new, scale, softcap, slopes,
+                   window, prefix_lens, None, 0)
+
+
+def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, prefix_blocks: torch.Tensor,
+                            prefix_len: int, block_tables: torch.Tensor, context_lens: torch.Tensor, *,
+                            scale: float | None = None, softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                            window: int = 0) -> torch.Tensor:
+    """A decode step, q [n, Hq, D], of n sequences that all begin with the same prefix_len tokens, cached once
+    in the blocks prefix_blocks (int32 [blocks]). block_tables [n, max_blocks] and context_lens [n] hold each
+    sequence's own tokens after the prefix, the new one among them, at position prefix_len +
+    context_lens[s] - 1. Otherwise as paged_attention over prefix and own tokens, to rounding; the prefix's
+    keys and values are read once for all sequences' rows."""
+    return _attend("shared_prefix_attention", q, k_pool, v_pool, block_tables, context_lens, None, None, scale, softcap, slopes,
+                   window, None, prefix_blocks, prefix_len)
