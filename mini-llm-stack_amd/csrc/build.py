@@ -32,7 +32,7 @@ ARCH = "gfx950"
 #   start, so the microsecond kernels issue their first loads without a scalar-load round
 #   trip for the arguments (their argument lists put what those loads need first). The code
 #   object keeps a prologue that loads them for firmware without preloading.
-# - gemv_mfma.hip (the skinny GEMM's INT4 kernels), gemm_small.hip, gemm_grouped.hip: MFMA
+# - gemv_mfma.hip (the skinny GEMM's INT4 kernels), gemm_small.hip, gemm_grouped.hip, paged_gqa_*.hip: MFMA
 #   results in VGPRs (the kernels scale MFMA results with VALU FMAs; in AGPRs each one is
 #   first copied back with v_accvgpr_read, 56 extra VALU instructions per wavefront in the
 #   skinny kernel at K = 4096). The skinny INT8 kernels (gemv_mfma8.hip) measured slower
@@ -47,6 +47,9 @@ EXTRA_FLAGS = {"gemv.hip": PRELOAD,
                "gemm_grouped.hip": VGPR_FORM,
                "grouped_skinny.hip": VGPR_FORM,
                "gemm_dw.hip": VGPR_FORM,
+               "paged_gqa_f32.hip": VGPR_FORM,
+               "paged_gqa_f16.hip": VGPR_FORM,
+               "paged_gqa_bf16.hip": VGPR_FORM,
                "split.hip": PRELOAD}
 
 

@@ -30,45 +30,51 @@ extern template void gqa_tiles<_Float16>(GqaShape&);
 
 namespace {
 
-// One wavefront per (row, head): lane i holds piece i's reference and sum (at most 64 pieces),
-// then the lanes run over D with every piece's factor broadcast.
+// One wavefront per (row, head): lane i holds piece i's reference and sum (at most 64 pieces); then DW / 4
+// lanes take a record, 4 floats each, as many records at once as the wavefront has lanes for, four
+// such loads in flight.
 template <typename T>
 __global__ __launch_bounds__(256) void gqa_join_kernel(const GqaArgs a) {
   const int lane = threadIdx.x & 63;
   const int Hq = a.Hkv * a.group;
   const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= (int64_t)a.T * Hq) return;
-  const int tok = (int)(item / Hq), head = (int)(item % Hq);
-  int live;
-  if (a.splits > 1) {
-    const int seq = a.cu ? __builtin_amdgcn_readfirstlane(gqa_find<false>(a, tok, lane)) : tok;
-    const int tok0 = a.cu ? (seq < 0 ? 0 : gqa_cu(a, seq)) : seq;
-    const int rt = ((tok - tok0) * a.group + head % a.group) >> a.bm_log;
-    live = a.piece0 + gqa_tile_plan(a, seq, rt, lane).live;
-  } else {
-    live = a.piece0 + 1;
-  }
-  if (live == 1) return;  // written by its only piece
+  const int live = a.piece0 + __builtin_amdgcn_readfirstlane(a.ws_live[item]);
   const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + item * a.pieces;
-  const float2 x = lane < live ? ml[lane] : make_float2(-3.402823466e38f, 0.0f);
-  const float M = wave_max(x.x);
-  const float f = __builtin_amdgcn_exp2f(x.x - M);
-  const float L = wave_sum(x.y * f);
+  const float2 x = ml[min(lane, live - 1)];
+  if (live == 1) return;  // written by its only piece
+  const float m = lane < live ? x.x : -3.402823466e38f;
+  const float M = wave_max(m);
+  const float f = lane < live ? __builtin_amdgcn_exp2f(m - M) : 0.0f;
+  const float L = lane_group_sum<64>(lane < live ? x.y * f : 0.0f);
   const float g = L == 0.0f ? 0.0f : f / L;
-  T* op = static_cast<T*>(a.out) + tok * a.o_st + head * a.o_sh;
-  const float* w = a.ws + item * a.pieces * a.DW;
-  for (int d0 = 0; d0 < a.D; d0 += 64) {
-    const int d = d0 + lane;
-    const float* wd = w + min(d, a.D - 1);
-    float acc = 0.0f;
-    for (int s0 = 0; s0 < live; s0 += 8) {  // eight records' loads in flight
-      float v[8];
+  const int lanes = a.DW / 4, per = 64 / lanes, sub = lane / lanes, d = (lane % lanes) * 4;
+  const float* w = a.ws + item * a.pieces * a.DW + d;
+  f32x4 acc{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < live; s0 += 4 * per) {
+    f32x4 v[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = wd[(int64_t)min(s0 + i, live - 1) * a.DW];
+    for (int i = 0; i < 4; ++i)
+      v[i] = *reinterpret_cast<const f32x4*>(w + (int64_t)min(s0 + i * per + sub, live - 1) * a.DW);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc = s0 + i < live ? fmaf(v[i], __shfl(g, s0 + i, 64), acc) : acc;
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i * per + sub;
+      const float h = __shfl(g, min(s, 63), 64);
+      if (s < live && sub < per) acc += v[i] * h;
     }
-    if (d < a.D) op[d] = from_f32<T>(acc);
+  }
+  f32x4 sum = acc;
+  for (int k = 1; k < per; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += __shfl(acc[i], lane + k * lanes, 64);
+  if (sub != 0) return;
+  T* op = static_cast<T*>(a.out) + (item / Hq) * a.o_st + (item % Hq) * a.o_sh + d;
+  if (a.o_vec && d + 4 <= a.D) {
+    store4<T>(op, sum[0], sum[1], sum[2], sum[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < a.D) op[i] = from_f32<T>(sum[i]);
   }
 }
 
@@ -183,9 +189,10 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   own.blocks = slots * Hkv * splits;
   pre.a.pieces = (int)pieces;
   if (slots > 0x3FFFFFFF || own.blocks > 0x7FFFFFFF || pre.blocks > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "%s: too large", fn);
-  need = pieces > 1 ? rows * pieces * (a.DW + 2) : 0;
+  need = pieces > 1 ? rows * (pieces * (a.DW + 2) + 1) : 0;
   own.a.ws = pre.a.ws = ws;
   own.a.ws_ml = pre.a.ws_ml = ws ? ws + rows * pieces * a.DW : nullptr;
+  own.a.ws_live = ws ? reinterpret_cast<int32_t*>(ws + rows * pieces * (a.DW + 2)) : nullptr;
   return MLS_OK;
 }
 

@@ -22,6 +22,7 @@ struct GqaArgs {
   int64_t o_st, o_sh;
   float* ws;     // [T][Hkv * group][pieces][DW]: O of each piece, not divided by its sum
   float* ws_ml;  // [T][Hkv * group][pieces][2]: its reference and sum
+  int32_t* ws_live;  // [T][Hkv * group]: pieces of the sequence's own keys that were made
   int64_t num_blocks;
   int n, T, Hkv, group, D, DW, BS;
   uint32_t bs_magic;  // ceil(2^32 / BS)
@@ -108,11 +109,8 @@ __device__ __forceinline__ int gqa_piece(const GqaArgs& a, int lane) {
     sum += (float)((((int64_t)nt * a.group + (1 << a.bm_log) - 1) >> a.bm_log) * t);
     if (nt > 0) most = max(most, t);
   }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    sum += __shfl_xor(sum, off, 64);
-    most = max(most, __shfl_xor(most, off, 64));
-  }
+  sum = lane_group_sum<64>(sum);
+  most = (int)lane_group_max<64>((float)min(most, 1 << 24));
   const int want = (int)fminf(ceilf(sum * a.Hkv / a.target), 1e9f);
   return __builtin_amdgcn_readfirstlane(max(max(want, (most + a.splits - 1) / a.splits), a.least));
 }
@@ -146,9 +144,11 @@ __device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int 
   if (a.shared) {
     pmin = 0x7FFFFFFF;
     pmax = a.front - 1;
-    for (int t = first + lane; t <= last; t += 64) pmin = min(pmin, a.front + max(a.lens[t], 0) - 1);
+    if (a.window > 0) {
+      for (int t = first + lane; t <= last; t += 64) pmin = min(pmin, a.front + max(a.lens[t], 0) - 1);
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) pmin = min(pmin, __shfl_xor(pmin, off, 64));
+      for (int off = 32; off >= 1; off >>= 1) pmin = min(pmin, __shfl_xor(pmin, off, 64));
+    }
   } else {
     pmin = p.pos0 + first;
     pmax = p.pos0 + last;
@@ -193,6 +193,35 @@ __device__ __forceinline__ void gqa_row_range(const GqaArgs& a, const GqaPlan& p
   pos = a.shared ? a.front + max(a.lens[tok], 0) - 1 : p.pos0 + (tok - p.tok0);
   hi = min(max(pos + 1, p.pfx), p.len);
   lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+}
+
+// Over the packed rows r0 .. r1 (none where r1 < r0) of one sequence, or of shared rows: the extremes
+// of the keys [lo, hi) that they see.
+__device__ __forceinline__ void gqa_wave_range(const GqaArgs& a, const GqaPlan& p, int r0, int r1, int lane, int& lo_min,
+                                               int& lo_max, int& hi_min, int& hi_max) {
+  lo_min = hi_min = 0x7FFFFFFF;
+  lo_max = hi_max = -0x7FFFFFFF;
+  if (r1 < r0) return;
+  const int t0 = p.tok0 + r0 / a.group, t1 = p.tok0 + r1 / a.group;
+  if (!a.shared) {  // (positions rise with the row)
+    int pos;
+    gqa_row_range(a, p, t0, lo_min, hi_min, pos);
+    gqa_row_range(a, p, t1, lo_max, hi_max, pos);
+    return;
+  }
+  hi_min = hi_max = p.len;
+  lo_min = lo_max = 0;
+  if (a.window <= 0) return;
+  int lo, hi, pos;
+  gqa_row_range(a, p, min(t0 + lane, t1), lo, hi, pos);  // (at most 32 rows)
+  lo_min = lo_max = lo;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    lo_min = min(lo_min, __shfl_xor(lo_min, off, 64));
+    lo_max = max(lo_max, __shfl_xor(lo_max, off, 64));
+  }
+  lo_min = __builtin_amdgcn_readfirstlane(lo_min);
+  lo_max = __builtin_amdgcn_readfirstlane(lo_max);
 }
 
 }  // namespace mls
