@@ -25,9 +25,9 @@ namespace mls {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// 16 bytes of zeros: what a lane loads for a key outside its range, of a block id outside the
-// pool, or for elements past the head dim.
-static __device__ __align__(16) const uint32_t gqa_zeros[4] = {0, 0, 0, 0};
+// Zeros: what a lane loads for a key outside its range, of a block id outside the pool, or for
+// elements past the head dim. A whole row of the widest head.
+static __device__ __align__(16) const uint32_t gqa_zeros[256] = {};
 
 template <typename T>
 struct GqaType {
@@ -74,11 +74,6 @@ __device__ __forceinline__ uint32_t gqa_rest2(float lo, float hi, uint32_t p) {
   }
 }
 
-__device__ __forceinline__ void gqa_lds_load16(const void* g, void* lds) {
-  __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)g,
-                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
-}
-
 // Maximum over the four 16-lane rows of a wavefront, lane & 15 kept apart.
 __device__ __forceinline__ float gqa_row_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, 64));
@@ -90,7 +85,7 @@ __device__ __forceinline__ float gqa_row_sum(float v) {
 }
 
 // Geometry of a tile of BN keys in LDS: rows of DL elements (a power of two), CPR chunks a row.
-// Chunk c of K row r sits at c ^ (r & 7); of V row r at c ^ 2 (r & 7) (16-bit: the four rows that
+// Chunk c of K row r sits at c ^ (r & 15) (16 lanes read one chunk of 16 rows at once); of V row r at c ^ 2 (r & 7) (16-bit: the four rows that
 // one group of 16 lanes reads transposed, 32 bytes of each, lie in different banks) or, fp32,
 // c ^ 4 ((r >> 2) & 3) (four lane groups read 64 bytes of rows 4 apart).
 template <typename T, int DP>
@@ -98,64 +93,131 @@ struct GqaTile {
   static constexpr int CE = GqaType<T>::CE;
   static constexpr int DL = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;
   static constexpr int CPR = DL / CE, ROWB = DL * (int)sizeof(T);
-  __device__ static __forceinline__ int swz_k(int r) { return r & 7; }
+  __device__ static __forceinline__ int swz_k(int r) { return r & (CPR >= 16 ? 15 : 7); }
   __device__ static __forceinline__ int swz_v(int r) {
     if constexpr (GqaType<T>::F32) return ((r >> 2) & 3) << 2;
     return (r << 1) & (CPR >= 16 ? 14 : 6);
   }
 };
 
-// Loads the K rows (V = false) or V rows of BN keys into LDS, by WAVES wavefronts, of which this is
-// `wave`. off: lane i's is key i's byte offset in the pool, -1 for a key to be read as zeros. `whole`
-// (uniform): no such key, no padded elements, and an instruction's rows all lie in one cache block, so
-// that they need one address, in scalar registers. (With an address a row for every lane, the loads'
-// addresses alone are 78 vector instructions a tile of 64 keys, a third of the main loop's.)
-template <typename T, int DP, int BN, int WAVES, bool VEC, bool V>
-__device__ __forceinline__ void gqa_fill(const GqaArgs& a, uint8_t* dst, const uint8_t* base, int64_t off, bool whole, int wave,
-                                         int lane) {
+// Before a main loop: the loads so far (q, block ids) have landed, said in a way that the compiler
+// counts; else their first use in the loop would wait, in every pass, for the loop's loads.
+__device__ __forceinline__ void gqa_landed() { __builtin_amdgcn_s_waitcnt(0 | 0x70 | 0xF00); }
+
+// A sequence's block ids: 128 of them in two registers, a lane each, so that a tile's lookup is no
+// load (one that the counter of the tiles' own loads would make wait for those).
+struct GqaTable {
+  int tab, next, base;  // entries [base, base + 64) and [base + 64, base + 128)
+  __device__ __forceinline__ int load(const GqaArgs& a, const GqaPlan& p, int from, int lane) const {
+    const int e = from + lane;
+    const int blk = p.khi > 0 && e <= gqa_block_of(a, p.khi - 1) ? p.table[e] : -1;
+    return blk < a.num_blocks ? blk : -1;
+  }
+  __device__ __forceinline__ void start(const GqaArgs& a, const GqaPlan& p, int j0, int lane) {
+    base = gqa_block_of(a, j0);
+    tab = load(a, p, base, lane);
+    next = load(a, p, base + 64, lane);
+  }
+  // Lane i < n: the block of key j0 + i (tiles in rising order), negative for none; `ok`: the keys of them that
+  // any row of the tile sees.
+  __device__ __forceinline__ int at(const GqaArgs& a, const GqaPlan& p, int j0, int n, int lane, uint64_t& ok) {
+    ok = 0;
+    if (j0 >= p.khi) return -1;
+    const int first = gqa_block_of(a, j0);
+    while (first - base >= 64) {
+      tab = next;
+      base += 64;
+      next = load(a, p, base + 64, lane);
+      gqa_landed();  // (once in 64 blocks)
+    }
+    const int key = j0 + lane, i = gqa_block_of(a, key) - base;
+    const int x = __shfl(tab, i & 63, 64), y = __shfl(next, i & 63, 64);
+    const int blk = i < 64 ? x : y;
+    ok = __ballot(lane < n && key >= p.klo && key < p.khi && blk >= 0);
+    return blk;
+  }
+};
+
+// Loads of a tile of BN keys by WAVES wavefronts: rows of one instruction, instructions of one wavefront.
+template <typename T, int DP, int BN, int WAVES>
+struct GqaFill {
   using G = GqaTile<T, DP>;
-  constexpr int ROWS = 64 / G::CPR, ITER = BN / ROWS / WAVES;  // rows of one instruction; instructions
+  static constexpr int ROWS = 64 / G::CPR, ITER = BN / ROWS / WAVES;
   static_assert(BN <= 64 && ITER * ROWS * WAVES == BN, "whole instructions");
-  const int r = lane / G::CPR, c = lane % G::CPR;
-  if (VEC && whole) {
+  uint64_t at[ITER];  // uniform: each instruction's first row, bytes from a head's base
+  uint64_t ok;        // the keys that are there: the others are read as zeros
+
+  // One address an instruction, whose rows lie in one cache block (gqa_rows_of), made by scalar instructions. (With an address a row for
+  // every lane, the addresses alone are 78 vector instructions a tile of 64 keys, a third of the main loop's.)
+  __device__ __forceinline__ void place(const GqaArgs& a, int j0, int blk, uint64_t okmask, int wave) {
+    ok = okmask;
 #pragma unroll
     for (int u = 0; u < ITER; ++u) {
-      const int row = (u * WAVES + wave) * ROWS;  // (uniform)
-      const int64_t o = ((int64_t)__builtin_amdgcn_readlane((int)(off >> 32), row) << 32) |
-                        (uint32_t)__builtin_amdgcn_readlane((int)off, row);
+      const int row = (u * WAVES + wave) * ROWS, key = j0 + row;
+      const uint32_t b = __builtin_amdgcn_readlane(blk, row), t = key - gqa_block_of(a, key) * a.BS;
+      at[u] = (uint64_t)b * a.sb_bytes + (uint64_t)t * a.st_bytes;
+    }
+  }
+  // The K (V = false) or V rows straight into LDS. By buffer loads, whose bounds give the zeros; and the
+  // compiler takes LDS-direct loads of the global kind for accesses that may return in any order, so that
+  // every later LDS read would wait for all reads (lgkmcnt(0)) and some for all loads: 595 us for a prompt of 8192.
+  template <bool V>
+  __device__ __forceinline__ void load(const GqaArgs& a, uint8_t* dst, const uint8_t* base, int wave, int lane) const {
+    constexpr uint64_t FULL = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
+    const int r = lane / G::CPR, c = lane % G::CPR;
+    const bool whole = ok == FULL && a.D == G::DL;
+#pragma unroll
+    for (int u = 0; u < ITER; ++u) {
+      const int row = (u * WAVES + wave) * ROWS;
       const int cc = c ^ (V ? G::swz_v(row + r) : G::swz_k(row + r));
-      const uint32_t in = (uint32_t)r * (uint32_t)a.kv_st * (uint32_t)sizeof(T) + cc * 16;
-      gqa_lds_load16(base + o + in, dst + (u * WAVES + wave) * 1024);
+      uint32_t off = (uint32_t)r * a.st_bytes + cc * 16;
+      if (!whole && !(((uint32_t)(ok >> row) >> r & 1) && cc * G::CE < a.D)) off = 0xFFFFFFFFu;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(base + at[u]), (short)0, 0x7FFFFFFF, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(dst + (u * WAVES + wave) * 1024), 16, (int)off, 0, 0, 0);
     }
-    return;
   }
+  // Pools of any alignment and block size, through registers; blk: lane i's is key i's block
+  template <bool V>
+  __device__ __forceinline__ static void load_any(const GqaArgs& a, uint8_t* dst, const uint8_t* base, int j0, int blk, uint64_t ok,
+                                                  int wave, int lane) {
+    const int r = lane / G::CPR, c = lane % G::CPR;
 #pragma unroll
-  for (int u = 0; u < ITER; ++u) {
-    const int row = (u * WAVES + wave) * ROWS + r;
-    const int lo = __shfl((int)off, row, 64), hi = __shfl((int)(off >> 32), row, 64);
-    const int64_t o = ((int64_t)hi << 32) | (uint32_t)lo;
-    const int cc = c ^ (V ? G::swz_v(row) : G::swz_k(row));
-    uint8_t* d = dst + (u * WAVES + wave) * 1024;
-    if constexpr (VEC) {
-      const uint8_t* zero = reinterpret_cast<const uint8_t*>(gqa_zeros);
-      gqa_lds_load16(hi >= 0 && cc * G::CE < a.D ? base + o + cc * 16 : zero, d);
-    } else {
-      T x[G::CE];
+    for (int u = 0; u < ITER; ++u) {
+      const int row = (u * WAVES + wave) * ROWS + r, key = j0 + row;
+      const int b = __shfl(blk, row, 64);
+      const int64_t o = ((int64_t)b * a.kv_sb + (int64_t)(key - gqa_block_of(a, key) * a.BS) * a.kv_st) * (int64_t)sizeof(T);
+      const int cc = c ^ (V ? G::swz_v(row) : G::swz_k(row));
+      const bool in = (ok >> row) & 1;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (a.kv_vec) {
+        if (in && cc * G::CE < a.D) v = *reinterpret_cast<const uint4*>(base + o + cc * 16);
+      } else {
+        T x[G::CE];
 #pragma unroll
-      for (int e = 0; e < G::CE; ++e) {
-        const int dd = cc * G::CE + e;
-        x[e] = hi >= 0 && dd < a.D ? reinterpret_cast<const T*>(base + o)[dd] : (T)0.0f;
+        for (int e = 0; e < G::CE; ++e) {
+          const int dd = cc * G::CE + e;
+          x[e] = in && dd < a.D ? reinterpret_cast<const T*>(base + o)[dd] : (T)0.0f;
+        }
+        v = __builtin_bit_cast(uint4, x);
       }
-      *reinterpret_cast<uint4*>(d + lane * 16) = __builtin_bit_cast(uint4, x);
+      *reinterpret_cast<uint4*>(dst + (u * WAVES + wave) * 1024 + lane * 16) = v;
     }
   }
-}
+};
 
-// The place of key `key` in the pools (bytes from a head's base), from its block id.
-__device__ __forceinline__ int64_t gqa_key_offset(const GqaArgs& a, int key, int blk, bool in, int esz) {
-  const bool ok = in && blk >= 0 && blk < a.num_blocks;
-  const int t = key - gqa_block_of(a, key) * a.BS;
-  return ok ? ((int64_t)blk * a.kv_sb + (int64_t)t * a.kv_st) * esz : -1;
+// A tile's rows into LDS, with its addresses made here.
+template <typename T, int DP, int BN, int WAVES, bool VEC, bool V>
+__device__ __forceinline__ void gqa_fill(const GqaArgs& a, uint8_t* dst, const uint8_t* base, int j0, int blk, uint64_t ok, int wave,
+                                         int lane) {
+  using F = GqaFill<T, DP, BN, WAVES>;
+  if constexpr (VEC) {
+    F f;
+    f.place(a, j0, blk, ok, wave);
+    f.template load<V>(a, dst, base, wave, lane);
+  } else {
+    F::template load_any<V>(a, dst, base, j0, blk, ok, wave, lane);
+  }
 }
 
 // One wavefront's rows: 16 NT query rows with their softmax state. SPLIT: P as two parts of the
@@ -171,13 +233,16 @@ struct GqaRows {
   uint4 q[NT][QT];
   f32x4 o[NT][OT], ol[NT];
   float m[NT];
-  int lo[NT], hi[NT], pos[NT];  // the keys that a row sees: [lo, hi)
-  float slope[NT];              // times log2(e)
+  // in LDS, since only masked tiles and biased scores need it: the keys [x, y) that a row sees, its
+  // position and its slope's bits (times log2(e))
+  int4* at;
   int lo_min, lo_max, hi_min, hi_max;  // over the wavefront's rows
 
   // row0: the wavefront's first packed row of the tile's sequence
-  __device__ __forceinline__ void init(const GqaArgs& a, const GqaPlan& p, int row0, int kvh, int lane) {
+  // ranges: 16 NT places of the wavefront's own
+  __device__ __forceinline__ void init(const GqaArgs& a, const GqaPlan& p, int row0, int kvh, int4* ranges, int lane) {
     const int g = lane >> 4;
+    at = ranges;
     gqa_wave_range(a, p, row0, min(row0 + 16 * NT, p.rows) - 1, lane, lo_min, lo_max, hi_min, hi_max);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -188,8 +253,10 @@ struct GqaRows {
       const int r = row0 + 16 * n + (lane & 15);
       const bool in = r < p.rows;
       const int t = r / a.group, tok = min(p.tok0 + t, a.T - 1), head = kvh * a.group + r - t * a.group;
-      gqa_row_range(a, p, tok, lo[n], hi[n], pos[n]);
-      slope[n] = a.slopes ? a.slopes[head] * 1.44269504f : 0.0f;
+      int lo, hi, pos;
+      gqa_row_range(a, p, tok, lo, hi, pos);
+      const float slope = a.slopes ? a.slopes[head] * 1.44269504f : 0.0f;
+      if (g == 0) at[16 * n + lane] = make_int4(lo, hi, pos, __float_as_int(slope));
       const T* src = static_cast<const T*>(a.q) + tok * a.q_st + head * a.q_sh;
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
@@ -212,28 +279,81 @@ struct GqaRows {
   __device__ __forceinline__ bool sees_all(int j, int n) const { return lo_max <= j && j + n <= hi_min; }
   __device__ __forceinline__ bool sees_any(int j, int n) const { return lo_min < j + n && j < hi_max; }
 
-  // S = K Q^T for the BN keys in kt; a sub-tile's fragments are read while the one before it multiplies
-  template <int BN>
-  __device__ __forceinline__ void scores(const uint8_t* kt, int lane, f32x4 (&s)[NT][BN / 16]) const {
-    constexpr int KT = BN / 16;
+  // O^T += V^T P^T over the BN keys in vt (PV), then S = K Q^T for those in kt (QK). The fragments of both
+  // are one sequence, read DEPTH ahead of their use: the order is pinned, since the compiler, short of
+  // registers, reads each just before its use (a read's latency is four fragments' products; prompt of
+  // 8192 so, 2 wavefronts a SIMD taking turns: 972 us).
+  template <int BN, bool PV, bool QK>
+  __device__ __forceinline__ void matrix(const uint4 (&pf)[BN / 32 + (BN < 32)][NT], const uint4 (&pr)[BN / 32 + (BN < 32)][NT],
+                                         const uint8_t* vt, const uint8_t* kt, f32x4 (&s)[NT][BN / 16], int lane) {
+    constexpr int NV = PV ? BN / 32 * OT : 0, NK = QK ? BN / 16 * QT : 0, N = NV + NK, DEPTH = N < 6 ? N : 6;
     const int g = lane >> 4, c = lane & 15;
-    const uint8_t* at[QT];
+    const int vrow = 4 * g + (c >> 2);  // (and 16, 32 further on: the same swizzle)
+    const uint8_t* vbase = vt + vrow * G::ROWB + (c & 1) * 8;
+    const uint8_t* kbase = kt + c * G::ROWB;
+    auto read = [&](int x) __attribute__((always_inline)) {
+      if (x < NV) {
+        const int h = x / OT, d = x % OT;
+        const uint8_t* p = vbase + h * 32 * G::ROWB + (((2 * d + ((c >> 1) & 1)) ^ G::swz_v(vrow)) << 4);
+        struct {
+          s16x4 a, b;
+        } v{__builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p),
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 16 * G::ROWB))};
+        return __builtin_bit_cast(uint4, v);
+      }
+      const int k = (x - NV) / QT, t = (x - NV) % QT;
+      return *reinterpret_cast<const uint4*>(kbase + k * 16 * G::ROWB + (((4 * t + g) ^ G::swz_k(c)) << 4));
+    };
+    uint4 f[DEPTH];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) at[t] = kt + c * G::ROWB + (((4 * t + g) ^ G::swz_k(c)) << 4);
-    uint4 kf[2][QT];
+    for (int x = 0; x < DEPTH; ++x) f[x] = read(x);
 #pragma unroll
-    for (int t = 0; t < QT; ++t) kf[0][t] = *reinterpret_cast<const uint4*>(at[t]);
+    for (int x = 0; x < N; ++x) {
+      const uint4 v = f[x % DEPTH];
+      if (x < NV) {
+        const int h = x / OT, d = x % OT;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[n][d] = gqa_mma<T>(v, pf[h][n], o[n][d]);
+        if constexpr (SPLIT)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) o[n][d] = gqa_mma<T>(v, pr[h][n], o[n][d]);
+        if (d == OT - 1) {
+          constexpr uint32_t ONE = __is_same(T, __bf16) ? 0x3F803F80u : 0x3C003C00u;
+          const uint4 ones = make_uint4(ONE, ONE, ONE, ONE);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            ol[n] = gqa_mma<T>(ones, pf[h][n], ol[n]);
+            if constexpr (SPLIT) ol[n] = gqa_mma<T>(ones, pr[h][n], ol[n]);
+          }
+        }
+      } else {
+        const int k = (x - NV) / QT, t = (x - NV) % QT;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][k] = gqa_mma<T>(v, q[n][t], t == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[n][k]);
+      }
+      if (x + DEPTH < N) f[x % DEPTH] = read(x + DEPTH);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // S = K Q^T for the BN keys in kt
+  template <int BN>
+  __device__ __forceinline__ void scores(const uint8_t* kt, int lane, f32x4 (&s)[NT][BN / 16]) {
+    const uint4 none[BN / 32 + (BN < 32)][NT] = {};
+    matrix<BN, false, true>(none, none, nullptr, kt, s, lane);
+  }
+
+  // The same from fragments in registers
+  template <int KT>
+  __device__ __forceinline__ void scores_of(const uint4 (&kf)[KT][QT], f32x4 (&s)[NT][KT]) const {
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
-      if (k + 1 < KT)
 #pragma unroll
-        for (int t = 0; t < QT; ++t) kf[(k + 1) & 1][t] = *reinterpret_cast<const uint4*>(at[t] + (k + 1) * 16 * G::ROWB);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][k] = gqa_mma<T>(kf[k & 1][0], q[n][0], f32x4{0.f, 0.f, 0.f, 0.f});
+      for (int n = 0; n < NT; ++n) s[n][k] = gqa_mma<T>(kf[k][0], q[n][0], f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
       for (int t = 1; t < QT; ++t)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][k] = gqa_mma<T>(kf[k & 1][t], q[n][t], s[n][k]);
+        for (int n = 0; n < NT; ++n) s[n][k] = gqa_mma<T>(kf[k][t], q[n][t], s[n][k]);
     }
   }
 
@@ -247,20 +367,22 @@ struct GqaRows {
     float cc = a.c;
     if (!a.simple) {
       cc = 1.0f;
-      scored<KT>(a, s, j0, g);
+      scored<KT>(a, s, j0, lane);
     }
     constexpr uint64_t FULL = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
     if (okmask != FULL || !sees_all(j0, BN)) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        const int4 x = at[16 * n + (lane & 15)];
 #pragma unroll
         for (int k = 0; k < KT; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int kk = 16 * k + 4 * g + i, j = j0 + kk;
-            const bool see = lo[n] <= j && j < hi[n] && ((okmask >> kk) & 1);
+            const bool see = x.x <= j && j < x.y && ((okmask >> kk) & 1);
             s[n][k][i] = see ? s[n][k][i] : -__builtin_huge_valf();
           }
+      }
     }
     float mx[NT];
     bool over = false;
@@ -298,7 +420,7 @@ struct GqaRows {
 
   // Raw products -> scores in log2 units, with the cap and the bias by distance
   template <int KT>
-  __device__ __forceinline__ void scored(const GqaArgs& a, f32x4 (&s)[NT][KT], int j0, int g) const {
+  __device__ __forceinline__ void scored(const GqaArgs& a, f32x4 (&s)[NT][KT], int j0, int lane) const {
     if (a.cap > 0.0f) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -321,73 +443,57 @@ struct GqaRows {
     }
     if (a.slopes) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        const int4 x = at[16 * n + (lane & 15)];
+        const float slope = __int_as_float(x.w);
+        const int gap = x.z - j0 - 4 * (lane >> 4);
 #pragma unroll
         for (int k = 0; k < KT; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s[n][k][i] = fmaf(-slope[n], fabsf((float)(pos[n] - (j0 + 16 * k + 4 * g + i))), s[n][k][i]);
+          for (int i = 0; i < 4; ++i) s[n][k][i] = fmaf(-slope, fabsf((float)(gap - (16 * k + i))), s[n][k][i]);
+      }
     }
   }
 
   // O^T += V^T P^T, and the weights' sums
   template <int BN>
-  __device__ __forceinline__ void product(const f32x4 (&s)[NT][BN / 16], const uint8_t* vt, int lane) {
-    const int g = lane >> 4, c = lane & 15;
+  __device__ __forceinline__ void product(f32x4 (&s)[NT][BN / 16], const uint8_t* vt, int lane) {
     if constexpr (K::F32) {
+      const int g = lane >> 4, c = lane & 15;
+      constexpr int N = BN / 4 * OT, DEPTH = 8;
+      auto read = [&](int x) __attribute__((always_inline)) {
+        const int i = x / OT % 4, row = 16 * (x / OT / 4) + 4 * g + i, d = x % OT;
+        const int ch = (4 * d + (c >> 2)) ^ G::swz_v(row);
+        return *reinterpret_cast<const float*>(vt + row * G::ROWB + ch * 16 + (c & 3) * 4);
+      };
+      float f[DEPTH];
 #pragma unroll
-      for (int k = 0; k < BN / 16; ++k)
+      for (int x = 0; x < DEPTH; ++x) f[x] = read(x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = 16 * k + 4 * g + i;
+      for (int x = 0; x < N; ++x) {
+        const float v = f[x % DEPTH];
+        const int k = x / OT / 4, i = x / OT % 4, d = x % OT;
 #pragma unroll
-          for (int d = 0; d < OT; ++d) {
-            const int ch = (4 * d + (c >> 2)) ^ G::swz_v(row);
-            const float v = *reinterpret_cast<const float*>(vt + row * G::ROWB + ch * 16 + (c & 3) * 4);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[n][k][i], o[n][d], 0, 0, 0);
-          }
-        }
-    } else {
-      constexpr uint32_t ONE = __is_same(T, __bf16) ? 0x3F803F80u : 0x3C003C00u;
-      const uint4 ones = make_uint4(ONE, ONE, ONE, ONE);
-      const int row = 4 * g + (c >> 2);  // (and 16, 32 further on: the same swizzle)
-      const uint8_t* at[OT];
-#pragma unroll
-      for (int d = 0; d < OT; ++d)
-        at[d] = vt + row * G::ROWB + (c & 1) * 8 + (((2 * d + ((c >> 1) & 1)) ^ G::swz_v(row)) << 4);
-#pragma unroll
-      for (int h = 0; h < BN / 32; ++h) {
-        uint4 pf[NT], pr[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const f32x4 x = s[n][2 * h], y = s[n][2 * h + 1];
-          pf[n] = make_uint4(gqa_pack2<T>(x[0], x[1]), gqa_pack2<T>(x[2], x[3]), gqa_pack2<T>(y[0], y[1]), gqa_pack2<T>(y[2], y[3]));
-          if constexpr (SPLIT)
-            pr[n] = make_uint4(gqa_rest2<T>(x[0], x[1], pf[n].x), gqa_rest2<T>(x[2], x[3], pf[n].y),
-                               gqa_rest2<T>(y[0], y[1], pf[n].z), gqa_rest2<T>(y[2], y[3], pf[n].w));
-        }
-#pragma unroll
-        for (int d = 0; d < OT; ++d) {
-          const uint8_t* p = at[d] + h * 32 * G::ROWB;
-          struct {
-            s16x4 a, b;
-          } v{__builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p),
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 16 * G::ROWB))};
-          const uint4 vf = __builtin_bit_cast(uint4, v);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) o[n][d] = gqa_mma<T>(vf, pf[n], o[n][d]);
-          if constexpr (SPLIT)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[n][d] = gqa_mma<T>(vf, pr[n], o[n][d]);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          ol[n] = gqa_mma<T>(ones, pf[n], ol[n]);
-          if constexpr (SPLIT) ol[n] = gqa_mma<T>(ones, pr[n], ol[n]);
-        }
+        for (int n = 0; n < NT; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[n][k][i], o[n][d], 0, 0, 0);
+        if (x + DEPTH < N) f[x % DEPTH] = read(x + DEPTH);
+        if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
+      uint4 pf[BN / 32][NT], pr[BN / 32][NT];
+#pragma unroll
+      for (int h = 0; h < BN / 32; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) pack(s[n][2 * h], s[n][2 * h + 1], pf[h][n], pr[h][n]);
+      matrix<BN, true, false>(pf, pr, vt, nullptr, s, lane);
     }
+  }
+
+  // The weights of 32 keys as operands of the product with V
+  __device__ __forceinline__ static void pack(const f32x4& x, const f32x4& y, uint4& p, uint4& rest) {
+    p = make_uint4(gqa_pack2<T>(x[0], x[1]), gqa_pack2<T>(x[2], x[3]), gqa_pack2<T>(y[0], y[1]), gqa_pack2<T>(y[2], y[3]));
+    if constexpr (SPLIT)
+      rest = make_uint4(gqa_rest2<T>(x[0], x[1], p.x), gqa_rest2<T>(x[2], x[3], p.y), gqa_rest2<T>(y[0], y[1], p.z),
+                        gqa_rest2<T>(y[2], y[3], p.w));
   }
 
   __device__ __forceinline__ float sum_of(int n) const { return LMMA ? ol[n][0] : gqa_row_sum(ol[n][0]); }
@@ -428,14 +534,15 @@ constexpr int gqa_bn() {
 
 template <typename T, int DP, int NT, int BN, bool VEC>
 __device__ __forceinline__ void gqa_rows_step(const GqaArgs& a, GqaRows<T, DP, NT, false>& rows, const uint8_t* __restrict__ cur,
-                                              uint8_t* __restrict__ nxt, const uint8_t* kbase, const uint8_t* vbase, int64_t off,
-                                              bool more, bool whole, int j0, uint64_t okmask, int wave, int lane) {
+                                              uint8_t* __restrict__ nxt, const uint8_t* __restrict__ kbase,
+                                              const uint8_t* __restrict__ vbase, int blk, uint64_t ok1, bool now,
+                                              bool more, int j0, uint64_t okmask, int wave, int lane) {
   constexpr int TB = BN * GqaTile<T, DP>::ROWB;
   if (more) {
-    gqa_fill<T, DP, BN, 4, VEC, false>(a, nxt, kbase, off, whole, wave, lane);
-    gqa_fill<T, DP, BN, 4, VEC, true>(a, nxt + TB, vbase, off, whole, wave, lane);
+    gqa_fill<T, DP, BN, 4, VEC, false>(a, nxt, kbase, j0 + BN, blk, ok1, wave, lane);
+    gqa_fill<T, DP, BN, 4, VEC, true>(a, nxt + TB, vbase, j0 + BN, blk, ok1, wave, lane);
   }
-  if (!rows.sees_any(j0, BN)) return;
+  if (!now || !rows.sees_any(j0, BN)) return;
   f32x4 s[NT][BN / 16];
   rows.template scores<BN>(cur, lane, s);
   rows.template weigh<BN>(a, s, j0, okmask, lane);
@@ -445,7 +552,6 @@ __device__ __forceinline__ void gqa_rows_step(const GqaArgs& a, GqaRows<T, DP, N
 template <typename T, int DP, int NT, bool VEC>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void gqa_rows_kernel(const GqaArgs a) {
   constexpr int BN = gqa_bn<T, DP>(), TB = BN * GqaTile<T, DP>::ROWB;
-  constexpr uint64_t FULL = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int kvh, split;
@@ -453,33 +559,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void gqa_rows_kernel(const 
   if (split >= p.live || p.rows <= p.row0) return;
   GqaRows<T, DP, NT, false> rows;
   const int row0 = p.row0 + wave * 16 * NT;
-  rows.init(a, p, row0, kvh, lane);
+  rows.init(a, p, row0, kvh, reinterpret_cast<int4*>(smem + 4 * TB) + wave * 16 * NT, lane);
   const uint8_t* kbase = static_cast<const uint8_t*>(a.kp) + kvh * a.kv_sh * (int64_t)sizeof(T);
   const uint8_t* vbase = static_cast<const uint8_t*>(a.vp) + kvh * a.kv_sh * (int64_t)sizeof(T);
-  const bool blocks = a.D == GqaTile<T, DP>::DL && a.BS % (64 / GqaTile<T, DP>::CPR) == 0 && a.kv_st < (1 << 24);
   const int t0 = split * p.per, t1 = min(p.tiles, t0 + p.per);
-  // lane i looks up key i of a tile, two tiles ahead of its use
-  auto key_in = [&](int t) { const int j = p.lo + t * BN + lane; return lane < BN && t < t1 && j >= p.klo && j < p.khi; };
-  auto look = [&](int t) { return key_in(t) ? p.table[gqa_block_of(a, p.lo + t * BN + lane)] : -1; };
   if (t0 < t1) {
-    int blk = look(t0);
-    int64_t off = gqa_key_offset(a, p.lo + t0 * BN + lane, blk, key_in(t0), sizeof(T));
-    uint64_t ok = __ballot(off >= 0);
-    blk = look(t0 + 1);
-    gqa_fill<T, DP, BN, 4, VEC, false>(a, smem, kbase, off, blocks && ok == FULL, wave, lane);
-    gqa_fill<T, DP, BN, 4, VEC, true>(a, smem + TB, vbase, off, blocks && ok == FULL, wave, lane);
-    auto step = [&](int t, const uint8_t* cur, uint8_t* nxt) __attribute__((always_inline)) {
+    GqaTable tab;
+    tab.start(a, p, p.lo + t0 * BN, lane);
+    gqa_landed();
+    uint64_t ok = 0;
+    for (int t = t0 - 1; t < t1; ++t) {  // (the first only loads)
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      off = gqa_key_offset(a, p.lo + (t + 1) * BN + lane, blk, key_in(t + 1), sizeof(T));
-      const uint64_t ok1 = __ballot(off >= 0);
-      blk = look(t + 2);
-      gqa_rows_step<T, DP, NT, BN, VEC>(a, rows, cur, nxt, kbase, vbase, off, t + 1 < t1, blocks && ok1 == FULL, p.lo + t * BN, ok,
-                                        wave, lane);
+      uint64_t ok1 = 0;
+      const int blk = t + 1 < t1 ? tab.at(a, p, p.lo + (t + 1) * BN, BN, lane, ok1) : -1;
+      const int cur = ((t - t0) & 1) * 2 * TB;
+      gqa_rows_step<T, DP, NT, BN, VEC>(a, rows, smem + cur, smem + (2 * TB - cur), kbase, vbase, blk, ok1, t >= t0,
+                                        t + 1 < t1, p.lo + t * BN, ok, wave, lane);
       ok = ok1;
-    };
-    for (int t = t0; t < t1; t += 2) {  // (in pairs: LDS addresses are constants then)
-      step(t, smem, smem + 2 * TB);
-      if (t + 1 < t1) step(t + 1, smem + 2 * TB, smem);
     }
   }
   const int g = lane >> 4;
@@ -497,41 +593,152 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void gqa_rows_kernel(const 
   }
 }
 
+// Many rows of 16-bit types: 8 wavefronts, two a SIMD, in two groups half a step apart: while one
+// group's matrix instructions run (the last tile's product with V, this tile's with K), the other
+// does its softmax on the vector unit, and a barrier swaps them. Left to themselves the two
+// wavefronts of a SIMD overlap by chance only (prompt of 8192, 32 heads of 128 over 8, 4 wavefronts a block:
+// 649 us, matrix unit busy 36%, vector unit 41%).
+// K and V tiles go through rings of 3: tile i + 2 of K and i + 1 of V are loaded from the start of step i.
+template <typename T, int DP>
+constexpr int gqa_pair_bn() { return DP <= 128 ? 64 : 32; }
+
+template <typename T, int DP, int NT>
+struct GqaPair {
+  static constexpr int BN = gqa_pair_bn<T, DP>(), TB = BN * GqaTile<T, DP>::ROWB, PER = TB / 1024 / 8;
+  using Fill = GqaFill<T, DP, BN, 8>;
+  GqaRows<T, DP, NT, false> rows;
+  f32x4 s[NT][BN / 16];
+  uint4 pf[BN / 32][NT];
+
+  // kr, vr: tiles i of K, i - 1 of V; kw, vw: the slots of tiles i + 2 and i + 1. (Every pointer is __restrict, the loads' sources
+  // too, or the loads would hold up the reads; no wait is in here, since one would not order accesses through them.)
+  __device__ __forceinline__ void multiply(const GqaArgs& a, const uint8_t* __restrict__ kr, uint8_t* __restrict__ kw,
+                                           const uint8_t* __restrict__ vr, uint8_t* __restrict__ vw,
+                                           const uint8_t* __restrict__ kbase, const uint8_t* __restrict__ vbase,
+                                           const Fill& kat, const Fill& vat, bool kmore, bool vmore, int wave, int lane) {
+    if (vmore) vat.template load<true>(a, vw, vbase, wave, lane);
+    if (kmore) kat.template load<false>(a, kw, kbase, wave, lane);
+    rows.template matrix<BN, true, true>(pf, pf, vr, kr, s, lane);
+  }
+  __device__ __forceinline__ void soften(const GqaArgs& a, int j0, uint64_t okmask, int lane) {
+    rows.template weigh<BN>(a, s, j0, okmask, lane);
+    uint4 none;
+#pragma unroll
+    for (int h = 0; h < BN / 32; ++h)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) GqaRows<T, DP, NT, false>::pack(s[n][2 * h], s[n][2 * h + 1], pf[h][n], none);
+  }
+};
+
+template <typename T, int DP, int NT>
+__global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
+  using P = GqaPair<T, DP, NT>;
+  constexpr int BN = P::BN, TB = P::TB;
+  extern __shared__ __align__(1024) uint8_t smem[];  // 3 tiles of K, 3 of V
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int kvh, split;
+  const GqaPlan p = gqa_block_plan(a, blockIdx.x, lane, kvh, split);
+  if (split >= p.live || p.rows <= p.row0) return;
+  const uint8_t* kbase = static_cast<const uint8_t*>(a.kp) + kvh * a.kv_sh * (int64_t)sizeof(T);
+  const uint8_t* vbase = static_cast<const uint8_t*>(a.vp) + kvh * a.kv_sh * (int64_t)sizeof(T);
+  const int t0 = split * p.per, n = min(p.tiles - t0, p.per), j0 = p.lo + t0 * BN;
+  P w;
+  const int row0 = p.row0 + wave * 16 * NT;
+  w.rows.init(a, p, row0, kvh, reinterpret_cast<int4*>(smem + 6 * TB) + wave * 16 * NT, lane);
+  if (n > 0) {
+    GqaTable tab;
+    tab.start(a, p, j0, lane);
+    gqa_landed();
+    typename P::Fill f0, f1, f2;  // tiles i, i + 1 and i + 2
+    f0.ok = f1.ok = f2.ok = 0;
+    const int b0 = tab.at(a, p, j0, BN, lane, f0.ok);
+    const int b1 = n > 1 ? tab.at(a, p, j0 + BN, BN, lane, f1.ok) : -1, b2 = n > 2 ? tab.at(a, p, j0 + 2 * BN, BN, lane, f2.ok) : -1;
+    gqa_fill<T, DP, BN, 8, true, false>(a, smem, kbase, j0, b0, f0.ok, wave, lane);
+    gqa_fill<T, DP, BN, 8, true, true>(a, smem + 3 * TB, vbase, j0, b0, f0.ok, wave, lane);
+    if (n > 1) gqa_fill<T, DP, BN, 8, true, false>(a, smem + TB, kbase, j0 + BN, b1, f1.ok, wave, lane);
+    f1.place(a, j0 + BN, b1, f1.ok, wave);
+    f2.place(a, j0 + 2 * BN, b2, f2.ok, wave);
+    uint64_t ok0 = f0.ok;
+    // V's tile -1: zeros, with weights of 0
+    for (int e = threadIdx.x; e < TB / 16; e += 512) reinterpret_cast<uint4*>(smem + 5 * TB)[e] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int h = 0; h < BN / 32; ++h)
+#pragma unroll
+      for (int m = 0; m < NT; ++m) w.pf[h][m] = make_uint4(0, 0, 0, 0);
+    gqa_landed();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (wave >= 4) asm volatile("s_barrier" ::: "memory");  // half a step behind
+    int s0 = 0, s1 = TB, s2 = 2 * TB;  // slots of tiles i, i + 1, i + 2 (and so of i - 1)
+    for (int i = 0; i < n; ++i) {
+      w.multiply(a, smem + s0, smem + s2, smem + 3 * TB + s2, smem + 3 * TB + s1, kbase, vbase, f2, f1, i + 2 < n,
+                 i + 1 < n, wave, lane);
+      // the last step's loads have landed (this one's may be on their way)
+      if (i + 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * P::PER) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      w.soften(a, j0 + i * BN, ok0, lane);
+      const int t = s0;
+      s0 = s1, s1 = s2, s2 = t;
+      ok0 = f1.ok;
+      f1 = f2;
+      uint64_t ok = 0;
+      const int b2 = i + 3 < n ? tab.at(a, p, j0 + (i + 3) * BN, BN, lane, ok) : -1;
+      f2.place(a, j0 + (i + 3) * BN, b2, ok, wave);
+      asm volatile("s_barrier" ::: "memory");
+    }
+    w.rows.template matrix<BN, true, false>(w.pf, w.pf, smem + 3 * TB + s2, nullptr, w.s, lane);
+    if (!(wave >= 4)) asm volatile("s_barrier" ::: "memory");
+  }
+  const int g = lane >> 4;
+#pragma unroll
+  for (int m = 0; m < NT; ++m) {
+    const int r = row0 + 16 * m + (lane & 15);
+    const float l = w.rows.sum_of(m);
+    if (r < p.rows) {
+      const int tok = p.tok0 + r / a.group, head = kvh * a.group + r % a.group;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+        gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, 16 * d + 4 * g, w.rows.o[m][d], w.rows.m[m], l);
+      if (g == 0) gqa_store_live(a, tok, head, split, p.live);
+    }
+  }
+}
+
 // Few rows: the NW wavefronts of a block hold the same 16 NT rows and take WK keys each of a
-// step of NW WK keys, each with LDS of its own, so that no wavefront waits for another before the end,
-// where their states are joined through LDS. A wavefront has one K and one V buffer: the next K
-// tile is on its way from the moment this one's scores are done, the next V tile from the end of
-// this one's product, so that 8 wavefronts a CU (64 KB of LDS a block) keep 64 to 128 KB of loads in
-// flight. (With two buffers of each and 4 wavefronts a CU, 64 KB in flight at most: 40
-// sequences of 1 to 4096 tokens, 32 heads of 128 over 8 K/V heads, 45 us.)
+// step of NW WK keys, so that no wavefront waits for another before the end, where their states are
+// joined through LDS. K's fragments are loaded straight into registers (16 rows of 64 bytes an
+// instruction), the next tile's as soon as this one's scores are made; V tiles go through LDS, to be read
+// transposed, the next one's loads issued after this one's product. (With two K and two V buffers in LDS and
+// 4 wavefronts a CU: 40 sequences of 1 to 4096 tokens, 32 heads of 128 over 8 K/V heads, 45 us.)
 template <typename T, int DP>
 constexpr int gqa_wk() { return GqaType<T>::F32 ? (DP <= 64 ? 32 : 16) : 32; }
 template <typename T, int DP>
 constexpr int gqa_nw() { return gqa_wk<T, DP>() * GqaTile<T, DP>::ROWB > 8192 ? 2 : 4; }
 
-template <typename T, int DP, int NT, int WK>
-__device__ __forceinline__ void gqa_keys_step(const GqaArgs& a, GqaRows<T, DP, NT, !GqaType<T>::F32>& rows, uint8_t* __restrict__ kt,
-                                              uint8_t* __restrict__ vt, const uint8_t* kbase, const uint8_t* vbase, int64_t off,
-                                              bool more, bool whole, int j0, uint64_t okmask, int lane) {
-  constexpr int PER = WK * GqaTile<T, DP>::ROWB / 1024;  // loads of a K or V tile
-  f32x4 s[NT][WK / 16];
-  // loads complete in order, and this K tile's are older than the V tile's (a table entry may follow those)
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
-  rows.template scores<WK>(kt, lane, s);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (K is read)
-  if (more) gqa_fill<T, DP, WK, 1, true, false>(a, kt, kbase, off, whole, 0, lane);
-  rows.template weigh<WK>(a, s, j0, okmask, lane);
-  if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
-  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  rows.template product<WK>(s, vt, lane);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (V is read)
-  if (more) gqa_fill<T, DP, WK, 1, true, true>(a, vt, vbase, off, whole, 0, lane);
+// The K fragments of keys j0 .. j0 + 16 KT; blk: lane i's is key i's block.
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void gqa_load_k(const GqaArgs& a, uint4 (&kf)[KT][DP / (4 * GqaType<T>::CE)], const uint8_t* base, int j0,
+                                           int blk, uint64_t ok, int lane) {
+  constexpr int CE = GqaType<T>::CE, QT = DP / (4 * CE);
+  const int g = lane >> 4, c = lane & 15;
+  const uint8_t* zero = reinterpret_cast<const uint8_t*>(gqa_zeros) + g * 16;
+#pragma unroll
+  for (int k = 0; k < KT; ++k) {
+    const int b = __shfl(blk, 16 * k + c, 64), key = j0 + 16 * k + c;
+    const int64_t o = ((int64_t)b * a.kv_sb + (int64_t)(key - gqa_block_of(a, key) * a.BS) * a.kv_st) * (int64_t)sizeof(T);
+    const uint8_t* row = (ok >> (16 * k + c)) & 1 ? base + o + g * 16 : zero;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const uint8_t* from = a.D == DP || (4 * t + g) * CE < a.D ? row : zero;
+      // (said to be global memory: chosen between two pointers, it would be a load of the flat kind)
+      kf[k][t] = __builtin_bit_cast(
+          uint4, __builtin_nontemporal_load((const __attribute__((address_space(1))) i32x4*)(from + t * 64)));
+    }
+  }
 }
 
 template <typename T, int DP, int NT>
 __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void gqa_keys_kernel(const GqaArgs a) {
   constexpr int WK = gqa_wk<T, DP>(), NW = gqa_nw<T, DP>(), TB = WK * GqaTile<T, DP>::ROWB, BN = NW * WK;
-  constexpr uint64_t FULL = (1ull << WK) - 1;
   constexpr int OL = DP + 4;  // floats of an output row in LDS
   extern __shared__ __align__(1024) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -541,33 +748,42 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
   GqaRows<T, DP, NT, !GqaType<T>::F32> rows;
   const uint8_t* kbase = static_cast<const uint8_t*>(a.kp) + kvh * a.kv_sh * (int64_t)sizeof(T);
   const uint8_t* vbase = static_cast<const uint8_t*>(a.vp) + kvh * a.kv_sh * (int64_t)sizeof(T);
-  const bool blocks = a.D == GqaTile<T, DP>::DL && a.BS % (64 / GqaTile<T, DP>::CPR) == 0 && a.kv_st < (1 << 24);
   int t0 = split * p.per, t1 = min(p.tiles, t0 + p.per);
   // this wavefront's first and last steps may hold none of its keys
   if (p.lo + t0 * BN + (wave + 1) * WK <= p.klo) ++t0;
   t1 = min(t1, (p.khi - p.lo - wave * WK + BN - 1) / BN);
-  uint8_t *kt = smem + wave * 2 * TB, *vt = kt + TB;
+  uint8_t* vt = smem + wave * TB;
   auto first = [&](int t) { return p.lo + t * BN + wave * WK; };
-  auto key_in = [&](int t) { const int j = first(t) + lane; return lane < WK && t < t1 && j >= p.klo && j < p.khi; };
-  auto look = [&](int t) { return key_in(t) ? p.table[gqa_block_of(a, first(t) + lane)] : -1; };
-  int64_t off = -1;
+  GqaTable tab;
+  rows.init(a, p, p.row0, kvh, reinterpret_cast<int4*>(smem + NW * TB) + wave * 16 * NT, lane);
+  if (t0 < t1) tab.start(a, p, first(t0), lane);
+  gqa_landed();
   uint64_t ok = 0;
-  int blk = -1;
   if (t0 < t1) {
-    blk = look(t0);
-    off = gqa_key_offset(a, first(t0) + lane, blk, key_in(t0), sizeof(T));
-    ok = __ballot(off >= 0);
-    gqa_fill<T, DP, WK, 1, true, false>(a, kt, kbase, off, blocks && ok == FULL, 0, lane);
-    gqa_fill<T, DP, WK, 1, true, true>(a, vt, vbase, off, blocks && ok == FULL, 0, lane);
-  }
-  rows.init(a, p, p.row0, kvh, lane);
-  blk = t0 + 1 < t1 ? look(t0 + 1) : -1;
-  for (int t = t0; t < t1; ++t) {
-    off = gqa_key_offset(a, first(t + 1) + lane, blk, key_in(t + 1), sizeof(T));
-    const uint64_t ok1 = __ballot(off >= 0);
-    blk = look(t + 2);
-    gqa_keys_step<T, DP, NT, WK>(a, rows, kt, vt, kbase, vbase, off, t + 1 < t1, blocks && ok1 == FULL, first(t), ok, lane);
-    ok = ok1;
+    constexpr int KT = WK / 16, PER = KT * (DP / (4 * GqaType<T>::CE));  // loads of a K tile
+    uint4 kf[KT][DP / (4 * GqaType<T>::CE)];
+    int blk = tab.at(a, p, first(t0), WK, lane, ok);
+    gqa_load_k<T, DP, KT>(a, kf, kbase, first(t0), blk, ok, lane);
+    gqa_fill<T, DP, WK, 1, true, true>(a, vt, vbase, first(t0), blk, ok, 0, lane);
+    for (int t = t0; t < t1 - 1; ++t) {
+      uint64_t ok1;
+      blk = tab.at(a, p, first(t + 1), WK, lane, ok1);
+      f32x4 s[NT][KT];
+      rows.scores_of(kf, s);
+      gqa_load_k<T, DP, KT>(a, kf, kbase, first(t + 1), blk, ok1, lane);
+      rows.template weigh<WK>(a, s, first(t), ok, lane);
+      // loads complete in order: this V tile's are older than the K fragments'
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
+      rows.template product<WK>(s, vt, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (V is read)
+      gqa_fill<T, DP, WK, 1, true, true>(a, vt, vbase, first(t + 1), blk, ok1, 0, lane);
+      ok = ok1;
+    }
+    f32x4 s[NT][KT];
+    rows.scores_of(kf, s);
+    rows.template weigh<WK>(a, s, first(t1 - 1), ok, lane);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    rows.template product<WK>(s, vt, lane);
   }
   // join the wavefronts' states
   float* ol = reinterpret_cast<float*>(smem);                // [NW][16 NT][OL]
@@ -610,7 +826,7 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
 template <typename T, int DP, int NT>
 constexpr int gqa_keys_lds() {
   constexpr int NW = gqa_nw<T, DP>();
-  constexpr int tiles = NW * 2 * gqa_wk<T, DP>() * GqaTile<T, DP>::ROWB, join = NW * 16 * NT * (DP + 4 + 2) * 4;
+  constexpr int tiles = NW * (gqa_wk<T, DP>() * GqaTile<T, DP>::ROWB + 256 * NT), join = NW * 16 * NT * (DP + 4 + 2) * 4;
   return tiles > join ? tiles : join;
 }
 
@@ -635,15 +851,24 @@ int gqa_launch_dp(const GqaArgs& a, const GqaShape& s, int64_t blocks, hipStream
     if (s.nt == 1) return gqa_launch_kernel<gqa_keys_kernel<T, DP, 1>>(a, blocks, threads, l1, st);
     return gqa_launch_kernel<gqa_keys_kernel<T, DP, 2>>(a, blocks, threads, l2, st);
   }
-  constexpr int lds = 4 * gqa_bn<T, DP>() * GqaTile<T, DP>::ROWB;
+  if constexpr (!GqaType<T>::F32) {
+    if (s.pair) {
+      constexpr int NT = DP <= 128 ? 2 : 1;
+      return gqa_launch_kernel<gqa_pair_kernel<T, DP, NT>>(a, blocks, 512, 6 * GqaPair<T, DP, NT>::TB + 8 * 256 * NT, st);
+    }
+  }
+  constexpr int lds = 4 * gqa_bn<T, DP>() * GqaTile<T, DP>::ROWB + 4 * 256 * 2;
   if (!s.vec) return gqa_launch_kernel<gqa_rows_kernel<T, DP, 1, false>>(a, blocks, 256, lds, st);
-  if (s.nt == 1) return gqa_launch_kernel<gqa_rows_kernel<T, DP, 1, true>>(a, blocks, 256, lds, st);
-  return gqa_launch_kernel<gqa_rows_kernel<T, DP, 2, true>>(a, blocks, 256, lds, st);
+  if constexpr (GqaType<T>::F32)
+    if (s.nt == 2) return gqa_launch_kernel<gqa_rows_kernel<T, DP, 2, true>>(a, blocks, 256, lds, st);
+  return gqa_launch_kernel<gqa_rows_kernel<T, DP, 1, true>>(a, blocks, 256, lds, st);
 }
 
 template <typename T, int DP>
 void gqa_tiles_dp(GqaShape& s) {
-  s.bn = s.keys ? gqa_nw<T, DP>() * gqa_wk<T, DP>() : gqa_bn<T, DP>();
+  s.bn = s.keys ? gqa_nw<T, DP>() * gqa_wk<T, DP>() : s.pair ? gqa_pair_bn<T, DP>() : gqa_bn<T, DP>();
+  s.group_rows = 64 / GqaTile<T, DP>::CPR;
+  s.bm = s.keys ? 16 * s.nt : s.pair ? (DP <= 128 ? 256 : 128) : 64 * s.nt;
 }
 
 template <typename T>

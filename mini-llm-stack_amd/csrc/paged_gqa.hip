@@ -91,16 +91,18 @@ struct Pass {
 };
 
 // Row tile and kernel for `rows` packed rows a sequence.
-void choose_shape(GqaShape& s, int64_t rows, int dt, int64_t D, bool vec) {
-  s.vec = vec;
-  s.keys = vec && rows <= 32;
-  s.nt = s.keys ? (rows <= 16 ? 1 : 2) : (!vec || rows <= 64 ? 1 : 2);
+void choose_shape(GqaShape& s, int64_t rows, int dt, int64_t D, int64_t BS, bool vec) {
   s.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
   if (dt == MLS_F32) gqa_tiles<float>(s);
   else gqa_tiles<_Float16>(s);
+  vec = vec && BS % s.group_rows == 0;
+  s.vec = vec;
+  s.keys = vec && rows <= 32;
+  s.pair = vec && !s.keys && dt != MLS_F32 && rows > 64;
+  s.nt = s.keys ? (rows <= 16 ? 1 : 2) : (dt == MLS_F32 && vec && rows > 64 ? 2 : 1);
+  if (dt == MLS_F32) gqa_tiles<float>(s);
+  else gqa_tiles<_Float16>(s);
 }
-
-int bm_log_of(const GqaShape& s) { return (s.keys ? 4 : 6) + (s.nt == 2 ? 1 : 0); }
 
 // Validates a call and lays out its launches; need: floats of workspace.
 int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass& own, Pass& pre, bool& shared, int64_t& need) {
@@ -138,6 +140,9 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   a.DW = (int)cdiv(D, 4) * 4, a.BS = (int)BS;
   a.bs_magic = (uint32_t)((0xFFFFFFFFull / (uint64_t)BS) + 1);  // ceil(2^32 / BS) for BS > 1
   a.max_blocks = (int)p->max_blocks, a.window = (int)p->window;
+  if (vec && p->kv_sb * esz <= 0xFFFFFFFFll && p->kv_st * esz * std::max<int64_t>(BS, 64) < 0x7FFFFFFFll)
+    a.sb_bytes = (uint32_t)(p->kv_sb * esz), a.st_bytes = (uint32_t)(p->kv_st * esz);
+  a.kv_vec = vec;
   constexpr double LOG2E = 1.4426950408889634;
   a.c = (float)(p->scale * LOG2E);
   a.cap = (float)(p->softcap * LOG2E);
@@ -148,9 +153,10 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
 
   // the sequences' own keys
   own.a = a;
+  own.s = pre.s = GqaShape{};
   const int64_t most = p->cu_seqlens ? (p->max_new > 0 ? std::min(p->max_new, T) : cdiv(T, std::max<int64_t>(n, 1))) : 1;
-  choose_shape(own.s, most * G, p->dt, D, vec);
-  own.a.bm_log = bm_log_of(own.s);
+  choose_shape(own.s, most * G, p->dt, D, BS, a.sb_bytes != 0);
+  own.a.bm_log = __builtin_ctz(own.s.bm);
   own.a.bn = own.s.bn;
   const int64_t bm = 1ll << own.a.bm_log;
   const int64_t slots = p->cu_seqlens ? T * G / bm + n + 2 : n * cdiv(G, bm);
@@ -164,11 +170,11 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   int64_t sp = 0;
   if (shared) {
     pre.a = a;
-    choose_shape(pre.s, n * G, p->dt, D, vec);
+    choose_shape(pre.s, n * G, p->dt, D, BS, a.sb_bytes != 0);
     pre.a.shared = 1;
     pre.a.front = (int)std::min<int64_t>(p->prefix_len, p->prefix_count * BS);
     pre.a.bt = p->prefix_blocks, pre.a.bt_ss = 0, pre.a.max_blocks = (int)p->prefix_count;
-    pre.a.bm_log = bm_log_of(pre.s);
+    pre.a.bm_log = __builtin_ctz(pre.s.bm);
     pre.a.bn = pre.s.bn;
     pre.a.slots = (int)cdiv(n * G, 1ll << pre.a.bm_log);
     const int64_t pt = pre.a.slots * Hkv, ps = std::max<int64_t>(cdiv(pre.a.front, pre.s.bn), 1);

@@ -26,6 +26,7 @@ struct GqaArgs {
   int64_t num_blocks;
   int n, T, Hkv, group, D, DW, BS;
   uint32_t bs_magic;  // ceil(2^32 / BS)
+  uint32_t sb_bytes, st_bytes;  // kv_sb, kv_st in bytes where they fit (0: not)
   int max_blocks;
   int window;
   int front;   // shared: keys of the prefix
@@ -38,12 +39,13 @@ struct GqaArgs {
   int piece0;            // first record of this launch's pieces (before it: the shared prefix's)
   int splits, least, cap_tiles;  // pieces a context may have, least steps of one; n > 1024: steps of one
   float target;                  // blocks to aim at
-  int q_vec, o_vec;
+  int q_vec, o_vec, kv_vec;  // 16-byte accesses of q, 4 elements at once of out, 16-byte ones of the pools
 };
 
 struct GqaShape {
-  bool keys, vec;
-  int nt, dp, bn;
+  bool keys, pair, vec;
+  int nt, dp, bn, bm;
+  int group_rows;  // cache rows that one load instruction covers: of one block each, where vec
 };
 
 struct GqaPlan {
