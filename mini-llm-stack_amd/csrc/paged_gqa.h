@@ -100,6 +100,13 @@ struct GqaTile {
   }
 };
 
+// A value that the compiler takes as new here: what rarely taken branches make of it is not made
+// ahead of the loop around them, in registers that the loop then lacks.
+__device__ __forceinline__ int gqa_here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // Before a main loop: the loads so far (q, block ids) have landed, said in a way that the compiler
 // counts; else their first use in the loop would wait, in every pass, for the loop's loads.
 __device__ __forceinline__ void gqa_landed() { __builtin_amdgcn_s_waitcnt(0 | 0x70 | 0xF00); }
@@ -108,21 +115,23 @@ __device__ __forceinline__ void gqa_landed() { __builtin_amdgcn_s_waitcnt(0 | 0x
 // load (one that the counter of the tiles' own loads would make wait for those).
 struct GqaTable {
   int tab, next, base;  // entries [base, base + 64) and [base + 64, base + 128)
-  __device__ __forceinline__ int load(const GqaArgs& a, const GqaPlan& p, int from, int lane) const {
+  bool holes;           // an id of these that the tile may use is outside the pool
+  __device__ __forceinline__ int load(const GqaArgs& a, const GqaPlan& p, int from, int lane) {
     const int e = from + lane;
-    const int blk = p.khi > 0 && e <= gqa_block_of(a, p.khi - 1) ? p.table[e] : -1;
+    const bool in = p.khi > 0 && e <= gqa_block_of(a, p.khi - 1);
+    const int blk = in ? p.table[e] : -1;
+    holes = holes || __any(in && (blk < 0 || blk >= a.num_blocks));
     return blk < a.num_blocks ? blk : -1;
   }
   __device__ __forceinline__ void start(const GqaArgs& a, const GqaPlan& p, int j0, int lane) {
+    holes = false;
     base = gqa_block_of(a, j0);
     tab = load(a, p, base, lane);
     next = load(a, p, base + 64, lane);
   }
-  // Lane i < n: the block of key j0 + i (tiles in rising order), negative for none; `ok`: the keys of them that
-  // any row of the tile sees.
-  __device__ __forceinline__ int at(const GqaArgs& a, const GqaPlan& p, int j0, int n, int lane, uint64_t& ok) {
-    ok = 0;
-    if (j0 >= p.khi) return -1;
+  // Moves on to the tile from key j0 on (tiles in rising order).
+  __device__ __forceinline__ void advance(const GqaArgs& a, const GqaPlan& p, int j0, int lane) {
+    if (j0 >= p.khi) return;
     const int first = gqa_block_of(a, j0);
     while (first - base >= 64) {
       tab = next;
@@ -130,11 +139,26 @@ struct GqaTable {
       next = load(a, p, base + 64, lane);
       gqa_landed();  // (once in 64 blocks)
     }
-    const int key = j0 + lane, i = gqa_block_of(a, key) - base;
+  }
+  // Lane i: the block of the tile's key j0 + i, negative for none.
+  __device__ __forceinline__ int block(const GqaArgs& a, int j0, int lane) const {
+    const int i = gqa_block_of(a, j0 + lane) - base;
     const int x = __shfl(tab, i & 63, 64), y = __shfl(next, i & 63, 64);
-    const int blk = i < 64 ? x : y;
-    ok = __ballot(lane < n && key >= p.klo && key < p.khi && blk >= 0);
-    return blk;
+    return i < 64 ? x : y;
+  }
+  // The same for one key, uniform
+  __device__ __forceinline__ int block_at(const GqaArgs& a, int key) const {
+    const int i = gqa_block_of(a, key) - base;
+    const int x = __builtin_amdgcn_readlane(tab, i & 63), y = __builtin_amdgcn_readlane(next, i & 63);
+    return i < 64 ? x : y;
+  }
+  // The keys of the tile that any row sees
+  template <int N>
+  __device__ __forceinline__ uint64_t seen(const GqaArgs& a, const GqaPlan& p, int j0, int lane) const {
+    if (j0 >= p.klo && j0 + N <= p.khi && !holes) return N == 64 ? ~0ull : (1ull << (N & 63)) - 1;
+    if (j0 >= p.khi) return 0;
+    const int here = gqa_here(lane), key = j0 + here;
+    return __ballot(here < N && key >= p.klo && key < p.khi && block(a, j0, here) >= 0);
   }
 };
 
@@ -149,12 +173,12 @@ struct GqaFill {
 
   // One address an instruction, whose rows lie in one cache block (gqa_rows_of), made by scalar instructions. (With an address a row for
   // every lane, the addresses alone are 78 vector instructions a tile of 64 keys, a third of the main loop's.)
-  __device__ __forceinline__ void place(const GqaArgs& a, int j0, int blk, uint64_t okmask, int wave) {
+  __device__ __forceinline__ void place(const GqaArgs& a, const GqaTable& tab, int j0, uint64_t okmask, int wave) {
     ok = okmask;
 #pragma unroll
     for (int u = 0; u < ITER; ++u) {
-      const int row = (u * WAVES + wave) * ROWS, key = j0 + row;
-      const uint32_t b = __builtin_amdgcn_readlane(blk, row), t = key - gqa_block_of(a, key) * a.BS;
+      const int key = j0 + (u * WAVES + wave) * ROWS;
+      const uint32_t b = tab.block_at(a, key), t = key - gqa_block_of(a, key) * a.BS;
       at[u] = (uint64_t)b * a.sb_bytes + (uint64_t)t * a.st_bytes;
     }
   }
@@ -162,12 +186,13 @@ struct GqaFill {
   // compiler takes LDS-direct loads of the global kind for accesses that may return in any order, so that
   // every later LDS read would wait for all reads (lgkmcnt(0)) and some for all loads: 595 us for a prompt of 8192.
   template <bool V>
-  __device__ __forceinline__ void load(const GqaArgs& a, uint8_t* dst, const uint8_t* base, int wave, int lane) const {
+  __device__ __forceinline__ void load(const GqaArgs& a, uint8_t* dst, const uint8_t* base, int wave, int lane, int only = -1) const {
     constexpr uint64_t FULL = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
     const int r = lane / G::CPR, c = lane % G::CPR;
     const bool whole = ok == FULL && a.D == G::DL;
 #pragma unroll
     for (int u = 0; u < ITER; ++u) {
+      if (only >= 0 && u != only) continue;
       const int row = (u * WAVES + wave) * ROWS;
       const int cc = c ^ (V ? G::swz_v(row + r) : G::swz_k(row + r));
       uint32_t off = (uint32_t)r * a.st_bytes + cc * 16;
@@ -206,17 +231,20 @@ struct GqaFill {
   }
 };
 
-// A tile's rows into LDS, with its addresses made here.
-template <typename T, int DP, int BN, int WAVES, bool VEC, bool V>
-__device__ __forceinline__ void gqa_fill(const GqaArgs& a, uint8_t* dst, const uint8_t* base, int j0, int blk, uint64_t ok, int wave,
-                                         int lane) {
+// A tile's K and V rows into LDS, with the addresses made here.
+template <typename T, int DP, int BN, int WAVES, bool VEC>
+__device__ __forceinline__ void gqa_fill(const GqaArgs& a, const GqaTable& tab, uint8_t* kt, uint8_t* vt, const uint8_t* kbase,
+                                         const uint8_t* vbase, int j0, uint64_t ok, int wave, int lane) {
   using F = GqaFill<T, DP, BN, WAVES>;
   if constexpr (VEC) {
     F f;
-    f.place(a, j0, blk, ok, wave);
-    f.template load<V>(a, dst, base, wave, lane);
+    f.place(a, tab, j0, ok, wave);
+    if (kt) f.template load<false>(a, kt, kbase, wave, lane);
+    if (vt) f.template load<true>(a, vt, vbase, wave, lane);
   } else {
-    F::template load_any<V>(a, dst, base, j0, blk, ok, wave, lane);
+    const int blk = tab.block(a, j0, lane);
+    F::template load_any<false>(a, kt, kbase, j0, blk, ok, wave, lane);
+    F::template load_any<true>(a, vt, vbase, j0, blk, ok, wave, lane);
   }
 }
 
@@ -283,9 +311,9 @@ struct GqaRows {
   // are one sequence, read DEPTH ahead of their use: the order is pinned, since the compiler, short of
   // registers, reads each just before its use (a read's latency is four fragments' products; prompt of
   // 8192 so, 2 wavefronts a SIMD taking turns: 972 us).
-  template <int BN, bool PV, bool QK>
+  template <int BN, bool PV, bool QK, typename F>
   __device__ __forceinline__ void matrix(const uint4 (&pf)[BN / 32 + (BN < 32)][NT], const uint4 (&pr)[BN / 32 + (BN < 32)][NT],
-                                         const uint8_t* vt, const uint8_t* kt, f32x4 (&s)[NT][BN / 16], int lane) {
+                                         const uint8_t* vt, const uint8_t* kt, f32x4 (&s)[NT][BN / 16], int lane, F beside) {
     constexpr int NV = PV ? BN / 32 * OT : 0, NK = QK ? BN / 16 * QT : 0, N = NV + NK, DEPTH = N < 6 ? N : 6;
     const int g = lane >> 4, c = lane & 15;
     const int vrow = 4 * g + (c >> 2);  // (and 16, 32 further on: the same swizzle)
@@ -301,7 +329,7 @@ struct GqaRows {
             __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 16 * G::ROWB))};
         return __builtin_bit_cast(uint4, v);
       }
-      const int k = (x - NV) / QT, t = (x - NV) % QT;
+      const int k = (x - NV) % (BN / 16), t = (x - NV) / (BN / 16);  // (a product of the same scores each BN / 16 fragments)
       return *reinterpret_cast<const uint4*>(kbase + k * 16 * G::ROWB + (((4 * t + g) ^ G::swz_k(c)) << 4));
     };
     uint4 f[DEPTH];
@@ -327,11 +355,12 @@ struct GqaRows {
           }
         }
       } else {
-        const int k = (x - NV) / QT, t = (x - NV) % QT;
+        const int k = (x - NV) % (BN / 16), t = (x - NV) / (BN / 16);
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n][k] = gqa_mma<T>(v, q[n][t], t == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[n][k]);
       }
       if (x + DEPTH < N) f[x % DEPTH] = read(x + DEPTH);
+      beside(x);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -340,7 +369,7 @@ struct GqaRows {
   template <int BN>
   __device__ __forceinline__ void scores(const uint8_t* kt, int lane, f32x4 (&s)[NT][BN / 16]) {
     const uint4 none[BN / 32 + (BN < 32)][NT] = {};
-    matrix<BN, false, true>(none, none, nullptr, kt, s, lane);
+    matrix<BN, false, true>(none, none, nullptr, kt, s, lane, [](int) {});
   }
 
   // The same from fragments in registers
@@ -362,26 +391,28 @@ struct GqaRows {
   template <int BN>
   __device__ __forceinline__ void weigh(const GqaArgs& a, f32x4 (&s)[NT][BN / 16], int j0, uint64_t okmask, int lane) {
     constexpr int KT = BN / 16;
-    const int g = lane >> 4;
     // scores in log2 units: s * cc
     float cc = a.c;
     if (!a.simple) {
       cc = 1.0f;
-      scored<KT>(a, s, j0, lane);
+      scored<KT>(a, s, j0, gqa_here(lane));
     }
     constexpr uint64_t FULL = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
     if (okmask != FULL || !sees_all(j0, BN)) {
+      const int here = gqa_here(lane), g = here >> 4;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int4 x = at[16 * n + (lane & 15)];
+        const int4 x = at[16 * n + (here & 15)];
 #pragma unroll
-        for (int k = 0; k < KT; ++k)
+        for (int k = 0; k < KT; ++k) {
+          const uint32_t there = (uint32_t)(okmask >> (16 * k)) >> (4 * g);
+          const int j = j0 + 16 * k + 4 * g;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int kk = 16 * k + 4 * g + i, j = j0 + kk;
-            const bool see = x.x <= j && j < x.y && ((okmask >> kk) & 1);
+            const bool see = x.x <= j + i && j + i < x.y && ((there >> i) & 1);
             s[n][k][i] = see ? s[n][k][i] : -__builtin_huge_valf();
           }
+        }
       }
     }
     float mx[NT];
@@ -484,7 +515,7 @@ struct GqaRows {
       for (int h = 0; h < BN / 32; ++h)
 #pragma unroll
         for (int n = 0; n < NT; ++n) pack(s[n][2 * h], s[n][2 * h + 1], pf[h][n], pr[h][n]);
-      matrix<BN, true, false>(pf, pr, vt, nullptr, s, lane);
+      matrix<BN, true, false>(pf, pr, vt, nullptr, s, lane, [](int) {});
     }
   }
 
@@ -533,15 +564,12 @@ constexpr int gqa_bn() {
 }
 
 template <typename T, int DP, int NT, int BN, bool VEC>
-__device__ __forceinline__ void gqa_rows_step(const GqaArgs& a, GqaRows<T, DP, NT, false>& rows, const uint8_t* __restrict__ cur,
+__device__ __forceinline__ void gqa_rows_step(const GqaArgs& a, const GqaTable& tab, GqaRows<T, DP, NT, false>& rows, const uint8_t* __restrict__ cur,
                                               uint8_t* __restrict__ nxt, const uint8_t* __restrict__ kbase,
-                                              const uint8_t* __restrict__ vbase, int blk, uint64_t ok1, bool now,
+                                              const uint8_t* __restrict__ vbase, uint64_t ok1, bool now,
                                               bool more, int j0, uint64_t okmask, int wave, int lane) {
   constexpr int TB = BN * GqaTile<T, DP>::ROWB;
-  if (more) {
-    gqa_fill<T, DP, BN, 4, VEC, false>(a, nxt, kbase, j0 + BN, blk, ok1, wave, lane);
-    gqa_fill<T, DP, BN, 4, VEC, true>(a, nxt + TB, vbase, j0 + BN, blk, ok1, wave, lane);
-  }
+  if (more) gqa_fill<T, DP, BN, 4, VEC>(a, tab, nxt, nxt + TB, kbase, vbase, j0 + BN, ok1, wave, lane);
   if (!now || !rows.sees_any(j0, BN)) return;
   f32x4 s[NT][BN / 16];
   rows.template scores<BN>(cur, lane, s);
@@ -571,9 +599,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void gqa_rows_kernel(const 
     for (int t = t0 - 1; t < t1; ++t) {  // (the first only loads)
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       uint64_t ok1 = 0;
-      const int blk = t + 1 < t1 ? tab.at(a, p, p.lo + (t + 1) * BN, BN, lane, ok1) : -1;
+      if (t + 1 < t1) {
+        tab.advance(a, p, p.lo + (t + 1) * BN, lane);
+        ok1 = tab.seen<BN>(a, p, p.lo + (t + 1) * BN, lane);
+      }
       const int cur = ((t - t0) & 1) * 2 * TB;
-      gqa_rows_step<T, DP, NT, BN, VEC>(a, rows, smem + cur, smem + (2 * TB - cur), kbase, vbase, blk, ok1, t >= t0,
+      gqa_rows_step<T, DP, NT, BN, VEC>(a, tab, rows, smem + cur, smem + (2 * TB - cur), kbase, vbase, ok1, t >= t0,
                                         t + 1 < t1, p.lo + t * BN, ok, wave, lane);
       ok = ok1;
     }
@@ -616,9 +647,18 @@ struct GqaPair {
                                            const uint8_t* __restrict__ vr, uint8_t* __restrict__ vw,
                                            const uint8_t* __restrict__ kbase, const uint8_t* __restrict__ vbase,
                                            const Fill& kat, const Fill& vat, bool kmore, bool vmore, int wave, int lane) {
-    if (vmore) vat.template load<true>(a, vw, vbase, wave, lane);
-    if (kmore) kat.template load<false>(a, kw, kbase, wave, lane);
-    rows.template matrix<BN, true, true>(pf, pf, vr, kr, s, lane);
+    // The loads go between the fragments (at the head of the step: prompt of 8192, 565 us against 550), but in the
+    // widest heads, whose tiles' products are as many for half the keys (chunks of D = 256: 139 against 152).
+    constexpr bool BETWEEN = DP <= 128;
+    if (!BETWEEN && vmore) vat.template load<true>(a, vw, vbase, wave, lane);
+    if (!BETWEEN && kmore) kat.template load<false>(a, kw, kbase, wave, lane);
+    rows.template matrix<BN, true, true>(pf, pf, vr, kr, s, lane, [&](int x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < PER && BETWEEN; ++u) {
+        if (x == 4 + 8 * u && vmore) vat.template load<true>(a, vw, vbase, wave, lane, u);
+        if (x == 8 + 8 * u && kmore) kat.template load<false>(a, kw, kbase, wave, lane, u);
+      }
+    });
   }
   __device__ __forceinline__ void soften(const GqaArgs& a, int j0, uint64_t okmask, int lane) {
     rows.template weigh<BN>(a, s, j0, okmask, lane);
@@ -649,16 +689,18 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
     GqaTable tab;
     tab.start(a, p, j0, lane);
     gqa_landed();
-    typename P::Fill f0, f1, f2;  // tiles i, i + 1 and i + 2
-    f0.ok = f1.ok = f2.ok = 0;
-    const int b0 = tab.at(a, p, j0, BN, lane, f0.ok);
-    const int b1 = n > 1 ? tab.at(a, p, j0 + BN, BN, lane, f1.ok) : -1, b2 = n > 2 ? tab.at(a, p, j0 + 2 * BN, BN, lane, f2.ok) : -1;
-    gqa_fill<T, DP, BN, 8, true, false>(a, smem, kbase, j0, b0, f0.ok, wave, lane);
-    gqa_fill<T, DP, BN, 8, true, true>(a, smem + 3 * TB, vbase, j0, b0, f0.ok, wave, lane);
-    if (n > 1) gqa_fill<T, DP, BN, 8, true, false>(a, smem + TB, kbase, j0 + BN, b1, f1.ok, wave, lane);
-    f1.place(a, j0 + BN, b1, f1.ok, wave);
-    f2.place(a, j0 + 2 * BN, b2, f2.ok, wave);
-    uint64_t ok0 = f0.ok;
+    typename P::Fill f1, f2;  // tiles i + 1 and i + 2
+    uint64_t ok0 = tab.seen<BN>(a, p, j0, lane);
+    gqa_fill<T, DP, BN, 8, true>(a, tab, smem, smem + 3 * TB, kbase, vbase, j0, ok0, wave, lane);
+    auto place = [&](typename P::Fill& f, int i) __attribute__((always_inline)) {
+      if (i < n) {
+        tab.advance(a, p, j0 + i * BN, lane);
+        f.place(a, tab, j0 + i * BN, tab.seen<BN>(a, p, j0 + i * BN, lane), wave);
+      }
+    };
+    place(f1, 1);
+    if (n > 1) f1.template load<false>(a, smem + TB, kbase, wave, lane);
+    place(f2, 2);
     // V's tile -1: zeros, with weights of 0
     for (int e = threadIdx.x; e < TB / 16; e += 512) reinterpret_cast<uint4*>(smem + 5 * TB)[e] = make_uint4(0, 0, 0, 0);
 #pragma unroll
@@ -670,8 +712,10 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
     if (wave >= 4) asm volatile("s_barrier" ::: "memory");  // half a step behind
     int s0 = 0, s1 = TB, s2 = 2 * TB;  // slots of tiles i, i + 1, i + 2 (and so of i - 1)
     for (int i = 0; i < n; ++i) {
+      __builtin_amdgcn_s_setprio(1);  // (its matrix instructions before the other's exponentials: 620 us without)
       w.multiply(a, smem + s0, smem + s2, smem + 3 * TB + s2, smem + 3 * TB + s1, kbase, vbase, f2, f1, i + 2 < n,
                  i + 1 < n, wave, lane);
+      __builtin_amdgcn_s_setprio(0);
       // the last step's loads have landed (this one's may be on their way)
       if (i + 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * P::PER) : "memory");
       else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -680,12 +724,10 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
       s0 = s1, s1 = s2, s2 = t;
       ok0 = f1.ok;
       f1 = f2;
-      uint64_t ok = 0;
-      const int b2 = i + 3 < n ? tab.at(a, p, j0 + (i + 3) * BN, BN, lane, ok) : -1;
-      f2.place(a, j0 + (i + 3) * BN, b2, ok, wave);
+      place(f2, i + 3);  // (here and not among the products, which are what a step waits for)
       asm volatile("s_barrier" ::: "memory");
     }
-    w.rows.template matrix<BN, true, false>(w.pf, w.pf, smem + 3 * TB + s2, nullptr, w.s, lane);
+    w.rows.template matrix<BN, true, false>(w.pf, w.pf, smem + 3 * TB + s2, nullptr, w.s, lane, [](int) {});
     if (!(wave >= 4)) asm volatile("s_barrier" ::: "memory");
   }
   const int g = lane >> 4;
@@ -762,21 +804,21 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
   if (t0 < t1) {
     constexpr int KT = WK / 16, PER = KT * (DP / (4 * GqaType<T>::CE));  // loads of a K tile
     uint4 kf[KT][DP / (4 * GqaType<T>::CE)];
-    int blk = tab.at(a, p, first(t0), WK, lane, ok);
-    gqa_load_k<T, DP, KT>(a, kf, kbase, first(t0), blk, ok, lane);
-    gqa_fill<T, DP, WK, 1, true, true>(a, vt, vbase, first(t0), blk, ok, 0, lane);
+    ok = tab.seen<WK>(a, p, first(t0), lane);
+    gqa_load_k<T, DP, KT>(a, kf, kbase, first(t0), tab.block(a, first(t0), lane), ok, lane);
+    gqa_fill<T, DP, WK, 1, true>(a, tab, nullptr, vt, nullptr, vbase, first(t0), ok, 0, lane);
     for (int t = t0; t < t1 - 1; ++t) {
-      uint64_t ok1;
-      blk = tab.at(a, p, first(t + 1), WK, lane, ok1);
+      tab.advance(a, p, first(t + 1), lane);
+      const uint64_t ok1 = tab.seen<WK>(a, p, first(t + 1), lane);
       f32x4 s[NT][KT];
       rows.scores_of(kf, s);
-      gqa_load_k<T, DP, KT>(a, kf, kbase, first(t + 1), blk, ok1, lane);
+      gqa_load_k<T, DP, KT>(a, kf, kbase, first(t + 1), tab.block(a, first(t + 1), lane), ok1, lane);
       rows.template weigh<WK>(a, s, first(t), ok, lane);
       // loads complete in order: this V tile's are older than the K fragments'
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
       rows.template product<WK>(s, vt, lane);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (V is read)
-      gqa_fill<T, DP, WK, 1, true, true>(a, vt, vbase, first(t + 1), blk, ok1, 0, lane);
+      gqa_fill<T, DP, WK, 1, true>(a, tab, nullptr, vt, nullptr, vbase, first(t + 1), ok1, 0, lane);
       ok = ok1;
     }
     f32x4 s[NT][KT];

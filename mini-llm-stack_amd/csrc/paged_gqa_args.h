@@ -60,8 +60,8 @@ struct GqaPlan {
 
 // key / BS
 __device__ __forceinline__ int gqa_block_of(const GqaArgs& a, int key) {
-  int b = a.BS == 1 ? key : (int)__umulhi((uint32_t)key, a.bs_magic);  // (one too many at most)
-  return b - (b * (int64_t)a.BS > key ? 1 : 0);
+  const uint32_t b = a.BS == 1 ? (uint32_t)key : __umulhi((uint32_t)key, a.bs_magic);  // (one too many at most)
+  return (int)(b - (b * (uint32_t)a.BS > (uint32_t)key ? 1 : 0));
 }
 
 // The last s of [0, n] whose start(s) is at most `at`, -1: none; by 64 probes a round.
