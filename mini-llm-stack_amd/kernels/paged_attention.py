@@ -24,8 +24,8 @@ import struct
 import torch
 
 import kernels
-from kernels._hip import dt_code, require_hip, stream
-from kernels.paged_kv import int32, no_grad_of, pools
+from kernels._hip import _DT, dt_code, require_hip, stream
+from kernels.paged_kv import _raw_stream, fresh, int32, no_grad_of, one_device, pools
 
 _ARGS = struct.Struct("=10Q21q2d")  # mlsx_paged_attention_args
 
@@ -75,54 +75,70 @@ def paged_attention_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
 
 def _attend(fn, q, k_pool, v_pool, block_tables, context_lens, cu_seqlens, max_new, scale, softcap, slopes, window, prefix_lens,
             prefix_blocks, prefix_len):
-    if q.dim() != 3:
-        raise ValueError(f"{fn}: q {tuple(q.shape)}, expected [tokens, heads, head_dim]")
-    T, Hq, D = q.shape
+    qs, ps, dt, int32_t = q.shape, k_pool.shape, q.dtype, torch.int32
+    if len(qs) != 3:
+        raise ValueError(f"{fn}: q {tuple(qs)}, expected [tokens, heads, head_dim]")
+    T, Hq, D = qs
     kv_sb, kv_sh, kv_st, _ = pools(k_pool, v_pool, fn)
-    num_blocks, Hkv, block_size, Dk = k_pool.shape
+    num_blocks, Hkv, block_size, Dk = ps
     if Dk != D or Hkv < 1 or Hq % Hkv:
-        raise ValueError(f"{fn}: q {tuple(q.shape)}, pools {tuple(k_pool.shape)}: head dims differ, or query heads are no "
-                         f"multiple of K/V heads")
-    if q.dtype != k_pool.dtype:
-        raise TypeError(f"{fn}: q {q.dtype} and pools {k_pool.dtype} must have one dtype")
+        raise ValueError(f"{fn}: q {tuple(qs)}, pools {tuple(ps)}: head dims differ, or query heads are no multiple of K/V heads")
+    if k_pool.dtype != dt:
+        raise TypeError(f"{fn}: q {dt} and pools {k_pool.dtype} must have one dtype")
     n = context_lens.shape[0] if context_lens.dim() == 1 else -1
-    lens = int32(context_lens, "context_lens", fn, (None,))
-    tables = int32(block_tables, "block_tables", fn, (n, None))
-    cu = prefix = shared = None
+    if context_lens.dtype != int32_t or n < 0 or context_lens.stride(0) != 1:
+        context_lens = int32(context_lens, "context_lens", fn, (None,))
+    ts = block_tables.shape
+    if block_tables.dtype != int32_t or len(ts) != 2 or ts[0] != n or block_tables.stride(1) != 1:
+        block_tables = int32(block_tables, "block_tables", fn, (n, None))
+    cu_at = prefix_at = shared_at = slopes_at = shared_blocks = 0
     if cu_seqlens is not None:
-        cu = int32(cu_seqlens, "cu_seqlens", fn, (n + 1,))
+        if cu_seqlens.dtype != int32_t or cu_seqlens.shape != (n + 1,) or cu_seqlens.stride(0) != 1:
+            cu_seqlens = int32(cu_seqlens, "cu_seqlens", fn, (n + 1,))
+        cu_at = cu_seqlens.data_ptr()
     elif n != T:
         raise ValueError(f"{fn}: {T} rows for {n} sequences: without cu_seqlens, each has one")
     if prefix_lens is not None:
-        prefix = int32(prefix_lens, "prefix_lens", fn, (n,))
+        prefix_lens = int32(prefix_lens, "prefix_lens", fn, (n,))
+        prefix_at = prefix_lens.data_ptr()
     if prefix_blocks is not None:
-        shared = int32(prefix_blocks, "prefix_blocks", fn, (None,))
-        if not 0 <= prefix_len <= shared.shape[0] * block_size:
-            raise ValueError(f"{fn}: a prefix of {prefix_len} tokens in {shared.shape[0]} blocks of {block_size}")
+        prefix_blocks = int32(prefix_blocks, "prefix_blocks", fn, (None,))
+        shared_blocks = prefix_blocks.shape[0]
+        if not 0 <= prefix_len <= shared_blocks * block_size:
+            raise ValueError(f"{fn}: a prefix of {prefix_len} tokens in {shared_blocks} blocks of {block_size}")
+        shared_at = prefix_blocks.data_ptr() if prefix_len else 0
     if slopes is not None:
         if slopes.shape != (Hq,) or slopes.dtype != torch.float32:
             raise ValueError(f"{fn}: slopes must be float32 [{Hq}], got {slopes.dtype} {tuple(slopes.shape)}")
         slopes = slopes.contiguous()
+        slopes_at = slopes.data_ptr()
     if not 0.0 <= softcap < 3e38:
         raise ValueError(f"{fn}: softcap {softcap}: a positive cap, or 0 for none")
     if window < 0 or max_new is not None and max_new < 0:
         raise ValueError(f"{fn}: window {window}, max_new {max_new}: not negative")
-    no_grad_of(fn, q, k_pool, v_pool, slopes)
-    dev = require_hip(fn, *(t for t in (q, k_pool, v_pool, tables, lens, cu, prefix, shared, slopes) if t is not None))
-    if q.stride(2) != 1 and D > 1 or q.stride(1) < D and Hq > 1:
+    if torch.is_grad_enabled():
+        no_grad_of(fn, q, k_pool, v_pool, slopes)
+    dev = one_device(fn, q, k_pool, v_pool, block_tables, context_lens, cu_seqlens, prefix_lens, prefix_blocks, slopes)
+    q_st, q_sh, inner = q.stride()
+    if inner != 1 and D > 1 or q_sh < D and Hq > 1:
         q = q.contiguous()
-    out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+        q_st, q_sh, _ = q.stride()
+    out = fresh(q, qs)
     args = _ARGS.pack(
-        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), tables.data_ptr(), lens.data_ptr(),
-        0 if cu is None else cu.data_ptr(), 0 if prefix is None else prefix.data_ptr(),
-        0 if not prefix_len else shared.data_ptr(), 0 if slopes is None else slopes.data_ptr(), out.data_ptr(),
-        dt_code(q.dtype, fn), q.stride(0), max(q.stride(1), D), Hq * D, D, kv_sb, max(kv_sh, D), max(kv_st, D),
-        tables.stride(0), num_blocks, n, T, Hkv, Hq // Hkv, D, block_size, tables.shape[1], min(window, 0x7FFFFFFF),
-        prefix_len, 0 if shared is None else shared.shape[0], max_new or 0, D ** -0.5 if scale is None else scale, softcap)
+        q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), cu_at, prefix_at,
+        shared_at, slopes_at, out.data_ptr(), _DT[dt] if dt in _DT else dt_code(dt, fn), q_st, q_sh if q_sh > D else D,
+        Hq * D, D, kv_sb, kv_sh if kv_sh > D else D, kv_st if kv_st > D else D, block_tables.stride(0), num_blocks, n, T, Hkv,
+        Hq // Hkv, D, block_size, block_tables.shape[1], window if window < 0x7FFFFFFF else 0x7FFFFFFF, prefix_len, shared_blocks,
+        max_new or 0, D ** -0.5 if scale is None else scale, softcap)
     L = kernels.lib()
     need = L.mlsx_paged_attention_ws(args)
-    ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
-    kernels.check(L.mlsx_paged_attention(args, ws.data_ptr() if need else None, need, stream(dev)), fn)
+    if need:
+        ws = q.new_empty(need if dt == torch.float32 else 2 * need)  # (`need` floats)
+        rc = L.mlsx_paged_attention(args, ws.data_ptr(), need, _raw_stream(dev))
+    else:
+        rc = L.mlsx_paged_attention(args, None, 0, _raw_stream(dev))
+    if rc:
+        kernels.check(rc, fn)
     return out
 
 

@@ -13,7 +13,7 @@ import struct
 import torch
 
 import kernels
-from kernels._hip import dt_code, require_hip, stream
+from kernels._hip import _DT, dt_code, require_hip
 
 _ARGS = struct.Struct("=10Q23q")  # mlsx_paged_append_args
 
@@ -31,15 +31,36 @@ def int32(t: torch.Tensor, name: str, fn: str, shape: tuple) -> torch.Tensor:
 
 def pools(k_pool: torch.Tensor, v_pool: torch.Tensor, fn: str) -> tuple:
     """Strides of the pools, which are read and written in place: never copied."""
-    if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype:
+    ps = k_pool.shape
+    if len(ps) != 4 or v_pool.shape != ps or v_pool.dtype != k_pool.dtype:
         raise ValueError(f"{fn}: pools {tuple(k_pool.shape)} {k_pool.dtype} / {tuple(v_pool.shape)} {v_pool.dtype}: expected "
                          f"two of one shape [num_blocks, kv_heads, block_size, head_dim] and type")
+    if ps[2] < 1:
+        raise ValueError(f"{fn}: blocks of no tokens")
     st = k_pool.stride()
     if v_pool.stride() != st or st[3] != 1 and k_pool.shape[3] > 1:
         raise ValueError(f"{fn}: pools need the same strides, 1 for the last dimension, got {st} / {v_pool.stride()}")
-    if k_pool.shape[2] < 1:
-        raise ValueError(f"{fn}: blocks of no tokens")
     return st
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # (a device index's current stream, as kernels._hip.stream)
+
+
+def one_device(fn: str, *tensors) -> int:
+    """The index of the HIP device that all of these (None: not given) are on."""
+    first = tensors[0].get_device()
+    if first >= 0:
+        for t in tensors:
+            if t is not None and t.get_device() != first:
+                break
+        else:
+            return first
+    return require_hip(fn, *(t for t in tensors if t is not None)).index
+
+
+def fresh(like: torch.Tensor, shape: tuple) -> torch.Tensor:
+    """A dense uninitialised tensor of `like`'s type and device (empty_like, half the host time, where it is dense)."""
+    return torch.empty_like(like) if like.shape == shape and like.is_contiguous() else like.new_empty(shape)
 
 
 def no_grad_of(fn: str, *tensors) -> None:
@@ -64,55 +85,73 @@ def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_
     first rot elements of each head are rotated, in pairs x[j], x[j + rot / 2], or, interleaved, x[2 j],
     x[2 j + 1]. A position outside rope comes out as NaN. All of one type (float32, float16, bfloat16)."""
     fn = "paged_kv_append"
-    if k.dim() != 3 or v.shape != k.shape:
-        raise ValueError(f"{fn}: k {tuple(k.shape)}, v {tuple(v.shape)}: expected two [tokens, kv_heads, head_dim]")
-    T, Hkv, D = k.shape
+    # (checks are compared in bulk; what differs is looked at by the helpers, which convert or refuse. A call's
+    # host time is most of what appending a decode step takes: 15.4 us a call with the helpers alone)
+    ks, ps, dt, int32_t = k.shape, k_pool.shape, k.dtype, torch.int32
+    if len(ks) != 3 or v.shape != ks:
+        raise ValueError(f"{fn}: k {tuple(ks)}, v {tuple(v.shape)}: expected two [tokens, kv_heads, head_dim]")
+    T, Hkv, D = ks
     kv_sb, kv_sh, kv_st, _ = pools(k_pool, v_pool, fn)
-    num_blocks, Hp, block_size, Dp = k_pool.shape
-    if (Hp, Dp) != (Hkv, D):
-        raise ValueError(f"{fn}: k {tuple(k.shape)}, pools {tuple(k_pool.shape)}: heads or head dims differ")
-    if k.dtype != k_pool.dtype or v.dtype != k.dtype or q is not None and q.dtype != k.dtype:
-        raise TypeError(f"{fn}: q, k, v and the pools must have one dtype, got {q.dtype if q is not None else None}, {k.dtype}, "
+    num_blocks, Hp, block_size, Dp = ps
+    if Hp != Hkv or Dp != D:
+        raise ValueError(f"{fn}: k {tuple(ks)}, pools {tuple(ps)}: heads or head dims differ")
+    if k_pool.dtype != dt or v.dtype != dt or q is not None and q.dtype != dt:
+        raise TypeError(f"{fn}: q, k, v and the pools must have one dtype, got {q.dtype if q is not None else None}, {dt}, "
                         f"{v.dtype}, {k_pool.dtype}")
-    if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != D):
-        raise ValueError(f"{fn}: q {tuple(q.shape)} for k {tuple(k.shape)}")
-    rot = 0
+    Hq = 0
+    if q is not None:
+        qs = q.shape
+        if len(qs) != 3 or qs[0] != T or qs[2] != D:
+            raise ValueError(f"{fn}: q {tuple(qs)} for k {tuple(ks)}")
+        Hq = qs[1]
+    rot = positions = rope_ld = 0
     if rope is not None:
         if rope.dim() != 2 or rope.dtype != torch.float32:
             raise ValueError(f"{fn}: rope must be float32 [positions, rot], got {rope.dtype} {tuple(rope.shape)}")
-        rot = rope.shape[1]
+        positions, rot = rope.shape
         if rot % 2 or rot > D:
             raise ValueError(f"{fn}: rope rotates {rot} of {D} elements: an even number up to the head dim is needed")
-        if rope.stride(1) != 1 or rope.stride(0) < rot:
+        rope_ld, inner = rope.stride()
+        if inner != 1 or rope_ld < rot:
             rope = rope.contiguous()
+            rope_ld = rot
     n = context_lens.shape[0] if context_lens.dim() == 1 else -1
-    lens = int32(context_lens, "context_lens", fn, (None,))
-    tables = int32(block_tables, "block_tables", fn, (n, None))
-    cu = None
+    if context_lens.dtype != int32_t or n < 0 or context_lens.stride(0) != 1:
+        context_lens = int32(context_lens, "context_lens", fn, (None,))
+    ts = block_tables.shape
+    if block_tables.dtype != int32_t or len(ts) != 2 or ts[0] != n or block_tables.stride(1) != 1:
+        block_tables = int32(block_tables, "block_tables", fn, (n, None))
     if cu_seqlens is not None:
-        cu = int32(cu_seqlens, "cu_seqlens", fn, (n + 1,))
+        if cu_seqlens.dtype != int32_t or cu_seqlens.shape != (n + 1,) or cu_seqlens.stride(0) != 1:
+            cu_seqlens = int32(cu_seqlens, "cu_seqlens", fn, (n + 1,))
     elif n != T:
         raise ValueError(f"{fn}: {T} rows for {n} sequences: without cu_seqlens, each has one")
-    no_grad_of(fn, q, k, v, k_pool, v_pool)
-    dev = require_hip(fn, *(t for t in (k, v, k_pool, v_pool, tables, lens, q, cu, rope) if t is not None))
-    if k.stride(2) != 1 and D > 1:
+    if torch.is_grad_enabled():
+        no_grad_of(fn, q, k, v, k_pool, v_pool)
+    dev = one_device(fn, k, v, k_pool, v_pool, block_tables, context_lens, q, cu_seqlens, rope)
+    k_st, k_sh, inner = k.stride()
+    if inner != 1 and D > 1:
         k = k.contiguous()
-    if v.stride(2) != 1 and D > 1:
+        k_st, k_sh, _ = k.stride()
+    v_st, v_sh, inner = v.stride()
+    if inner != 1 and D > 1:
         v = v.contiguous()
+        v_st, v_sh, _ = v.stride()
     turn = q is not None and rot > 0
-    out, q_st, q_sh, Hq = q, 0, 0, 0
+    out, q_st, q_sh, q_at, out_at = q, 0, 0, 0, 0
     if turn:
-        if q.stride(2) != 1 and D > 1:
+        q_st, q_sh, inner = q.stride()
+        if inner != 1 and D > 1:
             q = q.contiguous()
-        Hq = q.shape[1]
-        q_st, q_sh, _ = q.stride()
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    k_st, k_sh, _ = k.stride()
-    v_st, v_sh, _ = v.stride()
-    kernels.check(kernels.lib().mlsx_paged_append(_ARGS.pack(
-        q.data_ptr() if turn else 0, k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-        out.data_ptr() if turn else 0, tables.data_ptr(), lens.data_ptr(), cu.data_ptr() if cu is not None else 0,
-        rope.data_ptr() if rot else 0, dt_code(k.dtype, fn), q_st, q_sh, k_st, k_sh, v_st, v_sh, kv_sb, max(kv_sh, D), max(kv_st, D),
-        tables.stride(0), rope.stride(0) if rot else 0, num_blocks, n, T, Hq, Hkv, D, block_size, tables.shape[1],
-        rope.shape[0] if rot else 0, rot, interleaved), stream(dev)), fn)
+            q_st, q_sh, _ = q.stride()
+        out = fresh(q, (T, Hq, D))
+        q_at, out_at = q.data_ptr(), out.data_ptr()
+    rc = kernels.lib().mlsx_paged_append(_ARGS.pack(
+        q_at, k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out_at, block_tables.data_ptr(),
+        context_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(), rope.data_ptr() if rot else 0,
+        _DT[dt] if dt in _DT else dt_code(dt, fn), q_st, q_sh, k_st, k_sh, v_st, v_sh, kv_sb, kv_sh if kv_sh > D else D,
+        kv_st if kv_st > D else D, block_tables.stride(0), rope_ld, num_blocks, n, T, Hq, Hkv, D, block_size,
+        block_tables.shape[1], positions if rot else 0, rot, interleaved), _raw_stream(dev))
+    if rc:
+        kernels.check(rc, fn)
     return out
