@@ -557,6 +557,81 @@ __device__ __forceinline__ void gqa_store_live(const GqaArgs& a, int tok, int he
   if (split == 0 && a.ws_live) a.ws_live[(int64_t)tok * a.Hkv * a.group + head] = live;
 }
 
+// The rows (a bit each) of 16 whose sums are not finite: an infinity or NaN among the values, which the matrix
+// products multiply with the weights 0 of the rows that do not see its key, or one that they do see.
+template <int OT>
+__device__ __forceinline__ uint32_t gqa_odd_rows(const f32x4 (&o)[OT]) {
+  float z = 0.0f;
+#pragma unroll
+  for (int d = 0; d < OT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z = fmaf(o[d][i], 0.0f, z);
+  uint64_t b = __ballot(z != 0.0f);
+  b |= b >> 32;
+  return (uint32_t)(b | b >> 16) & 0xFFFFu;
+}
+
+// Such a row over the keys [lo, hi) again, by one wavefront: a lane makes a key's score, then 4 elements of the sum,
+// to which only keys that the row sees add. After the last use of the kernels' own registers, so that it takes none of
+// their loops' (it costs a prompt of 8192 bf16 rows under 1%; a check of each tile in the loop 14%, a function on a stack 5%).
+template <typename T>
+__device__ __forceinline__ void gqa_row_again(const GqaArgs& a, const int32_t* table, int kvh, int tok, int head, int lo, int hi,
+                                                        int pos, int piece, bool direct, int lane) {
+  const T* q = static_cast<const T*>(a.q) + tok * a.q_st + head * a.q_sh;
+  const T* kp = static_cast<const T*>(a.kp) + kvh * a.kv_sh;
+  const T* vp = static_cast<const T*>(a.vp) + kvh * a.kv_sh;
+  const float slope = a.slopes ? a.slopes[head] * 1.44269504f : 0.0f;
+  float m = -3.402823466e38f, l = 0.0f;
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int j = lo; j < hi; j += 64) {
+    const int key = j + lane, blk = key < hi ? table[gqa_block_of(a, key)] : -1;
+    const bool there = blk >= 0 && blk < a.num_blocks;
+    const int64_t at = there ? (int64_t)blk * a.kv_sb + (int64_t)(key - gqa_block_of(a, key) * a.BS) * a.kv_st : 0;
+    float s = -__builtin_huge_valf();
+    if (there) {
+      float x = 0.0f;
+#pragma unroll 1
+      for (int d = 0; d < a.D; ++d) x = fmaf(to_f32(q[d]), to_f32(kp[at + d]), x);
+      s = a.cap > 0.0f ? tanhf(x * a.to_cap) * a.cap : x * a.c;
+      if (a.slopes) s = fmaf(-slope, fabsf((float)(pos - key)), s);
+    }
+    const float mn = fmaxf(m, lane_group_max<64>(s)), f = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(s - mn);
+    m = mn;
+    l = fmaf(l, f, w);
+    o *= f;
+#pragma unroll 1
+    for (uint64_t left = __ballot(there); left; left &= left - 1) {
+      const int k = __builtin_ctzll(left);
+      const float wk = __shfl(w, k, 64);
+      const int64_t ak = __shfl((long long)at, k, 64);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * lane + i < a.D) o[i] = fmaf(wk, to_f32(vp[ak + 4 * lane + i]), o[i]);
+    }
+  }
+  l = lane_group_sum<64>(l);
+  if (4 * lane < a.D) gqa_store<T>(a, tok, head, piece, direct, 4 * lane, o, m, l);
+}
+
+// Bit i: row r0 + i is one of the tile's sequence
+__device__ __forceinline__ uint32_t gqa_rows_of(const GqaPlan& p, int r0) {
+  return r0 + 16 <= p.rows ? 0xFFFFu : r0 < p.rows ? (1u << (p.rows - r0)) - 1 : 0;
+}
+
+// The rows r0 + i of `odd`'s bits again, over the piece's keys [from, to)
+template <typename T>
+__device__ __forceinline__ void gqa_again(const GqaArgs& a, const GqaPlan& p, uint32_t odd, int r0, int kvh, int piece, int from, int to, int lane) {
+#pragma unroll 1
+  while (__builtin_expect(odd != 0, 0)) {
+    const int r = r0 + __builtin_ctz(odd), tok = p.tok0 + r / a.group;
+    odd &= odd - 1;
+    int lo, hi, pos;
+    gqa_row_range(a, p, tok, lo, hi, pos);
+    gqa_row_again<T>(a, p.table, kvh, tok, kvh * a.group + r % a.group, max(lo, from), min(hi, to), pos, piece, p.direct, gqa_here(lane));
+  }
+}
+
 // Many rows: 4 wavefronts of 16 NT rows each share tiles of BN keys, in two LDS buffers.
 template <typename T, int DP>
 constexpr int gqa_bn() {
@@ -610,18 +685,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void gqa_rows_kernel(const 
     }
   }
   const int g = lane >> 4;
+  uint32_t odd = 0;  // a bit a row
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = row0 + 16 * n + (lane & 15);
     const float l = rows.sum_of(n);
+    odd |= (gqa_odd_rows(rows.o[n]) & gqa_rows_of(p, row0 + 16 * n)) << (16 * n);
     if (r < p.rows) {
       const int tok = p.tok0 + r / a.group, head = kvh * a.group + r % a.group;
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d)
-        gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, 16 * d + 4 * g, rows.o[n][d], rows.m[n], l);
+        if (!((odd >> (16 * n + (lane & 15))) & 1)) gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, 16 * d + 4 * g, rows.o[n][d], rows.m[n], l);
       if (g == 0) gqa_store_live(a, tok, head, split, p.live);
     }
   }
+  gqa_again<T>(a, p, odd, row0, kvh, a.piece0 + split, p.lo + t0 * BN, p.lo + t1 * BN, lane);
 }
 
 // Many rows of 16-bit types: 8 wavefronts, two a SIMD, in two groups half a step apart: while one
@@ -731,18 +809,21 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
     if (!(wave >= 4)) asm volatile("s_barrier" ::: "memory");
   }
   const int g = lane >> 4;
+  uint32_t odd = 0;  // a bit a row
 #pragma unroll
   for (int m = 0; m < NT; ++m) {
     const int r = row0 + 16 * m + (lane & 15);
     const float l = w.rows.sum_of(m);
+    odd |= (gqa_odd_rows(w.rows.o[m]) & gqa_rows_of(p, row0 + 16 * m)) << (16 * m);
     if (r < p.rows) {
       const int tok = p.tok0 + r / a.group, head = kvh * a.group + r % a.group;
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d)
-        gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, 16 * d + 4 * g, w.rows.o[m][d], w.rows.m[m], l);
+        if (!((odd >> (16 * m + (lane & 15))) & 1)) gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, 16 * d + 4 * g, w.rows.o[m][d], w.rows.m[m], l);
       if (g == 0) gqa_store_live(a, tok, head, split, p.live);
     }
   }
+  gqa_again<T>(a, p, odd, row0, kvh, a.piece0 + split, j0, j0 + n * BN, lane);
 }
 
 // Few rows: the NW wavefronts of a block hold the same 16 NT rows and take WK keys each of a
@@ -830,21 +911,29 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
   // join the wavefronts' states
   float* ol = reinterpret_cast<float*>(smem);                // [NW][16 NT][OL]
   float* ml = ol + NW * 16 * NT * OL;                        // [NW][16 NT][2]
+  uint32_t* odd = reinterpret_cast<uint32_t*>(ml + NW * 16 * NT * 2);  // [NW]: rows whose sums are not finite
   __syncthreads();
+  uint32_t mine = 0;
   const int g = lane >> 4;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = 16 * n + (lane & 15);
     const float l = rows.sum_of(n);
+    mine |= (gqa_odd_rows(rows.o[n]) & gqa_rows_of(p, p.row0 + 16 * n)) << (16 * n);
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
       *reinterpret_cast<f32x4*>(ol + (wave * 16 * NT + r) * OL + 16 * d + 4 * g) = rows.o[n][d];
     if (g == 0) *reinterpret_cast<float2*>(ml + (wave * 16 * NT + r) * 2) = make_float2(rows.m[n], l);
   }
+  if (lane == 0) odd[wave] = mine;
   __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) all |= __builtin_amdgcn_readfirstlane(odd[w]);
   for (int e = threadIdx.x; e < 16 * NT * (DP / 4); e += NW * 64) {
     const int rr = e / (DP / 4), d = (e % (DP / 4)) * 4, r = p.row0 + rr;
     if (r >= p.rows || d >= a.D) continue;
+    const bool again = (all >> rr) & 1;
     float M = -3.402823466e38f, L = 0.0f;
     float2 x[NW];
 #pragma unroll
@@ -860,15 +949,18 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
       acc += *reinterpret_cast<const f32x4*>(ol + (w * 16 * NT + rr) * OL + d) * f;
     }
     const int tok = p.tok0 + r / a.group, head = kvh * a.group + r % a.group;
-    gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, d, acc, M, L);
+    if (!again) gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, d, acc, M, L);
     if (d == 0) gqa_store_live(a, tok, head, split, p.live);
   }
+  // (a wavefront takes every NW-th row)
+  gqa_again<T>(a, p, all & ((NW == 4 ? 0x11111111u : 0x55555555u) << wave), p.row0, kvh, a.piece0 + split,
+               p.lo + split * p.per * BN, p.lo + (split + 1) * p.per * BN, lane);
 }
 
 template <typename T, int DP, int NT>
 constexpr int gqa_keys_lds() {
   constexpr int NW = gqa_nw<T, DP>();
-  constexpr int tiles = NW * (gqa_wk<T, DP>() * GqaTile<T, DP>::ROWB + 256 * NT), join = NW * 16 * NT * (DP + 4 + 2) * 4;
+  constexpr int tiles = NW * (gqa_wk<T, DP>() * GqaTile<T, DP>::ROWB + 256 * NT), join = NW * 16 * NT * (DP + 4 + 2) * 4 + 4 * NW;
   return tiles > join ? tiles : join;
 }
 

@@ -266,3 +266,31 @@ def test_empty_calls(dev):
     assert paged_attention(q, kp, vp, tab, ctx, offsets([0, 0])).shape == (0, 4, 64)
     assert paged_attention(q, kp, vp, tab[:0], ctx[:0]).shape == (0, 4, 64)
     assert bool((paged_attention(_q(3, 4, 64, BF), kp, vp, tab[:0], ctx[:0], offsets([])) == 0).all())
+
+
+@pytest.mark.parametrize("dtype,D,group", [(BF, 128, 4), (HF, 64, 1), (FP, 64, 2), (BF, 256, 2), (FP, 128, 1), (HF, 80, 3)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("new,past", [([200, 9], [0, 40]), ([5, 3], [60, 0]), ([40], [300]), ([300], [70])])
+def test_values_that_only_later_rows_see(dev, dtype, D, group, bad, new, past):
+    """A cached value that is no number reaches the rows that see its token, in its own element, and no others."""
+    lens = [a + b for a, b in zip(new, past)]
+    for window in (0, 25):
+        kp, vp, tab, ctx = cache(lens, 1, D, 16, dtype, 21)
+        q = _q(sum(new), group, D, dtype)
+        want, bound = attention(q, kp, vp, tab, lens, new, window=window)
+        row = 0
+        for s, (cnt, n) in enumerate(zip(new, lens)):
+            for j in (n - 1, n - cnt // 2 - 1, max(0, n - cnt - 3)):
+                vp[int(tab[s, j // 16]), 0, j % 16, j % D] = bad
+                pos = torch.arange(n - cnt, n, device=dev)
+                sees = (pos >= j) & ((pos - j < window) if window else True)
+                part = want[row:row + cnt, :, j % D]
+                add = torch.full_like(part, bad)
+                want[row:row + cnt, :, j % D] = torch.where(sees[:, None], part + add, part)
+            row += cnt
+        y = paged_attention(q, kp, vp, tab, ctx, offsets(new), window=window).double()
+        odd = ~torch.isfinite(want)
+        assert bool((~torch.isfinite(y) == odd).all()), f"{int((~torch.isfinite(y) != odd).sum())} elements"
+        if bad == bad:
+            assert bool((y[odd] == want[odd]).all())
+        check(torch.where(odd, 0.0, y), torch.where(odd, 0.0, want), bound.nan_to_num(0.0, 0.0, 0.0) + torch.where(odd, 1e-30, 0.0))
