@@ -8,9 +8,9 @@ only. The library is bound on first use; if it is missing, or a CPU tensor
 reaches a kernel entry point, the call raises instead of computing elsewhere.
 
 Overlay. This package replaces only the reference's quantized-linear modules
-(dequant_matmul, fp8_matmul, moe_routing, paged_attention). Its search path is
-extended over every ``kernels`` directory on ``sys.path`` (pkgutil.extend_path),
-so with this directory first and a reference checkout after it, the reference's
+(dequant_matmul, fp8_matmul, moe_routing, paged_attention), and adds its own beside
+them (moe_grouped, int8_ste, paged_kv). Its search path is extended over every
+``kernels`` directory on ``sys.path`` (pkgutil.extend_path), so with this directory first and a reference checkout after it, the reference's
 other modules (attention_fwd, attention_bwd, autograd_ops, moe_backward,
 fusion_compiler) import from the checkout and bind this package's GEMMs. Both
 roots must be on ``sys.path`` before the first ``import kernels``.

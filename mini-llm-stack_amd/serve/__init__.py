@@ -1,6 +1,6 @@
-"""Serving-side quantization for the gfx950 quantized-linear path.
+"""Serving-side quantization and paged attention for the gfx950 path.
 
-This package provides only ``serve.quantize``. Its search path is extended over
+This package provides ``serve.quantize`` and ``serve.paged_layer``. Its search path is extended over
 every ``serve`` directory on ``sys.path`` (pkgutil.extend_path), so a reference
 checkout placed after this directory still supplies the engine, KV cache,
 speculative decoding and API modules, which then bind this ``serve.quantize``.
