@@ -143,7 +143,7 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   a.num_blocks = p->num_blocks, a.n = (int)n, a.T = (int)T, a.Hkv = (int)Hkv, a.group = (int)G, a.D = (int)D;
   a.DW = (int)cdiv(D, 4) * 4, a.BS = (int)BS;
   a.bs_magic = (uint32_t)((0xFFFFFFFFull / (uint64_t)BS) + 1);  // ceil(2^32 / BS) for BS > 1
-  a.max_blocks = (int)p->max_blocks, a.window = (int)p->window;
+  a.max_keys = (int)std::min<int64_t>(p->max_blocks * BS, 0x7FFFFFFF), a.window = (int)p->window;
   if (vec && p->kv_sb * esz <= 0xFFFFFFFFll && p->kv_st * esz * std::max<int64_t>(BS, 64) < 0x7FFFFFFFll)
     a.sb_bytes = (uint32_t)(p->kv_sb * esz), a.st_bytes = (uint32_t)(p->kv_st * esz);
   a.kv_vec = vec;
@@ -161,7 +161,7 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   const int64_t most = p->cu_seqlens ? (p->max_new > 0 ? std::min(p->max_new, T) : cdiv(T, std::max<int64_t>(n, 1))) : 1;
   choose_shape(own.s, most * G, T * G * Hkv, p->dt, D, BS, a.sb_bytes != 0);
   own.a.bm_log = __builtin_ctz(own.s.bm);
-  own.a.bn = own.s.bn;
+  own.a.bn_log = __builtin_ctz(own.s.bn);
   const int64_t bm = 1ll << own.a.bm_log;
   const int64_t slots = p->cu_seqlens ? T * G / bm + n + 2 : n * cdiv(G, bm);
   int64_t steps = cdiv(std::max<int64_t>(p->max_blocks * BS, 1), own.s.bn);
@@ -177,9 +177,9 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
     choose_shape(pre.s, n * G, n * G * Hkv, p->dt, D, BS, a.sb_bytes != 0);
     pre.a.shared = 1;
     pre.a.front = (int)std::min<int64_t>(p->prefix_len, p->prefix_count * BS);
-    pre.a.bt = p->prefix_blocks, pre.a.bt_ss = 0, pre.a.max_blocks = (int)p->prefix_count;
+    pre.a.bt = p->prefix_blocks, pre.a.bt_ss = 0;
     pre.a.bm_log = __builtin_ctz(pre.s.bm);
-    pre.a.bn = pre.s.bn;
+    pre.a.bn_log = __builtin_ctz(pre.s.bn);
     pre.a.slots = (int)cdiv(n * G, 1ll << pre.a.bm_log);
     const int64_t pt = pre.a.slots * Hkv, ps = std::max<int64_t>(cdiv(pre.a.front, pre.s.bn), 1);
     const int64_t ptarget = pre.s.pair ? 256 : 512;

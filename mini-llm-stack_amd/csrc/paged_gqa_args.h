@@ -27,13 +27,13 @@ struct GqaArgs {
   int n, T, Hkv, group, D, DW, BS;
   uint32_t bs_magic;  // ceil(2^32 / BS)
   uint32_t sb_bytes, st_bytes;  // kv_sb, kv_st in bytes where they fit (0: not)
-  int max_blocks;
+  int max_keys;           // a table's tokens
   int window;
   int front;   // shared: keys of the prefix
   int shared;  // the rows of all sequences (one each) over the one table's `front` keys
   float c, cap, to_cap;  // scale log2(e); cap log2(e) (0: none), scale / cap
   int simple;            // scores are positive multiples of the products: no cap, no slopes
-  int bm_log, bn;        // rows of a tile (log2) and keys of a step
+  int bm_log, bn_log;    // rows of a tile and keys of a step (log2)
   int slots;             // row tiles that the grid has room for
   int pieces;            // records a row has in the workspace
   int piece0;            // first record of this launch's pieces (before it: the shared prefix's)
@@ -94,7 +94,7 @@ __device__ __forceinline__ int gqa_find(const GqaArgs& a, int at, int lane) {
 }
 
 __device__ __forceinline__ int gqa_keys_of(const GqaArgs& a, int s) {
-  return (int)min((int64_t)max(a.lens[s], 0), (int64_t)a.max_blocks * a.BS);
+  return min(max(a.lens[s], 0), a.max_keys);
 }
 
 // Steps of a piece: what makes about `target` blocks of the batch's own lengths, and at most
@@ -105,10 +105,10 @@ __device__ __forceinline__ int gqa_piece(const GqaArgs& a, int lane) {
   int most = 0;
   for (int s = lane; s < a.n; s += 64) {
     const int nt = a.cu ? max(gqa_cu(a, s + 1) - gqa_cu(a, s), 0) : 1;
-    int64_t keys = gqa_keys_of(a, s);
-    if (a.window > 0) keys = min(keys, (int64_t)a.window + nt);
-    const int t = (int)((keys + a.bn - 1) / a.bn);
-    sum += (float)((((int64_t)nt * a.group + (1 << a.bm_log) - 1) >> a.bm_log) * t);
+    uint32_t keys = gqa_keys_of(a, s);
+    if (a.window > 0) keys = min(keys, (uint32_t)a.window + nt);
+    const int t = (int)((keys + (1u << a.bn_log) - 1) >> a.bn_log);
+    sum += (float)((nt * a.group + (1 << a.bm_log) - 1) >> a.bm_log) * (float)t;
     if (nt > 0) most = max(most, t);
   }
   sum = lane_group_sum<64>(sum);
@@ -117,8 +117,8 @@ __device__ __forceinline__ int gqa_piece(const GqaArgs& a, int lane) {
   return __builtin_amdgcn_readfirstlane(max(max(want, (most + a.splits - 1) / a.splits), a.least));
 }
 
-// Row tile rt of sequence seq (-1 and n: rows that no sequence holds, which see nothing).
-__device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int rt, int lane) {
+// Row tile rt of sequence seq (-1 and n: rows that no sequence holds, which see nothing), for its piece `split`.
+__device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int rt, int split, int lane) {
   GqaPlan p;
   const bool real = seq >= 0 && seq < a.n;
   int ntok;
@@ -157,11 +157,11 @@ __device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int 
   }
   p.khi = __builtin_amdgcn_readfirstlane(min(max(pmax + 1, p.pfx), p.len));
   p.klo = __builtin_amdgcn_readfirstlane(a.window > 0 ? max(0, pmin - a.window + 1) : 0);
-  p.lo = p.klo - p.klo % a.bn;
-  p.tiles = p.khi > p.klo ? (p.khi - p.lo + a.bn - 1) / a.bn : 0;
+  p.lo = p.klo >> a.bn_log << a.bn_log;
+  p.tiles = p.khi > p.klo ? (int)(((uint32_t)(p.khi - p.lo) + (1u << a.bn_log) - 1) >> a.bn_log) : 0;
   if (a.shared) {
     p.live = a.splits;
-  } else if (a.splits > 1) {
+  } else if (a.splits > 1 && p.tiles > max(split, 1)) {  // (a piece has a step or more: others need no lengths of the batch)
     const int piece = gqa_piece(a, lane);
     p.live = min(max((p.tiles + piece - 1) / piece, 1), a.splits);
   } else {
@@ -181,13 +181,13 @@ __device__ __forceinline__ GqaPlan gqa_block_plan(const GqaArgs& a, int block, i
   const int rest = block / a.Hkv;
   split = rest / a.slots;
   const int slot = a.slots - 1 - rest % a.slots;
-  if (a.shared) return gqa_tile_plan(a, 0, slot, lane);
+  if (a.shared) return gqa_tile_plan(a, 0, slot, split, lane);
   if (!a.cu) {
     const int per = (a.group + (1 << a.bm_log) - 1) >> a.bm_log;
-    return gqa_tile_plan(a, slot / per, slot % per, lane);
+    return gqa_tile_plan(a, slot / per, slot % per, split, lane);
   }
   const int seq = __builtin_amdgcn_readfirstlane(gqa_find<true>(a, slot, lane));
-  return gqa_tile_plan(a, seq, seq < 0 ? slot : slot - __builtin_amdgcn_readfirstlane(gqa_slot_of(a, seq)), lane);
+  return gqa_tile_plan(a, seq, seq < 0 ? slot : slot - __builtin_amdgcn_readfirstlane(gqa_slot_of(a, seq)), split, lane);
 }
 
 // The keys [lo, hi) that the row of token `tok` sees, and its position.
