@@ -12,8 +12,9 @@
 //
 // Softmax with a lazy maximum: m is a row's reference, any value within 2^8 of what the row has
 // seen; only a tile with a score above m + 8 (in log2 units) reduces the maximum over lanes and
-// rescales l and O. l is a per-lane partial sum until the end. All statistics are fp32. P is
-// rounded to the inputs' type for the product with V (half a step, unbiased), l sums it unrounded.
+// rescales l and O. All statistics are fp32. For the product with V, P is rounded to the inputs' type (half a
+// step of each weight; l sums the weights as rounded, so that a row's shares still add to 1), but in the kernel over
+// keys, whose matrix unit has room: there P is two parts of that type.
 #pragma once
 
 #include <atomic>
@@ -184,7 +185,7 @@ struct GqaFill {
   }
   // The K (V = false) or V rows straight into LDS. By buffer loads, whose bounds give the zeros; and the
   // compiler takes LDS-direct loads of the global kind for accesses that may return in any order, so that
-  // every later LDS read would wait for all reads (lgkmcnt(0)) and some for all loads: 595 us for a prompt of 8192.
+  // every later LDS read would wait for all reads (lgkmcnt(0)) and some for all loads.
   template <bool V>
   __device__ __forceinline__ void load(const GqaArgs& a, uint8_t* dst, const uint8_t* base, int wave, int lane, int only = -1) const {
     constexpr uint64_t FULL = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
@@ -831,7 +832,9 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
 // joined through LDS. K's fragments are loaded straight into registers (16 rows of 64 bytes an
 // instruction), the next tile's as soon as this one's scores are made; V tiles go through LDS, to be read
 // transposed, the next one's loads issued after this one's product. (With two K and two V buffers in LDS and
-// 4 wavefronts a CU: 40 sequences of 1 to 4096 tokens, 32 heads of 128 over 8 K/V heads, 45 us.)
+// 4 wavefronts a CU: 40 sequences of 1 to 4096 tokens, 32 heads of 128 over 8 K/V heads, 45 us; so 35. 64 of 2048: 104,
+// 5.2 TB/s.) What a block takes before its first key (lengths, table, keys: three loads one after the other, 7 us by its clock) is
+// most of what short contexts take, and code that runs once costs as much as the loads: it is fetched anew in each launch.
 template <typename T, int DP>
 constexpr int gqa_wk() { return GqaType<T>::F32 ? (DP <= 64 ? 32 : 16) : 32; }
 template <typename T, int DP>

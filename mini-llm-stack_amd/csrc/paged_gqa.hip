@@ -6,14 +6,15 @@
 // with a window w, p - j < w. Its score is x = scale q.k, capped c tanh(x / c), less
 // slope |p - j|; out = sum_j softmax(x)_j v_j, 0 where it sees nothing.
 //
-// Two kernels:
+// Three kernels:
 // - gqa_keys_kernel, up to 32 packed rows (new tokens x group) a sequence: HBM-bound. Each
 //   wavefront streams keys of its own, all hold the same rows.
-// - gqa_rows_kernel: MFMA-bound. The wavefronts of a block hold 16 or 32 rows each and share the
-//   K/V tiles.
+// - gqa_pair_kernel, many rows of 16-bit types: MFMA-bound. 8 wavefronts of 32 rows (16 of D > 128) share the K/V
+//   tiles, in two groups of which one multiplies while the other makes its softmax.
+// - gqa_rows_kernel, the rest (fp32, rows between, any alignment): 4 wavefronts of 16 or 32 rows share the tiles.
 // Where row tiles are fewer than the GPU has room for, contexts are cut into pieces, whose
-// (O, reference, sum) a third kernel joins. A shared prefix is a pass of its own: the rows of all
-// sequences against its keys, read once for 128 rows instead of once a sequence.
+// (O, reference, sum) a fourth kernel joins. A shared prefix is a pass of its own: the rows of all
+// sequences against its keys, read once for a tile of rows instead of once a sequence.
 #include <algorithm>
 
 #include "paged_gqa_args.h"
@@ -94,7 +95,8 @@ struct Pass {
 // - Up to 32 rows: the kernel over keys.
 // - 16-bit types: the paired kernel's tiles of 256 rows (128 of D > 128) where they are at least half full, since it is
 //   1.7 times as fast a row as tiles of 64 (prompt of 8192: 550 us, 915 in tiles of 64).
-// - fp32: tiles of 128 rows where there are enough to fill the GPU (a step of one takes 3.4 us: 5 prompts of up to 700 tokens, 8 heads of 64, 47 us so, 31 in tiles of 64).
+// - fp32: tiles of 128 rows where there are enough to fill the GPU (a step of one takes 3.4 us: 5 prompts of up to 700 tokens, 8 heads of 64,
+//   47 us so, 31 in tiles of 64).
 void choose_shape(GqaShape& s, int64_t rows, int64_t all, int dt, int64_t D, int64_t BS, bool vec) {
   s.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
   if (dt == MLS_F32) gqa_tiles<float>(s);
@@ -166,6 +168,8 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   const int64_t slots = p->cu_seqlens ? T * G / bm + n + 2 : n * cdiv(G, bm);
   int64_t steps = cdiv(std::max<int64_t>(p->max_blocks * BS, 1), own.s.bn);
   if (p->window > 0) steps = std::min(steps, cdiv(p->window + most, own.s.bn) + 1);
+  // two blocks of the kernel over keys run on a CU: 512 pieces would be one round, but twice as many even out
+  // unequal lengths (40 sequences of 1 to 4096 tokens: 41.7 us against 46.9)
   const int64_t target = own.s.pair ? 768 : 1024, tiles = slots * Hkv;
   const int64_t room = own.s.keys ? cdiv(2 * target, tiles) : target / tiles;
   int64_t splits = std::max<int64_t>(1, std::min<int64_t>({room, steps, 64}));
@@ -182,6 +186,8 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
     pre.a.bn_log = __builtin_ctz(pre.s.bn);
     pre.a.slots = (int)cdiv(n * G, 1ll << pre.a.bm_log);
     const int64_t pt = pre.a.slots * Hkv, ps = std::max<int64_t>(cdiv(pre.a.front, pre.s.bn), 1);
+    // a block a CU, or two: half of it leaves CUs idle (64 sequences behind 8192 tokens, 256 rows a K/V head: 67 us
+    // against 58), the smaller tiles' kernel with two blocks a CU takes as long (57) and 256 of them longer (63)
     const int64_t ptarget = pre.s.pair ? 256 : 512;
     sp = std::max<int64_t>(1, std::min<int64_t>({ptarget / pt, ps, 48}));
     pre.a.splits = (int)sp;
