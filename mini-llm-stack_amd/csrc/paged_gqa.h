@@ -827,7 +827,7 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
   gqa_again<T>(a, p, odd, row0, kvh, a.piece0 + split, j0, j0 + n * BN, lane);
 }
 
-// Few rows: the NW wavefronts of a block hold the same 16 NT rows and take WK keys each of a
+// Few rows: the NW wavefronts of a block hold the same 16 rows and take WK keys each of a
 // step of NW WK keys, so that no wavefront waits for another before the end, where their states are
 // joined through LDS. K's fragments are loaded straight into registers (16 rows of 64 bytes an
 // instruction), the next tile's as soon as this one's scores are made; V tiles go through LDS, to be read
@@ -862,8 +862,9 @@ __device__ __forceinline__ void gqa_load_k(const GqaArgs& a, uint4 (&kf)[KT][DP 
   }
 }
 
-template <typename T, int DP, int NT>
+template <typename T, int DP>
 __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void gqa_keys_kernel(const GqaArgs a) {
+  constexpr int NT = 1;
   constexpr int WK = gqa_wk<T, DP>(), NW = gqa_nw<T, DP>(), TB = WK * GqaTile<T, DP>::ROWB, BN = NW * WK;
   constexpr int OL = DP + 4;  // floats of an output row in LDS
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -960,10 +961,10 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
                p.lo + split * p.per * BN, p.lo + (split + 1) * p.per * BN, lane);
 }
 
-template <typename T, int DP, int NT>
+template <typename T, int DP>
 constexpr int gqa_keys_lds() {
   constexpr int NW = gqa_nw<T, DP>();
-  constexpr int tiles = NW * (gqa_wk<T, DP>() * GqaTile<T, DP>::ROWB + 256 * NT), join = NW * 16 * NT * (DP + 4 + 2) * 4 + 4 * NW;
+  constexpr int tiles = NW * (gqa_wk<T, DP>() * GqaTile<T, DP>::ROWB + 256), join = NW * 16 * (DP + 4 + 2) * 4 + 4 * NW;
   return tiles > join ? tiles : join;
 }
 
@@ -983,11 +984,7 @@ int gqa_launch_kernel(const GqaArgs& a, int64_t blocks, int threads, int lds, hi
 
 template <typename T, int DP>
 int gqa_launch_dp(const GqaArgs& a, const GqaShape& s, int64_t blocks, hipStream_t st) {
-  if (s.keys) {
-    constexpr int threads = gqa_nw<T, DP>() * 64, l1 = gqa_keys_lds<T, DP, 1>(), l2 = gqa_keys_lds<T, DP, 2>();
-    if (s.nt == 1) return gqa_launch_kernel<gqa_keys_kernel<T, DP, 1>>(a, blocks, threads, l1, st);
-    return gqa_launch_kernel<gqa_keys_kernel<T, DP, 2>>(a, blocks, threads, l2, st);
-  }
+  if (s.keys) return gqa_launch_kernel<gqa_keys_kernel<T, DP>>(a, blocks, gqa_nw<T, DP>() * 64, gqa_keys_lds<T, DP>(), st);
   if constexpr (!GqaType<T>::F32) {
     if (s.pair) {
       constexpr int NT = DP <= 128 ? 2 : 1;
@@ -1005,7 +1002,7 @@ template <typename T, int DP>
 void gqa_tiles_dp(GqaShape& s) {
   s.bn = s.keys ? gqa_nw<T, DP>() * gqa_wk<T, DP>() : s.pair ? gqa_pair_bn<T, DP>() : gqa_bn<T, DP>();
   s.group_rows = 64 / GqaTile<T, DP>::CPR;
-  s.bm = s.keys ? 16 * s.nt : s.pair ? (DP <= 128 ? 256 : 128) : 64 * s.nt;
+  s.bm = s.keys ? 16 : s.pair ? (DP <= 128 ? 256 : 128) : 64 * s.nt;
 }
 
 template <typename T>

@@ -7,7 +7,7 @@
 // slope |p - j|; out = sum_j softmax(x)_j v_j, 0 where it sees nothing.
 //
 // Three kernels:
-// - gqa_keys_kernel, up to 32 packed rows (new tokens x group) a sequence: HBM-bound. Each
+// - gqa_keys_kernel, up to 16 packed rows (new tokens x group) a sequence: HBM-bound. Each
 //   wavefront streams keys of its own, all hold the same rows.
 // - gqa_pair_kernel, many rows of 16-bit types: MFMA-bound. 8 wavefronts of 32 rows (16 of D > 128) share the K/V
 //   tiles, in two groups of which one multiplies while the other makes its softmax.
@@ -92,9 +92,12 @@ struct Pass {
 };
 
 // Row tile and kernel for `rows` packed rows a sequence, `all` of them over all sequences and K/V heads.
-// - Up to 32 rows: the kernel over keys.
+// - Up to 16 rows: the kernel over keys (40 sequences of 1 to 4096 tokens, 4 rows: 40 us, the next one 58). With 32 rows a
+//   wavefront it is out of registers: 32 rows, 12 sequences of up to 2048, 40 us against 28; 64 of 2000 to 6000, 323
+//   against 239 (20 rows: 230 against 241).
 // - 16-bit types: the paired kernel's tiles of 256 rows (128 of D > 128) where they are at least half full, since it is
-//   1.7 times as fast a row as tiles of 64 (prompt of 8192: 550 us, 915 in tiles of 64).
+//   1.7 times as fast a row as tiles of 64 (prompt of 8192: 550 us, 915 in tiles of 64; 12 sequences of 192 new rows
+//   52 against 57; of 96 rows 47 in the paired kernel, 37 in tiles of 64).
 // - fp32: tiles of 128 rows where there are enough to fill the GPU (a step of one takes 3.4 us: 5 prompts of up to 700 tokens, 8 heads of 64,
 //   47 us so, 31 in tiles of 64).
 void choose_shape(GqaShape& s, int64_t rows, int64_t all, int dt, int64_t D, int64_t BS, bool vec) {
@@ -103,9 +106,9 @@ void choose_shape(GqaShape& s, int64_t rows, int64_t all, int dt, int64_t D, int
   else gqa_tiles<_Float16>(s);
   vec = vec && BS % s.group_rows == 0;
   s.vec = vec;
-  s.keys = vec && rows <= 32;
+  s.keys = vec && rows <= 16;
   s.pair = vec && !s.keys && dt != MLS_F32 && rows > (s.dp <= 128 ? 128 : 64);
-  s.nt = s.keys ? (rows <= 16 ? 1 : 2) : (dt == MLS_F32 && vec && rows > 64 && all >= 128 * 512 ? 2 : 1);
+  s.nt = dt == MLS_F32 && vec && rows > 64 && all >= 128 * 512 ? 2 : 1;
   if (dt == MLS_F32) gqa_tiles<float>(s);
   else gqa_tiles<_Float16>(s);
 }
