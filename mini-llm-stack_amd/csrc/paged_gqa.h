@@ -141,7 +141,8 @@ struct GqaTable {
       gqa_landed();  // (once in 64 blocks)
     }
   }
-  // Lane i: the block of the tile's key j0 + i, negative for none.
+  // Lane i: the block of the tile's key j0 + i, negative for none. Called with all lanes on: ids come from
+  // other lanes' registers, and a lane that is off gives 0, a block of the pool.
   __device__ __forceinline__ int block(const GqaArgs& a, int j0, int lane) const {
     const int i = gqa_block_of(a, j0 + lane) - base;
     const int x = __shfl(tab, i & 63, 64), y = __shfl(next, i & 63, 64);
@@ -159,7 +160,8 @@ struct GqaTable {
     if (j0 >= p.klo && j0 + N <= p.khi && !holes) return N == 64 ? ~0ull : (1ull << (N & 63)) - 1;
     if (j0 >= p.khi) return 0;
     const int here = gqa_here(lane), key = j0 + here;
-    return __ballot(here < N && key >= p.klo && key < p.khi && block(a, j0, here) >= 0);
+    const int blk = block(a, j0, here);  // (not within the condition, which switches lanes off)
+    return __ballot(here < N && key >= p.klo && key < p.khi && blk >= 0);
   }
 };
 

@@ -1,0 +1,55 @@
+"""paged_attention, shared_prefix_attention and paged_kv_append at the edges of what they take: ids outside the
+pool deep in a context, views whose heads or tokens share memory, tables and windows at their ends, large caps, and values that are
+no numbers. Tolerances: paged_plain.attention's bound where nothing else is said."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from paged_plain import attention, cache, check, offsets
+
+from kernels.paged_attention import paged_attention
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def _q(T, H, D, dtype, seed=5):
+    return torch.randn(T, H, D, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype,D,bs", [(BF, 128, 16), (HF, 64, 8), (FP, 64, 8), (FP, 256, 16), (BF, 256, 32), (BF, 64, 5), (HF, 33, 16)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 4, 2], [50, 20, 33], [200, 70, 150]])
+def test_ids_outside_the_pool_deep_in_a_context(dev, dtype, D, bs, new):
+    """With more than 1024 sequences a piece is 2048 keys or more: the ids lie 20 to 200 blocks behind its start, before and
+    past the registers' first 64, and in a last tile of few keys. (64, 5) and (33, 16) load their tiles by elements."""
+    lens = [1500, 21 * bs + 3, 1000] + [0] * 1100
+    kp, vp, tab, ctx = cache(lens, 1, D, bs, dtype, 31)
+    bad = (-1, -7, kp.shape[0], 2 ** 31 - 1, -2 ** 31)
+    for i, at in enumerate((20, 40, 41, 63, 64, 70, 93, 150, 187)):
+        if at * bs < lens[0]:
+            tab[0, at] = bad[i % 5]
+    tab[1, 21] = -1  # the last 3 keys
+    tab[2, 1000 // bs - 2], tab[2, 0] = kp.shape[0], -3
+    new = new + [0] * 1100 if max(new) > 1 else [1] * len(lens)
+    q = _q(sum(new), 4, D, dtype)
+    cu = offsets(new) if max(new) > 1 else None
+    want = attention(q, kp, vp, tab, lens, new)
+    for hint in (None, max(new)):
+        check(paged_attention(q, kp, vp, tab, ctx, cu, max_new=hint), *want, f"{hint}")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("new", [1, 6, 90, 300])
+def test_ids_outside_the_pool_in_one_context(dev, dtype, new):
+    """The same for a batch of one, in pieces: every id of a run of blocks in turn."""
+    lens = [1061]
+    kp, vp, tab, ctx = cache(lens, 8, 64, 16, dtype, 32)
+    q = _q(new, 16, 64, dtype)
+    good = tab.clone()
+    for at in (1, 2, 3, 34, 35, 36, 64, 65, 66):
+        tab.copy_(good)
+        tab[0, at] = -1 - at
+        check(paged_attention(q, kp, vp, tab, ctx, offsets([new])), *attention(q, kp, vp, tab, lens, [new]), f"{at}")
