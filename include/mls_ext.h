@@ -49,9 +49,9 @@ int mlsx_paged_attention_decode(const void* q, int q_dt, int64_t q_ss, int64_t q
 /* Attention of new tokens over a paged cache with grouped heads (no reference counterpart; the
  * one-token, one-head-a-K/V-head form is kernels/paged_attention.py:93-118). Every field has 8
  * bytes. q and out: [tokens][kv_heads * group][head_dim], inner stride 1; pools [num_blocks]
- * [kv_heads][block_size][head_dim], inner stride 1, K and V with one set of strides; all of
- * type dt. Sequence s has the rows cu_seqlens[s] .. cu_seqlens[s + 1] (null: row s), its
- * last context_lens[s] - 1 the position of its last row. Rows of no sequence get zeros. A block
+ * [kv_heads][block_size][head_dim], inner stride 1, K and V with one set of strides (of heads and
+ * tokens head_dim or more, or 0: all of them in one place); all of type dt. Sequence s has the rows
+ * cu_seqlens[s] .. cu_seqlens[s + 1] (null: row s), context_lens[s] - 1 the position of its last row. Rows of no sequence get zeros. A block
  * id outside the pool holds no keys. With prefix_blocks, the prefix_len keys in those
  * prefix_count blocks come before every sequence's own (one row each), whose positions
  * count from there. max_new: the longest sequence's rows if known (0: not), which only chooses

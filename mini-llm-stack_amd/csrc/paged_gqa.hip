@@ -129,8 +129,8 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
     return fail(MLS_ERR_ARG, "%s: null pointer", fn);
   if (!p->cu_seqlens && T != n) return fail(MLS_ERR_ARG, "%s: %lld rows for %lld sequences of one", fn, (long long)T, (long long)n);
   if (shared && p->cu_seqlens) return fail(MLS_ERR_ARG, "%s: a shared prefix takes one token a sequence", fn);
-  if (p->q_sh < D || p->q_st < 0 || p->o_sh < D || p->o_st < Hkv * G * D || p->kv_st < D || p->kv_sh < D || p->kv_sb < 0 ||
-      p->bt_ss < 0)
+  if (p->q_sh < D || p->q_st < 0 || p->o_sh < D || p->o_st < Hkv * G * D || p->kv_sb < 0 || p->bt_ss < 0 ||
+      (p->kv_st < D && p->kv_st != 0) || (p->kv_sh < D && p->kv_sh != 0))
     return fail(MLS_ERR_ARG, "%s: bad strides", fn);
   if (D > 256) return fail(MLS_ERR_UNSUPPORTED, "%s: head dim %lld above 256", fn, (long long)D);
   if (T * G > 0x3FFFFFFF || T * Hkv * G > 0x3FFFFFFFFll || n > 0x3FFFFFFF || BS > 0x3FFFFFFF || p->max_blocks > 0x7FFFFFFF ||

@@ -79,7 +79,7 @@ def _attend(fn, q, k_pool, v_pool, block_tables, context_lens, cu_seqlens, max_n
     if len(qs) != 3:
         raise ValueError(f"{fn}: q {tuple(qs)}, expected [tokens, heads, head_dim]")
     T, Hq, D = qs
-    kv_sb, kv_sh, kv_st, _ = pools(k_pool, v_pool, fn)
+    kv_sb, kv_sh, kv_st = pools(k_pool, v_pool, fn)
     num_blocks, Hkv, block_size, Dk = ps
     if Dk != D or Hkv < 1 or Hq % Hkv:
         raise ValueError(f"{fn}: q {tuple(qs)}, pools {tuple(ps)}: head dims differ, or query heads are no multiple of K/V heads")
@@ -127,8 +127,8 @@ def _attend(fn, q, k_pool, v_pool, block_tables, context_lens, cu_seqlens, max_n
     args = _ARGS.pack(
         q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), cu_at, prefix_at,
         shared_at, slopes_at, out.data_ptr(), _DT[dt] if dt in _DT else dt_code(dt, fn), q_st, q_sh if q_sh > D else D,
-        Hq * D, D, kv_sb, kv_sh if kv_sh > D else D, kv_st if kv_st > D else D, block_tables.stride(0), num_blocks, n, T, Hkv,
-        Hq // Hkv, D, block_size, block_tables.shape[1], window if window < 0x7FFFFFFF else 0x7FFFFFFF, prefix_len, shared_blocks,
+        Hq * D, D, kv_sb, kv_sh, kv_st, block_tables.stride(0), num_blocks, n, T, Hkv, Hq // Hkv, D, block_size,
+        block_tables.shape[1], window if window < 0x7FFFFFFF else 0x7FFFFFFF, prefix_len, shared_blocks,
         max_new or 0, D ** -0.5 if scale is None else scale, softcap)
     L = kernels.lib()
     need = L.mlsx_paged_attention_ws(args)
@@ -149,7 +149,8 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     """Attention of q [T, Hq, D] over the cached keys and values of each row's sequence; [T, Hq, D].
 
     k_pool / v_pool [num_blocks, Hkv, block_size, D] of q's type, Hq a multiple of Hkv (query head h reads
-    K/V head h // (Hq / Hkv)), any strides with 1 for the last dimension. Sequence s holds rows
+    K/V head h // (Hq / Hkv)), any strides with 1 for the last dimension, also 0 for heads, tokens or blocks (an expanded
+    view: what they share is read for each). Sequence s holds rows
     cu_seqlens[s] .. cu_seqlens[s + 1] (int32 [n + 1]; None: row s), the newest tokens of its
     context_lens[s] cached ones (written before, as by kernels.paged_kv.paged_kv_append); token j of it is
     slot j % block_size of block block_tables[s, j // block_size]. max_new: the longest sequence's rows where the

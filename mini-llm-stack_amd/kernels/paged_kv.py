@@ -29,18 +29,35 @@ def int32(t: torch.Tensor, name: str, fn: str, shape: tuple) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def pools(k_pool: torch.Tensor, v_pool: torch.Tensor, fn: str) -> tuple:
-    """Strides of the pools, which are read and written in place: never copied."""
+def pools(k_pool: torch.Tensor, v_pool: torch.Tensor, fn: str, write: bool = False) -> tuple:
+    """Strides (block, head, token) of the pools, which are read and written in place: never copied. A dimension of size 1
+    counts as dense. Heads or tokens of stride 0 (expanded views) can be read, not written."""
     ps = k_pool.shape
     if len(ps) != 4 or v_pool.shape != ps or v_pool.dtype != k_pool.dtype:
         raise ValueError(f"{fn}: pools {tuple(k_pool.shape)} {k_pool.dtype} / {tuple(v_pool.shape)} {v_pool.dtype}: expected "
                          f"two of one shape [num_blocks, kv_heads, block_size, head_dim] and type")
-    if ps[2] < 1:
+    _, heads, tokens, D = ps
+    if tokens < 1:
         raise ValueError(f"{fn}: blocks of no tokens")
     st = k_pool.stride()
-    if v_pool.stride() != st or st[3] != 1 and k_pool.shape[3] > 1:
+    sb, sh, sw, inner = st
+    if v_pool.stride() != st or inner != 1 and D > 1:
         raise ValueError(f"{fn}: pools need the same strides, 1 for the last dimension, got {st} / {v_pool.stride()}")
-    return st
+    if heads == 1:
+        sh = D
+    if tokens == 1:
+        sw = D
+    if sh < D and sh or sw < D and sw:
+        raise ValueError(f"{fn}: pools of strides {st}: heads or tokens overlap within head dims of {D}")
+    if write and not (sh and sw and (sh >= sw * (tokens - 1) + D or sw >= sh * (heads - 1) + D)
+                      and sb >= sh * (heads - 1) + sw * (tokens - 1) + D):
+        end = 1  # (another order of the dimensions, or elements that share memory)
+        for step, size in sorted((t, n) for t, n in zip(st, ps) if n > 1):
+            if step < end:
+                raise ValueError(f"{fn}: pools of shape {tuple(ps)} and strides {st} share memory between elements: they can "
+                                 f"be read, not written")
+            end += step * (size - 1)
+    return sb, sh, sw
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # (a device index's current stream, as kernels._hip.stream)
@@ -79,7 +96,8 @@ def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_
     Sequence s holds rows cu_seqlens[s] .. cu_seqlens[s + 1] (int32 [n + 1]; None: row s); its last row is
     at position context_lens[s] - 1 (the new tokens counted). A row at position p goes to slot
     p % block_size of block block_tables[s, p // block_size]. Positions outside the table and block ids
-    outside the pool store nothing; rows of no sequence store nothing, and their q comes out as zeros.
+    outside the pool store nothing; rows of no sequence store nothing, and their rotated q is zeros. Pools have any
+    strides, 1 for the last dimension, and no two elements in one place.
 
     rope: float32 [positions, rot], the cosines of a position's rot / 2 angles, then their sines; the
     first rot elements of each head are rotated, in pairs x[j], x[j + rot / 2], or, interleaved, x[2 j],
@@ -91,7 +109,7 @@ def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_
     if len(ks) != 3 or v.shape != ks:
         raise ValueError(f"{fn}: k {tuple(ks)}, v {tuple(v.shape)}: expected two [tokens, kv_heads, head_dim]")
     T, Hkv, D = ks
-    kv_sb, kv_sh, kv_st, _ = pools(k_pool, v_pool, fn)
+    kv_sb, kv_sh, kv_st = pools(k_pool, v_pool, fn, write=True)
     num_blocks, Hp, block_size, Dp = ps
     if Hp != Hkv or Dp != D:
         raise ValueError(f"{fn}: k {tuple(ks)}, pools {tuple(ps)}: heads or head dims differ")
@@ -149,9 +167,9 @@ def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_
     rc = kernels.lib().mlsx_paged_append(_ARGS.pack(
         q_at, k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out_at, block_tables.data_ptr(),
         context_lens.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(), rope.data_ptr() if rot else 0,
-        _DT[dt] if dt in _DT else dt_code(dt, fn), q_st, q_sh, k_st, k_sh, v_st, v_sh, kv_sb, kv_sh if kv_sh > D else D,
-        kv_st if kv_st > D else D, block_tables.stride(0), rope_ld, num_blocks, n, T, Hq, Hkv, D, block_size,
-        block_tables.shape[1], positions if rot else 0, rot, interleaved), _raw_stream(dev))
+        _DT[dt] if dt in _DT else dt_code(dt, fn), q_st, q_sh, k_st, k_sh, v_st, v_sh, kv_sb, kv_sh, kv_st,
+        block_tables.stride(0), rope_ld, num_blocks, n, T, Hq, Hkv, D, block_size, block_tables.shape[1], positions if rot else 0, rot,
+        interleaved), _raw_stream(dev))
     if rc:
         kernels.check(rc, fn)
     return out

@@ -9,7 +9,8 @@ import torch
 
 from paged_plain import attention, cache, check, offsets
 
-from kernels.paged_attention import paged_attention
+from kernels.paged_attention import paged_attention, shared_prefix_attention
+from kernels.paged_kv import paged_kv_append
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +54,24 @@ def test_ids_outside_the_pool_in_one_context(dev, dtype, new):
         tab.copy_(good)
         tab[0, at] = -1 - at
         check(paged_attention(q, kp, vp, tab, ctx, offsets([new])), *attention(q, kp, vp, tab, lens, [new]), f"{at}")
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 64), (HF, 50)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [30, 200, 2]])
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_expanded_pools(dev, dtype, D, new, dim):
+    """One block, head or token seen as several: read as the copy of the view is, and not written."""
+    lens = [90, 333, 5]
+    kp, vp, tab, ctx = cache(lens, 4, D, 16, dtype, 33)
+    kp, vp = (t.narrow(dim, 0, 1).contiguous().expand(t.shape) for t in (kp, vp))  # (the last block's reads end at the storage's end)
+    q = _q(sum(new), 8, D, dtype)
+    cu = offsets(new) if max(new) > 1 else None
+    check(paged_attention(q, kp, vp, tab, ctx, cu), *attention(q, kp, vp, tab, lens, new))
+    if cu is None:
+        pre = tab[1, :20].contiguous()
+        check(shared_prefix_attention(q, kp, vp, pre, 300, tab, ctx), *attention(q, kp, vp, tab, lens, shared=pre, shared_len=300))
+    k = _q(sum(new), 4, D, dtype)
+    before = kp.clone()
+    with pytest.raises(ValueError, match="share memory"):
+        paged_kv_append(q, k, k.clone(), kp, vp, tab, ctx, cu)
+    assert torch.equal(kp, before)

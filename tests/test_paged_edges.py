@@ -1,0 +1,100 @@
+"""What the paged serving wrappers hand to the C entries at the edges of what they take, on CPU tensors: the entries are
+replaced by ones that keep the packed arguments, and nothing is launched."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import kernels
+from kernels import paged_attention as attention_mod, paged_kv as append_mod
+from kernels.paged_attention import paged_attention
+from kernels.paged_kv import paged_kv_append
+from test_paged_refusals import APPEND, ATTEND, _c_attend
+
+I, BF = torch.int32, torch.bfloat16
+
+
+@pytest.fixture
+def packed(monkeypatch):
+    """The fields of the last call of an entry, by name."""
+    seen = {}
+
+    class Library:
+        def mlsx_paged_attention_ws(self, args):
+            return 0
+
+        def mlsx_paged_attention(self, args, *_):
+            seen.update(zip(ATTEND, attention_mod._ARGS.unpack(args)))
+            return 0
+
+        def mlsx_paged_append(self, args, *_):
+            seen.update(zip(APPEND, append_mod._ARGS.unpack(args)))
+            return 0
+
+    monkeypatch.setattr(kernels, "lib", lambda: Library())
+    for mod in (attention_mod, append_mod):
+        monkeypatch.setattr(mod, "one_device", lambda fn, *tensors: 0)
+        monkeypatch.setattr(mod, "_raw_stream", lambda index: 0)
+    return seen
+
+
+def _call(kp, vp, heads, write, dtype=BF):
+    n, D = 4, kp.shape[3]
+    tab, lens = torch.zeros(n, 3, dtype=I), torch.ones(n, dtype=I)
+    if write:
+        k = torch.zeros(n, kp.shape[1], D, dtype=dtype)
+        return paged_kv_append(None, k, k.clone(), kp, vp, tab, lens)
+    return paged_attention(torch.zeros(n, heads, D, dtype=dtype), kp, vp, tab, lens)
+
+
+def _pair(make):
+    return make(), make()
+
+
+READ_ONLY = [  # views whose elements share memory, with their strides
+    (lambda: torch.zeros(8, 1, 16, 64, dtype=BF).expand(-1, 4, -1, -1), (1024, 0, 64)),
+    (lambda: torch.zeros(8, 4, 1, 64, dtype=BF).expand(-1, -1, 16, -1), (256, 64, 0)),
+    (lambda: torch.zeros(1, 4, 16, 64, dtype=BF).expand(8, -1, -1, -1), (0, 1024, 64)),
+    (lambda: torch.zeros(99999, dtype=BF).as_strided((8, 4, 16, 64), (1024, 256, 64, 1)), (1024, 256, 64)),
+]
+
+
+@pytest.mark.parametrize("make,strides", READ_ONLY)
+def test_views_that_share_memory_are_read_with_their_strides(packed, make, strides):
+    _call(*_pair(make), 4, False)
+    assert tuple(packed[f] for f in ("kv_sb", "kv_sh", "kv_st")) == strides
+
+
+@pytest.mark.parametrize("make,strides", READ_ONLY)
+def test_views_that_share_memory_are_not_written(packed, make, strides):
+    with pytest.raises(ValueError, match="share memory"):
+        _call(*_pair(make), 4, True)
+    assert not packed
+
+
+@pytest.mark.parametrize("write", [False, True])
+@pytest.mark.parametrize("strides", [(1024, 256, 32, 1), (4096, 32, 128, 1)])
+def test_rows_that_overlap_are_refused(packed, write, strides):
+    with pytest.raises(ValueError):
+        _call(*_pair(lambda: torch.zeros(99999, dtype=BF).as_strided((8, 4, 16, 64), strides)), 4, write)
+    assert not packed
+
+
+@pytest.mark.parametrize("write", [False, True])
+@pytest.mark.parametrize("make,strides", [
+    (lambda: torch.zeros(8, 16, 4, 64, dtype=BF).transpose(1, 2), (4096, 64, 256)),  # token-major
+    (lambda: torch.zeros(4, 8, 16, 64, dtype=BF).transpose(0, 1), (1024, 8192, 64)),  # a head at a time
+    (lambda: torch.zeros(8, 2, 4, 16, 64, dtype=BF)[:, 1], (8192, 1024, 64)),  # K and V of a block side by side
+    (lambda: torch.zeros(8, 1, 16, 64, dtype=BF).as_strided((8, 1, 16, 64), (1024, 3, 64, 1)), (1024, 64, 64)),  # one head: its
+    (lambda: torch.zeros(8, 4, 1, 64, dtype=BF).as_strided((8, 4, 1, 64), (256, 64, 0, 1)), (256, 64, 64)),  # .. stride is none
+])
+def test_orders_of_a_pool(packed, write, make, strides):
+    _call(*_pair(make), 4, write)
+    assert tuple(packed[f] for f in ("kv_sb", "kv_sh", "kv_st")) == strides
+
+
+def test_c_attention_takes_shared_heads_and_tokens():
+    for over in (dict(kv_sh=0), dict(kv_st=0), dict(kv_sb=0)):
+        rc, need = _c_attend(**over)  # (past the checks of strides: a workspace is missing)
+        assert rc == kernels.MLS_ERR_ARG and need > 0
