@@ -51,8 +51,9 @@ int mlsx_paged_attention_decode(const void* q, int q_dt, int64_t q_ss, int64_t q
  * bytes. q and out: [tokens][kv_heads * group][head_dim], inner stride 1; pools [num_blocks]
  * [kv_heads][block_size][head_dim], inner stride 1, K and V with one set of strides (of heads and
  * tokens head_dim or more, or 0: all of them in one place); all of type dt. Sequence s has the rows
- * cu_seqlens[s] .. cu_seqlens[s + 1] (null: row s), context_lens[s] - 1 the position of its last row. Rows of no sequence get zeros. A block
- * id outside the pool holds no keys. With prefix_blocks, the prefix_len keys in those
+ * cu_seqlens[s] .. cu_seqlens[s + 1] (null: row s), context_lens[s] - 1 the position of its last
+ * row. (Offsets that do not rise leave rows undefined, and nothing else.) Rows of no sequence get
+ * zeros. A block id outside the pool holds no keys. With prefix_blocks, the prefix_len keys in those
  * prefix_count blocks come before every sequence's own (one row each), whose positions
  * count from there. max_new: the longest sequence's rows if known (0: not), which only chooses
  * kernels. The 16-byte aligned workspace holds mlsx_paged_attention_ws floats (0: none). */

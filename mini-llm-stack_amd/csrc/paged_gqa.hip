@@ -40,7 +40,8 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const GqaArgs a) {
   const int Hq = a.Hkv * a.group;
   const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (item >= (int64_t)a.T * Hq) return;
-  const int live = a.piece0 + __builtin_amdgcn_readfirstlane(a.ws_live[item]);
+  // (where offsets do not rise, no tile may have held the row: its count is whatever the workspace held)
+  const int live = a.piece0 + min(max(__builtin_amdgcn_readfirstlane(a.ws_live[item]), 1), a.pieces - a.piece0);
   const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + item * a.pieces;
   const float2 x = ml[min(lane, live - 1)];
   if (live == 1) return;  // written by its only piece

@@ -136,11 +136,15 @@ __device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int 
   p.pfx = real && a.prefix ? a.prefix[seq] : 0;
   p.table = a.bt + (a.shared || !real ? 0 : seq * a.bt_ss);
   p.rows = ntok * a.group;
-  p.row0 = rt << a.bm_log;
   p.live = p.tiles = p.per = 0;
   p.klo = p.khi = p.lo = 0;
   p.direct = false;
-  if (p.row0 >= p.rows) return p;
+  // (offsets that do not rise can lead the search to a sequence that begins behind the slot: rt < 0)
+  if (rt < 0 || ((int64_t)rt << a.bm_log) >= p.rows) {
+    p.row0 = p.rows = 0;
+    return p;
+  }
+  p.row0 = rt << a.bm_log;
   const int first = p.row0 / a.group, last = (min(p.row0 + (1 << a.bm_log), p.rows) - 1) / a.group;
   int pmin, pmax;
   if (a.shared) {

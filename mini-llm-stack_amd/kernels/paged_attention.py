@@ -153,7 +153,8 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     view: what they share is read for each). Sequence s holds rows
     cu_seqlens[s] .. cu_seqlens[s + 1] (int32 [n + 1]; None: row s), the newest tokens of its
     context_lens[s] cached ones (written before, as by kernels.paged_kv.paged_kv_append); token j of it is
-    slot j % block_size of block block_tables[s, j // block_size]. max_new: the longest sequence's rows where the
+    slot j % block_size of block block_tables[s, j // block_size]. Offsets rise; where they do not, rows are
+    undefined, but no memory besides is touched. max_new: the longest sequence's rows where the
     caller knows them; it only chooses between kernels.
 
     The row at position p sees token j when j <= p or j < prefix_lens[s] (int32 [n]), and, with a window, when

@@ -9,7 +9,9 @@ import torch
 
 from paged_plain import attention, cache, check, offsets
 
-from kernels.paged_attention import paged_attention, shared_prefix_attention
+import kernels
+from kernels._hip import stream
+from kernels.paged_attention import _ARGS, paged_attention, shared_prefix_attention
 from kernels.paged_kv import paged_kv_append
 
 pytestmark = pytest.mark.gpu
@@ -75,3 +77,28 @@ def test_expanded_pools(dev, dtype, D, new, dim):
     with pytest.raises(ValueError, match="share memory"):
         paged_kv_append(q, k, k.clone(), kp, vp, tab, ctx, cu)
     assert torch.equal(kp, before)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 64)])
+@pytest.mark.parametrize("cu", [[0, 100, 0, 0], [0, 4000, 0, 0], [50, 10, 90, 20], [4000, 3000, 2000, 0], [-5, 9999, 3, 4001],
+                                [3999] * 900 + [0] + [4000] * 900])
+@pytest.mark.parametrize("max_new", [1, 40, 4000])
+def test_offsets_that_do_not_rise(dev, dtype, D, cu, max_new):
+    """Rows are undefined then, but outputs and workspace end where they end, and counts that no tile wrote bound the join."""
+    T, H, kvh, guard = 4000, 4, 2, 1 << 16
+    n = len(cu) - 1
+    kp, vp, tab, ctx = cache([900] * min(n, 3), kvh, D, 16, dtype, 34)
+    tab, ctx = (t.repeat(-(-n // 3), *[1] * (t.dim() - 1))[:n].contiguous() for t in (tab, ctx))
+    q = _q(T, H, D, dtype)
+    off = torch.tensor(cu, dtype=torch.int32, device=dev)
+    big = torch.full((T * H * D + 2 * guard,), 3.0, dtype=dtype, device=dev)
+    out = big[guard:-guard]
+    args = _ARGS.pack(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), tab.data_ptr(), ctx.data_ptr(), off.data_ptr(), 0, 0, 0,
+                      out.data_ptr(), {BF: kernels.MLS_BF16, FP: kernels.MLS_F32}[dtype], H * D, D, H * D, D, *kp.stride()[:3],
+                      tab.stride(0), kp.shape[0], n, T, kvh, H // kvh, D, 16, tab.shape[1], 0, 0, 0, max_new, D ** -0.5, 0.0)
+    need = kernels.lib().mlsx_paged_attention_ws(args)
+    work = torch.full((need + 2 * guard,), 0x7F7F7F7F, dtype=torch.int32, device=dev)  # a count far past every record
+    kernels.check(kernels.lib().mlsx_paged_attention(args, work[guard:].data_ptr(), need, stream(q.device)), "mlsx_paged_attention")
+    torch.cuda.synchronize()
+    for t, value in ((big, 3.0), (work, 0x7F7F7F7F)):
+        assert bool((t[:guard] == value).all()) and bool((t[-guard:] == value).all())
