@@ -210,6 +210,7 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   pre.a.pieces = (int)pieces;
   if (slots > 0x3FFFFFFF || own.blocks > 0x7FFFFFFF || pre.blocks > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "%s: too large", fn);
   need = pieces > 1 ? rows * (pieces * (a.DW + 2) + 1) : 0;
+  if (need == 0) ws = nullptr;  // (one piece writes no records and no counts, also where a workspace is given)
   own.a.ws = pre.a.ws = ws;
   own.a.ws_ml = pre.a.ws_ml = ws ? ws + rows * pieces * a.DW : nullptr;
   own.a.ws_live = ws ? reinterpret_cast<int32_t*>(ws + rows * pieces * (a.DW + 2)) : nullptr;

@@ -102,3 +102,22 @@ def test_offsets_that_do_not_rise(dev, dtype, D, cu, max_new):
     torch.cuda.synchronize()
     for t, value in ((big, 3.0), (work, 0x7F7F7F7F)):
         assert bool((t[:guard] == value).all()) and bool((t[-guard:] == value).all())
+
+
+@pytest.mark.parametrize("dtype,D,cu", [(BF, 128, None), (FP, 64, None), (BF, 128, [0, 300, 500]), (HF, 256, [0, 100, 200])])
+def test_a_workspace_that_is_not_needed(dev, dtype, D, cu):
+    """A call of one piece writes nothing into a workspace that it is given all the same."""
+    lens = [1] * 2000 if cu is None else [300, 200]
+    kp, vp, tab, ctx = cache(lens, 2, D, 16, dtype, 37)
+    T, n = (len(lens), len(lens)) if cu is None else (cu[-1], 2)
+    q, off = _q(T, 8, D, dtype), None if cu is None else torch.tensor(cu, dtype=torch.int32, device=dev)
+    out = torch.empty_like(q)
+    args = _ARGS.pack(q.data_ptr(), kp.data_ptr(), vp.data_ptr(), tab.data_ptr(), ctx.data_ptr(), 0 if cu is None else off.data_ptr(), 0, 0,
+                      0, out.data_ptr(), {BF: kernels.MLS_BF16, HF: kernels.MLS_F16, FP: kernels.MLS_F32}[dtype], 8 * D, D, 8 * D, D,
+                      *kp.stride()[:3], tab.stride(0), kp.shape[0], n, T, 2, 4, D, 16, 1 if cu is None else 2, 0, 0, 0, T, D ** -0.5, 0.0)
+    assert kernels.lib().mlsx_paged_attention_ws(args) == 0
+    work = torch.full((T * 8 * (2 * D + 5),), 7, dtype=torch.int32, device=dev)  # room for what a piece's records would take
+    kernels.check(kernels.lib().mlsx_paged_attention(args, work.data_ptr(), work.numel(), stream(q.device)), "mlsx_paged_attention")
+    assert bool((work == 7).all())
+    new = None if cu is None else [cu[1], cu[2] - cu[1]]
+    check(out, *attention(q, kp, vp, tab[:, :1 if cu is None else 2], lens, new))
