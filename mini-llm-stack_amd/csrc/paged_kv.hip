@@ -185,6 +185,7 @@ extern "C" int mlsx_paged_append(const mlsx_paged_append_args* p, mls_stream_t s
     return fail(MLS_ERR_ARG, "%s: null pointer", fn);
   if (!p->cu_seqlens && p->tokens != p->n_seqs)
     return fail(MLS_ERR_ARG, "%s: %lld rows for %lld sequences of one", fn, (long long)p->tokens, (long long)p->n_seqs);
+  if (!p->rope && p->rot > 0) return fail(MLS_ERR_ARG, "%s: %lld rotated elements without a table", fn, (long long)p->rot);
   if (p->rope && (p->rot < 0 || p->rot % 2 != 0 || p->rot > p->head_dim || p->rope_ld < p->rot))
     return fail(MLS_ERR_ARG, "%s: %lld rotated elements of %lld, table rows of %lld", fn, (long long)p->rot,
                 (long long)p->head_dim, (long long)p->rope_ld);

@@ -129,6 +129,8 @@ def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_
         positions, rot = rope.shape
         if rot % 2 or rot > D:
             raise ValueError(f"{fn}: rope rotates {rot} of {D} elements: an even number up to the head dim is needed")
+        if not positions and rot:
+            rope = rope.new_empty(1, rot)  # (an address: that of no elements is null. No row of it counts)
         rope_ld, inner = rope.stride()
         if inner != 1 or rope_ld < rot:
             rope = rope.contiguous()

@@ -13,6 +13,7 @@ import kernels
 from kernels._hip import stream
 from kernels.paged_attention import _ARGS, paged_attention, shared_prefix_attention
 from kernels.paged_kv import paged_kv_append
+from serve.paged_layer import PagedAttentionLayer, rope_table
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +122,30 @@ def test_a_workspace_that_is_not_needed(dev, dtype, D, cu):
     assert bool((work == 7).all())
     new = None if cu is None else [cu[1], cu[2] - cu[1]]
     check(out, *attention(q, kp, vp, tab[:, :1 if cu is None else 2], lens, new))
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rot", [64, 32])
+def test_a_rotation_table_without_rows(dev, dtype, interleaved, rot):
+    """Every position is outside it: NaN in the rotated elements of q and k, the others and v as they are."""
+    lens = [3, 20]
+    kp, vp, tab, ctx = cache(lens, 2, 64, 16, dtype, 35)
+    q, k, v = _q(2, 4, 64, dtype, 1), _q(2, 2, 64, dtype, 2), _q(2, 2, 64, dtype, 3)
+    table = torch.zeros(9, rot, device=dev)[9:]
+    kw, vw = kp.clone(), vp.clone()
+    y = paged_kv_append(q, k, v, kp, vp, tab, ctx, rope=table, interleaved=interleaved)
+    for s, n in enumerate(lens):
+        at = int(tab[s, (n - 1) // 16]), slice(None), (n - 1) % 16
+        kw[at], vw[at] = k[s], v[s]
+        kw[at][:, :rot] = float("nan")
+    want = q.clone()
+    want[..., :rot] = float("nan")
+    for a, b in ((y, want), (kp, kw), (vp, vw)):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+def test_layer_behind_a_prefix_as_long_as_its_table(dev):
+    mods = [torch.nn.Linear(128, n, bias=False, device=dev) for n in (256, 128, 128)] + [torch.nn.Linear(256, 128, bias=False, device=dev)]
+    layer = PagedAttentionLayer(*mods, head_dim=64, rope=rope_table(32, 64, device=dev))
+    kp, vp, tab, ctx = cache([1, 1, 32], 2, 64, 16, FP, 36)
+    y = layer(torch.randn(2, 128, device=dev), kp, vp, tab[:2], ctx[:2], prefix=(tab[2].contiguous(), 32))
+    assert bool(y.isnan().all())

@@ -98,3 +98,19 @@ def test_c_attention_takes_shared_heads_and_tokens():
     for over in (dict(kv_sh=0), dict(kv_st=0), dict(kv_sb=0)):
         rc, need = _c_attend(**over)  # (past the checks of strides: a workspace is missing)
         assert rc == kernels.MLS_ERR_ARG and need > 0
+
+
+@pytest.mark.parametrize("table", [torch.zeros(9, 64)[9:], torch.zeros(0, 32), torch.zeros(9, 128)[9:, ::2]])
+def test_a_rotation_table_without_rows_is_one(packed, table):
+    z = lambda *s: torch.zeros(*s, dtype=BF)
+    paged_kv_append(z(4, 4, 64), z(4, 2, 64), z(4, 2, 64), z(8, 2, 16, 64), z(8, 2, 16, 64), torch.zeros(4, 3, dtype=I),
+                    torch.ones(4, dtype=I), rope=table)
+    assert packed["rope"] != 0 and packed["rot"] == packed["rope_ld"] == table.shape[1] and packed["rope_rows"] == 0
+    assert packed["q"] != 0 and packed["q_out"] != 0
+
+
+def test_c_append_rejects_rotation_without_a_table():
+    a = dict.fromkeys(APPEND, 64) | dict(cu_seqlens=0, rope=0, dt=kernels.MLS_BF16, num_blocks=8, n_seqs=2, tokens=2, heads=4, kv_heads=2,
+                                         block_size=16, max_blocks=3, rope_rows=0, interleaved=0)
+    rc = kernels.lib().mlsx_paged_append(append_mod._ARGS.pack(*(a[f] for f in APPEND)), None)
+    assert rc == kernels.MLS_ERR_ARG and b"without a table" in kernels.lib().mls_last_error()
