@@ -19,12 +19,15 @@ _ARGS = struct.Struct("=10Q23q")  # mlsx_paged_append_args
 
 
 def int32(t: torch.Tensor, name: str, fn: str, shape: tuple) -> torch.Tensor:
-    """An index tensor of the given shape (None: any size) as int32 with unit inner stride."""
+    """An index tensor of the given shape (None: any size) as int32 with unit inner stride; what does not fit becomes the
+    nearest value, which is no block id and past every table."""
     if t.dim() != len(shape) or any(w is not None and w != s for w, s in zip(shape, t.shape)):
         raise ValueError(f"{fn}: {name} {tuple(t.shape)}, expected {tuple('any' if w is None else w for w in shape)}")
     if t.dtype != torch.int32:
         if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
             raise TypeError(f"{fn}: {name} must hold integers, got {t.dtype}")
+        if t.dtype in (torch.int64, torch.uint64, torch.uint32):
+            t = t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
         t = t.to(torch.int32)
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 

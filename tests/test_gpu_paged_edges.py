@@ -122,6 +122,8 @@ def test_a_workspace_that_is_not_needed(dev, dtype, D, cu):
     assert bool((work == 7).all())
     new = None if cu is None else [cu[1], cu[2] - cu[1]]
     check(out, *attention(q, kp, vp, tab[:, :1 if cu is None else 2], lens, new))
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("rot", [64, 32])
@@ -149,3 +151,16 @@ def test_layer_behind_a_prefix_as_long_as_its_table(dev):
     kp, vp, tab, ctx = cache([1, 1, 32], 2, 64, 16, FP, 36)
     y = layer(torch.randn(2, 128, device=dev), kp, vp, tab[:2], ctx[:2], prefix=(tab[2].contiguous(), 32))
     assert bool(y.isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint32])
+def test_indexes_wider_than_the_kernels(dev, dtype):
+    """Ids whose low 32 bits are an id of the pool hold no tokens."""
+    lens = [70, 200]
+    kp, vp, tab, ctx = cache(lens, 2, 64, 16, FP, 38)
+    q = _q(2, 4, 64, FP)
+    wide = tab.clamp(min=0).to(torch.int64)
+    wide[0, 1], wide[1, 3] = (2 ** 32 + int(tab[0, 1]), -2 ** 33 + int(tab[1, 3])) if dtype == torch.int64 else (2 ** 31 + 1, 2 ** 32 - 1)
+    tab[0, 1] = tab[1, 3] = -1
+    y = paged_attention(q, kp, vp, wide.to(dtype), ctx.to(dtype))
+    check(y, *attention(q, kp, vp, tab, lens))

@@ -114,3 +114,12 @@ def test_c_append_rejects_rotation_without_a_table():
                                          block_size=16, max_blocks=3, rope_rows=0, interleaved=0)
     rc = kernels.lib().mlsx_paged_append(append_mod._ARGS.pack(*(a[f] for f in APPEND)), None)
     assert rc == kernels.MLS_ERR_ARG and b"without a table" in kernels.lib().mls_last_error()
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8, torch.uint32, torch.uint64])
+def test_indexes_of_any_width(dtype):
+    """What int32 cannot hold stays outside every pool and table: its low bits could be an id of one."""
+    values = [0, 5, 100] + ([-1, -128] if dtype.is_signed else []) + {4: [2 ** 31 - 1], 8: [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5]}.get(dtype.itemsize, [])
+    values += [2 ** 31, 2 ** 32 - 1] if dtype == torch.uint32 else [-2 ** 33 + 5, -2 ** 32] if dtype == torch.int64 else []
+    got = append_mod.int32(torch.tensor(values, dtype=dtype), "block_tables", "f", (None,))
+    assert got.dtype == I and got.tolist() == [min(max(v, -2 ** 31), 2 ** 31 - 1) for v in values]
