@@ -117,6 +117,16 @@ __device__ __forceinline__ int gqa_piece(const GqaArgs& a, int lane) {
   return __builtin_amdgcn_readfirstlane(max(max(want, (most + a.splits - 1) / a.splits), a.least));
 }
 
+// First key within the window of a row at `pos` (which may be far below 0, and the window up to 2^31 - 1)
+__device__ __forceinline__ int gqa_window_from(const GqaArgs& a, int pos) {
+  return a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
+}
+
+// Shared: the position of sequence s's row, behind the prefix; at most 2^31 - 2, for any length
+__device__ __forceinline__ int gqa_shared_pos(const GqaArgs& a, int s) {
+  return (int)min((uint32_t)a.front + (uint32_t)max(a.lens[s], 0), 0x7FFFFFFFu) - 1;
+}
+
 // Row tile rt of sequence seq (-1 and n: rows that no sequence holds, which see nothing), for its piece `split`.
 __device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int rt, int split, int lane) {
   GqaPlan p;
@@ -151,7 +161,7 @@ __device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int 
     pmin = 0x7FFFFFFF;
     pmax = a.front - 1;
     if (a.window > 0) {
-      for (int t = first + lane; t <= last; t += 64) pmin = min(pmin, a.front + max(a.lens[t], 0) - 1);
+      for (int t = first + lane; t <= last; t += 64) pmin = min(pmin, gqa_shared_pos(a, t));
 #pragma unroll
       for (int off = 32; off >= 1; off >>= 1) pmin = min(pmin, __shfl_xor(pmin, off, 64));
     }
@@ -160,7 +170,7 @@ __device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int 
     pmax = p.pos0 + last;
   }
   p.khi = __builtin_amdgcn_readfirstlane(min(max(pmax + 1, p.pfx), p.len));
-  p.klo = __builtin_amdgcn_readfirstlane(a.window > 0 ? max(0, pmin - a.window + 1) : 0);
+  p.klo = __builtin_amdgcn_readfirstlane(gqa_window_from(a, pmin));
   p.lo = p.klo >> a.bn_log << a.bn_log;
   p.tiles = p.khi > p.klo ? (int)(((uint32_t)(p.khi - p.lo) + (1u << a.bn_log) - 1) >> a.bn_log) : 0;
   if (a.shared) {
@@ -196,9 +206,9 @@ __device__ __forceinline__ GqaPlan gqa_block_plan(const GqaArgs& a, int block, i
 
 // The keys [lo, hi) that the row of token `tok` sees, and its position.
 __device__ __forceinline__ void gqa_row_range(const GqaArgs& a, const GqaPlan& p, int tok, int& lo, int& hi, int& pos) {
-  pos = a.shared ? a.front + max(a.lens[tok], 0) - 1 : p.pos0 + (tok - p.tok0);
+  pos = a.shared ? gqa_shared_pos(a, tok) : p.pos0 + (tok - p.tok0);
   hi = min(max(pos + 1, p.pfx), p.len);
-  lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  lo = gqa_window_from(a, pos);
 }
 
 // Over the packed rows r0 .. r1 (none where r1 < r0) of one sequence, or of shared rows: the extremes

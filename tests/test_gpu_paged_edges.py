@@ -164,3 +164,28 @@ def test_indexes_wider_than_the_kernels(dev, dtype):
     tab[0, 1] = tab[1, 3] = -1
     y = paged_attention(q, kp, vp, wide.to(dtype), ctx.to(dtype))
     check(y, *attention(q, kp, vp, tab, lens))
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 64), (HF, 80)])
+@pytest.mark.parametrize("new", [[40, 5, 9], [200, 3, 130]])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 40, 2 ** 31 - 30])
+def test_windows_of_any_size(dev, dtype, D, new, window):
+    """Rows far below position 0 (fewer cached tokens than rows), with a window as wide as can be said."""
+    lens = [25, 0, 5]
+    kp, vp, tab, ctx = cache(lens, 2, D, 16, dtype, 39)
+    q = _q(sum(new), 4, D, dtype)
+    for pl in (None, torch.tensor([9, 3, 4], dtype=torch.int32, device=dev)):
+        y = paged_attention(q, kp, vp, tab, ctx, offsets(new), window=window, prefix_lens=pl)
+        check(y, *attention(q, kp, vp, tab, lens, new, window=window, prefix_lens=pl))
+
+
+@pytest.mark.parametrize("window", [0, 50, 2 ** 40])
+@pytest.mark.parametrize("shared", [300, 5])
+def test_lengths_near_2_31_behind_a_prefix(dev, window, shared):
+    """A context past its table is cut there, and its position counts as it is, also where the prefix carries it past 2^31."""
+    kp, vp, tab, ctx = cache([40, 33, 2, 300], 2, 64, 16, BF, 40)
+    pre, tab, ctx = tab[3, :-(-shared // 16)].contiguous(), tab[:3, :3].contiguous(), ctx[:3].clone()
+    ctx[0], ctx[2] = 2 ** 31 - 1, 2 ** 31 - 200
+    q = _q(3, 4, 64, BF)
+    y = shared_prefix_attention(q, kp, vp, pre, shared, tab, ctx, window=window)
+    check(y, *attention(q, kp, vp, tab, ctx.tolist(), shared=pre, shared_len=shared, window=window))
