@@ -455,7 +455,16 @@ struct GqaRows {
   // Raw products -> scores in log2 units, with the cap and the bias by distance
   template <int KT>
   __device__ __forceinline__ void scored(const GqaArgs& a, f32x4 (&s)[NT][KT], int j0, int lane) const {
-    if (a.cap > 0.0f) {
+    // 1 - 2 / (e^2y + 1) is off by up to 2^-22 of the cap, for small y too: half as much as rounding a weight to
+    // fp16 leaves, at a cap of 256. Past that, and in fp32, tanh with its relative precision.
+    if (a.cap > 0.0f && (K::F32 || a.cap > 256.0f * 1.44269504f)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][k][i] = tanhf(s[n][k][i] * a.to_cap) * a.cap;
+    } else if (a.cap > 0.0f) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -463,11 +472,7 @@ struct GqaRows {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float y = s[n][k][i] * a.to_cap;  // scale / cap
-            // 1 - 2 / (e^2y + 1) is off by 2^-23 of the cap: too much for fp32 scores only
-            float t;
-            if constexpr (K::F32) t = tanhf(y);
-            else t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * 2.88539008f) + 1.0f);
-            s[n][k][i] = t * a.cap;  // cap log2(e)
+            s[n][k][i] = (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * 2.88539008f) + 1.0f)) * a.cap;  // cap log2(e)
           }
     } else {
 #pragma unroll

@@ -155,8 +155,10 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   a.kv_vec = vec;
   constexpr double LOG2E = 1.4426950408889634;
   a.c = (float)(p->scale * LOG2E);
-  a.cap = (float)(p->softcap * LOG2E);
-  a.to_cap = p->softcap > 0.0 ? (float)(p->scale / p->softcap) : 0.0f;
+  // (a cap is none for scores under 2^-12 of it, in fp32; past 1e30, scale / cap and the cap leave fp32's normal values)
+  const double cap = p->softcap <= 1e30 ? p->softcap : 0.0;
+  a.cap = (float)(cap * LOG2E);
+  a.to_cap = cap > 0.0 ? (float)std::clamp(p->scale / cap, -3e38, 3e38) : 0.0f;
   a.simple = a.cap == 0.0f && !a.slopes && a.c > 0.0f && a.c < 3e38f;
   a.q_vec = D % ce == 0 && p->q_st % ce == 0 && p->q_sh % ce == 0 && aligned(p->q, 16);
   a.o_vec = p->o_st % 4 == 0 && p->o_sh % 4 == 0 && aligned(p->out, 4 * esz);

@@ -189,3 +189,30 @@ def test_lengths_near_2_31_behind_a_prefix(dev, window, shared):
     q = _q(3, 4, 64, BF)
     y = shared_prefix_attention(q, kp, vp, pre, shared, tab, ctx, window=window)
     check(y, *attention(q, kp, vp, tab, ctx.tolist(), shared=pre, shared_len=shared, window=window))
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 64), (FP, 64), (HF, 256)])
+@pytest.mark.parametrize("cap", [257.0, 2e3, 1e4, 1e5, 1e6, 1e8, 9e29, 2e38])
+@pytest.mark.parametrize("lens,new", [([3, 9, 70], None), ([40, 7], [40, 5]), ([300], [200])])
+def test_caps_far_above_the_scores(dev, dtype, D, cap, lens, new):
+    """The cap changes little then, and costs no precision: no term of the cap's size in the bound, only tanh and its two
+    factors, 2^-21 of the largest score (at most the largest |q| |k| times the scale)."""
+    kp, vp, tab, ctx = cache(lens, 2, D, 16, dtype, 41)
+    T = sum(new) if new else len(lens)
+    q = _q(T, 8, D, dtype)
+    want, _ = attention(q, kp, vp, tab, lens, new, softcap=cap)
+    share, bound = attention(q, kp, vp.abs(), tab, lens, new)
+    score = float(q.double().norm(dim=-1).max() * kp.double().norm(dim=-1).max()) * D ** -0.5
+    y = paged_attention(q, kp, vp, tab, ctx, offsets(new) if new else None, softcap=cap)
+    check(y, want, bound + 2 * 2.0 ** -21 * score * share, f"{cap}")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_caps_far_below_the_scores(dev, dtype):
+    """All scores are the cap or its negative, and 0 where a product is 0: the mean of the values, to rounding."""
+    lens = [50]
+    kp, vp, tab, ctx = cache(lens, 1, 64, 16, dtype, 42)
+    kp[int(tab[0, 0]), 0, 3] = 0
+    q = _q(1, 4, 64, dtype)
+    for cap in (1e-6, 1e-30, 1e-40):
+        check(paged_attention(q, kp, vp, tab, ctx, softcap=cap), *attention(q, kp, vp, tab, lens, softcap=cap), f"{cap}")
