@@ -390,15 +390,15 @@ struct GqaRows {
   }
 
   // Scores -> weights (s becomes P), with the row's state rescaled where its reference moves. okmask: the
-  // keys of [j0, j0 + BN) that are there at all.
-  template <int BN>
+  // keys of [j0, j0 + BN) that are there at all. ANYCAP: also caps that need tanh in 16-bit types.
+  template <int BN, bool ANYCAP = true>
   __device__ __forceinline__ void weigh(const GqaArgs& a, f32x4 (&s)[NT][BN / 16], int j0, uint64_t okmask, int lane) {
     constexpr int KT = BN / 16;
     // scores in log2 units: s * cc
     float cc = a.c;
     if (!a.simple) {
       cc = 1.0f;
-      scored<KT>(a, s, j0, gqa_here(lane));
+      scored<KT, ANYCAP>(a, s, j0, gqa_here(lane));
     }
     constexpr uint64_t FULL = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
     if (okmask != FULL || !sees_all(j0, BN)) {
@@ -453,11 +453,9 @@ struct GqaRows {
   }
 
   // Raw products -> scores in log2 units, with the cap and the bias by distance
-  template <int KT>
+  template <int KT, bool ANYCAP>
   __device__ __forceinline__ void scored(const GqaArgs& a, f32x4 (&s)[NT][KT], int j0, int lane) const {
-    // 1 - 2 / (e^2y + 1) is off by up to 2^-22 of the cap, for small y too: half as much as rounding a weight to
-    // fp16 leaves, at a cap of 256. Past that, and in fp32, tanh with its relative precision.
-    if (a.cap > 0.0f && (K::F32 || a.cap > 256.0f * 1.44269504f)) {
+    if (a.cap > 0.0f && (K::F32 || (ANYCAP && gqa_cap_needs_tanh(a)))) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -747,7 +745,7 @@ struct GqaPair {
     });
   }
   __device__ __forceinline__ void soften(const GqaArgs& a, int j0, uint64_t okmask, int lane) {
-    rows.template weigh<BN>(a, s, j0, okmask, lane);
+    rows.template weigh<BN, false>(a, s, j0, okmask, lane);
     uint4 none;
 #pragma unroll
     for (int h = 0; h < BN / 32; ++h)

@@ -101,14 +101,14 @@ struct Pass {
 //   52 against 57; of 96 rows 47 in the paired kernel, 37 in tiles of 64).
 // - fp32: tiles of 128 rows where there are enough to fill the GPU (a step of one takes 3.4 us: 5 prompts of up to 700 tokens, 8 heads of 64,
 //   47 us so, 31 in tiles of 64).
-void choose_shape(GqaShape& s, int64_t rows, int64_t all, int dt, int64_t D, int64_t BS, bool vec) {
+void choose_shape(GqaShape& s, int64_t rows, int64_t all, int dt, int64_t D, int64_t BS, bool vec, bool tanh) {
   s.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
   if (dt == MLS_F32) gqa_tiles<float>(s);
   else gqa_tiles<_Float16>(s);
   vec = vec && BS % s.group_rows == 0;
   s.vec = vec;
   s.keys = vec && rows <= 16;
-  s.pair = vec && !s.keys && dt != MLS_F32 && rows > (s.dp <= 128 ? 128 : 64);
+  s.pair = vec && !s.keys && dt != MLS_F32 && !tanh && rows > (s.dp <= 128 ? 128 : 64);
   s.nt = dt == MLS_F32 && vec && rows > 64 && all >= 128 * 512 ? 2 : 1;
   if (dt == MLS_F32) gqa_tiles<float>(s);
   else gqa_tiles<_Float16>(s);
@@ -167,7 +167,7 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   own.a = a;
   own.s = pre.s = GqaShape{};
   const int64_t most = p->cu_seqlens ? (p->max_new > 0 ? std::min(p->max_new, T) : cdiv(T, std::max<int64_t>(n, 1))) : 1;
-  choose_shape(own.s, most * G, T * G * Hkv, p->dt, D, BS, a.sb_bytes != 0);
+  choose_shape(own.s, most * G, T * G * Hkv, p->dt, D, BS, a.sb_bytes != 0, gqa_cap_needs_tanh(a));
   own.a.bm_log = __builtin_ctz(own.s.bm);
   own.a.bn_log = __builtin_ctz(own.s.bn);
   const int64_t bm = 1ll << own.a.bm_log;
@@ -184,7 +184,7 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   int64_t sp = 0;
   if (shared) {
     pre.a = a;
-    choose_shape(pre.s, n * G, n * G * Hkv, p->dt, D, BS, a.sb_bytes != 0);
+    choose_shape(pre.s, n * G, n * G * Hkv, p->dt, D, BS, a.sb_bytes != 0, gqa_cap_needs_tanh(a));
     pre.a.shared = 1;
     pre.a.front = (int)std::min<int64_t>(p->prefix_len, p->prefix_count * BS);
     pre.a.bt = p->prefix_blocks, pre.a.bt_ss = 0;

@@ -42,6 +42,12 @@ struct GqaArgs {
   int q_vec, o_vec, kv_vec;  // 16-byte accesses of q, 4 elements at once of out, 16-byte ones of the pools
 };
 
+// 16-bit types: 1 - 2 / (e^2y + 1) is off by up to 2^-22, so a score by 2^-22 of the cap, for small scores too: at a cap of
+// 256 a quarter of what rounding a weight to fp16 leaves. Past that the scores take tanhf, precise relative to y, and the
+// paired kernel, which it would slow with any cap (chunks of D = 256, cap 30: 145 us against 138), is not taken (prompt of
+// 8192, cap 300: 1379 us against 1277 there; cap 50: 879).
+__host__ __device__ __forceinline__ bool gqa_cap_needs_tanh(const GqaArgs& a) { return a.cap > 256.0f * 1.44269504f; }
+
 struct GqaShape {
   bool keys, pair, vec;
   int nt, dp, bn, bm;
