@@ -22,6 +22,7 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 import kernels
 from kernels._hip import _DT, dt_code, require_hip, stream
@@ -116,7 +117,7 @@ def _attend(fn, q, k_pool, v_pool, block_tables, context_lens, cu_seqlens, max_n
         raise ValueError(f"{fn}: softcap {softcap}: a positive cap, or 0 for none")
     if window < 0 or max_new is not None and max_new < 0:
         raise ValueError(f"{fn}: window {window}, max_new {max_new}: not negative")
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         no_grad_of(fn, q, k_pool, v_pool, slopes)
     dev = one_device(fn, q, k_pool, v_pool, block_tables, context_lens, cu_seqlens, prefix_lens, prefix_blocks, slopes)
     q_st, q_sh, inner = q.stride()

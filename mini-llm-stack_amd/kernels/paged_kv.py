@@ -11,6 +11,7 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 import kernels
 from kernels._hip import _DT, dt_code, require_hip
@@ -84,10 +85,15 @@ def fresh(like: torch.Tensor, shape: tuple) -> torch.Tensor:
 
 
 def no_grad_of(fn: str, *tensors) -> None:
+    """Refuses tensors that a gradient or a tangent is asked of: the result would silently have none."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{fn} has no gradient: call it under torch.no_grad(), or detach its inputs")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{fn} has no derivative: its inputs must not carry tangents")
 
 
 def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -149,8 +155,8 @@ def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_
             cu_seqlens = int32(cu_seqlens, "cu_seqlens", fn, (n + 1,))
     elif n != T:
         raise ValueError(f"{fn}: {T} rows for {n} sequences: without cu_seqlens, each has one")
-    if torch.is_grad_enabled():
-        no_grad_of(fn, q, k, v, k_pool, v_pool)
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+        no_grad_of(fn, q, k, v, k_pool, v_pool, rope)
     dev = one_device(fn, k, v, k_pool, v_pool, block_tables, context_lens, q, cu_seqlens, rope)
     k_st, k_sh, inner = k.stride()
     if inner != 1 and D > 1:

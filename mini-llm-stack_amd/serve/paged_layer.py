@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 
 from kernels.paged_attention import paged_attention, shared_prefix_attention
-from kernels.paged_kv import paged_kv_append
+from kernels.paged_kv import no_grad_of, paged_kv_append
 from serve.quantize import QuantLinear
 
 
@@ -63,12 +63,17 @@ class PagedAttentionLayer(nn.Module):
             setattr(self, name, QuantLinear(getattr(self, name), bits, group_size))
         return self
 
-    @torch.no_grad()
     def forward(self, x: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,
                 context_lens: torch.Tensor, cu_seqlens: torch.Tensor | None = None, *, max_new: int | None = None,
                 prefix_lens: torch.Tensor | None = None, prefix: tuple[torch.Tensor, int] | None = None) -> torch.Tensor:
         """prefix: (its blocks, its tokens), cached once for all sequences of a decode step; block_tables and
-        context_lens then hold the tokens after it."""
+        context_lens then hold the tokens after it. For serving: the parameters get no gradient, and inputs that ask
+        for one are refused."""
+        no_grad_of("PagedAttentionLayer", x, k_pool, v_pool)
+        with torch.no_grad():
+            return self._forward(x, k_pool, v_pool, block_tables, context_lens, cu_seqlens, max_new, prefix_lens, prefix)
+
+    def _forward(self, x, k_pool, v_pool, block_tables, context_lens, cu_seqlens, max_new, prefix_lens, prefix):
         q, k, v = (w(x).unflatten(-1, (-1, self.head_dim)) for w in (self.wq, self.wk, self.wv))
         rope = self.rope
         if prefix is not None:

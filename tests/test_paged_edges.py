@@ -6,10 +6,13 @@ from __future__ import annotations
 import pytest
 import torch
 
+from torch.autograd import forward_ad
+
 import kernels
 from kernels import paged_attention as attention_mod, paged_kv as append_mod
 from kernels.paged_attention import paged_attention
 from kernels.paged_kv import paged_kv_append
+from serve.paged_layer import PagedAttentionLayer
 from test_paged_refusals import APPEND, ATTEND, _c_attend
 
 I, BF = torch.int32, torch.bfloat16
@@ -123,3 +126,49 @@ def test_indexes_of_any_width(dtype):
     values += [2 ** 31, 2 ** 32 - 1] if dtype == torch.uint32 else [-2 ** 33 + 5, -2 ** 32] if dtype == torch.int64 else []
     got = append_mod.int32(torch.tensor(values, dtype=dtype), "block_tables", "f", (None,))
     assert got.dtype == I and got.tolist() == [min(max(v, -2 ** 31), 2 ** 31 - 1) for v in values]
+
+
+def _inputs():
+    z = lambda *s: torch.randn(*s)
+    return dict(q=z(4, 4, 64), k=z(4, 2, 64), v=z(4, 2, 64), kp=z(8, 2, 16, 64), vp=z(8, 2, 16, 64), rope=z(9, 64), slopes=z(4))
+
+
+def _run(which, a):
+    tab, lens = torch.zeros(4, 3, dtype=I), torch.ones(4, dtype=I)
+    if which == "append":
+        return paged_kv_append(a["q"], a["k"], a["v"], a["kp"], a["vp"], tab, lens, rope=a["rope"])
+    return paged_attention(a["q"], a["kp"], a["vp"], tab, lens, slopes=a["slopes"])
+
+
+@pytest.mark.parametrize("which,name", [("append", n) for n in ("q", "k", "v", "kp", "vp", "rope")] + [("attend", n) for n in ("q", "kp", "vp", "slopes")])
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_tangents_and_gradients_are_refused(packed, which, name, grad_mode):
+    with torch.set_grad_enabled(grad_mode):
+        with forward_ad.dual_level():
+            a = _inputs()
+            a[name] = forward_ad.make_dual(a[name], torch.ones_like(a[name]))
+            with pytest.raises(ValueError, match="tangents"):
+                _run(which, a)
+            _run(which, _inputs())  # (others of the level carry none)
+        if grad_mode:
+            a = _inputs()
+            a[name].requires_grad_()
+            with pytest.raises(ValueError, match="no gradient"):
+                _run(which, a)
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda t: _run(which, {**_inputs(), name: t}), (_inputs()[name],), (_inputs()[name],))
+
+
+def test_layer_refuses_inputs_that_ask_for_a_gradient(packed):
+    mods = [torch.nn.Linear(128, n, bias=False) for n in (256, 128, 128)] + [torch.nn.Linear(256, 128, bias=False)]
+    layer = PagedAttentionLayer(*mods, head_dim=64)
+    a = _inputs()
+    rest = a["kp"], a["vp"], torch.zeros(4, 3, dtype=I), torch.ones(4, dtype=I)
+    x = torch.randn(4, 128)
+    assert not layer(x, *rest).requires_grad
+    with pytest.raises(ValueError, match="no gradient"):
+        layer(x.clone().requires_grad_(), *rest)
+    with torch.no_grad():
+        layer(x.clone().requires_grad_(), *rest)
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="tangents"):
+        layer(forward_ad.make_dual(x, x), *rest)
