@@ -165,6 +165,48 @@ struct GqaTable {
   }
 };
 
+// 16 bytes of T: whether a value is an infinity or NaN; the values with zeros for those; a bit for each NaN
+template <typename T>
+__device__ __forceinline__ bool gqa_odd(T x) { return !(to_f32(x) * 0.0f == 0.0f); }
+template <typename T>
+__device__ __forceinline__ bool gqa_odd_chunk(const uint4& v) {
+  const T* x = reinterpret_cast<const T*>(&v);
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < GqaType<T>::CE; ++e) odd = odd || gqa_odd<T>(x[e]);
+  return odd;
+}
+template <typename T>
+__device__ __forceinline__ uint4 gqa_finite(uint4 v) {
+  T* x = reinterpret_cast<T*>(&v);
+#pragma unroll
+  for (int e = 0; e < GqaType<T>::CE; ++e) x[e] = gqa_odd<T>(x[e]) ? (T)0.0f : x[e];
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t gqa_nans(const uint4& v) {
+  const T* x = reinterpret_cast<const T*>(&v);
+  uint32_t b = 0;
+#pragma unroll
+  for (int e = 0; e < GqaType<T>::CE; ++e) b |= (to_f32(x[e]) != to_f32(x[e]) ? 1u : 0u) << e;
+  return b;
+}
+
+// Elements [d, d + CE) of a row of D, zeros past its end
+template <typename T>
+__device__ __forceinline__ uint4 gqa_chunk(const GqaArgs& a, const T* row, int d) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (a.kv_vec) {
+    if (d < a.D) v = *reinterpret_cast<const uint4*>(row + d);
+  } else {
+    T x[GqaType<T>::CE];
+#pragma unroll
+    for (int e = 0; e < GqaType<T>::CE; ++e) x[e] = d + e < a.D ? row[d + e] : (T)0.0f;
+    v = __builtin_bit_cast(uint4, x);
+  }
+  return v;
+}
+
 // Loads of a tile of BN keys by WAVES wavefronts: rows of one instruction, instructions of one wavefront.
 template <typename T, int DP, int BN, int WAVES>
 struct GqaFill {
@@ -174,7 +216,7 @@ struct GqaFill {
   uint64_t at[ITER];  // uniform: each instruction's first row, bytes from a head's base
   uint64_t ok;        // the keys that are there: the others are read as zeros
 
-  // One address an instruction, whose rows lie in one cache block (gqa_rows_of), made by scalar instructions. (With an address a row for
+  // One address an instruction, whose rows lie in one cache block (GqaShape::group_rows), made by scalar instructions. (With an address a row for
   // every lane, the addresses alone are 78 vector instructions a tile of 64 keys, a third of the main loop's.)
   __device__ __forceinline__ void place(const GqaArgs& a, const GqaTable& tab, int j0, uint64_t okmask, int wave) {
     ok = okmask;
@@ -210,25 +252,14 @@ struct GqaFill {
   __device__ __forceinline__ static void load_any(const GqaArgs& a, uint8_t* dst, const uint8_t* base, int j0, int blk, uint64_t ok,
                                                   int wave, int lane) {
     const int r = lane / G::CPR, c = lane % G::CPR;
-#pragma unroll
+#pragma unroll 4
     for (int u = 0; u < ITER; ++u) {
       const int row = (u * WAVES + wave) * ROWS + r, key = j0 + row;
       const int b = __shfl(blk, row, 64);
-      const int64_t o = ((int64_t)b * a.kv_sb + (int64_t)(key - gqa_block_of(a, key) * a.BS) * a.kv_st) * (int64_t)sizeof(T);
+      const int64_t o = (int64_t)b * a.kv_sb + (int64_t)(key - gqa_block_of(a, key) * a.BS) * a.kv_st;
       const int cc = c ^ (V ? G::swz_v(row) : G::swz_k(row));
-      const bool in = (ok >> row) & 1;
       uint4 v = make_uint4(0, 0, 0, 0);
-      if (a.kv_vec) {
-        if (in && cc * G::CE < a.D) v = *reinterpret_cast<const uint4*>(base + o + cc * 16);
-      } else {
-        T x[G::CE];
-#pragma unroll
-        for (int e = 0; e < G::CE; ++e) {
-          const int dd = cc * G::CE + e;
-          x[e] = in && dd < a.D ? reinterpret_cast<const T*>(base + o)[dd] : (T)0.0f;
-        }
-        v = __builtin_bit_cast(uint4, x);
-      }
+      if ((ok >> row) & 1) v = gqa_chunk<T>(a, reinterpret_cast<const T*>(base) + o, cc * G::CE);
       *reinterpret_cast<uint4*>(dst + (u * WAVES + wave) * 1024 + lane * 16) = v;
     }
   }
@@ -563,61 +594,32 @@ __device__ __forceinline__ void gqa_store_live(const GqaArgs& a, int tok, int he
   if (split == 0 && a.ws_live) a.ws_live[(int64_t)tok * a.Hkv * a.group + head] = live;
 }
 
-// The rows (a bit each) of 16 whose sums are not finite: an infinity or NaN among the values, which the matrix
-// products multiply with the weights 0 of the rows that do not see its key, or one that they do see.
+// The rows (a bit each) of 16 with a NaN among their sums o, but not in their sum of weights l (a NaN score, which is for all
+// elements): V's infinities and NaN times the weight 0 of a row that does not see their key, or of one whose weight is too small for
+// its type or has a second part of another sign. (An infinite sum is right: it has no such term.)
 template <int OT>
-__device__ __forceinline__ uint32_t gqa_odd_rows(const f32x4 (&o)[OT]) {
+__device__ __forceinline__ uint32_t gqa_odd_rows(const f32x4 (&o)[OT], float l) {
   float z = 0.0f;
 #pragma unroll
   for (int d = 0; d < OT; ++d)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z = fmaf(o[d][i], 0.0f, z);
-  uint64_t b = __ballot(z != 0.0f);
+    for (int i = 0; i < 4; ++i) z += o[d][i];
+  uint64_t b = __ballot(z != z && l == l);
   b |= b >> 32;
   return (uint32_t)(b | b >> 16) & 0xFFFFu;
 }
 
-// Such a row over the keys [lo, hi) again, by one wavefront: a lane makes a key's score, then 4 elements of the sum,
-// to which only keys that the row sees add. After the last use of the kernels' own registers, so that it takes none of
-// their loops' (it costs a prompt of 8192 bf16 rows under 1%; a check of each tile in the loop 14%, a function on a stack 5%).
-template <typename T>
-__device__ __forceinline__ void gqa_row_again(const GqaArgs& a, const int32_t* table, int kvh, int tok, int head, int lo, int hi,
-                                                        int pos, int piece, bool direct, int lane) {
-  const T* q = static_cast<const T*>(a.q) + tok * a.q_st + head * a.q_sh;
-  const T* kp = static_cast<const T*>(a.kp) + kvh * a.kv_sh;
-  const T* vp = static_cast<const T*>(a.vp) + kvh * a.kv_sh;
-  const float slope = a.slopes ? a.slopes[head] * 1.44269504f : 0.0f;
-  float m = -3.402823466e38f, l = 0.0f;
-  f32x4 o{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int j = lo; j < hi; j += 64) {
-    const int key = j + lane, blk = key < hi ? table[gqa_block_of(a, key)] : -1;
-    const bool there = blk >= 0 && blk < a.num_blocks;
-    const int64_t at = there ? (int64_t)blk * a.kv_sb + (int64_t)(key - gqa_block_of(a, key) * a.BS) * a.kv_st : 0;
-    float s = -__builtin_huge_valf();
-    if (there) {
-      float x = 0.0f;
-#pragma unroll 1
-      for (int d = 0; d < a.D; ++d) x = fmaf(to_f32(q[d]), to_f32(kp[at + d]), x);
-      s = a.cap > 0.0f ? tanhf(x * a.to_cap) * a.cap : x * a.c;
-      if (a.slopes) s = fmaf(-slope, fabsf((float)(pos - key)), s);
-    }
-    const float mn = fmaxf(m, lane_group_max<64>(s)), f = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(s - mn);
-    m = mn;
-    l = fmaf(l, f, w);
-    o *= f;
-#pragma unroll 1
-    for (uint64_t left = __ballot(there); left; left &= left - 1) {
-      const int k = __builtin_ctzll(left);
-      const float wk = __shfl(w, k, 64);
-      const int64_t ak = __shfl((long long)at, k, 64);
+// The elements of 16 rows' sums that are NaN in any row: bytes of 1, others 0. By one wavefront, in LDS of its own.
+template <int OT>
+__device__ __forceinline__ void gqa_odd_elements(const f32x4 (&o)[OT], uint8_t* cols, int lane) {
+  for (int e = lane; e < 16 * OT / 4; e += 64) reinterpret_cast<uint32_t*>(cols)[e] = 0;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * lane + i < a.D) o[i] = fmaf(wk, to_f32(vp[ak + 4 * lane + i]), o[i]);
-    }
-  }
-  l = lane_group_sum<64>(l);
-  if (4 * lane < a.D) gqa_store<T>(a, tok, head, piece, direct, 4 * lane, o, m, l);
+  for (int d = 0; d < OT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (o[d][i] != o[d][i]) cols[16 * d + 4 * (lane >> 4) + i] = 1;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // Bit i: row r0 + i is one of the tile's sequence
@@ -625,16 +627,144 @@ __device__ __forceinline__ uint32_t gqa_rows_of(const GqaPlan& p, int r0) {
   return r0 + 16 <= p.rows ? 0xFFFFu : r0 < p.rows ? (1u << (p.rows - r0)) - 1 : 0;
 }
 
-// The rows r0 + i of `odd`'s bits again, over the piece's keys [from, to)
-template <typename T>
-__device__ __forceinline__ void gqa_again(const GqaArgs& a, const GqaPlan& p, uint32_t odd, int r0, int kvh, int piece, int from, int to, int lane) {
+// Whether each of the elements marked in `cols` is NaN in a key of [from, to), all of which the 16 rows see. By one wavefront, four
+// loads in flight.
+template <typename T, int DP>
+__device__ __forceinline__ bool gqa_explained(const GqaArgs& a, const GqaPlan& p, const T* vp, const uint8_t* cols, int from, int to, int lane) {
+  using G = GqaTile<T, DP>;
+  constexpr int ROWS = 64 / G::CPR, CE = G::CE;
+  const int c = lane % G::CPR * CE;
+  uint32_t left = 0;
+#pragma unroll
+  for (int e = 0; e < CE; ++e)
+    if (c + e < DP && cols[c + e]) left |= 1u << e;
 #pragma unroll 1
-  while (__builtin_expect(odd != 0, 0)) {
-    const int r = r0 + __builtin_ctz(odd), tok = p.tok0 + r / a.group;
-    odd &= odd - 1;
-    int lo, hi, pos;
-    gqa_row_range(a, p, tok, lo, hi, pos);
-    gqa_row_again<T>(a, p.table, kvh, tok, kvh * a.group + r % a.group, max(lo, from), min(hi, to), pos, piece, p.direct, gqa_here(lane));
+  for (int j = from; j < to && __any(left != 0); j += 4 * ROWS) {
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int key = j + u * ROWS + lane / G::CPR, blk = key < to ? p.table[gqa_block_of(a, key)] : -1;
+      v[u] = make_uint4(0, 0, 0, 0);
+      if (blk >= 0 && blk < a.num_blocks)
+        v[u] = gqa_chunk<T>(a, vp + (int64_t)blk * a.kv_sb + (int64_t)(key - gqa_block_of(a, key) * a.BS) * a.kv_st, c);
+    }
+    left &= ~(gqa_nans<T>(v[0]) | gqa_nans<T>(v[1]) | gqa_nans<T>(v[2]) | gqa_nans<T>(v[3]));
+#pragma unroll
+    for (int off = G::CPR; off < 64; off <<= 1) left &= __shfl_xor(left, off, 64);
+  }
+  return !__any(left != 0);
+}
+
+// Keys of a step of the second pass below, and the LDS that a wavefront needs for it
+template <typename T>
+constexpr int gqa_again_wk() { return GqaType<T>::F32 ? 16 : 32; }
+template <typename T, int DP>
+constexpr int gqa_again_lds() { return gqa_again_wk<T>() * GqaTile<T, DP>::ROWB; }
+
+// The V tile of the keys j .. j + WK in `lds`, as loaded: zeros for infinities and NaN, which are noted in the bits pos and neg (NaN: both) of
+// the lane's elements, 4 d + i, where its row sees [lo, hi) of the keys.
+template <typename T, int DP>
+__device__ __forceinline__ void gqa_clean(uint8_t* lds, int j, int lo, int hi, uint64_t& pos, uint64_t& neg, int lane) {
+  using G = GqaTile<T, DP>;
+  constexpr int ROWS = 64 / G::CPR, CE = G::CE, ITER = gqa_again_wk<T>() / ROWS;
+  const int g = lane >> 4;
+#pragma unroll 1
+  for (int u = 0; u < ITER; ++u) {
+    uint4* at = reinterpret_cast<uint4*>(lds + u * 1024) + lane;
+    const uint4 mine = *at;
+    const bool odd = gqa_odd_chunk<T>(mine);
+    const uint64_t all = __ballot(odd);
+    if (all == 0) continue;
+#pragma unroll 1
+    for (int r = 0; r < ROWS; ++r) {
+      if ((all >> (r * G::CPR) & (~0ull >> (64 - G::CPR))) == 0) continue;
+      const int row = u * ROWS + r;
+      const bool see = lo <= j + row && j + row < hi;
+#pragma unroll 1
+      for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = 16 * d + 4 * g + i;
+          const float f = to_f32(*reinterpret_cast<const T*>(lds + row * G::ROWB + ((e / CE ^ G::swz_v(row)) << 4) + e % CE * (int)sizeof(T)));
+          const bool bad = see && !(f * 0.0f == 0.0f);
+          pos |= (uint64_t)(bad && !(f < 0.0f)) << (4 * d + i);
+          neg |= (uint64_t)(bad && !(f > 0.0f)) << (4 * d + i);
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (odd) *at = gqa_finite<T>(mine);
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+// The rows of `odd`'s bits, whose sums over the block's keys have NaN elements. Their results are stored already, and right where
+// each such element is NaN in a key that all of 16 rows see (EXPLAIN: `ranges` holds the marks of gqa_odd_elements, 256 bytes
+// for each 16 rows). Where not, the 16 rows go over their keys again, with zeros for the infinities and NaN, and these are
+// added at the end to the rows that see their keys (a weight is positive: its size does not matter to them). By one
+// wavefront, a tile at a time. lds, ranges: the wavefront's own; row_of_tile: its first row's place in the block's tile.
+// Arguments and block plan are made anew: those of the kernel, kept from its start to here, cost its loops registers
+// and its start their spills (chunks of D = 256 134 -> 160 us, 36 rows of 12 sequences 28 -> 31; so: no difference).
+// Prompt of 2048, 32 heads of 128 over 8, bf16: 111 us; with a NaN in the first token 108, in the last 751 (each such row by
+// itself, key by key: 23 ms), infinities alone 7.4 ms; prompt of 8192 0.66, 0.72, 6.1 and 120 ms.
+template <typename T, int DP, int NT, bool SPLIT, bool EXPLAIN>
+__device__ __forceinline__ void gqa_again(uint32_t odd, int row_of_tile, uint8_t* lds, int4* ranges) {
+  constexpr int WK = gqa_again_wk<T>();
+  const int lane = gqa_here(threadIdx.x & 63);
+  int block = blockIdx.x, kvh, split;
+  auto* args = (const __attribute__((address_space(4))) GqaArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(block), "+s"(args));
+  const GqaArgs& a = *(const GqaArgs*)args;
+  const GqaPlan p = gqa_block_plan(a, block, lane, kvh, split);
+  const int row0 = p.row0 + row_of_tile, piece = a.piece0 + split;
+  const int from = max(p.lo + (split * p.per << a.bn_log), p.klo), to = min(p.lo + ((split + 1) * p.per << a.bn_log), p.khi);
+  using F = GqaFill<T, DP, WK, 1>;
+  const T* kp = static_cast<const T*>(a.kp) + kvh * a.kv_sh;
+  const T* vp = static_cast<const T*>(a.vp) + kvh * a.kv_sh;
+#pragma unroll 1
+  for (int n = 0; n < NT; ++n) {
+    const uint32_t mine = odd >> (16 * n) & 0xFFFFu;
+    if (mine == 0) continue;
+    const int r0 = row0 + 16 * n;
+    if constexpr (EXPLAIN) {
+      int lo_min, lo_max, hi_min, hi_max;
+      gqa_wave_range(a, p, r0, min(r0 + 16, p.rows) - 1, lane, lo_min, lo_max, hi_min, hi_max);
+      if (gqa_explained<T, DP>(a, p, vp, reinterpret_cast<const uint8_t*>(ranges + 16 * n), max(from, lo_max), min(to, hi_min), lane)) continue;
+    }
+    GqaRows<T, DP, 1, SPLIT> rows;
+    rows.init(a, p, r0, kvh, ranges, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int4 sees = ranges[lane & 15];  // (the keys [x, y))
+    uint64_t pos = 0, neg = 0;
+    const int hi = min(to, rows.hi_max);
+#pragma unroll 1
+    for (int j = max(from, rows.lo_min); j < hi; j += WK) {
+      const int blk = lane < WK && j + lane < hi ? p.table[gqa_block_of(a, j + lane)] : -1;
+      const uint64_t ok = __ballot(blk >= 0 && blk < a.num_blocks);
+      f32x4 s[1][WK / 16];
+      F::template load_any<false>(a, lds, reinterpret_cast<const uint8_t*>(kp), j, blk, ok, 0, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      rows.template scores<WK>(lds, lane, s);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      F::template load_any<true>(a, lds, reinterpret_cast<const uint8_t*>(vp), j, blk, ok, 0, lane);
+      rows.template weigh<WK>(a, s, j, ok, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      gqa_clean<T, DP>(lds, j, sees.x, sees.y, pos, neg, lane);
+      rows.template product<WK>(s, lds, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    const float l = rows.sum_of(0);
+    if (!(mine >> (lane & 15) & 1)) continue;
+    const int r = r0 + (lane & 15), tok = p.tok0 + r / a.group, head = kvh * a.group + r % a.group;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      f32x4 x = rows.o[0][d];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool up = pos >> (4 * d + i) & 1, down = neg >> (4 * d + i) & 1;
+        if (up || down) x[i] = up && down ? __builtin_nanf("") : up ? __builtin_huge_valf() : -__builtin_huge_valf();
+      }
+      gqa_store<T>(a, tok, head, piece, p.direct, 16 * d + 4 * (lane >> 4), x, rows.m[0], l);
+    }
   }
 }
 
@@ -696,16 +826,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void gqa_rows_kernel(const 
   for (int n = 0; n < NT; ++n) {
     const int r = row0 + 16 * n + (lane & 15);
     const float l = rows.sum_of(n);
-    odd |= (gqa_odd_rows(rows.o[n]) & gqa_rows_of(p, row0 + 16 * n)) << (16 * n);
+    odd |= (gqa_odd_rows(rows.o[n], l) & gqa_rows_of(p, row0 + 16 * n)) << (16 * n);
     if (r < p.rows) {
       const int tok = p.tok0 + r / a.group, head = kvh * a.group + r % a.group;
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d)
-        if (!((odd >> (16 * n + (lane & 15))) & 1)) gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, 16 * d + 4 * g, rows.o[n][d], rows.m[n], l);
+        gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, 16 * d + 4 * g, rows.o[n][d], rows.m[n], l);
       if (g == 0) gqa_store_live(a, tok, head, split, p.live);
     }
   }
-  gqa_again<T>(a, p, odd, row0, kvh, a.piece0 + split, p.lo + t0 * BN, p.lo + t1 * BN, lane);
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the tiles are read: their LDS can be used)
+  if (__builtin_expect(odd == 0, 1)) return;
+  static_assert(gqa_again_lds<T, DP>() <= TB, "a tile's LDS for each wavefront");
+#pragma unroll
+  for (int n = 0; n < NT; ++n) gqa_odd_elements(rows.o[n], reinterpret_cast<uint8_t*>(rows.at + 16 * n), lane);
+  gqa_again<T, DP, NT, false, true>(odd, wave * 16 * NT, smem + wave * TB, rows.at);
 }
 
 // Many rows of 16-bit types: 8 wavefronts, two a SIMD, in two groups half a step apart: while one
@@ -720,6 +855,7 @@ constexpr int gqa_pair_bn() { return DP <= 128 ? 64 : 32; }
 template <typename T, int DP, int NT>
 struct GqaPair {
   static constexpr int BN = gqa_pair_bn<T, DP>(), TB = BN * GqaTile<T, DP>::ROWB, PER = TB / 1024 / 8;
+  static constexpr int RANGES = 6 * TB > 8 * gqa_again_lds<T, DP>() ? 6 * TB : 8 * gqa_again_lds<T, DP>();  // rows' ranges, behind the tiles
   using Fill = GqaFill<T, DP, BN, 8>;
   GqaRows<T, DP, NT, false> rows;
   f32x4 s[NT][BN / 16];
@@ -768,7 +904,7 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
   const int t0 = split * p.per, n = min(p.tiles - t0, p.per), j0 = p.lo + t0 * BN;
   P w;
   const int row0 = p.row0 + wave * 16 * NT;
-  w.rows.init(a, p, row0, kvh, reinterpret_cast<int4*>(smem + 6 * TB) + wave * 16 * NT, lane);
+  w.rows.init(a, p, row0, kvh, reinterpret_cast<int4*>(smem + P::RANGES) + wave * 16 * NT, lane);
   if (n > 0) {
     GqaTable tab;
     tab.start(a, p, j0, lane);
@@ -820,16 +956,20 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
   for (int m = 0; m < NT; ++m) {
     const int r = row0 + 16 * m + (lane & 15);
     const float l = w.rows.sum_of(m);
-    odd |= (gqa_odd_rows(w.rows.o[m]) & gqa_rows_of(p, row0 + 16 * m)) << (16 * m);
+    odd |= (gqa_odd_rows(w.rows.o[m], l) & gqa_rows_of(p, row0 + 16 * m)) << (16 * m);
     if (r < p.rows) {
       const int tok = p.tok0 + r / a.group, head = kvh * a.group + r % a.group;
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d)
-        if (!((odd >> (16 * m + (lane & 15))) & 1)) gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, 16 * d + 4 * g, w.rows.o[m][d], w.rows.m[m], l);
+        gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, 16 * d + 4 * g, w.rows.o[m][d], w.rows.m[m], l);
       if (g == 0) gqa_store_live(a, tok, head, split, p.live);
     }
   }
-  gqa_again<T>(a, p, odd, row0, kvh, a.piece0 + split, j0, j0 + n * BN, lane);
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the tiles are read: their LDS can be used)
+  if (__builtin_expect(odd == 0, 1)) return;
+#pragma unroll
+  for (int m = 0; m < NT; ++m) gqa_odd_elements(w.rows.o[m], reinterpret_cast<uint8_t*>(w.rows.at + 16 * m), lane);
+  gqa_again<T, DP, NT, false, true>(odd, wave * 16 * NT, smem + wave * gqa_again_lds<T, DP>(), w.rows.at);
 }
 
 // Few rows: the NW wavefronts of a block hold the same 16 rows and take WK keys each of a
@@ -920,7 +1060,7 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
   // join the wavefronts' states
   float* ol = reinterpret_cast<float*>(smem);                // [NW][16 NT][OL]
   float* ml = ol + NW * 16 * NT * OL;                        // [NW][16 NT][2]
-  uint32_t* odd = reinterpret_cast<uint32_t*>(ml + NW * 16 * NT * 2);  // [NW]: rows whose sums are not finite
+  uint32_t* odd = reinterpret_cast<uint32_t*>(ml + NW * 16 * NT * 2);  // [NW]: rows with NaN sums
   __syncthreads();
   uint32_t mine = 0;
   const int g = lane >> 4;
@@ -928,7 +1068,7 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
   for (int n = 0; n < NT; ++n) {
     const int r = 16 * n + (lane & 15);
     const float l = rows.sum_of(n);
-    mine |= (gqa_odd_rows(rows.o[n]) & gqa_rows_of(p, p.row0 + 16 * n)) << (16 * n);
+    mine |= (gqa_odd_rows(rows.o[n], l) & gqa_rows_of(p, p.row0 + 16 * n)) << (16 * n);
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
       *reinterpret_cast<f32x4*>(ol + (wave * 16 * NT + r) * OL + 16 * d + 4 * g) = rows.o[n][d];
@@ -942,7 +1082,6 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
   for (int e = threadIdx.x; e < 16 * NT * (DP / 4); e += NW * 64) {
     const int rr = e / (DP / 4), d = (e % (DP / 4)) * 4, r = p.row0 + rr;
     if (r >= p.rows || d >= a.D) continue;
-    const bool again = (all >> rr) & 1;
     float M = -3.402823466e38f, L = 0.0f;
     float2 x[NW];
 #pragma unroll
@@ -958,12 +1097,14 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
       acc += *reinterpret_cast<const f32x4*>(ol + (w * 16 * NT + rr) * OL + d) * f;
     }
     const int tok = p.tok0 + r / a.group, head = kvh * a.group + r % a.group;
-    if (!again) gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, d, acc, M, L);
+    gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, d, acc, M, L);
     if (d == 0) gqa_store_live(a, tok, head, split, p.live);
   }
-  // (a wavefront takes every NW-th row)
-  gqa_again<T>(a, p, all & ((NW == 4 ? 0x11111111u : 0x55555555u) << wave), p.row0, kvh, a.piece0 + split,
-               p.lo + split * p.per * BN, p.lo + (split + 1) * p.per * BN, lane);
+  if (__builtin_expect(all == 0, 1)) return;
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (results are stored, their LDS is read)
+  static_assert(gqa_again_lds<T, DP>() <= TB, "a tile's LDS");
+  if (wave == 0)
+    gqa_again<T, DP, NT, !GqaType<T>::F32, false>(all, 0, smem, rows.at);
 }
 
 template <typename T, int DP>
@@ -993,7 +1134,7 @@ int gqa_launch_dp(const GqaArgs& a, const GqaShape& s, int64_t blocks, hipStream
   if constexpr (!GqaType<T>::F32) {
     if (s.pair) {
       constexpr int NT = DP <= 128 ? 2 : 1;
-      return gqa_launch_kernel<gqa_pair_kernel<T, DP, NT>>(a, blocks, 512, 6 * GqaPair<T, DP, NT>::TB + 8 * 256 * NT, st);
+      return gqa_launch_kernel<gqa_pair_kernel<T, DP, NT>>(a, blocks, 512, GqaPair<T, DP, NT>::RANGES + 8 * 256 * NT, st);
     }
   }
   constexpr int lds = 4 * gqa_bn<T, DP>() * GqaTile<T, DP>::ROWB + 4 * 256 * 2;

@@ -216,3 +216,86 @@ def test_caps_far_below_the_scores(dev, dtype):
     q = _q(1, 4, 64, dtype)
     for cap in (1e-6, 1e-30, 1e-40):
         check(paged_attention(q, kp, vp, tab, ctx, softcap=cap), *attention(q, kp, vp, tab, lens, softcap=cap), f"{cap}")
+
+
+def _spoil(vp, tab, lens, new, want, window, prefix_lens, places, shared=None, shared_len=0):
+    """Puts `places` (sequence, or -1 for the shared prefix; token; element; value) into vp, and adds each value to the rows of
+    `want` that see its token."""
+    bs = vp.shape[2]
+    for s, j, d, bad in places:
+        row = shared if s < 0 else tab[s]
+        vp[int(row[j // bs]), :, j % bs, d] = bad
+        first = 0
+        for i, (cnt, n) in enumerate(zip(new, lens)):
+            if s in (i, -1):
+                at = j + (shared_len if s >= 0 else 0)
+                pos = torch.arange(n - cnt, n, device=vp.device).clamp(min=-1 if shared is not None else -2 ** 31) + shared_len
+                sees = pos >= at
+                if prefix_lens is not None:
+                    sees = sees | (at < int(prefix_lens[i]))
+                if window:
+                    sees = sees & (pos - at < window)
+                part = want[first:first + cnt, :, d]
+                want[first:first + cnt, :, d] = torch.where(sees[:, None], part + torch.full_like(part, bad), part)
+            first += cnt
+
+
+def _check_spoilt(y, want, bound, what=""):
+    y, odd = y.double(), ~torch.isfinite(want)
+    assert bool((~torch.isfinite(y) == odd).all()), f"{what}: {int((~torch.isfinite(y) != odd).sum())} elements"
+    assert bool(((y == want) | (y.isnan() & want.isnan()))[odd].all()), what
+    check(torch.where(odd, 0.0, y), torch.where(odd, 0.0, want), torch.where(odd, 1e-30, bound), what)
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("dtype,D,bs", [(BF, 128, 16), (HF, 64, 8), (FP, 64, 16), (BF, 256, 16), (FP, 256, 8), (HF, 80, 24), (BF, 50, 5)])
+@pytest.mark.parametrize("group", [1, 4])
+@pytest.mark.parametrize("opts", ["plain", "window", "prefix", "all"])
+def test_rows_apart_from_values_that_are_no_numbers(dev, dtype, D, bs, group, opts):
+    """Bad values early (every row sees them), among the new tokens, at the edges of windows, of both signs in one element, in
+    tokens behind a prefix mask, beside tables with holes: each reaches its element of the rows that see its token."""
+    new, past = [300, 7, 70, 2], [5, 200, 0, 90]
+    lens = [a + b for a, b in zip(new, past)]
+    kp, vp, tab, ctx = cache(lens, 2, D, bs, dtype, 51)
+    tab[2, 1] = -1
+    q = _q(sum(new), 2 * group, D, dtype)
+    window = 40 if opts in ("window", "all") else 0
+    pl = torch.tensor([60, 205, 9, 0], dtype=torch.int32, device=dev) if opts in ("prefix", "all") else None
+    o = dict(window=window, prefix_lens=pl, **(dict(softcap=5.0, slopes=torch.full((2 * group,), 0.1, device=dev)) if opts == "all" else {}))
+    want, bound = attention(q, kp, vp, tab, lens, new, **o)
+    _spoil(vp, tab, lens, new, want, window, pl, [
+        (0, 0, 0, INF), (0, 150, 1, NAN), (0, 151, 2, INF), (0, 190, 2, -INF), (0, 304, 3, -INF), (0, 55, 4, NAN), (0, 62, 5, INF),
+        (1, 202, 6, INF), (1, 206, 7, NAN), (1, 170, 8, -INF), (2, 69, 9, NAN), (2, 3 * bs, 10, INF), (3, 91, 11, NAN), (3, 0, 12, INF)])
+    for hint in (None, 3, 300):
+        _check_spoilt(paged_attention(q, kp, vp, tab, ctx, offsets(new), max_new=hint, **o), want, bound, f"{hint}")
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 64), (HF, 256)])
+@pytest.mark.parametrize("n", [5, 90])
+@pytest.mark.parametrize("window", [0, 130])
+def test_rows_behind_a_prefix_of_values_that_are_no_numbers(dev, dtype, D, n, window):
+    """Sequences of other lengths see other parts of the prefix within their windows."""
+    shared = 300
+    lens = [(41 * i) % 150 for i in range(n)]
+    kp, vp, tab, ctx = cache(lens + [shared], 2, D, 16, dtype, 52)
+    pre, tab, ctx = tab[n, :-(-shared // 16)].contiguous(), tab[:n], ctx[:n]
+    q = _q(n, 8, D, dtype)
+    want, bound = attention(q, kp, vp, tab, lens, shared=pre, shared_len=shared, window=window)
+    _spoil(vp, tab, lens, [1] * n, want, window, None, [(-1, 200, 0, INF), (-1, 250, 1, NAN), (-1, 299, 2, -INF), (-1, 20, 3, NAN),
+                                                       (-1, 280, 2, INF), (4, 0, 5, NAN), (3, 100, 6, -INF)], pre, shared)
+    _check_spoilt(shared_prefix_attention(q, kp, vp, pre, shared, tab, ctx, window=window), want, bound)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 64)])
+@pytest.mark.parametrize("new", [[260, 3], [3, 2]])
+def test_all_values_infinite(dev, dtype, D, new):
+    """Every row sees infinities alone, but the rows that see nothing."""
+    lens = [255, 40]
+    kp, vp, tab, ctx = cache(lens, 2, D, 16, dtype, 53)
+    vp.fill_(INF)
+    q = _q(sum(new), 8, D, dtype)
+    y = paged_attention(q, kp, vp, tab, ctx, offsets(new))
+    empty = max(new[0] - lens[0], 0)
+    assert bool((y[:empty] == 0).all()) and bool((y[empty:] == INF).all())
