@@ -205,7 +205,6 @@ int prepare(const char* fn, const mlsx_paged_attention_args* p, float* ws, Pass&
   own.a.splits = (int)splits;
   own.a.piece0 = (int)sp;
   own.a.pieces = (int)pieces;
-  own.a.least = 1;
   own.a.cap_tiles = (int)std::max<int64_t>(cdiv(2048, own.s.bn), cdiv(steps, splits));
   own.a.target = (float)target;
   own.blocks = slots * Hkv * splits;

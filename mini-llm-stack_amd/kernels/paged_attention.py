@@ -160,7 +160,7 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
 
     The row at position p sees token j when j <= p or j < prefix_lens[s] (int32 [n]), and, with a window, when
     p - j < window. A score is scale q.k (scale: D^-0.5), capped softcap tanh(score / softcap), less
-    slopes[h] |p - j| (float32 [Hq]). A row that sees nothing gives zeros, as do rows of no sequence; block ids
+    slopes[h] |p - j| (float32 [Hq]). A row that sees nothing (or only scores of -inf) gives zeros, as do rows of no sequence; block ids
     outside the pool hold no tokens, a context longer than its table is cut at the table's end."""
     return _attend("paged_attention", q, k_pool, v_pool, block_tables, context_lens, cu_seqlens, max_new, scale, softcap, slopes,
                    window, prefix_lens, None, 0)
