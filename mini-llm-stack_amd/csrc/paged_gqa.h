@@ -703,7 +703,9 @@ __device__ __forceinline__ void gqa_clean(uint8_t* lds, int j, int lo, int hi, u
 // added at the end to the rows that see their keys (a weight is positive: its size does not matter to them). By one
 // wavefront, a tile at a time. lds, ranges: the wavefront's own; row_of_tile: its first row's place in the block's tile.
 // Arguments and block plan are made anew: those of the kernel, kept from its start to here, cost its loops registers
-// and its start their spills (chunks of D = 256 134 -> 160 us, 36 rows of 12 sequences 28 -> 31; so: no difference).
+// and its start their spills (chunks of D = 256 134 -> 160 us, 36 rows of 12 sequences 28 -> 31). For the same reason the calls
+// say that they are as good as never reached: the loops in here would count as the kernel's hottest otherwise, and its own
+// values be spilled for them (12 sequences of 49 tokens, 4 heads a K/V head, 45.0 us against 41.1).
 // Prompt of 2048, 32 heads of 128 over 8, bf16: 111 us; with a NaN in the first token 108, in the last 751 (each such row by
 // itself, key by key: 23 ms), infinities alone 7.4 ms; prompt of 8192 0.66, 0.72, 6.1 and 120 ms.
 template <typename T, int DP, int NT, bool SPLIT, bool EXPLAIN>
@@ -836,7 +838,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void gqa_rows_kernel(const 
     }
   }
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the tiles are read: their LDS can be used)
-  if (__builtin_expect(odd == 0, 1)) return;
+  if (__builtin_expect_with_probability(odd == 0, 1, 1.0)) return;
   static_assert(gqa_again_lds<T, DP>() <= TB, "a tile's LDS for each wavefront");
 #pragma unroll
   for (int n = 0; n < NT; ++n) gqa_odd_elements(rows.o[n], reinterpret_cast<uint8_t*>(rows.at + 16 * n), lane);
@@ -966,7 +968,7 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
     }
   }
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the tiles are read: their LDS can be used)
-  if (__builtin_expect(odd == 0, 1)) return;
+  if (__builtin_expect_with_probability(odd == 0, 1, 1.0)) return;
 #pragma unroll
   for (int m = 0; m < NT; ++m) gqa_odd_elements(w.rows.o[m], reinterpret_cast<uint8_t*>(w.rows.at + 16 * m), lane);
   gqa_again<T, DP, NT, false, true>(odd, wave * 16 * NT, smem + wave * gqa_again_lds<T, DP>(), w.rows.at);
@@ -1100,7 +1102,7 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
     gqa_store<T>(a, tok, head, a.piece0 + split, p.direct, d, acc, M, L);
     if (d == 0) gqa_store_live(a, tok, head, split, p.live);
   }
-  if (__builtin_expect(all == 0, 1)) return;
+  if (__builtin_expect_with_probability(all == 0, 1, 1.0)) return;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (results are stored, their LDS is read)
   static_assert(gqa_again_lds<T, DP>() <= TB, "a tile's LDS");
   if (wave == 0)

@@ -158,7 +158,7 @@ __device__ __forceinline__ GqaPlan gqa_tile_plan(const GqaArgs& a, int seq, int 
   p.klo = p.khi = p.lo = 0;
   p.direct = false;
   // (offsets that do not rise can lead the search to a sequence that begins behind the slot: rt < 0)
-  if (rt < 0 || ((int64_t)rt << a.bm_log) >= p.rows) {
+  if ((uint32_t)rt >= (uint32_t)(p.rows + (1 << a.bm_log) - 1) >> a.bm_log) {
     p.row0 = p.rows = 0;
     return p;
   }
