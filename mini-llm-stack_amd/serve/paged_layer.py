@@ -54,7 +54,8 @@ class PagedAttentionLayer(nn.Module):
         """Moves the tables with the module, but leaves them float32 under .half() and the like."""
         keep = self.rope, self.slopes
         super()._apply(fn, recurse)
-        self.rope, self.slopes = (t if t is None else t.to(to.device) for t, to in zip(keep, (self.rope, self.slopes)))
+        self.rope, self.slopes = (t if t is None else to.to(t.dtype) if t.is_meta else t.to(to.device)
+                                  for t, to in zip(keep, (self.rope, self.slopes)))
         return self
 
     def to_int(self, bits: int = 8, group_size: int = 32) -> "PagedAttentionLayer":

@@ -172,3 +172,16 @@ def test_layer_refuses_inputs_that_ask_for_a_gradient(packed):
         layer(x.clone().requires_grad_(), *rest)
     with forward_ad.dual_level(), pytest.raises(ValueError, match="tangents"):
         layer(forward_ad.make_dual(x, x), *rest)
+
+
+def test_layer_made_on_the_meta_device():
+    """to_empty gives its tables memory, float32 as they are."""
+    with torch.device("meta"):
+        mods = [torch.nn.Linear(128, n, bias=False) for n in (256, 128, 128)] + [torch.nn.Linear(256, 128, bias=False)]
+        layer = PagedAttentionLayer(*mods, head_dim=64, rope=torch.zeros(9, 64), slopes=torch.zeros(4))
+    layer = layer.half().to_empty(device="cpu")
+    assert layer.wq.weight.dtype == torch.float16 and layer.wq.weight.device.type == "cpu"
+    for t, shape in ((layer.rope, (9, 64)), (layer.slopes, (4,))):
+        assert t.dtype == torch.float32 and t.device.type == "cpu" and t.shape == shape
+    layer.rope.fill_(0.1)
+    assert torch.equal(layer.bfloat16().rope, torch.full((9, 64), 0.1))
