@@ -96,6 +96,7 @@ struct Pass {
 // - Up to 16 rows: the kernel over keys (40 sequences of 1 to 4096 tokens, 4 rows: 40 us, the next one 58). With 32 rows a
 //   wavefront it is out of registers: 32 rows, 12 sequences of up to 2048, 40 us against 28; 64 of 2000 to 6000, 323
 //   against 239 (20 rows: 230 against 241).
+//   (Weights are rounded once from here on: in two parts, 36 rows of 12 sequences 30.0 us against 28.2, 20 of 64 257 against 241.)
 // - 16-bit types: the paired kernel's tiles of 256 rows (128 of D > 128) where they are at least half full, since it is
 //   1.7 times as fast a row as tiles of 64 (prompt of 8192: 550 us, 915 in tiles of 64; 12 sequences of 192 new rows
 //   52 against 57; of 96 rows 47 in the paired kernel, 37 in tiles of 64).
