@@ -698,8 +698,8 @@ __device__ __forceinline__ void gqa_clean(uint8_t* lds, int j, int lo, int hi, u
 }
 
 // The rows of `odd`'s bits, whose sums over the block's keys have NaN elements. Their results are stored already, and right where
-// each such element is NaN in a key that all of 16 rows see (EXPLAIN: `ranges` holds the marks of gqa_odd_elements, 256 bytes
-// for each 16 rows). Where not, the 16 rows go over their keys again, with zeros for the infinities and NaN, and these are
+// each such element is NaN in a key that all of 16 rows see (`ranges` holds the marks of gqa_odd_elements, 256 bytes for
+// each 16 rows). Where not, the 16 rows go over their keys again, with zeros for the infinities and NaN, and these are
 // added at the end to the rows that see their keys (a weight is positive: its size does not matter to them). By one
 // wavefront, a tile at a time. lds, ranges: the wavefront's own; row_of_tile: its first row's place in the block's tile.
 // Arguments and block plan are made anew: those of the kernel, kept from its start to here, cost its loops registers
@@ -707,8 +707,9 @@ __device__ __forceinline__ void gqa_clean(uint8_t* lds, int j, int lo, int hi, u
 // say that they are as good as never reached: the loops in here would count as the kernel's hottest otherwise, and its own
 // values be spilled for them (12 sequences of 49 tokens, 4 heads a K/V head, 45.0 us against 41.1).
 // Prompt of 2048, 32 heads of 128 over 8, bf16: 111 us; with a NaN in the first token 108, in the last 751 (each such row by
-// itself, key by key: 23 ms), infinities alone 7.4 ms; prompt of 8192 0.66, 0.72, 6.1 and 120 ms.
-template <typename T, int DP, int NT, bool SPLIT, bool EXPLAIN>
+// itself, key by key: 23 ms), NaN alone 117, infinities alone 7.4 ms; prompt of 8192 0.66, 0.72, 6.1 and 120 ms. 64 sequences
+// of 2048, a token each: 104 us; a token of NaN 104, one element of it only 500, infinities alone 4.5 ms.
+template <typename T, int DP, int NT, bool SPLIT>
 __device__ __forceinline__ void gqa_again(uint32_t odd, int row_of_tile, uint8_t* lds, int4* ranges) {
   constexpr int WK = gqa_again_wk<T>();
   const int lane = gqa_here(threadIdx.x & 63);
@@ -727,11 +728,9 @@ __device__ __forceinline__ void gqa_again(uint32_t odd, int row_of_tile, uint8_t
     const uint32_t mine = odd >> (16 * n) & 0xFFFFu;
     if (mine == 0) continue;
     const int r0 = row0 + 16 * n;
-    if constexpr (EXPLAIN) {
-      int lo_min, lo_max, hi_min, hi_max;
-      gqa_wave_range(a, p, r0, min(r0 + 16, p.rows) - 1, lane, lo_min, lo_max, hi_min, hi_max);
-      if (gqa_explained<T, DP>(a, p, vp, reinterpret_cast<const uint8_t*>(ranges + 16 * n), max(from, lo_max), min(to, hi_min), lane)) continue;
-    }
+    int lo_min, lo_max, hi_min, hi_max;
+    gqa_wave_range(a, p, r0, min(r0 + 16, p.rows) - 1, lane, lo_min, lo_max, hi_min, hi_max);
+    if (gqa_explained<T, DP>(a, p, vp, reinterpret_cast<const uint8_t*>(ranges + 16 * n), max(from, lo_max), min(to, hi_min), lane)) continue;
     GqaRows<T, DP, 1, SPLIT> rows;
     rows.init(a, p, r0, kvh, ranges, lane);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -842,7 +841,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void gqa_rows_kernel(const 
   static_assert(gqa_again_lds<T, DP>() <= TB, "a tile's LDS for each wavefront");
 #pragma unroll
   for (int n = 0; n < NT; ++n) gqa_odd_elements(rows.o[n], reinterpret_cast<uint8_t*>(rows.at + 16 * n), lane);
-  gqa_again<T, DP, NT, false, true>(odd, wave * 16 * NT, smem + wave * TB, rows.at);
+  gqa_again<T, DP, NT, false>(odd, wave * 16 * NT, smem + wave * TB, rows.at);
 }
 
 // Many rows of 16-bit types: 8 wavefronts, two a SIMD, in two groups half a step apart: while one
@@ -971,7 +970,7 @@ __global__ __launch_bounds__(512, 2) void gqa_pair_kernel(const GqaArgs a) {
   if (__builtin_expect_with_probability(odd == 0, 1, 1.0)) return;
 #pragma unroll
   for (int m = 0; m < NT; ++m) gqa_odd_elements(w.rows.o[m], reinterpret_cast<uint8_t*>(w.rows.at + 16 * m), lane);
-  gqa_again<T, DP, NT, false, true>(odd, wave * 16 * NT, smem + wave * gqa_again_lds<T, DP>(), w.rows.at);
+  gqa_again<T, DP, NT, false>(odd, wave * 16 * NT, smem + wave * gqa_again_lds<T, DP>(), w.rows.at);
 }
 
 // Few rows: the NW wavefronts of a block hold the same 16 rows and take WK keys each of a
@@ -1105,8 +1104,11 @@ __global__ __launch_bounds__((gqa_nw<T, DP>() * 64), (gqa_nw<T, DP>() / 2)) void
   if (__builtin_expect_with_probability(all == 0, 1, 1.0)) return;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (results are stored, their LDS is read)
   static_assert(gqa_again_lds<T, DP>() <= TB, "a tile's LDS");
-  if (wave == 0)
-    gqa_again<T, DP, NT, !GqaType<T>::F32, false>(all, 0, smem, rows.at);
+  if (wave != 0) return;
+  // (which elements are NaN is not kept: all count, as a token that is no number makes them)
+  for (int e = lane; e < DP; e += 64) reinterpret_cast<uint8_t*>(rows.at)[e] = e < a.D;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  gqa_again<T, DP, NT, !GqaType<T>::F32>(all, 0, smem, rows.at);
 }
 
 template <typename T, int DP>

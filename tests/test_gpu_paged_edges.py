@@ -299,3 +299,19 @@ def test_all_values_infinite(dev, dtype, D, new):
     y = paged_attention(q, kp, vp, tab, ctx, offsets(new))
     empty = max(new[0] - lens[0], 0)
     assert bool((y[:empty] == 0).all()) and bool((y[empty:] == INF).all())
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (FP, 64), (HF, 80), (BF, 33), (FP, 256)])
+@pytest.mark.parametrize("new,past", [([1, 1, 1], [70, 2, 400]), ([3, 2, 4], [70, 2, 400]), ([150, 1, 90], [0, 33, 200])])
+def test_whole_tokens_of_no_numbers(dev, dtype, D, new, past):
+    """A token whose values are all NaN: every element of the rows that see it, nothing of the others; and a cache of NaN alone."""
+    lens = [a + b for a, b in zip(new, past)]
+    kp, vp, tab, ctx = cache(lens, 2, D, 16, dtype, 54)
+    q = _q(sum(new), 8, D, dtype)
+    cu = offsets(new) if max(new) > 1 else None
+    want, bound = attention(q, kp, vp, tab, lens, new)
+    places = [(0, lens[0] - new[0] // 2 - 1, d, NAN) for d in range(D)] + [(2, 50, d, NAN) for d in range(D)]
+    _spoil(vp, tab, lens, new, want, 0, None, places)
+    _check_spoilt(paged_attention(q, kp, vp, tab, ctx, cu), want, bound)
+    vp.fill_(NAN)
+    assert bool(paged_attention(q, kp, vp, tab, ctx, cu).isnan().all())
