@@ -43,7 +43,7 @@ struct GqaArgs {
 };
 
 // 16-bit types: 1 - 2 / (e^2y + 1) is off by up to 2^-22, so a score by 2^-22 of the cap, for small scores too: at a cap of
-// 256 a quarter of what rounding a weight to fp16 leaves. Past that the scores take tanhf, precise relative to y, and the
+// 256 an eighth of what rounding a weight to fp16 leaves. Past that the scores take tanhf, precise relative to y, and the
 // paired kernel, which it would slow with any cap (chunks of D = 256, cap 30: 145 us against 138), is not taken (prompt of
 // 8192, cap 300: 1379 us against 1277 there; cap 50: 879).
 __host__ __device__ __forceinline__ bool gqa_cap_needs_tanh(const GqaArgs& a) { return a.cap > 256.0f * 1.44269504f; }
