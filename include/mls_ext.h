@@ -126,6 +126,46 @@ int mlsx_dw_fp32_pays(int64_t M, int64_t N, int64_t K);
 int mlsx_dw_fp32(const float* dy, int64_t lddy, const float* x, int64_t ldx, float* dw, int64_t lddw, int64_t M,
                  int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream);
 
+/* ---------------------------------------------------------------- activations in 8 bits */
+
+/* Codes int8 [M][ldq] and scales fp32 [M] of x's rows (dt, [M][ldx]): scale = max(max|row| / 127, 1e-8),
+ * code = value / scale (IEEE) rounded half to even; a row with an infinity or NaN: that scale, codes 0. */
+int mlsx_quantize_rows(const void* x, int dt, int64_t ldx, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* s,
+                       mls_stream_t stream);
+
+/* c[m][n] = (sum_k x[m][k] w[n][k]) sw[n] sx[m] + bias[n], type c_dt, [M][ldc]. w: int8 [N][ldw]; sw: sw_dt (fp32 or
+ * fp16) [N]; bias: bias_dt [N], or null. x_dt -1: x holds codes int8 [M][ldx], sx their scales fp32 [M];
+ * otherwise x holds values of that type, quantized by rows as above, and sx is not read. 1 <= K <= 131071
+ * (sums of 32 bits). Every field has 8 bytes. The 16-byte aligned workspace holds mlsx_a8w8_ws bytes (0: none). */
+typedef struct mlsx_a8w8_args {
+  const void* x;
+  const float* sx;
+  const int8_t* w;
+  const void *sw, *bias;
+  void* c;
+  int64_t x_dt, sw_dt, bias_dt, c_dt, ldx, ldw, ldc, M, N, K;
+} mlsx_a8w8_args;
+int64_t mlsx_a8w8_ws(const mlsx_a8w8_args* args);
+int mlsx_a8w8(const mlsx_a8w8_args* args, void* ws, int64_t ws_bytes, mls_stream_t stream);
+
+/* Codes and scales, as mlsx_quantize_rows, of silu(gate) * up (fp32; gate, up: dt, [M][ld]). kept_q, kept_s (both or
+ * neither null): codes int8 [2][M][H] and scales fp32 [2][M][ceil(H / 128)] of gate and up by groups of 128
+ * columns. */
+int mlsx_silu_mul_quantize(const void* gate, int64_t ldg, const void* up, int64_t ldu, int dt, int64_t M, int64_t H,
+                           int8_t* q, int64_t ldq, float* s, int8_t* kept_q, float* kept_s, mls_stream_t stream);
+
+/* Gradients of gate and up (dt, [M][ldo]) from dh (dt, [M][lddh]) and such a checkpoint: row m of gate's codes at
+ * q + m * ldq, of up's q_step further; scales alike. */
+int mlsx_silu_mul_backward(const void* dh, int64_t lddh, int dt, const int8_t* q, int64_t ldq, int64_t q_step,
+                           const float* s, int64_t lds, int64_t s_step, int64_t M, int64_t H, void* dgate, void* dup,
+                           int64_t ldo, mls_stream_t stream);
+
+/* dw[n][k] = sum_m dy[m][n] s[m] q[m][k] (dy and dw: dt; fp32 sums; 16-bit dt: s q rounded to it). M >= 1. The
+ * 16-byte aligned workspace holds mlsx_dw_int8_workspace bytes (0: sizes it does not take). */
+int64_t mlsx_dw_int8_workspace(int dt, int64_t M, int64_t N, int64_t K);
+int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw,
+                 int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream);
+
 /* ---------------------------------------------------------------- FP8 training */
 
 /* The fp8 operands of train/fp8.py:62-95 padded for the K-contiguous GEMM:

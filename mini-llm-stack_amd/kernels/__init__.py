@@ -9,7 +9,7 @@ reaches a kernel entry point, the call raises instead of computing elsewhere.
 
 Overlay. This package replaces only the reference's quantized-linear modules
 (dequant_matmul, fp8_matmul, moe_routing, paged_attention), and adds its own beside
-them (moe_grouped, int8_ste, paged_kv). Its search path is extended over every
+them (moe_grouped, int8_ste, int8_act, paged_kv). Its search path is extended over every
 ``kernels`` directory on ``sys.path`` (pkgutil.extend_path), so with this directory first and a reference checkout after it, the reference's
 other modules (attention_fwd, attention_bwd, autograd_ops, moe_backward,
 fusion_compiler) import from the checkout and bind this package's GEMMs. Both
@@ -117,6 +117,13 @@ EXT_SIGNATURES = {
     "mlsx_dw_fp32_workspace": ([_I64, _I64, _I64], _I64),
     "mlsx_dw_fp32_pays": ([_I64, _I64, _I64], _I),
     "mlsx_dw_fp32": ([_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
+    "mlsx_quantize_rows": ([_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P], _I),
+    "mlsx_a8w8_ws": ([ctypes.c_char_p], _I64),  # (an argument struct, packed)
+    "mlsx_a8w8": ([ctypes.c_char_p, _P, _I64, _P], _I),
+    "mlsx_silu_mul_quantize": ([_P, _I64, _P, _I64, _I, _I64, _I64, _P, _I64, _P, _P, _P, _P], _I),
+    "mlsx_silu_mul_backward": ([_P, _I64, _I, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P], _I),
+    "mlsx_dw_int8_workspace": ([_I, _I64, _I64, _I64], _I64),
+    "mlsx_dw_int8": ([_P, _I, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
     "mlsx_fp8_encode_pad": ([_I, _P, _I, _I64, _I64, _I64, _F, _P, _I64, _P, _P, _P], _I),
     "mlsx_absmax_parts": ([_P, _I, _I64, _P, _P], _I),
     "mlsx_absmax_scales": ([_P, _I, _F, _P, _P, _P], _I),
