@@ -16,6 +16,11 @@ the reference's host op sequence, which is the definition the kernels match.
 QuantLinear(use_kernel=True) runs the fused HIP GEMMs of kernels.dequant_matmul;
 use_kernel=False keeps the reference's dequantize-then-matmul path.
 
+act_bits=8 (no reference counterpart): the input is quantized too, per token as it comes, and INT8 weights meet it
+on the 8-bit matrix cores (kernels.int8_act), at about twice the 16-bit rate for prompts. quantize_model(act_bits=8) also makes
+every SwiGLU an Int8SwiGLU, whose product with the down projection's codes is one kernel. Such layers serve: they have
+no gradient and refuse inputs that ask for one.
+
 Unlike the reference, this module does not import the model package (the
 reference imports train.model only for a type annotation, :15): quantize_model
 finds the Linear slots by attribute name.
@@ -90,20 +95,29 @@ def dequantize_int4(packed: torch.Tensor, scale: torch.Tensor, group_size: int):
     return w.reshape(N, K)
 
 
+def _act_bits(act_bits: int | None, bits: int) -> int | None:
+    if act_bits not in (None, 8) or act_bits == 8 and bits != 8:
+        raise ValueError(f"act_bits={act_bits} with bits={bits}: activations of 8 bits meet weights of 8, or stay as they are (None)")
+    return act_bits
+
+
 class QuantLinear(nn.Module):
     """Drop-in nn.Linear replacement holding quantized weights (serve/quantize.py:50-95).
 
     use_kernel=True runs the fused gfx950 dequant GEMM; False runs the
     reference path (explicit dequant then matmul), kept for correctness tests
-    and host execution.
+    and host execution. act_bits=8 (with bits=8): x is quantized per token too.
     """
 
+    act_bits: int | None = None
+
     def __init__(self, linear: nn.Linear, bits: int = 8, group_size: int = 32,
-                 use_kernel: bool = True):
+                 use_kernel: bool = True, act_bits: int | None = None):
         super().__init__()
         assert linear.bias is None
         assert bits in (4, 8)
         self.bits, self.group_size, self.use_kernel = bits, group_size, use_kernel
+        self.act_bits = _act_bits(act_bits, bits)
         self.out_features, self.in_features = linear.weight.shape
         w = linear.weight.detach().float()
         if bits == 8:
@@ -115,13 +129,14 @@ class QuantLinear(nn.Module):
 
     @classmethod
     def from_quantized(cls, w_q: torch.Tensor, scale: torch.Tensor, bits: int, group_size: int,
-                       in_features: int, use_kernel: bool = True) -> "QuantLinear":
+                       in_features: int, use_kernel: bool = True, act_bits: int | None = None) -> "QuantLinear":
         """A QuantLinear around buffers that are already quantized (a quantized
         checkpoint): no fp weight, no quantization pass."""
         assert bits in (4, 8)
         self = cls.__new__(cls)
         nn.Module.__init__(self)
         self.bits, self.group_size, self.use_kernel = bits, group_size, use_kernel
+        self.act_bits = _act_bits(act_bits, bits)
         self.out_features, self.in_features = w_q.shape[0], in_features
         want = in_features if bits == 8 else in_features // 2
         if w_q.dim() != 2 or w_q.shape[1] != want:
@@ -143,7 +158,13 @@ class QuantLinear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shape = x.shape
         flat = x.reshape(-1, self.in_features)
-        if self.use_kernel:
+        if self.act_bits == 8:
+            if self.use_kernel:
+                from kernels.int8_act import int8_dynamic_matmul
+                y = int8_dynamic_matmul(flat, self.w_q, self.scale)
+            else:
+                y = self.matmul_codes(*quantize_int8(flat.float()), flat.dtype)
+        elif self.use_kernel:
             from kernels.dequant_matmul import int4_matmul, int8_matmul
             if self.bits == 8:
                 y = int8_matmul(flat, self.w_q, self.scale)
@@ -153,29 +174,84 @@ class QuantLinear(nn.Module):
             y = flat @ self.dequant().to(flat.dtype).t()
         return y.reshape(*shape[:-1], self.out_features)
 
+    def matmul_codes(self, x_q: torch.Tensor, sx: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
+        """forward of an input that is quantized per token already: codes [M, K], scales [M]."""
+        if self.use_kernel:
+            from kernels.int8_act import int8_scaled_matmul
+            return int8_scaled_matmul(x_q, sx, self.w_q, self.scale, out_dtype=out_dtype)
+        return ((x_q.double() @ self.w_q.double().t()) * self.scale.double() * sx.double()[:, None]).to(out_dtype)
+
+
+class Int8SwiGLU(nn.Module):
+    """w_down(silu(w_gate(x)) * w_up(x)) of three QuantLinear(act_bits=8), under the names that the
+    reference's SwiGLU gives them (train/model.py:127-135): x is quantized once for gate and up, and the product
+    once more, in fp32, on its way to w_down."""
+
+    def __init__(self, w_gate: QuantLinear, w_up: QuantLinear, w_down: QuantLinear):
+        super().__init__()
+        for m in (w_gate, w_up, w_down):
+            if not (isinstance(m, QuantLinear) and m.act_bits == 8):
+                raise ValueError("Int8SwiGLU needs three QuantLinear with act_bits=8")
+        self.w_gate, self.w_up, self.w_down = w_gate, w_up, w_down
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        flat = x.reshape(-1, x.shape[-1])
+        if not self.w_gate.use_kernel:
+            xq = quantize_int8(flat.float())
+            g, u = (m.matmul_codes(*xq, flat.dtype).float() for m in (self.w_gate, self.w_up))
+            h = quantize_int8(g * torch.sigmoid(g) * u)
+        else:
+            from kernels.int8_act import quantize_rows, silu_mul_quantize
+            # (up to 16 rows the product quantizes them itself: one launch less)
+            if flat.shape[0] <= 16:
+                g, u = self.w_gate(flat), self.w_up(flat)
+            else:
+                xq = quantize_rows(flat)
+                g, u = (m.matmul_codes(*xq, flat.dtype) for m in (self.w_gate, self.w_up))
+            h = silu_mul_quantize(g, u)
+        return self.w_down.matmul_codes(*h, flat.dtype).reshape(*x.shape[:-1], self.w_down.out_features)
+
 
 _ATTN_SLOTS = ("wq", "wk", "wv", "wo")
 _MLP_SLOTS = ("w_gate", "w_up", "w_down")
 
 
+def _fuse_int8_mlps(model: nn.Module) -> None:
+    """Every SwiGLU of the blocks whose three projections have act_bits=8 becomes an Int8SwiGLU."""
+    def fused(m):
+        lins = [getattr(m, n, None) for n in _MLP_SLOTS]
+        ok = not isinstance(m, Int8SwiGLU) and all(isinstance(q, QuantLinear) and q.act_bits == 8 for q in lins)
+        return Int8SwiGLU(*lins).train(m.training) if ok else m
+    for blk in getattr(model, "blocks", []):
+        if getattr(blk, "is_moe", False):
+            for i, m in enumerate(blk.mlp.experts):
+                blk.mlp.experts[i] = fused(m)
+        elif hasattr(blk, "mlp"):
+            blk.mlp = fused(blk.mlp)
+
+
 def quantize_model(model: nn.Module, bits: int = 8, group_size: int = 32,
-                   use_kernel: bool = True) -> nn.Module:
+                   use_kernel: bool = True, act_bits: int | None = None) -> nn.Module:
     """Replace all block linears with QuantLinear (router/embed/head stay fp)
     (serve/quantize.py:98-115). Walks model.blocks; each block's .attn holds
     wq/wk/wv/wo and its .mlp holds w_gate/w_up/w_down, or, when blk.is_moe,
-    .mlp.experts is a list of such MLPs."""
+    .mlp.experts is a list of such MLPs. act_bits=8 (with bits=8): their inputs are
+    quantized per token too, and the MLPs become Int8SwiGLU."""
     import copy
+    _act_bits(act_bits, bits)
     model = copy.deepcopy(model)
     for blk in model.blocks:
         a = blk.attn
         for name in _ATTN_SLOTS:
-            setattr(a, name, QuantLinear(getattr(a, name), bits, group_size, use_kernel))
+            setattr(a, name, QuantLinear(getattr(a, name), bits, group_size, use_kernel, act_bits))
         mods = blk.mlp.experts if getattr(blk, "is_moe", False) else [blk.mlp]
         for m in mods:
             for name in _MLP_SLOTS:
-                setattr(m, name, QuantLinear(getattr(m, name), bits, group_size, use_kernel))
+                setattr(m, name, QuantLinear(getattr(m, name), bits, group_size, use_kernel, act_bits))
         if getattr(blk, "is_moe", False):
             stacked_int4_experts(mods)
+    if act_bits is not None:
+        _fuse_int8_mlps(model)
     return model
 
 
@@ -270,7 +346,8 @@ def model_weight_bytes(model: nn.Module) -> int:
 # so a load is a copy to the device and quantization runs once, on the GPU.
 #
 # Header ("__metadata__"): format = "mls-quantized", version = "1", and per quantized
-# module "q:<module name>" = "<bits>,<group_size>,<in_features>". Tensors: the model's
+# module "q:<module name>" = "<bits>,<group_size>,<in_features>", and "a:<module name>" = "8" where its
+# input is quantized too. Tensors: the model's
 # state dict (the QuantLinear buffers under their state-dict names, every other
 # parameter and buffer as stored), each saved as its own contiguous copy.
 
@@ -285,10 +362,12 @@ def save_quantized(model: nn.Module, path, extra_metadata: dict | None = None) -
     for name, m in model.named_modules():
         if isinstance(m, QuantLinear):
             meta[f"q:{name}"] = f"{m.bits},{m.group_size},{m.in_features}"
+            if m.act_bits is not None:
+                meta[f"a:{name}"] = str(m.act_bits)
     if len(meta) == 2:
         raise ValueError("save_quantized: the model holds no QuantLinear (run quantize_model first)")
     for k, v in (extra_metadata or {}).items():
-        if k in meta or k.startswith("q:"):
+        if k in meta or k.startswith(("q:", "a:")):
             raise ValueError(f"save_quantized: metadata key {k!r} is reserved")
         meta[k] = str(v)
     tensors = {k: v.detach().contiguous().clone() for k, v in model.state_dict().items()}
@@ -337,7 +416,8 @@ def load_quantized(model: nn.Module, path, device=None, use_kernel: bool = True)
         if w_q.shape[0] != out_features or in_features != old.in_features:
             raise ValueError(f"load_quantized: {name} stores {w_q.shape[0]}x{in_features}, "
                              f"the model has {out_features}x{old.in_features}")
-        _set_submodule(model, name, QuantLinear.from_quantized(w_q, scale, bits, group, in_features, use_kernel))
+        act = int(meta[f"a:{name}"]) if f"a:{name}" in meta else None
+        _set_submodule(model, name, QuantLinear.from_quantized(w_q, scale, bits, group, in_features, use_kernel, act))
     if dev is not None:
         model.to(dev)
     missing, unexpected = model.load_state_dict(tensors, strict=False)
@@ -346,6 +426,7 @@ def load_quantized(model: nn.Module, path, device=None, use_kernel: bool = True)
     missing = [k for k in missing if k not in quant_keys]
     if missing or unexpected:
         raise ValueError(f"load_quantized: missing {missing[:5]}, unexpected {unexpected[:5]}")
+    _fuse_int8_mlps(model)
     for blk in getattr(model, "blocks", []):
         if getattr(blk, "is_moe", False):
             stacked_int4_experts(blk.mlp.experts)

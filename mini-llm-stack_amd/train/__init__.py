@@ -1,6 +1,6 @@
-"""FP8 linear training caller of the gfx950 fp8 GEMM.
+"""FP8 and INT8 linear training callers of the gfx950 GEMMs.
 
-This package provides only ``train.fp8``. Its search path is extended over every
+This package provides ``train.fp8`` and ``train.int8``. Its search path is extended over every
 ``train`` directory on ``sys.path`` (pkgutil.extend_path), so a reference checkout
 placed after this directory still supplies the model, config, training loop and
 parallel modules, which then bind this ``train.fp8``.

@@ -1,0 +1,182 @@
+"""INT8 training layers whose activations live in 8 bits, on the gfx950 kernels (no reference counterpart; its
+INT8 estimator, kernels/autograd_ops.py:95-134, quantizes the weight alone and keeps x in full width).
+
+Forward: the weight (per output row) and the input (per token) are quantized, and their codes meet on the 8-bit
+matrix cores. What a layer keeps for its backward is those codes: a quarter of fp32's bytes, half of 16-bit types'.
+Backward, straight through both quantizers: dx = dy times the quantized weight, dw = dy^T times the kept codes,
+each operand the one that the forward used.
+
+Int8SwiGLU is a whole MLP, w_down(silu(w_gate(x)) * w_up(x)): the product goes to w_down as codes made in the
+kernel that computes it, and gate and up are kept in 8 bits with a scale for every 128 columns. For a batch of M
+tokens it keeps M (dim + 3 hidden) bytes and scales, where the plain layers keep M (dim + 3 hidden) values and silu's own.
+
+use_kernel=False runs the same arithmetic in torch ops, on the host or a device.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from serve.quantize import quantize_int8
+
+_GROUP = 128
+
+
+def _rows(x, use_kernel):
+    """Codes and scales of x's rows."""
+    if use_kernel:
+        from kernels.int8_act import quantize_rows
+        return quantize_rows(x)
+    return quantize_int8(x.float())
+
+
+def _matmul(x_q, sx, w_q, sw, bias, dtype, use_kernel):
+    if use_kernel:
+        from kernels.int8_act import int8_scaled_matmul
+        return int8_scaled_matmul(x_q, sx, w_q, sw, bias, out_dtype=dtype)
+    y = (x_q.double() @ w_q.double().t()) * sw.double() * sx.double()[:, None]
+    return (y if bias is None else y + bias.double()).to(dtype)
+
+
+def _input_grad(dy, w_q, sw, use_kernel):
+    if use_kernel:
+        from kernels.dequant_matmul import int8_dgrad
+        return int8_dgrad(dy, w_q, sw)
+    return (dy.float() @ (w_q.float() * sw.float()[:, None])).to(dy.dtype)
+
+
+def _weight_grad(dy, x_q, sx, use_kernel, dtype):
+    if use_kernel:
+        from kernels.int8_act import int8_weight_grad
+        return int8_weight_grad(dy, x_q, sx).to(dtype)
+    return (dy.float().t() @ (x_q.float() * sx[:, None])).to(dtype)
+
+
+def _silu_mul(g, u, use_kernel, keep):
+    """Codes and scales of silu(g) * u, and gate and up in 8 bits where they are kept."""
+    if use_kernel:
+        from kernels.int8_act import silu_mul_quantize
+        return silu_mul_quantize(g, u, checkpoint=True) if keep else (*silu_mul_quantize(g, u), None)
+    M, H = g.shape
+    g, u = g.float(), u.float()
+    kept = None
+    if keep:
+        pad = nn.functional.pad(torch.stack([g, u]), (0, -H % _GROUP))
+        q, s = quantize_int8(pad.reshape(-1, _GROUP))
+        kept = q.reshape(2, M, -1)[..., :H], s.reshape(2, M, -1)
+    return *quantize_int8(g * torch.sigmoid(g) * u), kept
+
+
+def _silu_mul_grad(dh, kept, use_kernel):
+    if use_kernel:
+        from kernels.int8_act import silu_mul_backward
+        return silu_mul_backward(dh, kept)
+    q, s = kept
+    g, u = q.float() * s.repeat_interleave(_GROUP, 2)[..., :q.shape[2]]
+    d, sig = dh.float(), torch.sigmoid(g)
+    return (d * u * sig * (1 + g * (1 - sig))).to(dh.dtype), (d * g * sig).to(dh.dtype)
+
+
+class _Int8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, use_kernel):
+        w_q, sw = _rows(w, use_kernel)
+        x_q, sx = _rows(x, use_kernel)
+        ctx.use_kernel, ctx.dtypes = use_kernel, (w.dtype, None if bias is None else bias.dtype)
+        need_x, need_w = ctx.needs_input_grad[:2]
+        ctx.save_for_backward(*((w_q, sw) if need_x else (None, None)), *((x_q, sx) if need_w else (None, None)))
+        return _matmul(x_q, sx, w_q, sw, bias, x.dtype, use_kernel)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        w_q, sw, x_q, sx = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        wt, bt = ctx.dtypes
+        dx = _input_grad(dy, w_q, sw, ctx.use_kernel) if need_x else None
+        dw = _weight_grad(dy, x_q, sx, ctx.use_kernel, wt) if need_w else None
+        return dx, dw, dy.sum(0, dtype=torch.float32).to(bt) if need_b else None, None
+
+
+class _Int8SwiGLUFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, use_kernel):
+        grad = any(ctx.needs_input_grad[:4])
+        weights = [_rows(w, use_kernel) for w in (w_gate, w_up, w_down)]
+        x_q, sx = _rows(x, use_kernel)
+        g, u = (_matmul(x_q, sx, *w, None, x.dtype, use_kernel) for w in weights[:2])
+        h_q, sh, kept = _silu_mul(g, u, use_kernel, grad)
+        ctx.use_kernel, ctx.dtypes = use_kernel, (w_gate.dtype, w_up.dtype, w_down.dtype)
+        if grad:
+            ctx.save_for_backward(x_q, sx, h_q, sh, *kept, *(t for w in weights for t in w))
+        return _matmul(h_q, sh, *weights[2], None, x.dtype, use_kernel)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x_q, sx, h_q, sh, kq, ks, gq, gs, uq, us, dq, ds = ctx.saved_tensors
+        k, (tg, tu, td) = ctx.use_kernel, ctx.dtypes
+        need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
+        dwd = _weight_grad(dy, h_q, sh, k, td) if need_d else None
+        if not (need_x or need_g or need_u):
+            return None, None, None, dwd, None
+        dg, du = _silu_mul_grad(_input_grad(dy, dq, ds, k), (kq, ks), k)
+        dwg = _weight_grad(dg, x_q, sx, k, tg) if need_g else None
+        dwu = _weight_grad(du, x_q, sx, k, tu) if need_u else None
+        dx = _input_grad(dg, gq, gs, k).add_(_input_grad(du, uq, us, k)) if need_x else None
+        return dx, dwg, dwu, dwd, None
+
+
+class Int8Linear(nn.Module):
+    """A linear layer for training with INT8 products: the parameters keep their dtype and are quantized at every
+    forward; x may be float32, float16 or bfloat16, and y has its dtype."""
+
+    def __init__(self, linear: nn.Linear, use_kernel: bool = True):
+        super().__init__()
+        self.weight = nn.Parameter(linear.weight.detach().clone())
+        self.bias = None if linear.bias is None else nn.Parameter(linear.bias.detach().clone())
+        self.use_kernel = use_kernel
+
+    def forward(self, x):
+        y = _Int8LinearFn.apply(x.reshape(-1, x.shape[-1]), self.weight, self.bias, self.use_kernel)
+        return y.reshape(*x.shape[:-1], self.weight.shape[0])
+
+
+class Int8SwiGLU(nn.Module):
+    """w_down(silu(w_gate(x)) * w_up(x)) for training with INT8 products and 8-bit activations, under the
+    parameter names of the reference's SwiGLU (train/model.py:127-135). No biases."""
+
+    def __init__(self, w_gate: nn.Linear, w_up: nn.Linear, w_down: nn.Linear, use_kernel: bool = True):
+        super().__init__()
+        if any(m.bias is not None for m in (w_gate, w_up, w_down)):
+            raise ValueError("Int8SwiGLU: projections with biases")
+        self.w_gate, self.w_up, self.w_down = (Int8Linear(m, use_kernel) for m in (w_gate, w_up, w_down))
+        self.use_kernel = use_kernel
+
+    def forward(self, x):
+        y = _Int8SwiGLUFn.apply(x.reshape(-1, x.shape[-1]), self.w_gate.weight, self.w_up.weight, self.w_down.weight,
+                                self.use_kernel)
+        return y.reshape(*x.shape[:-1], self.w_down.weight.shape[0])
+
+
+def convert_linears_to_int8(model: nn.Module, use_kernel: bool = True) -> nn.Module:
+    """A copy of the model whose attention projections (wq/wk/wv/wo) are Int8Linear and whose SwiGLU MLPs (modules with
+    w_gate/w_up/w_down) are Int8SwiGLU; embeddings, head, router and norms stay as they are. Modules are recognised by their slot names, as
+    train.fp8.convert_linears_to_fp8 does; the state dict keeps its names."""
+    import copy
+    model = copy.deepcopy(model)
+    slots = lambda m, names: [getattr(m, n, None) for n in names]
+    linears = lambda ms: all(isinstance(m, nn.Linear) for m in ms)
+    for m in list(model.modules()):
+        attn = slots(m, ("wq", "wk", "wv", "wo"))
+        if linears(attn):
+            for n, lin in zip(("wq", "wk", "wv", "wo"), attn):
+                setattr(m, n, Int8Linear(lin, use_kernel))
+        for name, child in list(m.named_children()):
+            mlp = slots(child, ("w_gate", "w_up", "w_down"))
+            if linears(mlp):
+                setattr(m, name, Int8SwiGLU(*mlp, use_kernel=use_kernel).train(child.training))
+    mlp = slots(model, ("w_gate", "w_up", "w_down"))
+    return Int8SwiGLU(*mlp, use_kernel=use_kernel).train(model.training) if linears(mlp) else model
