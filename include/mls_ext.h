@@ -136,7 +136,8 @@ int mlsx_quantize_rows(const void* x, int dt, int64_t ldx, int64_t M, int64_t K,
 /* c[m][n] = (sum_k x[m][k] w[n][k]) sw[n] sx[m] + bias[n], type c_dt, [M][ldc]. w: int8 [N][ldw]; sw: sw_dt (fp32 or
  * fp16) [N]; bias: bias_dt [N], or null. x_dt -1: x holds codes int8 [M][ldx], sx their scales fp32 [M];
  * otherwise x holds values of that type, quantized by rows as above, and sx is not read. 1 <= K <= 131071
- * (sums of 32 bits). Every field has 8 bytes. The 16-byte aligned workspace holds mlsx_a8w8_ws bytes (0: none). */
+ * (sums of 32 bits). Every field has 8 bytes. The 16-byte aligned workspace holds mlsx_a8w8_ws bytes (0: none); a call that
+ * needs one and has none (ws null, ws_bytes 0) enqueues nothing and returns those bytes. */
 typedef struct mlsx_a8w8_args {
   const void* x;
   const float* sx;
@@ -146,7 +147,7 @@ typedef struct mlsx_a8w8_args {
   int64_t x_dt, sw_dt, bias_dt, c_dt, ldx, ldw, ldc, M, N, K;
 } mlsx_a8w8_args;
 int64_t mlsx_a8w8_ws(const mlsx_a8w8_args* args);
-int mlsx_a8w8(const mlsx_a8w8_args* args, void* ws, int64_t ws_bytes, mls_stream_t stream);
+int64_t mlsx_a8w8(const mlsx_a8w8_args* args, void* ws, int64_t ws_bytes, mls_stream_t stream);
 
 /* Codes and scales, as mlsx_quantize_rows, of silu(gate) * up (fp32; gate, up: dt, [M][ld]). kept_q, kept_s (both or
  * neither null): codes int8 [2][M][H] and scales fp32 [2][M][ceil(H / 128)] of gate and up by groups of 128

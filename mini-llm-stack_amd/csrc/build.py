@@ -47,6 +47,8 @@ EXTRA_FLAGS = {"gemv.hip": PRELOAD,
                "gemm_grouped.hip": VGPR_FORM,
                "grouped_skinny.hip": VGPR_FORM,
                "gemm_dw.hip": VGPR_FORM,
+               "gemm_a8.hip": VGPR_FORM,
+               "gemm_dw8.hip": VGPR_FORM,
                "paged_gqa_f32.hip": VGPR_FORM,
                "paged_gqa_f16.hip": VGPR_FORM,
                "paged_gqa_bf16.hip": VGPR_FORM,

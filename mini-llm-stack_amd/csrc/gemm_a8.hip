@@ -34,14 +34,13 @@ __device__ __forceinline__ float float_at(const void* p, int dt, int64_t i) {
 // already small.
 __device__ __forceinline__ float scaled(int acc, float sw, float sx, float bias) { return (float)acc * sw * sx + bias; }
 
-__device__ __forceinline__ i32x4 mma8(const uint4& a, const uint4& b, const i32x4& c) {
-  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+__device__ __forceinline__ i32x4 mma8(const i32x4& a, const i32x4& b, const i32x4& c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
 struct Int8Op {
   using Acc = i32x4;
-  static constexpr bool kZeroB = false;  // whole numbers times zero are zero
-  __device__ static __forceinline__ i32x4 mma(const uint4& a, const uint4& b, const i32x4& c) { return mma8(a, b, c); }
+  __device__ static __forceinline__ i32x4 mma(const i32x4& a, const i32x4& b, const i32x4& c) { return mma8(a, b, c); }
 };
 
 // ---------------------------------------------------------------- tiles
@@ -54,38 +53,62 @@ struct TileArgs {
   int m_tiles, n_tiles, splits;
 };
 
-template <typename CT, int BM, int BN, int WM, int WN, bool PARTIAL>
-__global__ __launch_bounds__(64 * WM * WN) void a8_tile_kernel(const TileArgs p) {
-  using T = NtTile<Int8Op, BM, BN, WM, WN>;
+// T: a form of tile (nt_tile.h)
+template <typename CT, class T, bool PARTIAL>
+__global__ __launch_bounds__(T::THREADS) void a8_tile_kernel(const TileArgs p) {
+  extern __shared__ __align__(16) uint8_t lds[];
   int sp, mt, nt;
   nt_place(p.m_tiles, p.n_tiles, sp, mt, nt);
   const int units = (p.o.K + 127) / 128;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   i32x4 acc[T::TN][T::TM];
-  T::run(p.o, mt * BM, nt * BN, (int)((int64_t)units * sp / p.splits), (int)((int64_t)units * (sp + 1) / p.splits), wave,
-         lane, acc);
-  const int N = p.o.N;
-  T::each(p.o, mt * BM, nt * BN, wave, lane, acc, [&](int m, int n, const i32x4& v) __attribute__((always_inline)) {
-    const bool whole = n + 3 < N;
-    if constexpr (PARTIAL) {
-      int* dst = (int*)p.c + ((int64_t)sp * p.o.M + m) * N + n;
-      if (whole && N % 4 == 0) {
-        *reinterpret_cast<int4*>(dst) = make_int4(v[0], v[1], v[2], v[3]);
-      } else {
+  if (!T::run(p.o, lds, mt * T::BM, nt * T::BN, (int)((int64_t)units * sp / p.splits), (int)((int64_t)units * (sp + 1) / p.splits), wave,
+              lane, acc))
+    return;
+  const int M = p.o.M, N = p.o.N, m0 = T::row(mt * T::BM, wave, lane), n0 = T::column(nt * T::BN, wave, lane);
+  if constexpr (PARTIAL) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < N) dst[e] = v[e];
+    for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+      for (int j = 0; j < T::TM; ++j) {
+        const int m = m0 + 16 * j, n = n0 + 16 * i;
+        if (m >= M || n >= N) continue;
+        const i32x4 v = acc[i][j];
+        int* dst = (int*)p.c + ((int64_t)sp * M + m) * N + n;
+        if (n + 3 < N && N % 4 == 0) {
+          *reinterpret_cast<int4*>(dst) = make_int4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < N) dst[e] = v[e];
+        }
       }
-    } else {
-      const float sx = p.s.sx[m];
+    return;
+  }
+  // all scales before the first store, which they would otherwise wait for one by one
+  float sx[T::TM], sw[T::TN][4], bias[T::TN][4];
+#pragma unroll
+  for (int j = 0; j < T::TM; ++j) sx[j] = p.s.sx[min(m0 + 16 * j, M - 1)];
+#pragma unroll
+  for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = min(n0 + 16 * i + e, N - 1);
+      sw[i][e] = float_at(p.s.sw, p.s.sw_dt, n);
+      bias[i][e] = p.s.bias ? float_at(p.s.bias, p.s.bias_dt, n) : 0.0f;
+    }
+  const bool v4 = p.ldc % 4 == 0 && ((uintptr_t)p.c & (4 * sizeof(CT) - 1)) == 0;
+#pragma unroll
+  for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+    for (int j = 0; j < T::TM; ++j) {
+      const int m = m0 + 16 * j, n = n0 + 16 * i;
+      if (m >= M || n >= N) continue;
       CT* dst = (CT*)p.c + (int64_t)m * p.ldc + n;
       float y[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int ne = min(n + e, N - 1);
-        y[e] = scaled(v[e], float_at(p.s.sw, p.s.sw_dt, ne), sx, p.s.bias ? float_at(p.s.bias, p.s.bias_dt, ne) : 0.0f);
-      }
-      if (whole && p.ldc % 4 == 0 && ((uintptr_t)p.c & (4 * sizeof(CT) - 1)) == 0) {
+      for (int e = 0; e < 4; ++e) y[e] = scaled(acc[i][j][e], sw[i][e], sx[j], bias[i][e]);
+      if (n + 3 < N && v4) {
         store4<CT>(dst, y[0], y[1], y[2], y[3]);
       } else {
 #pragma unroll
@@ -93,7 +116,6 @@ __global__ __launch_bounds__(64 * WM * WN) void a8_tile_kernel(const TileArgs p)
           if (n + e < N) dst[e] = from_f32<CT>(y[e]);
       }
     }
-  });
 }
 
 // Adds the K ranges' sums: 4 columns a thread.
@@ -149,12 +171,12 @@ constexpr int kFewWaves = 16;
 template <typename XT, typename CT, int C>
 __global__ __launch_bounds__(64 * kFewWaves) void a8_few_kernel(const FewArgs p) {
   constexpr bool CODES = __is_same(XT, int8_t);
-  constexpr int U = 2;  // steps in flight
   extern __shared__ __align__(16) uint8_t codes[];  // [M][ldq]
   __shared__ __align__(16) int sums[kFewWaves][64][4];
   __shared__ uint32_t tops[kFewWaves];
   __shared__ float scales[16];
 
+  constexpr int U = 2;  // steps in flight
   const int n0 = blockIdx.x * 16;
   const int lane = threadIdx.x & 63, lr = lane & 15, lk = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -228,19 +250,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void a8_few_kernel(const FewArgs p)
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) acc = mma8(wv[u][h], xv[u][h], acc);
+      for (int h = 0; h < 2; ++h) acc = mma8(__builtin_bit_cast(i32x4, wv[u][h]), __builtin_bit_cast(i32x4, xv[u][h]), acc);
     if (step + U * kFewWaves < steps) load_w(step + U * kFewWaves);
   }
   *reinterpret_cast<int4*>(sums[wave][lane]) = make_int4(acc[0], acc[1], acc[2], acc[3]);
   __syncthreads();
-  const int t = threadIdx.x, m = t / 16, n = t % 16;
-  if (m >= p.M || m >= 16 || n0 + n >= p.N) return;
+  const int t = threadIdx.x, m = t / 16, n = n0 + t % 16;
+  if (m >= min(p.M, 16) || n >= p.N) return;
   int total = 0;
 #pragma unroll
-  for (int i = 0; i < kFewWaves; ++i) total += sums[i][n / 4 * 16 + m][n % 4];
+  for (int i = 0; i < kFewWaves; ++i) total += sums[i][t % 16 / 4 * 16 + m][t % 4];
   const float sx = CODES ? p.s.sx[m] : scales[m];
-  ((CT*)p.c)[m * p.ldc + n0 + n] = from_f32<CT>(scaled(total, float_at(p.s.sw, p.s.sw_dt, n0 + n), sx,
-                                                        p.s.bias ? float_at(p.s.bias, p.s.bias_dt, n0 + n) : 0.0f));
+  ((CT*)p.c)[m * p.ldc + n] =
+      from_f32<CT>(scaled(total, float_at(p.s.sw, p.s.sw_dt, n), sx, p.s.bias ? float_at(p.s.bias, p.s.bias_dt, n) : 0.0f));
 }
 
 // Chunks of 8 values a lane that quantizing M rows of K takes in a few-rows block.
@@ -252,13 +274,45 @@ int few_chunks(int64_t M, int64_t K) {
 
 // ---------------------------------------------------------------- host
 
+// The forms of tile, and what they take: us a stage of 128 k on a CU, alone (first) and with all CUs at work. From
+// timed calls of 48 to 4096 rows with weights that no cache holds. A CU takes its blocks one after another or side by side; either way their
+// stages add up, bound by what its L1 gives (64 bytes a clock: 64 x 64 reads four times as much a product as 256 x 256)
+// and, at 256 x 256, by the matrix cores at the clock that they leave it (64 x 64 x 128 on every CU of 4096 x 8192 x 8192).
+struct TileForm {
+  int bm, bn;
+  float alone, busy;
+};
+constexpr TileForm kForms[] = {{64, 64, 0.24f, 0.23f}, {128, 64, 0.36f, 0.45f}, {128, 128, 0.52f, 0.60f}, {128, 128, 9.0f, 0.55f}, {256, 256, 1.35f, 1.85f}};
+
 struct Plan {
   bool few, fused;        // the kernel for few rows; which quantizes x itself
   bool pad_w, own_x;      // operands copied (or codes made) into the workspace
   int64_t kpad;
-  int tile, splits;       // tile: side
+  int form, splits;       // of kForms; K ranges
   int64_t x_at, s_at, w_at, part_at, bytes;
 };
+
+// The quickest form and number of K ranges by these figures: 4 us for a launch and its first stage; K ranges cost a second launch
+// and their sums' way through memory. (333 x 4096 x 11008: 128 x 128 in two ranges 35 us, whole 49, 128 x 64 35, 64 x 64 43.)
+void choose_form(int64_t M, int64_t N, int64_t K, Plan& p) {
+  const int64_t units = cdiv(K, 128);
+  float best = 3e38f;
+  for (int f = 0; f < 5; ++f) {
+    const TileForm& t = kForms[f];
+    const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn);
+    for (int s = 1; s <= (f < 3 ? 8 : 1) && (s == 1 || units / s >= 4); ++s) {
+      const int64_t deep = cdiv(tiles * s, 256);
+      const float stage = deep > 1 ? t.busy : t.alone + (t.busy - t.alone) * (float)(tiles * s) / 256.0f;
+      const float us = 4.0f + (float)(deep * cdiv(units, s)) * (f == 3 && deep == 1 ? t.alone : stage) +
+                       (s > 1 ? 6.0f + (float)s * (float)M * (float)N * 4.0f / 2.5e6f : 0.0f);
+      if (us < best) {
+        best = us;
+        p.form = f;
+        p.splits = s;
+      }
+    }
+  }
+}
 
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -272,15 +326,11 @@ Plan make_plan(const mlsx_a8w8_args& a) {
   p.kpad = (a.K + 15) / 16 * 16;
   p.pad_w = !rows_fit(a.w, a.ldw, a.K);
   p.few = a.M <= 16;
-  p.fused = a.x_dt == a.c_dt && p.few && few_chunks(a.M, a.K) <= 8;
+  // a block's quantizing takes about 0.25 us a chunk, in every round of blocks; a launch of its own 3 us
+  p.fused = a.x_dt == a.c_dt && p.few && few_chunks(a.M, a.K) <= 6 && few_chunks(a.M, a.K) * cdiv(a.N, 4096) <= 6;
   p.own_x = codes ? !rows_fit(a.x, a.ldx, a.K) : !p.fused;
-  const bool big = a.M > 128 && cdiv(a.M, 256) * cdiv(a.N, 256) >= 128;
-  p.tile = big ? 256 : 128;
   p.splits = 1;
-  if (!p.few && !big) {
-    const int64_t tiles = cdiv(a.M, 128) * cdiv(a.N, 128), units = cdiv(a.K, 128);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, units / 4, 16}));
-  }
+  if (!p.few) choose_form(a.M, a.N, a.K, p);
   int64_t at = 0;
   if (p.own_x) {
     p.x_at = at;
@@ -300,20 +350,27 @@ Plan make_plan(const mlsx_a8w8_args& a) {
   return p;
 }
 
-template <typename CT, int B, int WM, int WN>
-int launch_tile(TileArgs t, void* part, hipStream_t st) {
-  t.m_tiles = (int)cdiv(t.o.M, B);
-  t.n_tiles = (int)cdiv(t.o.N, B);
+template <typename CT, class T, bool PARTIAL>
+int launch_tiles(TileArgs t, hipStream_t st) {
+  t.m_tiles = (int)cdiv(t.o.M, T::BM);
+  t.n_tiles = (int)cdiv(t.o.N, T::BN);
   const int64_t blocks = (int64_t)t.m_tiles * t.n_tiles * t.splits;
   if (blocks > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "a8w8: %d x %d", t.o.M, t.o.N);
-  if (t.splits == 1) {
-    hipLaunchKernelGGL((a8_tile_kernel<CT, B, B, WM, WN, false>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, st, t);
-    return check_launch("a8w8");
-  }
+  auto kern = a8_tile_kernel<CT, T, PARTIAL>;
+  constexpr int lds = T::LDS;
+  // (a call a launch: the limit is the function's on the current device)
+  if (lds > 32768 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+    return fail(MLS_ERR_HIP, "a8w8: cannot reserve %d bytes of LDS", lds);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(T::THREADS), lds, st, t);
+  return check_launch("a8w8");
+}
+
+template <typename CT, class T>
+int launch_tile(TileArgs t, void* part, hipStream_t st) {
+  if (t.splits == 1) return launch_tiles<CT, T, false>(t, st);
   void* c = t.c;
   t.c = part;
-  hipLaunchKernelGGL((a8_tile_kernel<CT, B, B, WM, WN, true>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, st, t);
-  if (const int rc = check_launch("a8w8")) return rc;
+  if (const int rc = launch_tiles<CT, T, true>(t, st)) return rc;
   hipLaunchKernelGGL(a8_join_kernel<CT>, dim3((unsigned)cdiv(t.o.N, 1024), (unsigned)t.o.M), dim3(256), 0, st, (const int*)part,
                      t.splits, (CT*)c, t.ldc, t.s, t.o.M, t.o.N);
   return check_launch("a8w8 (join)");
@@ -334,7 +391,7 @@ int launch_fused(const FewArgs& f, int chunks, hipStream_t st) {
   if (chunks <= 1) return launch_few<T, T, 1>(f, st);
   if (chunks <= 2) return launch_few<T, T, 2>(f, st);
   if (chunks <= 4) return launch_few<T, T, 4>(f, st);
-  return launch_few<T, T, 8>(f, st);
+  return launch_few<T, T, 6>(f, st);
 }
 
 template <typename CT>
@@ -372,8 +429,14 @@ int run(const mlsx_a8w8_args& a, const Plan& p, uint8_t* ws, hipStream_t st) {
     return launch_fused<CT>(f, few_chunks(a.M, a.K), st);
   }
   TileArgs t{{x, w, (int)ldx, (int)ldw, (int)a.M, (int)a.N, (int)K}, a.c, s, a.ldc, 0, 0, p.splits};
-  if (p.tile == 256) return launch_tile<CT, 256, 2, 4>(t, nullptr, st);
-  return launch_tile<CT, 128, 2, 2>(t, ws + p.part_at, st);
+  void* part = ws + p.part_at;
+  switch (p.form) {
+    case 0: return launch_tile<CT, NtSmall<Int8Op, 64, 64, 5, 4, 4>>(t, part, st);
+    case 1: return launch_tile<CT, NtSmall<Int8Op, 128, 64, 6, 4, 4>>(t, part, st);
+    case 2: return launch_tile<CT, NtSmall<Int8Op, 128, 128, 4, 8, 4>>(t, part, st);
+    case 3: return launch_tiles<CT, NtTile<Int8Op, 128, 2>, false>(t, st);
+    default: return launch_tiles<CT, NtTile<Int8Op, 256, 2>, false>(t, st);
+  }
 }
 
 int check_args(const mlsx_a8w8_args& a, const char* fn) {
@@ -400,12 +463,13 @@ extern "C" int64_t mlsx_a8w8_ws(const mlsx_a8w8_args* args) {
   return make_plan(*args).bytes;
 }
 
-extern "C" int mlsx_a8w8(const mlsx_a8w8_args* args, void* ws, int64_t ws_bytes, mls_stream_t stream) {
+extern "C" int64_t mlsx_a8w8(const mlsx_a8w8_args* args, void* ws, int64_t ws_bytes, mls_stream_t stream) {
   const char* fn = "mlsx_a8w8";
   if (!args) return fail(MLS_ERR_ARG, "%s: null pointer", fn);
   if (const int rc = check_args(*args, fn)) return rc;
   if (args->M == 0 || args->N == 0) return MLS_OK;
   const Plan p = make_plan(*args);
+  if (p.bytes && !ws && ws_bytes == 0) return p.bytes;
   if (p.bytes > ws_bytes || (p.bytes && (!ws || !aligned(ws, 16)))) return fail(MLS_ERR_ARG, "%s: workspace too small or misaligned", fn);
   const hipStream_t st = (hipStream_t)stream;
   if (args->c_dt == MLS_F32) return run<float>(*args, p, (uint8_t*)ws, st);

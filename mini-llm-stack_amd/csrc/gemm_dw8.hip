@@ -17,8 +17,9 @@ namespace {
 template <typename T>
 struct Op16 {
   using Acc = f32x4;
-  static constexpr bool kZeroB = true;  // (a zero times an infinity would be NaN)
-  __device__ static __forceinline__ f32x4 mma(const uint4& a, const uint4& b, const f32x4& c) { return Mfma16<T>::mma(a, b, c); }
+  __device__ static __forceinline__ f32x4 mma(const i32x4& a, const i32x4& b, const f32x4& c) {
+    return Mfma16<T>::mma(__builtin_bit_cast(uint4, a), __builtin_bit_cast(uint4, b), c);
+  }
 };
 
 struct TurnArgs {
@@ -77,28 +78,36 @@ struct Dw8Args {
   int m_tiles, n_tiles, splits;
 };
 
-template <typename T, int B, int WM, int WN, bool PARTIAL>
-__global__ __launch_bounds__(64 * WM * WN) void dw8_kernel(const Dw8Args p) {
-  using G = NtTile<Op16<T>, B, B, WM, WN>;
+template <typename T, int B, int NB, bool PARTIAL>
+__global__ __launch_bounds__(512) void dw8_kernel(const Dw8Args p) {
+  using G = NtTile<Op16<T>, B, NB>;
+  extern __shared__ __align__(16) uint8_t lds[];
   int sp, mt, nt;
   nt_place(p.m_tiles, p.n_tiles, sp, mt, nt);
   const int units = (p.o.K + 127) / 128;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x4 acc[G::TN][G::TM];
-  G::run(p.o, mt * B, nt * B, (int)((int64_t)units * sp / p.splits), (int)((int64_t)units * (sp + 1) / p.splits), wave, lane, acc);
+  (void)G::run(p.o, lds, mt * B, nt * B, (int)((int64_t)units * sp / p.splits), (int)((int64_t)units * (sp + 1) / p.splits), wave, lane, acc);
   using CT = std::conditional_t<PARTIAL, float, T>;
   CT* c = (CT*)p.c + (PARTIAL ? (int64_t)sp * p.o.M * p.ldc : 0);
   const bool v4 = p.ldc % 4 == 0 && ((uintptr_t)p.c & (4 * sizeof(CT) - 1)) == 0;
-  G::each(p.o, mt * B, nt * B, wave, lane, acc, [&](int m, int n, const f32x4& v) __attribute__((always_inline)) {
-    CT* dst = c + m * p.ldc + n;
-    if (n + 3 < p.o.N && v4) {
-      store4<CT>(dst, v[0], v[1], v[2], v[3]);
-    } else {
+  const int M = p.o.M, N = p.o.N, m0 = G::row(mt * B, wave, lane), n0 = G::column(nt * B, wave, lane);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.o.N) dst[e] = from_f32<CT>(v[e]);
+  for (int i = 0; i < G::TN; ++i)
+#pragma unroll
+    for (int j = 0; j < G::TM; ++j) {
+      const int m = m0 + 16 * j, n = n0 + 16 * i;
+      if (m >= M || n >= N) continue;
+      const f32x4 v = acc[i][j];
+      CT* dst = c + m * p.ldc + n;
+      if (n + 3 < N && v4) {
+        store4<CT>(dst, v[0], v[1], v[2], v[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < N) dst[e] = from_f32<CT>(v[e]);
+      }
     }
-  });
 }
 
 // Adds the ranges' sums in their order: 4 columns a thread; part [splits][N][ldp], ldp a multiple of 4.
@@ -158,6 +167,19 @@ DwPlan make_plan(int dt, int64_t M, int64_t N, int64_t K) {
   return p;
 }
 
+template <typename T, int B, int NB, bool PARTIAL>
+int launch_dw8(const Dw8Args& a, hipStream_t st) {
+  const char* fn = "mlsx_dw_int8";
+  const int64_t blocks = (int64_t)a.m_tiles * a.n_tiles * a.splits;
+  if (blocks > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "%s: %d x %d", fn, a.o.M, a.o.N);
+  auto kern = dw8_kernel<T, B, NB, PARTIAL>;
+  constexpr int lds = NtTile<Op16<T>, B, NB>::LDS;
+  if (lds > 32768 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+    return fail(MLS_ERR_HIP, "%s: cannot reserve %d bytes of LDS", fn, lds);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(512), lds, st, a);
+  return check_launch(fn);
+}
+
 template <typename T>
 int run16(const void* dy, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw, int64_t lddw, int64_t M, int64_t N,
           int64_t K, const DwPlan& p, uint8_t* ws, hipStream_t st) {
@@ -167,20 +189,10 @@ int run16(const void* dy, int64_t lddy, const int8_t* q, int64_t ldq, const floa
   if (const int rc = check_launch(fn)) return rc;
   const int ld = (int)p.Mp * 2;
   Dw8Args a{{ws, ws + p.xt_at, ld, ld, (int)N, (int)K, ld}, dw, lddw, (int)cdiv(N, p.tile), (int)cdiv(K, p.tile), p.splits};
-  const int64_t blocks = (int64_t)a.m_tiles * a.n_tiles * a.splits;
-  if (blocks > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "%s: %lld x %lld", fn, (long long)N, (long long)K);
-  if (p.tile == 256) {
-    hipLaunchKernelGGL((dw8_kernel<T, 256, 2, 4, false>), dim3((unsigned)blocks), dim3(512), 0, st, a);
-    return check_launch(fn);
-  }
-  if (p.splits == 1) {
-    hipLaunchKernelGGL((dw8_kernel<T, 128, 2, 2, false>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    return check_launch(fn);
-  }
+  if (p.splits == 1) return p.tile == 256 ? launch_dw8<T, 256, 2, false>(a, st) : launch_dw8<T, 128, 4, false>(a, st);
   a.c = ws + p.part_at;
   a.ldc = p.ldp;
-  hipLaunchKernelGGL((dw8_kernel<T, 128, 2, 2, true>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-  if (const int rc = check_launch(fn)) return rc;
+  if (const int rc = launch_dw8<T, 128, 4, true>(a, st)) return rc;
   hipLaunchKernelGGL(dw8_join_kernel<T>, dim3((unsigned)cdiv(K, 1024), (unsigned)N), dim3(256), 0, st,
                      (const float*)(ws + p.part_at), p.splits, p.ldp, (T*)dw, lddw, (int)N, (int)K);
   return check_launch(fn);

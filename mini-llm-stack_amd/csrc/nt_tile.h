@@ -1,13 +1,21 @@
-// A tile of a product of two matrices whose rows both run along the reduction axis: 128 bytes of every row a
-// stage, brought into LDS by loads that write it directly, two buffers, one barrier a stage.
+// A tile of a product of two matrices whose rows both run along the reduction axis, by two groups of wavefronts
+// half a stage apart.
 //
 // Op: the matrix instruction of 16 rows by 16 rows over 64 bytes of each (int8: 64 values, 16-bit types: 32):
 // Acc and mma(first, second, acc). Lane (lr, lk) = (lane & 15, lane >> 4) gives row lr's 16-byte chunk lk of both and
 // ends with the products of second's row lr and first's rows 4 lk .. 4 lk + 3.
 //
-// LDS: row r's chunk c lies in slot r * 8 + (c ^ (r & 7)), so that the 16 rows of an operand read, and the 8
-// lanes that fill a row, cover all banks. The LDS-direct loads write lane l's chunk to slot base + l: each lane loads
-// the chunk that belongs there.
+// A block is 8 wavefronts on a tile of B x B, group g = wavefronts 4 g .. 4 g + 3, one of each group on every SIMD. A step is 64 bytes
+// of every row. In phase 2 s + g group g moves step s from LDS to registers, in the next phase it multiplies, and the other group
+// does the opposite: the matrix cores always have a wavefront whose operands are there. A barrier ends a phase.
+//
+// A stage is two steps: 128 bytes of every row, whole cache lines (64 bytes a row and load: twice the requests, and L2 gives half as
+// much). LDS holds NB stages, filled by loads that write it directly, group 0 a's rows, group 1 b's. Stage t + NB - 1 is asked for
+// from phase 4 t on, when the last read of stage t - 1 is over, and waited for at the end of phase 4 (t + NB - 1) - 1, the last
+// before it is read.
+//
+// Row r's chunk c of a stage lies in slot r * 8 + (c ^ (r & 7)): the 16 rows of an operand cover all banks. Loads write
+// lane l's chunk to slot base + l, so each lane loads the chunk that belongs there.
 #pragma once
 
 #include "common.h"
@@ -44,35 +52,70 @@ __device__ __forceinline__ void nt_place(int m_tiles, int n_tiles, int& split, i
   nt = r / size;
 }
 
-template <class Op, int BM, int BN, int WM, int WN>
+// One stage's operands of a wavefront from LDS, waited for: a's 16-row tiles lie 2048 bytes apart from address
+// `a`, b's from `b`.
+template <int TM, int TN>
+__device__ __forceinline__ void nt_read(uint32_t a, uint32_t b, i32x4 (&x)[TM], i32x4 (&y)[TN]) {
+  static_assert((TM == 8 && TN == 4) || (TM == 4 && TN == 2) || (TM == 2 && TN == 1), "a half by a quarter of a square");
+  if constexpr (TM == 8) {
+    asm volatile(
+        "ds_read_b128 %8, %13\n\tds_read_b128 %0, %12\n\tds_read_b128 %9, %13 offset:2048\n\t"
+        "ds_read_b128 %10, %13 offset:4096\n\tds_read_b128 %11, %13 offset:6144\n\t"
+        "ds_read_b128 %1, %12 offset:2048\n\tds_read_b128 %2, %12 offset:4096\n\tds_read_b128 %3, %12 offset:6144\n\t"
+        "ds_read_b128 %4, %12 offset:8192\n\tds_read_b128 %5, %12 offset:10240\n\tds_read_b128 %6, %12 offset:12288\n\t"
+        "ds_read_b128 %7, %12 offset:14336\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7]), "=&v"(y[0]),
+          "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+        : "v"(a), "v"(b)
+        : "memory");
+  } else if constexpr (TM == 4) {
+    asm volatile(
+        "ds_read_b128 %4, %7\n\tds_read_b128 %0, %6\n\tds_read_b128 %5, %7 offset:2048\n\tds_read_b128 %1, %6 offset:2048\n\t"
+        "ds_read_b128 %2, %6 offset:4096\n\tds_read_b128 %3, %6 offset:6144\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1])
+        : "v"(a), "v"(b)
+        : "memory");
+  } else {
+    asm volatile("ds_read_b128 %2, %4\n\tds_read_b128 %0, %3\n\tds_read_b128 %1, %3 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(y[0])
+                 : "v"(a), "v"(b)
+                 : "memory");
+  }
+}
+
+template <class Op, int B, int NB>
 struct NtTile {
-  static constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
-  static constexpr int PA = BM * 8 / (64 * NW), PB = BN * 8 / (64 * NW);  // chunks a lane and stage
-  static_assert(PA >= 1 && PB >= 1 && BM * 8 % (64 * NW) == 0 && BN * 8 % (64 * NW) == 0, "whole loads");
+  static constexpr int BM = B, BN = B, THREADS = 512;
+  static constexpr int WTM = B / 2, WTN = B / 4, TM = WTM / 16, TN = WTN / 16;
+  static constexpr int STAGE = 2 * B * 128;  // bytes
+  static constexpr int LDS = NB * STAGE;
+  static constexpr int PW = B * 8 / 256;     // loads of 64 chunks a wavefront and stage
+  static_assert(B % 64 == 0 && NB >= 2 && (NB - 2) * PW < 64, "whole loads, and a count that vmcnt holds");
   using Acc = typename Op::Acc;
 
-  // Stages k_lo .. k_hi of 128 bytes of the tile at (m0, n0). acc[i][j]: b's rows wn0 + 16 i .., a's 16 j ..
-  __device__ static __forceinline__ void run(const NtOperands& p, int m0, int n0, int k_lo, int k_hi, int wave, int lane,
+  __device__ static __forceinline__ void phase_end() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // Stages k_lo .. k_hi of 128 bytes of the tile at (m0, n0), in `lds` of LDS bytes. acc[i][j]: b's rows
+  // 16 i .. of this wavefront's WTN, a's 16 j .. of its WTM.
+  __device__ static __forceinline__ bool run(const NtOperands& p, uint8_t* lds, int m0, int n0, int k_lo, int k_hi, int wave, int lane,
                                              Acc (&acc)[TN][TM]) {
-    // separate arrays: the loads into one pair are known not to touch the pair being read
-    __shared__ __align__(16) uint4 A0[BM * 8], B0[BN * 8], A1[BM * 8], B1[BN * 8];
-    const int wm0 = (wave / WN) * WTM, wn0 = (wave % WN) * WTN;
-    const __amdgpu_buffer_rsrc_t rsa = nt_rows(p.a, m0, p.lda, min(BM, p.M - m0), p.K);
-    const __amdgpu_buffer_rsrc_t rsb = nt_rows(p.b, n0, p.ldb, min(BN, p.N - n0), p.K);
-    const int lc = (lane & 7) ^ ((lane >> 3) & 7);
-    int a_off[PA], b_off[PB];
+    const int g = wave >> 2, w = wave & 3;
+    const __amdgpu_buffer_rsrc_t rs = g == 0 ? nt_rows(p.a, m0, p.lda, min(B, p.M - m0), p.K) : nt_rows(p.b, n0, p.ldb, min(B, p.N - n0), p.K);
+    const int ld = g == 0 ? p.lda : p.ldb;
+    const int lc = ((lane & 7) ^ ((lane >> 3) & 7)) * 16;  // (a load's 8 rows begin at a multiple of 8)
+    int off[PW];
 #pragma unroll
-    for (int i = 0; i < PA; ++i) a_off[i] = ((i * NW + wave) * 8 + (lane >> 3)) * p.lda + lc * 16;
-#pragma unroll
-    for (int i = 0; i < PB; ++i) b_off[i] = ((i * NW + wave) * 8 + (lane >> 3)) * p.ldb + lc * 16;
-    auto dma = [&](uint4* as, uint4* bs, int kt) __attribute__((always_inline)) {
-      const int k0 = kt * 128;
-      // past K: a reads zeros, and b whatever its next row holds
-      const bool in = k0 + lc * 16 < p.K;
-#pragma unroll
-      for (int i = 0; i < PA; ++i) nt_lds_load16(rsa, as + (i * NW + wave) * 64, in ? a_off[i] + k0 : kNtOutside);
-#pragma unroll
-      for (int i = 0; i < PB; ++i) nt_lds_load16(rsb, bs + (i * NW + wave) * 64, in || !Op::kZeroB ? b_off[i] + k0 : kNtOutside);
+    for (int i = 0; i < PW; ++i) off[i] = ((w * PW + i) * 8 + (lane >> 3)) * ld + lc;
+    uint8_t* const fill = lds + (g * B + w * PW * 8) * 128;
+    auto ask = [&](int i, int t, int buf) __attribute__((always_inline)) {
+      const int k0 = t * 128;
+      // past K, and past the last stage: zeros, and no memory is read
+      const bool in = t < k_hi && k0 + lc < p.K;
+      nt_lds_load16(rs, fill + buf * STAGE + i * 1024, in ? off[i] + k0 : kNtOutside);
     };
 #pragma unroll
     for (int i = 0; i < TN; ++i)
@@ -80,52 +123,168 @@ struct NtTile {
       for (int j = 0; j < TM; ++j) acc[i][j] = Acc{0, 0, 0, 0};
 
     const int lr = lane & 15, lk = lane >> 4;
-    // Stage kt lies in one pair of buffers; at its start the loads of stage kt + 1 go into the other pair,
-    // last read before the barrier that ended stage kt - 1. The closing wait covers them.
-    auto stage = [&](const uint4* as, const uint4* bs, uint4* an, uint4* bn, int kt) __attribute__((always_inline)) {
-      __builtin_amdgcn_sched_barrier(0);
-      if (kt + 1 < k_hi) dma(an, bn, kt + 1);
-      __builtin_amdgcn_sched_barrier(0);
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + lr * 128 + (lk ^ (lr & 7)) * 16;
+    const uint32_t at_a = base + g * WTM * 128, at_b = base + (B + w * WTN) * 128;
+
+    constexpr int left = (NB - 2) * PW;  // loads of later stages
+    constexpr int wait_code = (left & 15) | (left >> 4) << 14 | 0x70 | 0xF00;
+    for (int t = 0; t < NB - 1; ++t)
+#pragma unroll
+      for (int i = 0; i < PW; ++i) ask(i, k_lo + t, t);
+    __builtin_amdgcn_s_waitcnt(wait_code);
+    phase_end();
+    if (g == 1) phase_end();  // half a step later
+    int buf = 0;
+    for (int t = k_lo; t < k_hi; ++t) {
+      const int last = buf == 0 ? NB - 1 : buf - 1;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint4 bop[TN];
+        i32x4 x[TM], y[TN];
+        nt_read<TM, TN>((at_a + buf * STAGE) ^ (h * 64), (at_b + buf * STAGE) ^ (h * 64), x, y);
+        if (h == 1 && g == 1) __builtin_amdgcn_s_waitcnt(wait_code);
+        // half of the next stage's loads behind the first step's reads, half among its products: all of them at one place
+        // hold up that phase
+        if (h == 0) {
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < TN; ++i) {
-          const int row = wn0 + i * 16 + lr;
-          bop[i] = bs[row * 8 + ((lk + 4 * h) ^ (row & 7))];
+          for (int i = 0; i < PW / 2; ++i) ask(i, t + NB - 1, last);
         }
+        phase_end();
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
-          const int row = wm0 + j * 16 + lr;
-          const uint4 aop = as[row * 8 + ((lk + 4 * h) ^ (row & 7))];
 #pragma unroll
-          for (int i = 0; i < TN; ++i) acc[i][j] = Op::mma(bop[i], aop, acc[i][j]);
+          for (int i = 0; i < TN; ++i) acc[i][j] = Op::mma(y[i], x[j], acc[i][j]);
+          if (h == 0 && j < PW - PW / 2) {
+            __builtin_amdgcn_sched_barrier(0);
+            ask(PW / 2 + j, t + NB - 1, last);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (h == 1 && g == 0) __builtin_amdgcn_s_waitcnt(wait_code);
+        phase_end();
       }
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    if (k_lo < k_hi) dma(A0, B0, k_lo);
-    __syncthreads();
-    int kt = k_lo;
-    for (; kt + 2 <= k_hi; kt += 2) {
-      stage(A0, B0, A1, B1, kt);
-      stage(A1, B1, A0, B0, kt + 1);
+      buf = buf == NB - 1 ? 0 : buf + 1;
     }
-    if (kt < k_hi) stage(A0, B0, A1, B1, kt);
+    if (g == 0) phase_end();
+    __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // no load writes LDS after the block
+    return true;
   }
 
-  // f(m, n, acc): the outputs (m, n .. n + 3) of this lane, m < M, n < N
-  template <class F>
-  __device__ static __forceinline__ void each(const NtOperands& p, int m0, int n0, int wave, int lane, const Acc (&acc)[TN][TM], F f) {
-    const int mb = m0 + (wave / WN) * WTM + (lane & 15), nb = n0 + (wave % WN) * WTN + 4 * (lane >> 4);
+  // This wavefront's first output: the lane holds, in acc[i][j][e], row + 16 j and column + 16 i + e.
+  __device__ static __forceinline__ int row(int m0, int wave, int lane) { return m0 + (wave >> 2) * WTM + (lane & 15); }
+  __device__ static __forceinline__ int column(int n0, int wave, int lane) { return n0 + (wave & 3) * WTN + 4 * (lane >> 4); }
+};
+
+
+// Both steps' operands of a stage, waited for: a's 16-row tiles lie 2048 bytes apart from address `a`, b's from `b`.
+template <int TM, int TN>
+__device__ __forceinline__ void nt_read_stage(uint32_t a, uint32_t b, i32x4 (&x)[2][TM], i32x4 (&y)[2][TN]) {
+  static_assert((TM == 4 && TN == 2) || (TM == 2 && TN == 2), "32 or 64 rows by 32");
+  if constexpr (TM == 4) {
+    asm volatile(
+        "ds_read_b128 %8, %14\n\tds_read_b128 %9, %14 offset:2048\n\t"
+        "ds_read_b128 %0, %12\n\tds_read_b128 %1, %12 offset:2048\n\t"
+        "ds_read_b128 %2, %12 offset:4096\n\tds_read_b128 %3, %12 offset:6144\n\t"
+        "ds_read_b128 %10, %15\n\tds_read_b128 %11, %15 offset:2048\n\t"
+        "ds_read_b128 %4, %13\n\tds_read_b128 %5, %13 offset:2048\n\t"
+        "ds_read_b128 %6, %13 offset:4096\n\tds_read_b128 %7, %13 offset:6144\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[0][3]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[1][2]),
+          "=&v"(x[1][3]), "=&v"(y[0][0]), "=&v"(y[0][1]), "=&v"(y[1][0]), "=&v"(y[1][1])
+        : "v"(a), "v"(a ^ 64), "v"(b), "v"(b ^ 64)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b128 %4, %10\n\tds_read_b128 %5, %10 offset:2048\n\t"
+        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:2048\n\t"
+        "ds_read_b128 %6, %11\n\tds_read_b128 %7, %11 offset:2048\n\t"
+        "ds_read_b128 %2, %9\n\tds_read_b128 %3, %9 offset:2048\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(y[0][0]), "=&v"(y[0][1]), "=&v"(y[1][0]),
+          "=&v"(y[1][1])
+        : "v"(a), "v"(a ^ 64), "v"(b), "v"(b ^ 64)
+        : "memory");
+  }
+}
+
+// The same product on a tile of BM x BN, one barrier a stage: CW wavefronts of 2 x CW / 2 multiply, 4 more only load. A
+// wavefront's load of 64 chunks takes about 40 ns to go out, whatever comes of it, so that loads in front of a
+// small tile's few products would take longer than they (64 x 64: 255 ns a stage, with loaders ...).
+template <class Op, int BM_, int BN_, int NB, int CW, int LW>
+struct NtSmall {
+  static constexpr int BM = BM_, BN = BN_, THREADS = 64 * (CW + LW);
+  static constexpr int WN = CW / 2, WTM = BM / 2, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
+  static constexpr int STAGE = (BM + BN) * 128, LDS = NB * STAGE;
+  static constexpr int PW = (BM + BN) / (8 * LW);
+  static_assert((BM + BN) % (8 * LW) == 0 && BM % 32 == 0 && BN % 32 == 0 && NB >= 2 && (NB - 2) * PW < 64, "whole loads, and a count that vmcnt holds");
+  using Acc = typename Op::Acc;
+
+  // Whether this wavefront has outputs.
+  __device__ static __forceinline__ bool run(const NtOperands& p, uint8_t* lds, int m0, int n0, int k_lo, int k_hi, int wave, int lane,
+                                             Acc (&acc)[TN][TM]) {
+    auto stage_begins = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if (wave >= CW) {
+      const int w = wave - CW;
+      const __amdgpu_buffer_rsrc_t rsa = nt_rows(p.a, m0, p.lda, min(BM, p.M - m0), p.K), rsb = nt_rows(p.b, n0, p.ldb, min(BN, p.N - n0), p.K);
+      const int lc = ((lane & 7) ^ ((lane >> 3) & 7)) * 16;  // (a load's 8 rows begin at a multiple of 8)
+      int off[PW];
+#pragma unroll
+      for (int i = 0; i < PW; ++i) {
+        const int q = w * PW + i;
+        off[i] = (q < BM / 8 ? (q * 8 + (lane >> 3)) * p.lda : (q * 8 - BM + (lane >> 3)) * p.ldb) + lc;
+      }
+      auto ask = [&](int t, int buf) __attribute__((always_inline)) {
+        const int k0 = t * 128;
+        // past K, and past the last stage: zeros, and no memory is read
+        const bool in = t < k_hi && k0 + lc < p.K;
+#pragma unroll
+        for (int i = 0; i < PW; ++i)
+          nt_lds_load16(w * PW + i < BM / 8 ? rsa : rsb, lds + buf * STAGE + (w * PW + i) * 1024, in ? off[i] + k0 : kNtOutside);
+      };
+      for (int t = 0; t < NB - 1; ++t) ask(k_lo + t, t);
+      int buf = NB - 1;
+      for (int t = k_lo; t < k_hi; ++t) {
+        constexpr int left = (NB - 2) * PW;  // loads of later stages
+        __builtin_amdgcn_s_waitcnt((left & 15) | (left >> 4) << 14 | 0x70 | 0xF00);
+        stage_begins();
+        ask(t + NB - 1, buf);  // the buffer of stage t - 1, which everyone has read
+        buf = buf == NB - 1 ? 0 : buf + 1;
+      }
+      __builtin_amdgcn_s_waitcnt(0x70 | 0xF00);  // no load writes LDS after the block
+      return false;
+    }
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
-      for (int j = 0; j < TM; ++j)
-        if (mb + 16 * j < p.M && nb + 16 * i < p.N) f(mb + 16 * j, nb + 16 * i, acc[i][j]);
+      for (int j = 0; j < TM; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+    const int lr = lane & 15, lk = lane >> 4;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + lr * 128 + (lk ^ (lr & 7)) * 16;
+    const uint32_t at_a = base + wave / WN * WTM * 128, at_b = base + (BM + wave % WN * WTN) * 128;
+    int buf = 0;
+    for (int t = k_lo; t < k_hi; ++t) {
+      stage_begins();
+      i32x4 x[2][TM], y[2][TN];
+      nt_read_stage<TM, TN>(at_a + buf * STAGE, at_b + buf * STAGE, x, y);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+          for (int i = 0; i < TN; ++i) acc[i][j] = Op::mma(y[h][i], x[h][j], acc[i][j]);
+      buf = buf == NB - 1 ? 0 : buf + 1;
+    }
+    return true;
   }
+
+  __device__ static __forceinline__ int row(int m0, int wave, int lane) { return m0 + wave / WN * WTM + (lane & 15); }
+  __device__ static __forceinline__ int column(int n0, int wave, int lane) { return n0 + wave % WN * WTN + 4 * (lane >> 4); }
 };
 
 }  // namespace mls

@@ -119,9 +119,10 @@ def _product(fn, x, sx, x_dt, w_q, sw, bias, out_dtype):
     args = _ARGS.pack(x.data_ptr(), 0 if sx is None else sx.data_ptr(), w_q.data_ptr(), sw.data_ptr(), b_at, y.data_ptr(), x_dt,
                       _DT[sw.dtype], b_dt, c_dt, x.stride(0) if M > 1 else K, w_q.stride(0) if N > 1 else K, N, M, N, K)
     lib = kernels.lib()
-    need = lib.mlsx_a8w8_ws(args)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    rc = lib.mlsx_a8w8(args, ws.data_ptr() if need else 0, need, _raw_stream(dev))
+    rc = lib.mlsx_a8w8(args, 0, 0, _raw_stream(dev))
+    if rc > 0:  # (the workspace that it needs)
+        ws = torch.empty(rc, dtype=torch.uint8, device=x.device)
+        rc = lib.mlsx_a8w8(args, ws.data_ptr(), rc, _raw_stream(dev))
     if rc:
         kernels.check(rc, fn)
     return y
