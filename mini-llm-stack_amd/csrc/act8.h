@@ -59,6 +59,20 @@ __device__ __forceinline__ void load8(const T* row, int64_t k, int64_t K, float 
   }
 }
 
+// 8 consecutive codes of a row from column k as values, zeros past K; any alignment.
+__device__ __forceinline__ void load_codes8(const int8_t* row, int64_t k, int64_t K, float s, float (&v)[8]) {
+  uint32_t w[2] = {0, 0};
+  if (k + 8 <= K) {
+    __builtin_memcpy(w, row + k, 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < K) w[e / 4] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e % 4));
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * s;
+}
+
 // n <= 8 values to a row; any alignment of a whole number of values.
 template <typename T>
 __device__ __forceinline__ void store8(T* dst, const float (&v)[8], int64_t n) {

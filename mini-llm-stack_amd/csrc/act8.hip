@@ -165,19 +165,6 @@ struct BackArgs {
   int64_t M, H, per;  // per: chunks of 8 columns a row
 };
 
-__device__ __forceinline__ void load_codes8(const int8_t* row, int64_t k, int64_t K, float s, float (&v)[8]) {
-  uint32_t w[2] = {0, 0};
-  if (k + 8 <= K) {
-    __builtin_memcpy(w, row + k, 8);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k + e < K) w[e / 4] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e % 4));
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * s;
-}
-
 template <typename T>
 __global__ __launch_bounds__(256) void silu_back_kernel(const BackArgs p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;

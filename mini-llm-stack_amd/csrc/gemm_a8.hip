@@ -274,45 +274,13 @@ int few_chunks(int64_t M, int64_t K) {
 
 // ---------------------------------------------------------------- host
 
-// The forms of tile, and what they take: us a stage of 128 k on a CU, alone (first) and with all CUs at work. From
-// timed calls of 48 to 4096 rows with weights that no cache holds. A CU takes its blocks one after another or side by side; either way their
-// stages add up, bound by what its L1 gives (64 bytes a clock: 64 x 64 reads four times as much a product as 256 x 256)
-// and, at 256 x 256, by the matrix cores at the clock that they leave it (64 x 64 x 128 on every CU of 4096 x 8192 x 8192).
-struct TileForm {
-  int bm, bn;
-  float alone, busy;
-};
-constexpr TileForm kForms[] = {{64, 64, 0.24f, 0.23f}, {128, 64, 0.36f, 0.45f}, {128, 128, 0.52f, 0.60f}, {128, 128, 9.0f, 0.55f}, {256, 256, 1.35f, 1.85f}};
-
 struct Plan {
   bool few, fused;        // the kernel for few rows; which quantizes x itself
   bool pad_w, own_x;      // operands copied (or codes made) into the workspace
   int64_t kpad;
-  int form, splits;       // of kForms; K ranges
+  int form, splits;       // of kNtForms; K ranges
   int64_t x_at, s_at, w_at, part_at, bytes;
 };
-
-// The quickest form and number of K ranges by these figures: 4 us for a launch and its first stage; K ranges cost a second launch
-// and their sums' way through memory. (333 x 4096 x 11008: 128 x 128 in two ranges 35 us, whole 49, 128 x 64 35, 64 x 64 43.)
-void choose_form(int64_t M, int64_t N, int64_t K, Plan& p) {
-  const int64_t units = cdiv(K, 128);
-  float best = 3e38f;
-  for (int f = 0; f < 5; ++f) {
-    const TileForm& t = kForms[f];
-    const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn);
-    for (int s = 1; s <= (f < 3 ? 8 : 1) && (s == 1 || units / s >= 4); ++s) {
-      const int64_t deep = cdiv(tiles * s, 256);
-      const float stage = deep > 1 ? t.busy : t.alone + (t.busy - t.alone) * (float)(tiles * s) / 256.0f;
-      const float us = 4.0f + (float)(deep * cdiv(units, s)) * (f == 3 && deep == 1 ? t.alone : stage) +
-                       (s > 1 ? 6.0f + (float)s * (float)M * (float)N * 4.0f / 2.5e6f : 0.0f);
-      if (us < best) {
-        best = us;
-        p.form = f;
-        p.splits = s;
-      }
-    }
-  }
-}
 
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -330,7 +298,7 @@ Plan make_plan(const mlsx_a8w8_args& a) {
   p.fused = a.x_dt == a.c_dt && p.few && few_chunks(a.M, a.K) <= 6 && few_chunks(a.M, a.K) * cdiv(a.N, 4096) <= 6;
   p.own_x = codes ? !rows_fit(a.x, a.ldx, a.K) : !p.fused;
   p.splits = 1;
-  if (!p.few) choose_form(a.M, a.N, a.K, p);
+  if (!p.few) nt_choose(a.M, a.N, a.K, p.form, p.splits);
   int64_t at = 0;
   if (p.own_x) {
     p.x_at = at;
@@ -367,13 +335,17 @@ int launch_tiles(TileArgs t, hipStream_t st) {
 
 template <typename CT, class T>
 int launch_tile(TileArgs t, void* part, hipStream_t st) {
-  if (t.splits == 1) return launch_tiles<CT, T, false>(t, st);
-  void* c = t.c;
-  t.c = part;
-  if (const int rc = launch_tiles<CT, T, true>(t, st)) return rc;
-  hipLaunchKernelGGL(a8_join_kernel<CT>, dim3((unsigned)cdiv(t.o.N, 1024), (unsigned)t.o.M), dim3(256), 0, st, (const int*)part,
-                     t.splits, (CT*)c, t.ldc, t.s, t.o.M, t.o.N);
-  return check_launch("a8w8 (join)");
+  if constexpr (T::RANGES) {
+    if (t.splits > 1) {
+      void* c = t.c;
+      t.c = part;
+      if (const int rc = launch_tiles<CT, T, true>(t, st)) return rc;
+      hipLaunchKernelGGL(a8_join_kernel<CT>, dim3((unsigned)cdiv(t.o.N, 1024), (unsigned)t.o.M), dim3(256), 0, st, (const int*)part,
+                         t.splits, (CT*)c, t.ldc, t.s, t.o.M, t.o.N);
+      return check_launch("a8w8 (join)");
+    }
+  }
+  return launch_tiles<CT, T, false>(t, st);
 }
 
 template <typename XT, typename CT, int C>
@@ -429,14 +401,7 @@ int run(const mlsx_a8w8_args& a, const Plan& p, uint8_t* ws, hipStream_t st) {
     return launch_fused<CT>(f, few_chunks(a.M, a.K), st);
   }
   TileArgs t{{x, w, (int)ldx, (int)ldw, (int)a.M, (int)a.N, (int)K}, a.c, s, a.ldc, 0, 0, p.splits};
-  void* part = ws + p.part_at;
-  switch (p.form) {
-    case 0: return launch_tile<CT, NtSmall<Int8Op, 64, 64, 5, 4, 4>>(t, part, st);
-    case 1: return launch_tile<CT, NtSmall<Int8Op, 128, 64, 6, 4, 4>>(t, part, st);
-    case 2: return launch_tile<CT, NtSmall<Int8Op, 128, 128, 4, 8, 4>>(t, part, st);
-    case 3: return launch_tiles<CT, NtTile<Int8Op, 128, 2>, false>(t, st);
-    default: return launch_tiles<CT, NtTile<Int8Op, 256, 2>, false>(t, st);
-  }
+  return nt_form<Int8Op>(p.form, [&](auto form) { return launch_tile<CT, typename decltype(form)::type>(t, ws + p.part_at, st); });
 }
 
 int check_args(const mlsx_a8w8_args& a, const char* fn) {

@@ -2,9 +2,14 @@
 // with a scale a token.
 //
 // 16-bit dy: the kept value q s is rounded to dy's type (off by half a step of it, as dy itself is) and the product runs on
-// the 16-bit matrix cores with fp32 sums. Both operands are turned first, so that their rows run along the
-// tokens (dw8_turn_kernel), then multiplied tile by tile (nt_tile.h).
+// the 16-bit matrix cores with fp32 sums. fp32: dy s, rounded once, becomes three bf16 parts that add up to it
+// (8 significant bits each), and each meets the codes, which bf16 holds exactly: three products where two fp32
+// operands would take six. Parts of values under 2^-110 lose bits below 2^-133, bf16's smallest.
+//
+// Both operands are turned first, so that their rows run along the tokens (dw8_turn_kernel; the rows' ends are padded with zeros to
+// 64 tokens), then multiplied tile by tile (nt_tile.h).
 #include <algorithm>
+#include <type_traits>
 
 #include "act8.h"
 #include "mfma16.h"
@@ -29,45 +34,75 @@ struct TurnArgs {
   int64_t ldq;
   const float* s;
   int M, N, K, Mp;
-  void* dyt;  // [N][Mp]
+  void* dyt;  // [N][Mp]; fp32: bf16 [N][3][Mp]
   void* xt;   // [K][Mp]
 };
 
-// 64 tokens x 64 columns through LDS. blockIdx.z: 0 dy, 1 the kept input. Tokens past M become zeros.
-template <typename T>
-__global__ __launch_bounds__(256) void dw8_turn_kernel(const TurnArgs p) {
-  __shared__ T tile[64][72];
-  const bool second = blockIdx.z != 0;
-  const int C = second ? p.K : p.N, c0 = blockIdx.x * 64, m0 = blockIdx.y * 64, tid = threadIdx.x;
+// n <= W consecutive values of a row, zeros past them
+template <int W, typename T>
+__device__ __forceinline__ void load_some(const T* src, int64_t n, float (&v)[W]) {
+  T raw[W];
+  if (n >= W) {
+    __builtin_memcpy(raw, src, sizeof(raw));
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = to_f32(raw[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = e < n ? to_f32(src[e]) : 0.0f;
+  }
+}
+
+// 8 tokens x W columns a lane, turned in registers, 8 x 8 lanes a wavefront: loads take 128 bytes (codes: 64) of each of 8
+// rows, stores 128 bytes of 8 of the results' rows. PARTS: of every value (the second and third of what is left).
+template <typename T, typename P, int W, int PARTS, bool CODES>
+__device__ __forceinline__ void turn(const TurnArgs& p, int C, P* dst) {
+  const int c0 = blockIdx.x * 8 * W + (threadIdx.x & 7) * W, m0 = blockIdx.y * 64 + (threadIdx.x >> 3) * 8;
   if (c0 >= C) return;
+  float v[8][W];  // [token][column]
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = i * 32 + tid / 8, c = (tid % 8) * 8, m = m0 + r;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (m < p.M && c0 + c < C) {
-      if (second) {
+  for (int r = 0; r < 8; ++r) {
+    const int m = m0 + r;
+    if (m >= p.M) {
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[r][e] = 0.0f;
+    } else if constexpr (CODES) {
+      // (fp32: the scale goes to dy)
+      load_codes8(p.q + (int64_t)m * p.ldq, c0, C, sizeof(T) == 4 ? 1.0f : p.s[m], v[r]);
+    } else {
+      load_some<W>((const T*)p.dy + (int64_t)m * p.lddy + c0, C - c0, v[r]);
+      if constexpr (sizeof(T) == 4) {
         const float s = p.s[m];
-        const int8_t* src = p.q + (int64_t)m * p.ldq + c0 + c;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c0 + c + e < C) v[e] = (float)src[e] * s;
-      } else {
-        load8((const T*)p.dy + (int64_t)m * p.lddy, c0 + c, C, v);
+        for (int e = 0; e < W; ++e) v[r][e] *= s;
       }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) tile[r][c + e] = from_f32<T>(v[e]);
   }
-  __syncthreads();
-  T* dst = (T*)(second ? p.xt : p.dyt);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int c = i * 32 + tid / 8, r0 = (tid % 8) * 8;
-    if (c0 + c >= C || m0 + r0 >= p.Mp) continue;  // (Mp is a multiple of 8)
-    T o[8];
+  for (int c = 0; c < W; ++c) {
+    if (c0 + c >= C) continue;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = tile[r0 + e][c];
-    __builtin_memcpy(__builtin_assume_aligned(dst + (int64_t)(c0 + c) * p.Mp + m0 + r0, 16), o, 16);
+    for (int t = 0; t < PARTS; ++t) {
+      P o[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        float part = v[r][c];
+        if (t + 1 < PARTS) split_f32(v[r][c], part, v[r][c]);
+        o[r] = (P)part;
+      }
+      __builtin_memcpy(__builtin_assume_aligned(dst + ((int64_t)(c0 + c) * PARTS + t) * p.Mp + m0, 16), o, 16);
+    }
+  }
+}
+
+// blockIdx.z: 0 dy, 1 the kept input
+template <typename T>
+__global__ __launch_bounds__(64) void dw8_turn_kernel(const TurnArgs p) {
+  if constexpr (sizeof(T) == 4) {
+    if (blockIdx.z == 0) turn<T, __bf16, 4, 3, false>(p, p.N, (__bf16*)p.dyt);
+    else turn<T, __bf16, 8, 1, true>(p, p.K, (__bf16*)p.xt);
+  } else {
+    if (blockIdx.z == 0) turn<T, T, 8, 1, false>(p, p.N, (T*)p.dyt);
+    else turn<T, T, 8, 1, true>(p, p.K, (T*)p.xt);
   }
 }
 
@@ -78,20 +113,22 @@ struct Dw8Args {
   int m_tiles, n_tiles, splits;
 };
 
-template <typename T, int B, int NB, bool PARTIAL>
-__global__ __launch_bounds__(512) void dw8_kernel(const Dw8Args p) {
-  using G = NtTile<Op16<T>, B, NB>;
+// G: a form of tile
+template <typename T, class G, bool PARTIAL>
+__global__ __launch_bounds__(G::THREADS) void dw8_kernel(const Dw8Args p) {
   extern __shared__ __align__(16) uint8_t lds[];
   int sp, mt, nt;
   nt_place(p.m_tiles, p.n_tiles, sp, mt, nt);
   const int units = (p.o.K + 127) / 128;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   f32x4 acc[G::TN][G::TM];
-  (void)G::run(p.o, lds, mt * B, nt * B, (int)((int64_t)units * sp / p.splits), (int)((int64_t)units * (sp + 1) / p.splits), wave, lane, acc);
+  if (!G::run(p.o, lds, mt * G::BM, nt * G::BN, (int)((int64_t)units * sp / p.splits), (int)((int64_t)units * (sp + 1) / p.splits), wave,
+              lane, acc))
+    return;
   using CT = std::conditional_t<PARTIAL, float, T>;
   CT* c = (CT*)p.c + (PARTIAL ? (int64_t)sp * p.o.M * p.ldc : 0);
   const bool v4 = p.ldc % 4 == 0 && ((uintptr_t)p.c & (4 * sizeof(CT) - 1)) == 0;
-  const int M = p.o.M, N = p.o.N, m0 = G::row(mt * B, wave, lane), n0 = G::column(nt * B, wave, lane);
+  const int M = p.o.M, N = p.o.N, m0 = G::row(mt * G::BM, wave, lane), n0 = G::column(nt * G::BN, wave, lane);
 #pragma unroll
   for (int i = 0; i < G::TN; ++i)
 #pragma unroll
@@ -128,38 +165,21 @@ __global__ __launch_bounds__(256) void dw8_join_kernel(const float* __restrict__
     if (k + e < K) c[n * ldc + k + e] = from_f32<T>(o[e]);
 }
 
-// fp32: the kept input itself
-__global__ __launch_bounds__(256) void dw8_values_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ s,
-                                                         float* __restrict__ x, int K) {
-  const int64_t m = blockIdx.y;
-  const int k = blockIdx.x * 256 + threadIdx.x;
-  if (k < K) x[m * K + k] = (float)q[m * ldq + k] * s[m];
-}
-
 struct DwPlan {
-  int64_t Mp, dyt_at, xt_at, part_at, ldp, bytes;
-  int tile, splits;
+  int64_t Mp, xt_at, part_at, ldp, bytes;
+  int form, splits;
 };
 
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 DwPlan make_plan(int dt, int64_t M, int64_t N, int64_t K) {
   DwPlan p{};
-  if (dt == MLS_F32) {
-    p.xt_at = up256(mlsx_dw_fp32_workspace(M, N, K));
-    p.bytes = p.xt_at ? p.xt_at + up256(M * K * 4) : 0;
-    return p;
-  }
-  p.Mp = cdiv(M, 8) * 8;
-  p.xt_at = up256(N * p.Mp * 2);
+  const int parts = dt == MLS_F32 ? 3 : 1;
+  p.Mp = cdiv(M, 64) * 64;
+  p.xt_at = up256(N * parts * p.Mp * 2);
   p.part_at = p.xt_at + up256(K * p.Mp * 2);
   p.bytes = p.part_at;
-  p.tile = cdiv(N, 256) * cdiv(K, 256) >= 128 ? 256 : 128;
-  p.splits = 1;
-  if (p.tile == 128) {
-    const int64_t tiles = cdiv(N, 128) * cdiv(K, 128), units = cdiv(M, 64);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, units / 4, 16}));
-  }
+  nt_choose(N, K, parts * p.Mp * 2, p.form, p.splits);
   if (p.splits > 1) {
     p.ldp = cdiv(K, 4) * 4;
     p.bytes += up256(p.splits * N * p.ldp * 4);
@@ -167,35 +187,43 @@ DwPlan make_plan(int dt, int64_t M, int64_t N, int64_t K) {
   return p;
 }
 
-template <typename T, int B, int NB, bool PARTIAL>
-int launch_dw8(const Dw8Args& a, hipStream_t st) {
+template <typename T, class G, bool PARTIAL>
+int launch_dw8(Dw8Args a, hipStream_t st) {
   const char* fn = "mlsx_dw_int8";
+  a.m_tiles = (int)cdiv(a.o.M, G::BM);
+  a.n_tiles = (int)cdiv(a.o.N, G::BN);
   const int64_t blocks = (int64_t)a.m_tiles * a.n_tiles * a.splits;
   if (blocks > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "%s: %d x %d", fn, a.o.M, a.o.N);
-  auto kern = dw8_kernel<T, B, NB, PARTIAL>;
-  constexpr int lds = NtTile<Op16<T>, B, NB>::LDS;
-  if (lds > 32768 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
-    return fail(MLS_ERR_HIP, "%s: cannot reserve %d bytes of LDS", fn, lds);
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(512), lds, st, a);
+  auto kern = dw8_kernel<T, G, PARTIAL>;
+  // (a call a launch: the limit is the function's on the current device)
+  if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS) != hipSuccess)
+    return fail(MLS_ERR_HIP, "%s: cannot reserve %d bytes of LDS", fn, G::LDS);
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(G::THREADS), G::LDS, st, a);
   return check_launch(fn);
 }
 
 template <typename T>
-int run16(const void* dy, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw, int64_t lddw, int64_t M, int64_t N,
-          int64_t K, const DwPlan& p, uint8_t* ws, hipStream_t st) {
+int run(const TurnArgs& t, void* dw, int64_t lddw, const DwPlan& p, uint8_t* ws, hipStream_t st) {
   const char* fn = "mlsx_dw_int8";
-  const TurnArgs t{dy, lddy, q, ldq, s, (int)M, (int)N, (int)K, (int)p.Mp, ws, ws + p.xt_at};
-  hipLaunchKernelGGL(dw8_turn_kernel<T>, dim3((unsigned)cdiv(std::max(N, K), 64), (unsigned)cdiv(M, 64), 2), dim3(256), 0, st, t);
+  hipLaunchKernelGGL(dw8_turn_kernel<T>, dim3((unsigned)std::max(cdiv(t.N, sizeof(T) == 4 ? 32 : 64), cdiv(t.K, 64)), (unsigned)(p.Mp / 64), 2), dim3(64), 0, st, t);
   if (const int rc = check_launch(fn)) return rc;
-  const int ld = (int)p.Mp * 2;
-  Dw8Args a{{ws, ws + p.xt_at, ld, ld, (int)N, (int)K, ld}, dw, lddw, (int)cdiv(N, p.tile), (int)cdiv(K, p.tile), p.splits};
-  if (p.splits == 1) return p.tile == 256 ? launch_dw8<T, 256, 2, false>(a, st) : launch_dw8<T, 128, 4, false>(a, st);
-  a.c = ws + p.part_at;
-  a.ldc = p.ldp;
-  if (const int rc = launch_dw8<T, 128, 4, true>(a, st)) return rc;
-  hipLaunchKernelGGL(dw8_join_kernel<T>, dim3((unsigned)cdiv(K, 1024), (unsigned)N), dim3(256), 0, st,
-                     (const float*)(ws + p.part_at), p.splits, p.ldp, (T*)dw, lddw, (int)N, (int)K);
-  return check_launch(fn);
+  const int parts = sizeof(T) == 4 ? 3 : 1, ld = (int)p.Mp * 2;
+  using P = std::conditional_t<sizeof(T) == 4, __bf16, T>;
+  Dw8Args a{{ws, ws + p.xt_at, parts * ld, ld, t.N, t.K, parts * ld, parts}, dw, lddw, 0, 0, p.splits};
+  return nt_form<Op16<P>>(p.form, [&](auto form) {
+    using G = typename decltype(form)::type;
+    if constexpr (G::RANGES) {
+      if (p.splits > 1) {
+        a.c = ws + p.part_at;
+        a.ldc = p.ldp;
+        if (const int rc = launch_dw8<T, G, true>(a, st)) return rc;
+        hipLaunchKernelGGL(dw8_join_kernel<T>, dim3((unsigned)cdiv(t.K, 1024), (unsigned)t.N), dim3(256), 0, st,
+                           (const float*)(ws + p.part_at), p.splits, p.ldp, (T*)dw, lddw, t.N, t.K);
+        return check_launch(fn);
+      }
+    }
+    return launch_dw8<T, G, false>(a, st);
+  });
 }
 
 }  // namespace
@@ -223,11 +251,8 @@ extern "C" int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* 
   const DwPlan p = make_plan(dt, M, N, K);
   const hipStream_t st = (hipStream_t)stream;
   uint8_t* w = (uint8_t*)ws;
-  if (dt == MLS_F16) return run16<_Float16>(dy, lddy, q, ldq, s, dw, lddw, M, N, K, p, w, st);
-  if (dt == MLS_BF16) return run16<__bf16>(dy, lddy, q, ldq, s, dw, lddw, M, N, K, p, w, st);
-  float* x = (float*)(w + p.xt_at);
-  if (M > 65535) return fail(MLS_ERR_UNSUPPORTED, "%s: M=%lld", fn, (long long)M);
-  hipLaunchKernelGGL(dw8_values_kernel, dim3((unsigned)cdiv(K, 256), (unsigned)M), dim3(256), 0, st, q, ldq, s, x, (int)K);
-  if (const int rc = check_launch(fn)) return rc;
-  return mlsx_dw_fp32((const float*)dy, lddy, x, K, (float*)dw, lddw, M, N, K, ws, p.xt_at, stream);
+  const TurnArgs t{dy, lddy, q, ldq, s, (int)M, (int)N, (int)K, (int)p.Mp, w, w + p.xt_at};
+  if (dt == MLS_F32) return run<float>(t, dw, lddw, p, w, st);
+  if (dt == MLS_F16) return run<_Float16>(t, dw, lddw, p, w, st);
+  return run<__bf16>(t, dw, lddw, p, w, st);
 }

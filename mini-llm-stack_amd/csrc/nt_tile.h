@@ -29,6 +29,7 @@ struct NtOperands {
   const uint8_t* b;  // [N][ldb]
   int lda, ldb;      // bytes, multiples of 16, as a and b
   int M, N, K;       // K: bytes of a row, a multiple of 16
+  int turns = 1;     // a's rows are that many parts of K / turns bytes, a multiple of 128 where there are several; each meets the same row of b
 };
 
 // The rows first .. first + rows of a matrix. The offsets that lanes give are checked against it.
@@ -40,6 +41,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t nt_rows(const void* base, int6
 __device__ __forceinline__ void nt_lds_load16(__amdgpu_buffer_rsrc_t rs, void* lds, int voff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, voff, 0, 0, 0);
 }
+
+// The stage of b that stage t of a meets; part: stages a part, or a large number.
+__device__ __forceinline__ int nt_stage_of_b(int t, int part) { return t < part ? t : t < 2 * part ? t - part : t - 2 * part; }
+__device__ __forceinline__ int nt_part(const NtOperands& p) { return p.turns == 1 ? 0x3FFFFFFF : p.K / p.turns / 128; }
 
 // Block -> (K range, row tile, column tile): consecutive tiles on one XCD, runs of 4 row tiles sweep all
 // column tiles.
@@ -86,6 +91,7 @@ __device__ __forceinline__ void nt_read(uint32_t a, uint32_t b, i32x4 (&x)[TM], 
 template <class Op, int B, int NB>
 struct NtTile {
   static constexpr int BM = B, BN = B, THREADS = 512;
+  static constexpr bool RANGES = false;  // (whether it is run on ranges of K)
   static constexpr int WTM = B / 2, WTN = B / 4, TM = WTM / 16, TN = WTN / 16;
   static constexpr int STAGE = 2 * B * 128;  // bytes
   static constexpr int LDS = NB * STAGE;
@@ -104,18 +110,19 @@ struct NtTile {
   __device__ static __forceinline__ bool run(const NtOperands& p, uint8_t* lds, int m0, int n0, int k_lo, int k_hi, int wave, int lane,
                                              Acc (&acc)[TN][TM]) {
     const int g = wave >> 2, w = wave & 3;
-    const __amdgpu_buffer_rsrc_t rs = g == 0 ? nt_rows(p.a, m0, p.lda, min(B, p.M - m0), p.K) : nt_rows(p.b, n0, p.ldb, min(B, p.N - n0), p.K);
+    const __amdgpu_buffer_rsrc_t rs = g == 0 ? nt_rows(p.a, m0, p.lda, min(B, p.M - m0), p.K) : nt_rows(p.b, n0, p.ldb, min(B, p.N - n0), p.K / p.turns);
     const int ld = g == 0 ? p.lda : p.ldb;
     const int lc = ((lane & 7) ^ ((lane >> 3) & 7)) * 16;  // (a load's 8 rows begin at a multiple of 8)
-    int off[PW];
-#pragma unroll
-    for (int i = 0; i < PW; ++i) off[i] = ((w * PW + i) * 8 + (lane >> 3)) * ld + lc;
+    const int off = (w * PW * 8 + (lane >> 3)) * ld + lc;
     uint8_t* const fill = lds + (g * B + w * PW * 8) * 128;
-    auto ask = [&](int i, int t, int buf) __attribute__((always_inline)) {
-      const int k0 = t * 128;
-      // past K, and past the last stage: zeros, and no memory is read
-      const bool in = t < k_hi && k0 + lc < p.K;
-      nt_lds_load16(rs, fill + buf * STAGE + i * 1024, in ? off[i] + k0 : kNtOutside);
+    const int part = g == 0 ? 0x3FFFFFFF : nt_part(p);
+    // where this lane's first chunk of stage t lies; past K, and past the last stage: outside, and the loads write zeros and
+    // read no memory (so are the chunks of the rows below it: 256 rows span less than 2^31 bytes)
+    auto start = [&](int t) __attribute__((always_inline)) {
+      return t < k_hi && t * 128 + lc < p.K ? off + nt_stage_of_b(t, part) * 128 : kNtOutside;
+    };
+    auto ask = [&](int i, int at, int buf) __attribute__((always_inline)) {
+      nt_lds_load16(rs, fill + buf * STAGE + i * 1024, at + i * 8 * ld);
     };
 #pragma unroll
     for (int i = 0; i < TN; ++i)
@@ -130,13 +137,13 @@ struct NtTile {
     constexpr int wait_code = (left & 15) | (left >> 4) << 14 | 0x70 | 0xF00;
     for (int t = 0; t < NB - 1; ++t)
 #pragma unroll
-      for (int i = 0; i < PW; ++i) ask(i, k_lo + t, t);
+      for (int i = 0; i < PW; ++i) ask(i, start(k_lo + t), t);
     __builtin_amdgcn_s_waitcnt(wait_code);
     phase_end();
     if (g == 1) phase_end();  // half a step later
     int buf = 0;
     for (int t = k_lo; t < k_hi; ++t) {
-      const int last = buf == 0 ? NB - 1 : buf - 1;
+      const int last = buf == 0 ? NB - 1 : buf - 1, at = start(t + NB - 1);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         i32x4 x[TM], y[TN];
@@ -147,7 +154,7 @@ struct NtTile {
         if (h == 0) {
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < PW / 2; ++i) ask(i, t + NB - 1, last);
+          for (int i = 0; i < PW / 2; ++i) ask(i, at, last);
         }
         phase_end();
         __builtin_amdgcn_s_setprio(1);
@@ -157,7 +164,7 @@ struct NtTile {
           for (int i = 0; i < TN; ++i) acc[i][j] = Op::mma(y[i], x[j], acc[i][j]);
           if (h == 0 && j < PW - PW / 2) {
             __builtin_amdgcn_sched_barrier(0);
-            ask(PW / 2 + j, t + NB - 1, last);
+            ask(PW / 2 + j, at, last);
             __builtin_amdgcn_sched_barrier(0);
           }
         }
@@ -212,10 +219,11 @@ __device__ __forceinline__ void nt_read_stage(uint32_t a, uint32_t b, i32x4 (&x)
 
 // The same product on a tile of BM x BN, one barrier a stage: CW wavefronts of 2 x CW / 2 multiply, 4 more only load. A
 // wavefront's load of 64 chunks takes about 40 ns to go out, whatever comes of it, so that loads in front of a
-// small tile's few products would take longer than they (64 x 64: 255 ns a stage, with loaders ...).
+// small tile's few products would take longer than they (64 x 64: 255 ns a stage; with loaders 140 to 180).
 template <class Op, int BM_, int BN_, int NB, int CW, int LW>
 struct NtSmall {
   static constexpr int BM = BM_, BN = BN_, THREADS = 64 * (CW + LW);
+  static constexpr bool RANGES = true;
   static constexpr int WN = CW / 2, WTM = BM / 2, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
   static constexpr int STAGE = (BM + BN) * 128, LDS = NB * STAGE;
   static constexpr int PW = (BM + BN) / (8 * LW);
@@ -232,7 +240,7 @@ struct NtSmall {
     };
     if (wave >= CW) {
       const int w = wave - CW;
-      const __amdgpu_buffer_rsrc_t rsa = nt_rows(p.a, m0, p.lda, min(BM, p.M - m0), p.K), rsb = nt_rows(p.b, n0, p.ldb, min(BN, p.N - n0), p.K);
+      const __amdgpu_buffer_rsrc_t rsa = nt_rows(p.a, m0, p.lda, min(BM, p.M - m0), p.K), rsb = nt_rows(p.b, n0, p.ldb, min(BN, p.N - n0), p.K / p.turns);
       const int lc = ((lane & 7) ^ ((lane >> 3) & 7)) * 16;  // (a load's 8 rows begin at a multiple of 8)
       int off[PW];
 #pragma unroll
@@ -240,13 +248,16 @@ struct NtSmall {
         const int q = w * PW + i;
         off[i] = (q < BM / 8 ? (q * 8 + (lane >> 3)) * p.lda : (q * 8 - BM + (lane >> 3)) * p.ldb) + lc;
       }
+      const int part = nt_part(p);
       auto ask = [&](int t, int buf) __attribute__((always_inline)) {
-        const int k0 = t * 128;
         // past K, and past the last stage: zeros, and no memory is read
-        const bool in = t < k_hi && k0 + lc < p.K;
+        const bool in = t < k_hi && t * 128 + lc < p.K;
+        const int tb = nt_stage_of_b(t, part);
 #pragma unroll
-        for (int i = 0; i < PW; ++i)
-          nt_lds_load16(w * PW + i < BM / 8 ? rsa : rsb, lds + buf * STAGE + (w * PW + i) * 1024, in ? off[i] + k0 : kNtOutside);
+        for (int i = 0; i < PW; ++i) {
+          const bool a = w * PW + i < BM / 8;
+          nt_lds_load16(a ? rsa : rsb, lds + buf * STAGE + (w * PW + i) * 1024, in ? off[i] + (a ? t : tb) * 128 : kNtOutside);
+        }
       };
       for (int t = 0; t < NB - 1; ++t) ask(k_lo + t, t);
       int buf = NB - 1;
@@ -286,5 +297,54 @@ struct NtSmall {
   __device__ static __forceinline__ int row(int m0, int wave, int lane) { return m0 + wave / WN * WTM + (lane & 15); }
   __device__ static __forceinline__ int column(int n0, int wave, int lane) { return n0 + wave % WN * WTN + 4 * (lane >> 4); }
 };
+
+// The forms of tile, and what they take: us a stage of 128 bytes on a CU, alone (first) and with all CUs at work. From
+// timed calls of 48 to 4096 rows with weights that no cache holds. A CU takes its blocks one after another or side by side; either way their
+// stages add up, bound by what its L1 gives (64 bytes a clock: 64 x 64 reads four times as much a product as 256 x 256)
+// and, at 256 x 256, by the matrix cores at the clock that they leave it (64 x 64 x 128 on every CU of 4096 x 8192 x 8192).
+struct NtForm {
+  int bm, bn;
+  float alone, busy;
+};
+inline constexpr NtForm kNtForms[] = {{64, 64, 0.24f, 0.23f}, {128, 64, 0.36f, 0.45f}, {128, 128, 0.52f, 0.60f}, {128, 128, 0.55f, 0.55f}, {256, 256, 1.35f, 1.85f}};
+
+// The quickest form and number of ranges of K (bytes) by these figures: 4 us for a launch and its first stage; K ranges cost a second launch
+// and their sums' way through memory. (int8, 333 x 4096 x 11008: 128 x 128 in two ranges 35 us, whole 49, 128 x 64 35, 64 x 64 43.)
+inline void nt_choose(int64_t M, int64_t N, int64_t K, int& form, int& splits) {
+  const int64_t units = cdiv(K, 128);
+  float best = 3e38f;
+  for (int f = 0; f < 5; ++f) {
+    const NtForm& t = kNtForms[f];
+    const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn);
+    for (int s = 1; s <= (f < 3 && M <= 65535 ? 8 : 1) && (s == 1 || units / s >= 4); ++s) {  // (the join has a block row a row)
+      // (128 x 128 in phases needs two blocks a CU, which begin and end together)
+      const int64_t deep = f == 3 ? 2 * cdiv(tiles, 512) : cdiv(tiles * s, 256);
+      const float stage = deep > 1 ? t.busy : t.alone + (t.busy - t.alone) * (float)(tiles * s) / 256.0f;
+      const float us = 4.0f + (float)(deep * cdiv(units, s)) * stage +
+                       (s > 1 ? 6.0f + (float)s * (float)M * (float)N * 4.0f / 2.5e6f : 0.0f);
+      if (us < best) {
+        best = us;
+        form = f;
+        splits = s;
+      }
+    }
+  }
+}
+
+// Calls f with the chosen form's type as Form<T>{}; those past the third take no ranges.
+template <class T>
+struct Form {
+  using type = T;
+};
+template <class Op, class F>
+int nt_form(int form, F f) {
+  switch (form) {
+    case 0: return f(Form<NtSmall<Op, 64, 64, 5, 4, 4>>{});
+    case 1: return f(Form<NtSmall<Op, 128, 64, 6, 4, 4>>{});
+    case 2: return f(Form<NtSmall<Op, 128, 128, 4, 8, 4>>{});
+    case 3: return f(Form<NtTile<Op, 128, 2>>{});
+    default: return f(Form<NtTile<Op, 256, 2>>{});
+  }
+}
 
 }  // namespace mls
