@@ -97,25 +97,44 @@ __global__ __launch_bounds__(T::THREADS) void a8_tile_kernel(const TileArgs p) {
       sw[i][e] = float_at(p.s.sw, p.s.sw_dt, n);
       bias[i][e] = p.s.bias ? float_at(p.s.bias, p.s.bias_dt, n) : 0.0f;
     }
-  const bool v4 = p.ldc % 4 == 0 && ((uintptr_t)p.c & (4 * sizeof(CT) - 1)) == 0;
+  const bool wide = (p.ldc * sizeof(CT)) % 16 == 0 && ((uintptr_t)p.c & 15) == 0;
+  if constexpr (sizeof(CT) == 2) {
+    const int lk = lane >> 4, nt0 = n0 - 4 * lk;
 #pragma unroll
-  for (int i = 0; i < T::TN; ++i)
+    for (int i = 0; i < T::TN; i += 2)
 #pragma unroll
-    for (int j = 0; j < T::TM; ++j) {
-      const int m = m0 + 16 * j, n = n0 + 16 * i;
-      if (m >= M || n >= N) continue;
-      CT* dst = (CT*)p.c + (int64_t)m * p.ldc + n;
-      float y[4];
+      for (int j = 0; j < T::TM; ++j) {
+        uint2 o[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = scaled(acc[i][j][e], sw[i][e], sx[j], bias[i][e]);
-      if (n + 3 < N && v4) {
-        store4<CT>(dst, y[0], y[1], y[2], y[3]);
-      } else {
+        for (int t = 0; t < 2; ++t) {
+          CT y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < N) dst[e] = from_f32<CT>(y[e]);
+          for (int e = 0; e < 4; ++e) y[e] = from_f32<CT>(scaled(acc[i + t][j][e], sw[i + t][e], sx[j], bias[i + t][e]));
+          o[t] = make_uint2(pack2_bits(y[0], y[1]), pack2_bits(y[2], y[3]));
+        }
+        const int m = m0 + 16 * j;
+        nt_store_pair((uint16_t*)p.c + (int64_t)m * p.ldc + nt0 + 16 * i, nt0 + 16 * i, N, o[0], o[1], lk, m < M, wide);
       }
-    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+      for (int j = 0; j < T::TM; ++j) {
+        const int m = m0 + 16 * j, n = n0 + 16 * i;
+        if (m >= M || n >= N) continue;
+        CT* dst = (CT*)p.c + (int64_t)m * p.ldc + n;
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = scaled(acc[i][j][e], sw[i][e], sx[j], bias[i][e]);
+        if (n + 3 < N && wide) {
+          store4<CT>(dst, y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < N) dst[e] = from_f32<CT>(y[e]);
+        }
+      }
+  }
 }
 
 // Adds the K ranges' sums: 4 columns a thread.

@@ -127,24 +127,41 @@ __global__ __launch_bounds__(G::THREADS) void dw8_kernel(const Dw8Args p) {
     return;
   using CT = std::conditional_t<PARTIAL, float, T>;
   CT* c = (CT*)p.c + (PARTIAL ? (int64_t)sp * p.o.M * p.ldc : 0);
-  const bool v4 = p.ldc % 4 == 0 && ((uintptr_t)p.c & (4 * sizeof(CT) - 1)) == 0;
+  const bool wide = (p.ldc * sizeof(CT)) % 16 == 0 && ((uintptr_t)p.c & 15) == 0;
   const int M = p.o.M, N = p.o.N, m0 = G::row(mt * G::BM, wave, lane), n0 = G::column(nt * G::BN, wave, lane);
+  if constexpr (sizeof(CT) == 2) {
+    const int lk = lane >> 4, nt0 = n0 - 4 * lk;
 #pragma unroll
-  for (int i = 0; i < G::TN; ++i)
+    for (int i = 0; i < G::TN; i += 2)
 #pragma unroll
-    for (int j = 0; j < G::TM; ++j) {
-      const int m = m0 + 16 * j, n = n0 + 16 * i;
-      if (m >= M || n >= N) continue;
-      const f32x4 v = acc[i][j];
-      CT* dst = c + m * p.ldc + n;
-      if (n + 3 < N && v4) {
-        store4<CT>(dst, v[0], v[1], v[2], v[3]);
-      } else {
+      for (int j = 0; j < G::TM; ++j) {
+        uint2 o[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < N) dst[e] = from_f32<CT>(v[e]);
+        for (int t = 0; t < 2; ++t) {
+          const f32x4 v = acc[i + t][j];
+          o[t] = make_uint2(pack2_bits(from_f32<CT>(v[0]), from_f32<CT>(v[1])), pack2_bits(from_f32<CT>(v[2]), from_f32<CT>(v[3])));
+        }
+        const int m = m0 + 16 * j;
+        nt_store_pair((uint16_t*)c + (int64_t)m * p.ldc + nt0 + 16 * i, nt0 + 16 * i, N, o[0], o[1], lk, m < M, wide);
       }
-    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < G::TN; ++i)
+#pragma unroll
+      for (int j = 0; j < G::TM; ++j) {
+        const int m = m0 + 16 * j, n = n0 + 16 * i;
+        if (m >= M || n >= N) continue;
+        const f32x4 v = acc[i][j];
+        CT* dst = c + m * p.ldc + n;
+        if (n + 3 < N && wide) {
+          store4<CT>(dst, v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < N) dst[e] = from_f32<CT>(v[e]);
+        }
+      }
+  }
 }
 
 // Adds the ranges' sums in their order: 4 columns a thread; part [splits][N][ldp], ldp a multiple of 4.

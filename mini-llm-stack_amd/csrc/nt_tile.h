@@ -186,6 +186,26 @@ struct NtTile {
 };
 
 
+// Outputs of two neighbouring tiles of 16 columns, 16-bit: lane (lr, lk) holds columns 4 lk .. 4 lk + 3 of both (lo: those
+// of the first). Odd and even lk trade halves (v_permlane16_swap), so that a lane stores 16 bytes, and a row's 4 lanes 64 in
+// one instruction. `row`: of the first column of the first tile, n: that column; wide: rows are 16-byte aligned.
+__device__ __forceinline__ void nt_store_pair(uint16_t* row, int n, int N, uint2 lo, uint2 hi, int lk, bool in, bool wide) {
+  const auto x = __builtin_amdgcn_permlane16_swap(lo.x, hi.x, false, false);
+  const uint32_t x0 = x[0], x1 = x[1];
+  const auto y = __builtin_amdgcn_permlane16_swap(lo.y, hi.y, false, false);
+  const uint32_t y0 = y[0], y1 = y[1];
+  const int c = 16 * (lk & 1) + 8 * (lk >> 1);
+  if (!in || n + c >= N) return;
+  if (wide && n + c + 8 <= N) {
+    *reinterpret_cast<uint4*>(row + c) = make_uint4(x0, y0, x1, y1);
+  } else {
+    const uint32_t w[4] = {x0, y0, x1, y1};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (n + c + e < N) row[c + e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+  }
+}
+
 // Both steps' operands of a stage, waited for: a's 16-row tiles lie 2048 bytes apart from address `a`, b's from `b`.
 template <int TM, int TN>
 __device__ __forceinline__ void nt_read_stage(uint32_t a, uint32_t b, i32x4 (&x)[2][TM], i32x4 (&y)[2][TN]) {
