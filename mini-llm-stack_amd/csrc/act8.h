@@ -13,6 +13,11 @@ namespace mls {
 // maximum over bits keeps a NaN (which fmaxf drops).
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
+template <int C>
+struct Dpp {
+  static constexpr int v = C;
+};
+
 struct Scale8 {
   float s, inv;
   uint32_t finite;  // all bits, or none: the codes under an infinite or NaN scale are 0
@@ -95,11 +100,21 @@ __device__ __forceinline__ uint32_t max_abs8(const float (&v)[8]) {
   return m;
 }
 
-// Maximum over each aligned group of W lanes, in all of them.
+// Maximum over each aligned group of W >= 16 lanes, in all of them.
 template <int W>
 __device__ __forceinline__ uint32_t group_max_bits(uint32_t v) {
-#pragma unroll
-  for (int off = 1; off < W; off *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, off, 64));
+  static_assert(W == 16 || W == 64, "a DPP row, or the wavefront");
+  auto dpp = [&](auto ctrl) __attribute__((always_inline)) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::v, 0xF, 0xF, false));
+  };
+  dpp(Dpp<0xB1>{});   // lane ^ 1
+  dpp(Dpp<0x4E>{});   // lane ^ 2
+  dpp(Dpp<0x141>{});  // the other quad of the octet
+  dpp(Dpp<0x140>{});  // the other octet
+  if constexpr (W == 64) {
+    v = max(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+    v = max(v, (uint32_t)__shfl_xor((int)v, 32, 64));
+  }
   return v;
 }
 
@@ -116,7 +131,12 @@ constexpr int kGroup8 = 128;  // columns that share a scale in a checkpoint
 // act8.hip: codes [M][ldq] (zeros in columns K .. kpad) and scales [M] of x's rows
 int launch_quantize_rows(const void* x, int dt, int64_t ldx, int64_t M, int64_t K, int64_t kpad, int8_t* q,
                          int64_t ldq, float* s, hipStream_t st);
-// bytes [rows][ld] -> [rows][kpad], kpad a multiple of 16, zeros from column K
-int launch_pad_rows(const uint8_t* src, int64_t ld, int64_t rows, int64_t K, int64_t kpad, uint8_t* dst, hipStream_t st);
+// bytes src [rows][ld] -> dst [rows][kpad], kpad a multiple of 16, zeros from column K, of two matrices in one launch
+struct PadRows {
+  const uint8_t* src;
+  int64_t ld, rows;
+  uint8_t* dst;
+};
+int launch_pad_rows(const PadRows& one, const PadRows& two, int64_t K, int64_t kpad, hipStream_t st);
 
 }  // namespace mls

@@ -114,11 +114,17 @@ int launch_rows(const RowArgs& p, hipStream_t st, const char* fn) {
 #define MLS_ROWS(TH, C)                                                                                          \
   hipLaunchKernelGGL((rows8_kernel<T, SILU, TH, C>), dim3((unsigned)(TH == 64 ? cdiv(p.M, 4) : p.M)),            \
                      dim3(TH == 64 ? 256 : TH), 0, st, p)
+  // Few rows: as many threads a row as it has chunks, since what a block does takes the longer the more a thread does
+  // (one row of 11008 bf16 gates and ups: 512 threads 5.9 us, 1024 4.3). Many: enough rows a CU at a time, blocks of 256.
+  const bool few = p.M <= 512;
   if (chunks <= 64) MLS_ROWS(64, 1);
   else if (chunks <= 128) MLS_ROWS(64, 2);
   else if (chunks <= 256) MLS_ROWS(256, 1);
+  else if (chunks <= 512 && few) MLS_ROWS(512, 1);
   else if (chunks <= 512) MLS_ROWS(256, 2);
+  else if (chunks <= 1024 && few) MLS_ROWS(1024, 1);
   else if (chunks <= 1024) MLS_ROWS(256, 4);
+  else if (chunks <= 2048 && few) MLS_ROWS(1024, 2);
   else if (chunks <= 2048) MLS_ROWS(512, 4);
   else if (chunks <= 4096) MLS_ROWS(1024, 4);
   else MLS_ROWS(1024, 0);
@@ -133,13 +139,16 @@ int launch_rows_dt(const RowArgs& p, int dt, hipStream_t st, const char* fn) {
   return launch_rows<__bf16, SILU>(p, st, fn);
 }
 
-__global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* __restrict__ src, int64_t ld, int64_t rows,
-                                                       int64_t K, int64_t kpad, uint8_t* __restrict__ dst) {
-  const int64_t per = kpad / 16, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * per) return;
+__global__ __launch_bounds__(256) void pad_rows_kernel(const PadRows one, const PadRows two, int64_t K, int64_t kpad) {
+  const int64_t per = kpad / 16;
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const bool second = i >= one.rows * per;
+  const PadRows p = second ? two : one;
+  if (second) i -= one.rows * per;
+  if (i >= p.rows * per) return;
   const int64_t r = i / per, k = (i - r * per) * 16;
   uint4 v = make_uint4(0, 0, 0, 0);
-  const uint8_t* s = src + r * ld + k;
+  const uint8_t* s = p.src + r * p.ld + k;
   if (k + 16 <= K) {
     __builtin_memcpy(&v, s, 16);
   } else {
@@ -149,7 +158,7 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t* __restrict
       if (k + e < K) w[e / 4] |= (uint32_t)s[e] << (8 * (e % 4));
     v = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  *reinterpret_cast<uint4*>(dst + r * kpad + k) = v;
+  *reinterpret_cast<uint4*>(p.dst + r * kpad + k) = v;
 }
 
 struct BackArgs {
@@ -202,11 +211,11 @@ int launch_quantize_rows(const void* x, int dt, int64_t ldx, int64_t M, int64_t 
   return launch_rows_dt<false>(p, dt, st, "quantize_rows");
 }
 
-int launch_pad_rows(const uint8_t* src, int64_t ld, int64_t rows, int64_t K, int64_t kpad, uint8_t* dst, hipStream_t st) {
-  const int64_t n = cdiv(rows * (kpad / 16), 256);
-  if (n > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "pad rows: %lld x %lld", (long long)rows, (long long)K);
+int launch_pad_rows(const PadRows& one, const PadRows& two, int64_t K, int64_t kpad, hipStream_t st) {
+  const int64_t n = cdiv((one.rows + two.rows) * (kpad / 16), 256);
+  if (n > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "pad rows: %lld x %lld", (long long)(one.rows + two.rows), (long long)K);
   if (n == 0) return MLS_OK;
-  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)n), dim3(256), 0, st, src, ld, rows, K, kpad, dst);
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)n), dim3(256), 0, st, one, two, K, kpad);
   return check_launch("pad rows");
 }
 

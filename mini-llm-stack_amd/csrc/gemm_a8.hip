@@ -310,7 +310,7 @@ bool rows_fit(const void* p, int64_t ld, int64_t K) {
 Plan make_plan(const mlsx_a8w8_args& a) {
   Plan p{};
   const bool codes = a.x_dt < 0;
-  p.kpad = (a.K + 15) / 16 * 16;
+  p.kpad = (a.K + 127) / 128 * 128;  // (rows of whole cache lines: 20% off a stage's loads against rows 64 bytes apart)
   p.pad_w = !rows_fit(a.w, a.ldw, a.K);
   p.few = a.M <= 16;
   // a block's quantizing takes about 0.25 us a chunk, in every round of blocks; a launch of its own 3 us
@@ -392,11 +392,12 @@ int run(const mlsx_a8w8_args& a, const Plan& p, uint8_t* ws, hipStream_t st) {
   const uint8_t* w = (const uint8_t*)a.w;
   int64_t ldx = a.ldx, ldw = a.ldw, K = a.K;
   Scales s{a.sx, a.sw, a.bias, (int)a.sw_dt, (int)a.bias_dt};
+  PadRows px{}, pw{};
   if (p.own_x) {
     x = ws + p.x_at;
     ldx = p.kpad;
     if (codes) {
-      if (const int rc = launch_pad_rows((const uint8_t*)a.x, a.ldx, a.M, a.K, p.kpad, ws + p.x_at, st)) return rc;
+      px = {(const uint8_t*)a.x, a.ldx, a.M, ws + p.x_at};
     } else {
       s.sx = (float*)(ws + p.s_at);
       if (const int rc = launch_quantize_rows(a.x, (int)a.x_dt, a.ldx, a.M, a.K, p.kpad, (int8_t*)(ws + p.x_at), p.kpad,
@@ -407,9 +408,11 @@ int run(const mlsx_a8w8_args& a, const Plan& p, uint8_t* ws, hipStream_t st) {
   if (p.pad_w) {
     w = ws + p.w_at;
     ldw = p.kpad;
-    if (const int rc = launch_pad_rows((const uint8_t*)a.w, a.ldw, a.N, a.K, p.kpad, ws + p.w_at, st)) return rc;
+    pw = {(const uint8_t*)a.w, a.ldw, a.N, ws + p.w_at};
   }
-  // padded operands: the products of the padding are zeros
+  if (const int rc = launch_pad_rows(px, pw, a.K, p.kpad, st)) return rc;
+  // Padded operands: the products of the padding are zeros. (A K that is no multiple of 16 pads both; a quantizing block
+  // pads its codes itself.)
   if ((p.own_x || p.fused) && p.pad_w) K = p.kpad;
   if (p.few) {
     FewArgs f{x, w, a.c, s, ldx, a.ldc, (int)ldw, (int)a.M, (int)a.N, (int)K, 0};
