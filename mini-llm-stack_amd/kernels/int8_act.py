@@ -68,6 +68,14 @@ def _scales(t: torch.Tensor, n: int, name: str, fn: str) -> torch.Tensor:
     return t if n <= 1 or t.stride(0) == 1 else t.contiguous()
 
 
+def _on(dev: int, entry, *args) -> int:
+    """entry(*args) with the tensors' device as the current one, whose kernels' limits the library sets."""
+    if torch._C._cuda_getDevice() == dev:
+        return entry(*args)
+    with torch.cuda.device(dev):
+        return entry(*args)
+
+
 def _no_grad(fn: str, *tensors) -> None:
     if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         no_grad_of(fn, *tensors)
@@ -84,8 +92,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     M, K = x.shape
     q = torch.empty(M, -(-K // 16) * 16, dtype=torch.int8, device=x.device)
     s = torch.empty(M, dtype=torch.float32, device=x.device)
-    kernels.check(kernels.lib().mlsx_quantize_rows(x.data_ptr(), dt, max(x.stride(0), K), M, K, q.data_ptr(), q.shape[1],
-                                                   s.data_ptr(), _raw_stream(dev)), fn)
+    kernels.check(_on(dev, kernels.lib().mlsx_quantize_rows, x.data_ptr(), dt, max(x.stride(0), K), M, K, q.data_ptr(), q.shape[1],
+                      s.data_ptr(), _raw_stream(dev)), fn)
     return q[:, :K] if q.shape[1] != K else q, s
 
 
@@ -118,11 +126,11 @@ def _product(fn, x, sx, x_dt, w_q, sw, bias, out_dtype):
         return y.zero_() if bias is None else y.copy_(bias.expand(M, N))
     args = _ARGS.pack(x.data_ptr(), 0 if sx is None else sx.data_ptr(), w_q.data_ptr(), sw.data_ptr(), b_at, y.data_ptr(), x_dt,
                       _DT[sw.dtype], b_dt, c_dt, x.stride(0) if M > 1 else K, w_q.stride(0) if N > 1 else K, N, M, N, K)
-    lib = kernels.lib()
-    rc = lib.mlsx_a8w8(args, 0, 0, _raw_stream(dev))
+    entry = kernels.lib().mlsx_a8w8
+    rc = _on(dev, entry, args, 0, 0, _raw_stream(dev))
     if rc > 0:  # (the workspace that it needs)
         ws = torch.empty(rc, dtype=torch.uint8, device=x.device)
-        rc = lib.mlsx_a8w8(args, ws.data_ptr(), rc, _raw_stream(dev))
+        rc = _on(dev, entry, args, ws.data_ptr(), rc, _raw_stream(dev))
     if rc:
         kernels.check(rc, fn)
     return y
@@ -169,9 +177,8 @@ def silu_mul_quantize(gate: torch.Tensor, up: torch.Tensor, *, checkpoint: bool 
     s = new(M, dtype=torch.float32)
     kept = (new(2, M, H, dtype=torch.int8), new(2, M, -(-H // GROUP), dtype=torch.float32)) if checkpoint else None
     kq, ks = (kept[0].data_ptr(), kept[1].data_ptr()) if checkpoint and H else (0, 0)
-    kernels.check(kernels.lib().mlsx_silu_mul_quantize(gate.data_ptr(), max(gate.stride(0), H), up.data_ptr(), max(up.stride(0), H),
-                                                       dt, M, H, q.data_ptr(), q.shape[1], s.data_ptr(), kq, ks,
-                                                       _raw_stream(dev)), fn)
+    kernels.check(_on(dev, kernels.lib().mlsx_silu_mul_quantize, gate.data_ptr(), max(gate.stride(0), H), up.data_ptr(),
+                      max(up.stride(0), H), dt, M, H, q.data_ptr(), q.shape[1], s.data_ptr(), kq, ks, _raw_stream(dev)), fn)
     q = q[:, :H] if q.shape[1] != H else q
     return (q, s, kept) if checkpoint else (q, s)
 
@@ -194,16 +201,16 @@ def silu_mul_backward(dh: torch.Tensor, kept: tuple[torch.Tensor, torch.Tensor])
     _no_grad(fn, dh, s)
     dev = one_device(fn, dh, q, s)
     dgate, dup = (torch.empty(M, H, dtype=dh.dtype, device=dh.device) for _ in range(2))
-    kernels.check(kernels.lib().mlsx_silu_mul_backward(
-        dh.data_ptr(), max(dh.stride(0), H), dt, q.data_ptr(), q.stride(1), q.stride(0), s.data_ptr(), s.stride(1), s.stride(0),
-        M, H, dgate.data_ptr(), dup.data_ptr(), H, _raw_stream(dev)), fn)
+    kernels.check(_on(dev, kernels.lib().mlsx_silu_mul_backward, dh.data_ptr(), max(dh.stride(0), H), dt, q.data_ptr(),
+                      max(q.stride(1), H), q.stride(0), s.data_ptr(), max(s.stride(1), G), s.stride(0), M, H, dgate.data_ptr(),
+                      dup.data_ptr(), H, _raw_stream(dev)), fn)
     return dgate, dup
 
 
 def int8_weight_grad(dy: torch.Tensor, x_q: torch.Tensor, sx: torch.Tensor) -> torch.Tensor:
     """dw [N, K] = dy [M, N]^T (x_q sx[:, None]) [M, K] in dy's dtype, fp32 sums: the gradient of a weight whose
     layer kept its input as quantize_rows' codes and scales. For 16-bit dy the kept values are rounded to
-    dy's dtype on the way to the matrix cores; fp32 loses nothing."""
+    dy's dtype on the way to the matrix cores; fp32 rounds dy * sx once, to fp32. Up to 2^20 tokens."""
     fn = "int8_weight_grad"
     dt = dt_code(dy.dtype, fn)
     dy, x_q = _two(dy, "dy", fn), _codes(x_q, "x_q", fn)
@@ -223,6 +230,6 @@ def int8_weight_grad(dy: torch.Tensor, x_q: torch.Tensor, sx: torch.Tensor) -> t
     lib = kernels.lib()
     need = lib.mlsx_dw_int8_workspace(dt, M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
-    kernels.check(lib.mlsx_dw_int8(dy.data_ptr(), dt, max(dy.stride(0), N), x_q.data_ptr(), max(x_q.stride(0), K), sx.data_ptr(),
-                                   dw.data_ptr(), K, M, N, K, ws.data_ptr(), need, _raw_stream(dev)), fn)
+    kernels.check(_on(dev, lib.mlsx_dw_int8, dy.data_ptr(), dt, max(dy.stride(0), N), x_q.data_ptr(), max(x_q.stride(0), K),
+                      sx.data_ptr(), dw.data_ptr(), K, M, N, K, ws.data_ptr(), need, _raw_stream(dev)), fn)
     return dw

@@ -10,6 +10,9 @@ Int8SwiGLU is a whole MLP, w_down(silu(w_gate(x)) * w_up(x)): the product goes t
 kernel that computes it, and gate and up are kept in 8 bits with a scale for every 128 columns. For a batch of M
 tokens it keeps M (dim + 3 hidden) bytes and scales, where the plain layers keep M (dim + 3 hidden) values and silu's own.
 
+In a captured graph take gradients with torch.autograd.grad, or capture before any eager backward of the same
+parameters: torch's accumulation into .grad stays on the stream where a parameter was first used.
+
 use_kernel=False runs the same arithmetic in torch ops, on the host or a device.
 """
 

@@ -204,6 +204,29 @@ def test_sizes_of_zero():
     assert a8.int8_weight_grad(torch.zeros(3, 0, device="cuda"), torch.zeros(3, 6, dtype=torch.int8, device="cuda"), torch.zeros(3, device="cuda")).shape == (0, 6)
 
 
+@pytest.mark.parametrize("M", [1, 16, 40, 300])
+def test_rows_behind_the_operands_are_not_read(M):
+    """Operands inside larger buffers whose other bytes are -128 and whose other scales are NaN, K no multiple of 128."""
+    K, N = 208, 70
+    q, s = a8.quantize_rows(rows_like(M, K, F32, M).cuda())
+    w, sw = weights(N, K)
+    def inside(t, fill, rows, cols):
+        big = torch.full((t.shape[0] + 2 * rows, t.shape[1] + 2 * cols), fill, dtype=t.dtype, device="cuda")
+        view = big[rows:-rows, cols:t.shape[1] + cols]
+        view.copy_(t)
+        return view
+    want = a8.int8_scaled_matmul(q, s, w, sw, out_dtype=F32)
+    for cols in (16, 3):
+        assert torch.equal(a8.int8_scaled_matmul(inside(q, -128, 2, cols), s, inside(w, -128, 2, cols), sw, out_dtype=F32), want)
+    y = torch.full((M + 2, N + 8), 7.0, device="cuda")  # the C entry's rows of any distance: what is beside them stays
+    args = a8._ARGS.pack(q.data_ptr(), s.data_ptr(), w.data_ptr(), sw.data_ptr(), 0, y[1:, 4:].data_ptr(), -1, 0, 0, 0, q.stride(0), K, N + 8, M, N, K)
+    ws = torch.empty(max(1, a8.kernels.lib().mlsx_a8w8_ws(args)), dtype=torch.uint8, device="cuda")
+    assert a8.kernels.lib().mlsx_a8w8(args, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(y[1:-1, 4:-4], want)
+    y[1:-1, 4:-4] = 7.0
+    assert bool((y == 7.0).all())
+
+
 # ---------------------------------------------------------------- silu_mul_quantize
 
 def sigmoid_error(g):

@@ -111,6 +111,18 @@ def test_convert_and_train_a_model():
     assert all(bool(torch.isfinite(p.grad).all()) and bool(p.grad.any()) for p in net.parameters())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_batches_of_no_tokens_and_expanded_gradients(dtype):
+    layer = Int8SwiGLU(*lins([(64, 96), (64, 96), (96, 64)], dtype=dtype))
+    x = torch.zeros(2, 0, 64, dtype=dtype, device="cuda", requires_grad=True)
+    layer(x).sum().backward()
+    assert x.grad.shape == x.shape and all(not bool(p.grad.any()) for p in layer.parameters())
+    x = torch.randn(2, 5, 64, device="cuda").to(dtype)
+    got = torch.autograd.grad(layer(x).sum(), layer.parameters())  # (a gradient of stride 0)
+    y = layer(x)
+    assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(y, layer.parameters(), torch.ones_like(y))))
+
+
 # ---------------------------------------------------------------- serving
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -135,6 +147,7 @@ def test_served_swiglu_is_its_operators_in_turn(M):
     g, u = qs[0](x), qs[1](x)
     want = qs[2].matmul_codes(*a8.silu_mul_quantize(g, u), BF16)
     assert torch.equal(ServeSwiGLU(*qs)(x), want)
+    assert ServeSwiGLU(*qs)(x[:0]).shape == (0, D)
 
 
 @torch.no_grad()
