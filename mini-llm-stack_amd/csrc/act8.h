@@ -50,6 +50,25 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], const Scale8& g) {
                     pack_codes(code8(v[4], g), code8(v[5], g), code8(v[6], g), code8(v[7], g)) & g.finite);
 }
 
+// 8 consecutive values of a row as they lie there, of a K that is a multiple of 8 (past K: others of the row). Without a
+// branch, so that several are on their way at once: a load8 is waited for within its own.
+template <typename T>
+struct Raw8 {
+  T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> fetch8(const T* row, int64_t k, int64_t K) {
+  Raw8<T> r;
+  const int64_t other = (threadIdx.x & 63) * 8;
+  __builtin_memcpy(&r, row + (k < K ? k : other < K ? other : 0), sizeof(r));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void widen8(const Raw8<T>& r, bool in, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = in ? to_f32(r.v[e]) : 0.0f;
+}
+
 // 8 consecutive values of a row from column k, zeros past K; any alignment of a whole number of values.
 template <typename T>
 __device__ __forceinline__ void load8(const T* row, int64_t k, int64_t K, float (&v)[8]) {
@@ -64,6 +83,11 @@ __device__ __forceinline__ void load8(const T* row, int64_t k, int64_t K, float 
   }
 }
 
+__device__ __forceinline__ void codes_to_values(uint32_t lo, uint32_t hi, float s, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? lo : hi) >> (8 * (e % 4))) * s;
+}
+
 // 8 consecutive codes of a row from column k as values, zeros past K; any alignment.
 __device__ __forceinline__ void load_codes8(const int8_t* row, int64_t k, int64_t K, float s, float (&v)[8]) {
   uint32_t w[2] = {0, 0};
@@ -74,8 +98,7 @@ __device__ __forceinline__ void load_codes8(const int8_t* row, int64_t k, int64_
     for (int e = 0; e < 8; ++e)
       if (k + e < K) w[e / 4] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e % 4));
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * s;
+  codes_to_values(w[0], w[1], s, v);
 }
 
 // n <= 8 values to a row; any alignment of a whole number of values.

@@ -42,13 +42,10 @@ __device__ __forceinline__ void keep8(const RowArgs& p, int which, int64_t m, in
   if (k % kGroup8 == 0) p.kept_s[row * p.groups + k / kGroup8] = g.s;
 }
 
-// 8 values of the row to quantize
+// From 8 values of gate (or x) and up: those of the row to quantize, and the checkpoint's codes
 template <typename T, bool SILU>
-__device__ __forceinline__ void value8(const RowArgs& p, int64_t m, int64_t k, bool keep, float (&v)[8]) {
-  load8((const T*)p.x + m * p.ldx, k, p.K, v);
+__device__ __forceinline__ void product8(const RowArgs& p, int64_t m, int64_t k, bool keep, float (&v)[8], const float (&u)[8]) {
   if constexpr (SILU) {
-    float u[8];
-    load8((const T*)p.u + m * p.ldu, k, p.K, u);
     if (keep) {
       keep8(p, 0, m, k, v);
       keep8(p, 1, m, k, u);
@@ -56,6 +53,14 @@ __device__ __forceinline__ void value8(const RowArgs& p, int64_t m, int64_t k, b
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = v[e] * sigmoid<T>(v[e]) * u[e];
   }
+}
+
+template <typename T, bool SILU>
+__device__ __forceinline__ void value8(const RowArgs& p, int64_t m, int64_t k, bool keep, float (&v)[8]) {
+  float u[8];
+  load8((const T*)p.x + m * p.ldx, k, p.K, v);
+  if constexpr (SILU) load8((const T*)p.u + m * p.ldu, k, p.K, u);
+  product8<T, SILU>(p, m, k, keep, v, u);
 }
 
 // THREADS threads a row, C chunks of 8 columns a thread (C = 0: any number, the row read twice). Rows of a
@@ -70,10 +75,29 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rows8_kernel(co
   float v[C ? C : 1][8];
   uint32_t top = 0;
   if constexpr (C != 0) {
+    if (p.K % 8 == 0 && p.K > 0) {
+      Raw8<T> x[C], u[SILU ? C : 1];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      value8<T, SILU>(p, m, (int64_t)(c * THREADS + t) * 8, keep, v[c]);
-      top = max(top, max_abs8(v[c]));
+      for (int c = 0; c < C; ++c) {
+        const int64_t k = (int64_t)(c * THREADS + t) * 8;
+        x[c] = fetch8((const T*)p.x + m * p.ldx, k, p.K);
+        if constexpr (SILU) u[c] = fetch8((const T*)p.u + m * p.ldu, k, p.K);
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int64_t k = (int64_t)(c * THREADS + t) * 8;
+        float uv[8];
+        widen8(x[c], k < p.K, v[c]);
+        if constexpr (SILU) widen8(u[c], k < p.K, uv);
+        product8<T, SILU>(p, m, k, keep, v[c], uv);
+        top = max(top, max_abs8(v[c]));
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        value8<T, SILU>(p, m, (int64_t)(c * THREADS + t) * 8, keep, v[c]);
+        top = max(top, max_abs8(v[c]));
+      }
     }
   } else {
     // (whole groups of lanes: keep8 needs them all)
@@ -178,12 +202,24 @@ template <typename T>
 __global__ __launch_bounds__(256) void silu_back_kernel(const BackArgs p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= p.M * p.per) return;
-  const int64_t m = i / p.per, k = (i - m * p.per) * 8;
-  float d[8], g[8], u[8];
-  load8((const T*)p.dh + m * p.lddh, k, p.H, d);
+  const int64_t m = (p.M * p.per) >> 32 ? i / p.per : (uint32_t)i / (uint32_t)p.per, k = (i - m * p.per) * 8;
   const float* s = p.s + m * p.lds + k / kGroup8;
-  load_codes8(p.q + m * p.ldq, k, p.H, s[0], g);
-  load_codes8(p.q + p.qs + m * p.ldq, k, p.H, s[p.ss], u);
+  const int8_t *q0 = p.q + m * p.ldq, *q1 = q0 + p.qs;
+  const T* dh = (const T*)p.dh + m * p.lddh;
+  float d[8], g[8], u[8];
+  if (p.H % 8 == 0) {
+    const Raw8<T> raw = fetch8(dh, k, p.H);
+    const Raw8<int8_t> c0 = fetch8(q0, k, p.H), c1 = fetch8(q1, k, p.H);
+    const float s0 = s[0], s1 = s[p.ss];
+    const uint2 w0 = __builtin_bit_cast(uint2, c0), w1 = __builtin_bit_cast(uint2, c1);
+    widen8(raw, true, d);
+    codes_to_values(w0.x, w0.y, s0, g);
+    codes_to_values(w1.x, w1.y, s1, u);
+  } else {
+    load8(dh, k, p.H, d);
+    load_codes8(q0, k, p.H, s[0], g);
+    load_codes8(q1, k, p.H, s[p.ss], u);
+  }
   float dg[8], du[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {

@@ -175,7 +175,7 @@ struct FewArgs {
   int64_t ldx, ldc;
   int ldw;
   int M, N, K;
-  int values;  // columns of x to quantize (K: those and the weights' padding)
+  int values;  // columns of x to quantize, a multiple of 8 (K: those and the weights' padding)
 };
 
 constexpr int kFewWaves = 16;
@@ -217,17 +217,23 @@ __global__ __launch_bounds__(64 * kFewWaves) void a8_few_kernel(const FewArgs p)
     int R = 1;
     while (R < p.M) R *= 2;
     const int P = kFewWaves / R, row = wave / P, part = wave % P;
+    // (no branch around a load: its merge would wait for the weights in flight)
+    const XT* src = (const XT*)p.x + min(row, p.M - 1) * p.ldx;
+    Raw8<XT> raw[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) raw[c] = fetch8(src, ((c * P + part) * 64 + lane) * 8, p.values);
+    // x of all wavefronts before any weights, behind which the last would get it
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    load_w(wave);
+    __builtin_amdgcn_sched_barrier(0);
     float v[C][8];
     uint32_t top = 0;
-    if (row < p.M) {
-      const XT* src = (const XT*)p.x + row * p.ldx;
 #pragma unroll
-      for (int c = 0; c < C; ++c) load8(src, ((c * P + part) * 64 + lane) * 8, p.values, v[c]);
-    }
-    load_w(wave);
-    if (row < p.M) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) top = max(top, max_abs8(v[c]));
+    for (int c = 0; c < C; ++c) {
+      widen8(raw[c], ((c * P + part) * 64 + lane) * 8 < p.values, v[c]);
+      top = max(top, max_abs8(v[c]));
     }
     top = group_max_bits<64>(top);
     if (lane == 0) tops[wave] = top;
@@ -314,7 +320,7 @@ Plan make_plan(const mlsx_a8w8_args& a) {
   p.pad_w = !rows_fit(a.w, a.ldw, a.K);
   p.few = a.M <= 16;
   // a block's quantizing takes about 0.25 us a chunk, in every round of blocks; a launch of its own 3 us
-  p.fused = a.x_dt == a.c_dt && p.few && few_chunks(a.M, a.K) <= 6 && few_chunks(a.M, a.K) * cdiv(a.N, 4096) <= 6;
+  p.fused = a.x_dt == a.c_dt && p.few && a.K % 8 == 0 && few_chunks(a.M, a.K) <= 6 && few_chunks(a.M, a.K) * cdiv(a.N, 4096) <= 6;
   p.own_x = codes ? !rows_fit(a.x, a.ldx, a.K) : !p.fused;
   p.splits = 1;
   if (!p.few) nt_choose(a.M, a.N, a.K, p.form, p.splits);

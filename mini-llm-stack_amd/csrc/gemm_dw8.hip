@@ -59,24 +59,40 @@ __device__ __forceinline__ void turn(const TurnArgs& p, int C, P* dst) {
   const int c0 = blockIdx.x * 8 * W + (threadIdx.x & 7) * W, m0 = blockIdx.y * 64 + (threadIdx.x >> 3) * 8;
   if (c0 >= C) return;
   float v[8][W];  // [token][column]
+  float scale[8];
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const int m = m0 + r;
-    if (m >= p.M) {
+  for (int r = 0; r < 8; ++r) scale[r] = p.s[min(m0 + r, p.M - 1)];
+  if ((int)(blockIdx.x + 1) * 8 * W <= C) {
+    // without branches, so that all rows are on their way at once
+    using Raw = std::conditional_t<CODES, int8_t, T>;
+    const Raw* src = CODES ? (const Raw*)p.q : (const Raw*)p.dy;
+    const int64_t ld = CODES ? p.ldq : p.lddy;
+    Raw raw[8][W];
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[r][e] = 0.0f;
-    } else if constexpr (CODES) {
-      // (fp32: the scale goes to dy)
-      load_codes8(p.q + (int64_t)m * p.ldq, c0, C, sizeof(T) == 4 ? 1.0f : p.s[m], v[r]);
-    } else {
-      load_some<W>((const T*)p.dy + (int64_t)m * p.lddy + c0, C - c0, v[r]);
-      if constexpr (sizeof(T) == 4) {
-        const float s = p.s[m];
+    for (int r = 0; r < 8; ++r) __builtin_memcpy(raw[r], src + min(m0 + r, p.M - 1) * ld + c0, sizeof(raw[r]));
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[r][e] *= s;
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        if constexpr (CODES) v[r][e] = (float)raw[r][e];
+        else v[r][e] = to_f32(raw[r][e]);
       }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int64_t m = min(m0 + r, p.M - 1);
+      if constexpr (CODES) load_codes8(p.q + m * p.ldq, c0, C, 1.0f, v[r]);
+      else load_some<W>((const T*)p.dy + m * p.lddy + c0, C - c0, v[r]);
     }
   }
+  // 16-bit: codes become values here; fp32: the scale goes to dy
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      if constexpr (CODES != (sizeof(T) == 4)) v[r][e] *= scale[r];
+      if (m0 + r >= p.M) v[r][e] = 0.0f;
+    }
 #pragma unroll
   for (int c = 0; c < W; ++c) {
     if (c0 + c >= C) continue;
