@@ -318,18 +318,20 @@ struct NtSmall {
   __device__ static __forceinline__ int column(int n0, int wave, int lane) { return n0 + wave % WN * WTN + 4 * (lane >> 4); }
 };
 
-// The forms of tile, and what they take: us a stage of 128 bytes on a CU, alone (first) and with all CUs at work. From
-// timed calls of 48 to 4096 rows with weights that no cache holds. A CU takes its blocks one after another or side by side; either way their
-// stages add up, bound by what its L1 gives (64 bytes a clock: 64 x 64 reads four times as much a product as 256 x 256)
-// and, at 256 x 256, by the matrix cores at the clock that they leave it (64 x 64 x 128 on every CU of 4096 x 8192 x 8192).
+// The forms of tile, and what they take: us a stage of 128 bytes on a CU, with few CUs at work (alone) and with all (busy),
+// from timed calls of 48 to 4096 rows whose weights no cache holds. A CU takes its blocks one after another or side by side; either
+// way their stages add up. Bounds: what a CU's loads to LDS bring (86 to 91 bytes a ns; 64 x 64 reads four times as
+// much a product as 256 x 256), a barrier a stage, and at 256 x 256 the matrix cores at the clock that they leave themselves.
 struct NtForm {
   int bm, bn;
   float alone, busy;
 };
 inline constexpr NtForm kNtForms[] = {{64, 64, 0.24f, 0.23f}, {128, 64, 0.36f, 0.45f}, {128, 128, 0.52f, 0.60f}, {128, 128, 0.55f, 0.55f}, {256, 256, 1.35f, 1.85f}};
 
-// The quickest form and number of ranges of K (bytes) by these figures: 4 us for a launch and its first stage; K ranges cost a second launch
-// and their sums' way through memory. (int8, 333 x 4096 x 11008: 128 x 128 in two ranges 35 us, whole 49, 128 x 64 35, 64 x 64 43.)
+// The quickest form and number of ranges of K (bytes) by these figures: 4 us for a launch and its first stage; ranges cost a
+// second launch and their sums' way through memory. Int8, us of each form (64 x 64, 128 x 64, 128 x 128, that in phases, 256 x 256; best
+// in ranges): 333 x 4096 x 11008 43, 36, 49, 89, 133; 35 in two of 128 x 128. 1024 x 4096 x 4096 27, 26, 20, 29, 43.
+// 2048 x 4096 x 4096 52, 50, 39, 38, 44. 4096 x 11008 x 4096 305, 339, 242, 238, 168. 64 x 4096 x 11008 31; 17 in four.
 inline void nt_choose(int64_t M, int64_t N, int64_t K, int& form, int& splits) {
   const int64_t units = cdiv(K, 128);
   float best = 3e38f;
@@ -341,7 +343,7 @@ inline void nt_choose(int64_t M, int64_t N, int64_t K, int& form, int& splits) {
       const int64_t deep = f == 3 ? 2 * cdiv(tiles, 512) : cdiv(tiles * s, 256);
       const float stage = deep > 1 ? t.busy : t.alone + (t.busy - t.alone) * (float)(tiles * s) / 256.0f;
       const float us = 4.0f + (float)(deep * cdiv(units, s)) * stage +
-                       (s > 1 ? 6.0f + (float)s * (float)M * (float)N * 4.0f / 2.5e6f : 0.0f);
+                       (s > 1 ? 8.0f + (float)s * (float)M * (float)N * 4.0f / 2.5e6f : 0.0f);
       if (us < best) {
         best = us;
         form = f;
