@@ -1,6 +1,6 @@
 // Activations in 8 bits: codes of rows for the int8 product, SwiGLU's product with its codes and the 8-bit
 // checkpoint of its two inputs, and its backward pass from that checkpoint. All are bound by memory: 2048 x 5632 bf16 gates and
-// ups with their checkpoint 21.6 us (3.8 TB/s), the backward of 4096 x 11008 73 us (5.0 TB/s, a copy's rate).
+// ups with their checkpoint 20.5 us (3.9 TB/s; 21 from cold memory), the backward of 4096 x 11008 73 us (5.0 TB/s, a copy's rate).
 //
 // Forward kernels: a row's values stay in registers between the pass that finds its largest and the one that makes codes, so every
 // input is read once. A row belongs to one wavefront (up to 1024 columns) or one block; the longest rows are read
@@ -35,7 +35,8 @@ __device__ __forceinline__ void store_codes(int8_t* dst, const uint2& c, int64_t
 }
 
 // The same of two chunks of a lane at columns ka and kb, the lanes' neighbours 8 columns on, n a multiple of 16: lanes 2 i and
-// 2 i + 1 trade a chunk, so that each stores 16 bytes of one (2048 rows of 5632 with their checkpoint: 21.6 us with stores of 8 bytes).
+// 2 i + 1 trade a chunk, so that each stores 16 bytes of one. Against stores of 8 bytes and no form of three chunks, with the checkpoint:
+// 4096 x 11008 76.8 -> 64.2 us, 2048 x 5632 21.3 -> 20.5, 4096 x 8192 equal; one row of 11008 5.7 -> 6.2, the price of the trade.
 __device__ __forceinline__ void store_two(int8_t* row, const uint2& a, const uint2& b, int64_t ka, int64_t kb, int64_t n, int t) {
   auto neighbour = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false); };
   const bool odd = t & 1;
@@ -188,6 +189,7 @@ int launch_rows(const RowArgs& p, hipStream_t st, const char* fn) {
                      dim3(TH == 64 ? 256 : TH), 0, st, p)
   // Few rows: as many threads a row as it has chunks, since what a block does takes the longer the more a thread does
   // (one row of 11008 bf16 gates and ups: 512 threads 5.9 us, 1024 4.3). Many: enough rows a CU at a time, blocks of 256.
+  // Three chunks where four would leave a quarter of the threads without columns (with the checkpoint's stores: the times at store_two).
   const bool few = p.M <= 512;
   if (chunks <= 64) MLS_ROWS(64, 1);
   else if (chunks <= 128) MLS_ROWS(64, 2);

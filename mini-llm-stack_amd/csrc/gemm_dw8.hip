@@ -7,7 +7,7 @@
 // operands would take six. Parts of values under 2^-110 lose bits below 2^-133, bf16's smallest.
 //
 // Both operands are turned first, so that their rows run along the tokens (dw8_turn_kernel; the rows' ends are padded with zeros to
-// 64 tokens), then multiplied tile by tile (nt_tile.h). 2100 tokens, 11008 x 4096, bf16: turn 22 us (bytes at a copy's rate 23.6), product 157
+// 64 tokens), then multiplied tile by tile (nt_tile.h). 2100 tokens, 11008 x 4096, bf16: turn 22 us (bytes at a copy's rate 23.6), product 155
 // (1.2 PFLOP/s); the library's product of full-width operands 244. fp32, 1000 tokens, 2048 x 1024: 11 and 21, the library's 37.
 #include <algorithm>
 #include <type_traits>

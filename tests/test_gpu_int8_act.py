@@ -77,6 +77,39 @@ def test_codes_are_the_definition(M, K, dtype):
     assert np.array_equal(q.cpu().numpy(), want_q)
 
 
+# Past 512 rows blocks hold fewer threads a row: both sides of each length at which their form changes, lengths that end inside a
+# block's last columns, and of 8 but not 16.
+MANY = [(513, K) for K in (1032, 2048, 2056, 4096, 4104, 5632, 6144, 6152, 8192, 8200, 11008, 12288, 12296, 16384, 16392, 32776)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K", MANY + [(520, 5633), (520, 11001)])
+def test_codes_of_many_rows_are_the_definition(M, K, dtype):
+    x = rows_like(M, K, dtype, K)
+    q, s = a8.quantize_rows(x.cuda())
+    want_q, want_s = codes_of(x)
+    assert np.array_equal(s.cpu().numpy(), want_s)
+    assert np.array_equal(q.cpu().numpy(), want_q)
+
+
+@pytest.mark.parametrize("M,H", MANY + [(520, 5633), (520, 11001)])
+def test_silu_mul_quantize_of_many_rows(M, H):
+    """What the rows give in two calls of fewer than 512, and the checkpoint's codes by their definition."""
+    dtype = TYPES[H // 8 % 3]
+    gate, up = (3 * torch.randn(M, H, generator=gen(H))).to(dtype).cuda(), rows_like(M, H, dtype, H + 1).cuda()
+    q, s, (kq, ks) = a8.silu_mul_quantize(gate, up, checkpoint=True)
+    q2, s2 = a8.silu_mul_quantize(gate, up)
+    assert torch.equal(q, q2) and torch.equal(s, s2)
+    parts = [a8.silu_mul_quantize(gate[i], up[i], checkpoint=True) for i in (slice(0, 256), slice(256, M))]
+    assert torch.equal(q, torch.cat([t[0] for t in parts])) and torch.equal(s, torch.cat([t[1] for t in parts]))
+    G = -(-H // 128)
+    for i, t in enumerate((gate, up)):
+        t = torch.nn.functional.pad(t.float().cpu(), (0, G * 128 - H)).reshape(M * G, 128)
+        want_q, want_s = codes_of(t)
+        assert np.array_equal(ks[i].cpu().numpy(), want_s.reshape(M, G))
+        assert np.array_equal(kq[i].cpu().numpy(), want_q.reshape(M, G * 128)[:, :H])
+
+
 def test_codes_next_to_ties_and_of_every_size():
     """Quotients at and beside every tie, and rows from 1e-45 to 3e38."""
     g = gen(3)
