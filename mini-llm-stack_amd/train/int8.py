@@ -105,8 +105,9 @@ class _Int8LinearFn(torch.autograd.Function):
 
 class _Int8SwiGLUFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, use_kernel):
-        grad = any(ctx.needs_input_grad[:4])
+    def forward(ctx, x, w_gate, w_up, w_down, use_kernel, grad):
+        # (grad: the caller's grad mode; needs_input_grad does not know of it)
+        grad = grad and any(ctx.needs_input_grad[:4])
         weights = [_rows(w, use_kernel) for w in (w_gate, w_up, w_down)]
         x_q, sx = _rows(x, use_kernel)
         g, u = (_matmul(x_q, sx, *w, None, x.dtype, use_kernel) for w in weights[:2])
@@ -124,12 +125,12 @@ class _Int8SwiGLUFn(torch.autograd.Function):
         need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
         dwd = _weight_grad(dy, h_q, sh, k, td) if need_d else None
         if not (need_x or need_g or need_u):
-            return None, None, None, dwd, None
+            return None, None, None, dwd, None, None
         dg, du = _silu_mul_grad(_input_grad(dy, dq, ds, k), (kq, ks), k)
         dwg = _weight_grad(dg, x_q, sx, k, tg) if need_g else None
         dwu = _weight_grad(du, x_q, sx, k, tu) if need_u else None
         dx = _input_grad(dg, gq, gs, k).add_(_input_grad(du, uq, us, k)) if need_x else None
-        return dx, dwg, dwu, dwd, None
+        return dx, dwg, dwu, dwd, None, None
 
 
 class Int8Linear(nn.Module):
@@ -160,7 +161,7 @@ class Int8SwiGLU(nn.Module):
 
     def forward(self, x):
         y = _Int8SwiGLUFn.apply(x.reshape(-1, x.shape[-1]), self.w_gate.weight, self.w_up.weight, self.w_down.weight,
-                                self.use_kernel)
+                                self.use_kernel, torch.is_grad_enabled())
         return y.reshape(*x.shape[:-1], self.w_down.weight.shape[0])
 
 

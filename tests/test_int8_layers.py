@@ -92,6 +92,19 @@ def test_gradients_that_nobody_asks_for_are_not_made():
     assert lin.weight.grad is not None
 
 
+def test_no_checkpoint_without_gradients(monkeypatch):
+    import train.int8 as t8
+    kept, made = [], t8._silu_mul
+    monkeypatch.setattr(t8, "_silu_mul", lambda *a: kept.append(a[3]) or made(*a))
+    layer, x = Int8SwiGLU(*mlp(), use_kernel=False), torch.randn(3, D)
+    y = layer(x)
+    with torch.no_grad():
+        z = layer(x)
+    with torch.inference_mode():
+        layer(x)
+    assert kept == [True, False, False] and torch.equal(y, z) and not z.requires_grad
+
+
 def test_second_derivatives_are_refused():
     layer = Int8Linear(nn.Linear(D, 8), use_kernel=False)
     x = torch.randn(3, D, requires_grad=True)
