@@ -139,8 +139,8 @@ class Int8Linear(nn.Module):
 
     def __init__(self, linear: nn.Linear, use_kernel: bool = True):
         super().__init__()
-        self.weight = nn.Parameter(linear.weight.detach().clone())
-        self.bias = None if linear.bias is None else nn.Parameter(linear.bias.detach().clone())
+        copy = lambda p: None if p is None else nn.Parameter(p.detach().clone(), requires_grad=p.requires_grad)
+        self.weight, self.bias = copy(linear.weight), copy(linear.bias)
         self.use_kernel = use_kernel
 
     def forward(self, x):

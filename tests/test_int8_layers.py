@@ -105,6 +105,21 @@ def test_no_checkpoint_without_gradients(monkeypatch):
     assert kept == [True, False, False] and torch.equal(y, z) and not z.requires_grad
 
 
+def test_frozen_parameters_stay_frozen():
+    lin = nn.Linear(D, 8)
+    lin.weight.requires_grad_(False)
+    layer = Int8Linear(lin, use_kernel=False)
+    assert not layer.weight.requires_grad and layer.bias.requires_grad
+    w = mlp()
+    w[1].requires_grad_(False)
+    swi = Int8SwiGLU(*w, use_kernel=False)
+    assert [m.weight.requires_grad for m in (swi.w_gate, swi.w_up, swi.w_down)] == [True, False, True]
+    swi(torch.randn(3, D)).sum().backward()
+    assert swi.w_up.weight.grad is None and swi.w_gate.weight.grad is not None
+    c = convert_linears_to_int8(_Model().requires_grad_(False), use_kernel=False)
+    assert not any(p.requires_grad for p in c.parameters())
+
+
 def test_second_derivatives_are_refused():
     layer = Int8Linear(nn.Linear(D, 8), use_kernel=False)
     x = torch.randn(3, D, requires_grad=True)
