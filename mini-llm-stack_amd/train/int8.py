@@ -57,6 +57,16 @@ def _weight_grad(dy, x_q, sx, use_kernel, dtype):
     return (dy.float().t() @ (x_q.float() * sx[:, None])).to(dtype)
 
 
+def _bias_grad(dy, use_kernel, dtype):
+    """dy's sums over tokens, in fp32: on a device as the weight gradient of an input of ones, rounded to dy's type like it,
+    since torch's sum over many rows clears memory with a memset, which a captured graph must not hold.
+    (bf16: 4096 x 11008 47 us, torch's sum 197; 2048 x 4096 26 and 18; 64 x 4096 25 and 10.)"""
+    if use_kernel:
+        ones = torch.ones(dy.shape[0], 1, dtype=torch.int8, device=dy.device)
+        return _weight_grad(dy, ones, torch.ones(dy.shape[0], device=dy.device), True, dtype).reshape(-1)
+    return dy.sum(0, dtype=torch.float32).to(dtype)
+
+
 def _silu_mul(g, u, use_kernel, keep):
     """Codes and scales of silu(g) * u, and gate and up in 8 bits where they are kept."""
     if use_kernel:
@@ -100,7 +110,7 @@ class _Int8LinearFn(torch.autograd.Function):
         wt, bt = ctx.dtypes
         dx = _input_grad(dy, w_q, sw, ctx.use_kernel) if need_x else None
         dw = _weight_grad(dy, x_q, sx, ctx.use_kernel, wt) if need_w else None
-        return dx, dw, dy.sum(0, dtype=torch.float32).to(bt) if need_b else None, None
+        return dx, dw, _bias_grad(dy, ctx.use_kernel, bt) if need_b else None, None
 
 
 class _Int8SwiGLUFn(torch.autograd.Function):

@@ -102,6 +102,41 @@ def test_a_training_step_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(eager.parameters(), captured.parameters()))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M,N", [(1, 33), (300, 130), (5000, 257)])
+def test_bias_gradient_eager_and_replayed(M, N, dtype):
+    """Sums of M values that the matrix cores add in fp32, fp32's as three exact parts: 3 M roundings of the sum of sizes at most, then
+    one to the type. A captured backward gives the same bits at each replay."""
+    lin, = lins([(64, N)], bias=True, dtype=dtype)
+    layer, x = Int8Linear(lin), torch.randn(M, 64, device="cuda").to(dtype)
+    dys = [(torch.randn(M, N, device="cuda", generator=torch.Generator("cuda").manual_seed(i)) * 0.1).to(dtype) for i in range(4)]
+    grads = lambda dy: torch.autograd.grad(layer(x), [layer.weight, layer.bias], dy)
+    static = dys[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = grads(static)
+    for dy in dys:
+        static.copy_(dy)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = grads(dy)
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        ref, size = dy.double().sum(0), dy.double().abs().sum(0)
+        tol = 3 * M * U * size * (1 + torch.finfo(dtype).eps) + torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -25
+        assert want[1].shape == (N,) and bool(((want[1].double() - ref).abs() <= tol).all())
+
+
+def test_bias_gradient_of_no_tokens():
+    layer = Int8Linear(lins([(64, 33)], bias=True)[0])
+    layer(torch.zeros(0, 64, device="cuda")).sum().backward()
+    assert layer.bias.grad.shape == (33,) and not bool(layer.bias.grad.any())
+
+
 def test_convert_and_train_a_model():
     from test_gpu_layers import _Net
     torch.manual_seed(0)
