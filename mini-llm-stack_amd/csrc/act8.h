@@ -160,6 +160,9 @@ struct PadRows {
   int64_t ld, rows;
   uint8_t* dst;
 };
+// Whether a launch stays below 2^32 threads, the most that a grid has.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= 0xFFFFFFFFll / threads; }
+
 int launch_pad_rows(const PadRows& one, const PadRows& two, int64_t K, int64_t kpad, hipStream_t st);
 
 }  // namespace mls

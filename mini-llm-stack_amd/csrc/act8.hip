@@ -16,6 +16,7 @@ struct RowArgs {
   const void* u;   // up
   int64_t ldx, ldu;
   int64_t M, K, kpad;
+  int64_t first;   // a launch's first row
   int8_t* q;
   int64_t ldq;
   float* s;
@@ -83,7 +84,7 @@ template <typename T, bool SILU, int THREADS, int C>
 __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rows8_kernel(const RowArgs p) {
   constexpr bool WAVE = THREADS == 64;
   const int t = WAVE ? threadIdx.x & 63 : threadIdx.x;
-  const int64_t m = WAVE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const int64_t m = p.first + (WAVE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);
   if (m >= p.M) return;
   const bool keep = SILU && p.kept_q != nullptr;
   float v[C ? C : 1][8];
@@ -180,12 +181,12 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rows8_kernel(co
   }
 }
 
+// Rows p.first .. p.first + rows.
 template <typename T, bool SILU>
-int launch_rows(const RowArgs& p, hipStream_t st, const char* fn) {
-  if (p.M > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "%s: %lld rows", fn, (long long)p.M);
+int launch_some_rows(const RowArgs& p, int64_t rows, hipStream_t st, const char* fn) {
   const int64_t chunks = cdiv(p.kpad, 8);
 #define MLS_ROWS(TH, C)                                                                                          \
-  hipLaunchKernelGGL((rows8_kernel<T, SILU, TH, C>), dim3((unsigned)(TH == 64 ? cdiv(p.M, 4) : p.M)),            \
+  hipLaunchKernelGGL((rows8_kernel<T, SILU, TH, C>), dim3((unsigned)(TH == 64 ? cdiv(rows, 4) : rows)),          \
                      dim3(TH == 64 ? 256 : TH), 0, st, p)
   // Few rows: as many threads a row as it has chunks, since what a block does takes the longer the more a thread does
   // (one row of 11008 bf16 gates and ups: 512 threads 5.9 us, 1024 4.3). Many: enough rows a CU at a time, blocks of 256.
@@ -206,6 +207,14 @@ int launch_rows(const RowArgs& p, hipStream_t st, const char* fn) {
   else MLS_ROWS(1024, 0);
 #undef MLS_ROWS
   return check_launch(fn);
+}
+
+template <typename T, bool SILU>
+int launch_rows(RowArgs p, hipStream_t st, const char* fn) {
+  constexpr int64_t kRows = 1 << 21;  // a launch's most: with 1024 threads each 2^31 threads, and a grid has less than 2^32
+  for (; p.M - p.first > kRows; p.first += kRows)
+    if (const int rc = launch_some_rows<T, SILU>(p, kRows, st, fn)) return rc;
+  return launch_some_rows<T, SILU>(p, p.M - p.first, st, fn);
 }
 
 template <bool SILU>
@@ -301,7 +310,7 @@ int launch_quantize_rows(const void* x, int dt, int64_t ldx, int64_t M, int64_t 
 
 int launch_pad_rows(const PadRows& one, const PadRows& two, int64_t K, int64_t kpad, hipStream_t st) {
   const int64_t n = cdiv((one.rows + two.rows) * (kpad / 16), 256);
-  if (n > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "pad rows: %lld x %lld", (long long)(one.rows + two.rows), (long long)K);
+  if (!grid_fits(n, 256)) return fail(MLS_ERR_UNSUPPORTED, "pad rows: %lld x %lld", (long long)(one.rows + two.rows), (long long)K);
   if (n == 0) return MLS_OK;
   hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)n), dim3(256), 0, st, one, two, K, kpad);
   return check_launch("pad rows");
@@ -332,7 +341,7 @@ extern "C" int mlsx_silu_mul_quantize(const void* gate, int64_t ldg, const void*
   if ((H > 0 && (!gate || !up || !q)) || !s || (kept_q == nullptr) != (kept_s == nullptr))
     return fail(MLS_ERR_ARG, "%s: null pointer", fn);
   if (ldg < H || ldu < H || ldq < H) return fail(MLS_ERR_ARG, "%s: bad leading dimension", fn);
-  RowArgs p{gate, up, ldg, ldu, M, H, H, q, ldq, s, kept_q, kept_s, cdiv(H, kGroup8)};
+  RowArgs p{gate, up, ldg, ldu, M, H, H, 0, q, ldq, s, kept_q, kept_s, cdiv(H, kGroup8)};
   return launch_rows_dt<true>(p, dt, (hipStream_t)stream, fn);
 }
 
@@ -347,7 +356,7 @@ extern "C" int mlsx_silu_mul_backward(const void* dh, int64_t lddh, int dt, cons
   if (lddh < H || ldq < H || lds < cdiv(H, kGroup8) || ldo < H) return fail(MLS_ERR_ARG, "%s: bad leading dimension", fn);
   const BackArgs p{dh, lddh, q, ldq, q_step, s, lds, s_step, dgate, dup, ldo, M, H, cdiv(H, 8)};
   const int64_t n = cdiv(M * p.per, 256);
-  if (n > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "%s: %lld x %lld", fn, (long long)M, (long long)H);
+  if (!grid_fits(n, 256)) return fail(MLS_ERR_UNSUPPORTED, "%s: %lld x %lld", fn, (long long)M, (long long)H);
   const dim3 grid((unsigned)n), block(256);
   if (dt == MLS_F32) hipLaunchKernelGGL(silu_back_kernel<float>, grid, block, 0, (hipStream_t)stream, p);
   else if (dt == MLS_F16) hipLaunchKernelGGL(silu_back_kernel<_Float16>, grid, block, 0, (hipStream_t)stream, p);

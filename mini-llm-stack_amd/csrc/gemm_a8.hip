@@ -351,7 +351,7 @@ int launch_tiles(TileArgs t, hipStream_t st) {
   t.m_tiles = (int)cdiv(t.o.M, T::BM);
   t.n_tiles = (int)cdiv(t.o.N, T::BN);
   const int64_t blocks = (int64_t)t.m_tiles * t.n_tiles * t.splits;
-  if (blocks > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "a8w8: %d x %d", t.o.M, t.o.N);
+  if (!grid_fits(blocks, T::THREADS)) return fail(MLS_ERR_UNSUPPORTED, "a8w8: %d x %d", t.o.M, t.o.N);
   auto kern = a8_tile_kernel<CT, T, PARTIAL>;
   constexpr int lds = T::LDS;
   // (a call a launch: the limit is the function's on the current device)

@@ -227,7 +227,7 @@ int launch_dw8(Dw8Args a, hipStream_t st) {
   a.m_tiles = (int)cdiv(a.o.M, G::BM);
   a.n_tiles = (int)cdiv(a.o.N, G::BN);
   const int64_t blocks = (int64_t)a.m_tiles * a.n_tiles * a.splits;
-  if (blocks > 0x7FFFFFFF) return fail(MLS_ERR_UNSUPPORTED, "%s: %d x %d", fn, a.o.M, a.o.N);
+  if (!grid_fits(blocks, G::THREADS)) return fail(MLS_ERR_UNSUPPORTED, "%s: %d x %d", fn, a.o.M, a.o.N);
   auto kern = dw8_kernel<T, G, PARTIAL>;
   // (a call a launch: the limit is the function's on the current device)
   if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS) != hipSuccess)

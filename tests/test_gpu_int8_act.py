@@ -110,6 +110,19 @@ def test_silu_mul_quantize_of_many_rows(M, H):
         assert np.array_equal(kq[i].cpu().numpy(), want_q.reshape(M, G * 128)[:, :H])
 
 
+@pytest.mark.parametrize("K", [8, 1032])
+def test_more_rows_than_a_launch(K):
+    """2^21 rows and some: those at both ends and around the second launch's first are what they are in a call of their own."""
+    M = 2 ** 21 + 5
+    x = torch.randn(M, K, device="cuda", dtype=BF16, generator=torch.Generator("cuda").manual_seed(1))
+    q, s = a8.quantize_rows(x)
+    h_q, h_s, (kq, ks) = a8.silu_mul_quantize(x, x, checkpoint=True)
+    for r in (slice(0, 9), slice(2 ** 21 - 9, 2 ** 21), slice(2 ** 21, M)):
+        a, (b, c, (d, e)) = a8.quantize_rows(x[r]), a8.silu_mul_quantize(x[r], x[r], checkpoint=True)
+        for got, want in ((q[r], a[0]), (s[r], a[1]), (h_q[r], b), (h_s[r], c), (kq[:, r], d), (ks[:, r], e)):
+            assert torch.equal(got, want)
+
+
 def test_codes_next_to_ties_and_of_every_size():
     """Quotients at and beside every tie, and rows from 1e-45 to 3e38."""
     g = gen(3)

@@ -116,3 +116,12 @@ def test_other_entries_refuse():
     for a in ((P, 2, 8, P, 8, P, P, 8, 0, 8, 8, P, need, None), (P, 9, 8, P, 8, P, P, 8, 10, 8, 8, P, need, None), (P, 2, 7, P, 8, P, P, 8, 10, 8, 8, P, need, None),
               (P, 2, 8, P, 8, P, P, 8, 10, 8, 8, P, need - 1, None), (P, 2, 8, P, 8, P, P, 8, 10, 8, 8, P + 4, need, None), (0, 2, 8, P, 8, P, P, 8, 10, 8, 8, P, need, None)):
         assert lib.mlsx_dw_int8(*a) == kernels.MLS_ERR_ARG
+
+
+def test_grids_past_32_bits_of_threads_are_refused():
+    """Sizes whose operands no GPU here holds: an error of the entry's own before any launch."""
+    lib, P = kernels.lib(), 1 << 20
+    assert lib.mlsx_silu_mul_backward(P, 1 << 14, 0, P, 1 << 14, 1 << 38, P, 128, 1 << 31, 1 << 24, 1 << 14, P, P, 1 << 14, None) == kernels.MLS_ERR_UNSUPPORTED
+    for K, ld in ((16, 16), (131071, 131071)):  # (tiles; rows to copy first)
+        args = a8._ARGS.pack(P, P, P, P, 0, P, -1, 0, 0, 0, ld, ld, 1 << 22, 1 << 22, 1 << 22, K)
+        assert lib.mlsx_a8w8(args, P, 1 << 60, None) == kernels.MLS_ERR_UNSUPPORTED
