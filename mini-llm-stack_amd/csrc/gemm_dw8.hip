@@ -2,7 +2,9 @@
 // with a scale a token.
 //
 // 16-bit dy: the kept value q s is rounded to dy's type (off by half a step of it, as dy itself is) and the product runs on
-// the 16-bit matrix cores with fp32 sums. fp32: dy s, rounded once, becomes three bf16 parts that add up to it
+// the 16-bit matrix cores with fp32 sums. fp16: the scales may stand for values past 65504 or below 2^-14 (a product of two
+// activations is quantized from fp32), so a power of two that brings the largest scale to [2^7, 2^8) is taken out of all and put back
+// into the sums: values stay below 2^15, and those of rows with 2^-22 of the largest scale still have all 11 bits. fp32: dy s, rounded once, becomes three bf16 parts that add up to it
 // (8 significant bits each), and each meets the codes, which bf16 holds exactly: three products where two fp32
 // operands would take six. Parts of values under 2^-110 lose bits below 2^-133, bf16's smallest.
 //
@@ -35,6 +37,7 @@ struct TurnArgs {
   int64_t ldq;
   const float* s;
   int M, N, K, Mp;
+  const float* unit;  // fp16: the power of two that the scales are divided by
   void* dyt;  // [N][Mp]; fp32: bf16 [N][3][Mp]
   void* xt;   // [K][Mp]
 };
@@ -53,6 +56,23 @@ __device__ __forceinline__ void load_some(const T* src, int64_t n, float (&v)[W]
   }
 }
 
+// unit: the power of two that divides the largest finite scale to [2^7, 2^8). One block.
+__global__ __launch_bounds__(1024) void dw8_unit_kernel(const float* s, int M, float* unit) {
+  __shared__ uint32_t red[16];
+  uint32_t top = 0;
+  for (int m = threadIdx.x; m < M; m += 1024) {
+    const uint32_t b = abs_bits(s[m]);
+    top = max(top, b < 0x7F800000u ? b : 0u);
+  }
+  top = group_max_bits<64>(top);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 0; w < 16; ++w) top = max(top, red[w]);
+  // (an exponent of 1 at least: its reciprocal is a normal number too)
+  *unit = __uint_as_float((uint32_t)max((int)(top >> 23) - 7, 1) << 23);
+}
+
 // 8 tokens x W columns a lane, turned in registers, 8 x 8 lanes a wavefront: loads take 128 bytes (codes: 64) of each of 8
 // rows, stores 128 bytes of 8 of the results' rows. PARTS: of every value (the second and third of what is left).
 template <typename T, typename P, int W, int PARTS, bool CODES>
@@ -63,6 +83,11 @@ __device__ __forceinline__ void turn(const TurnArgs& p, int C, P* dst) {
   float scale[8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) scale[r] = p.s[min(m0 + r, p.M - 1)];
+  if constexpr (CODES && __is_same(T, _Float16)) {
+    const float inv = 1.0f / *p.unit;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) scale[r] *= inv;
+  }
   if ((int)(blockIdx.x + 1) * 8 * W <= C) {
     // without branches, so that all rows are on their way at once
     using Raw = std::conditional_t<CODES, int8_t, T>;
@@ -128,6 +153,7 @@ struct Dw8Args {
   void* c;  // direct: [N][ldc]; partial: fp32 [splits][N][K]
   int64_t ldc;
   int m_tiles, n_tiles, splits;
+  const float* unit;  // fp16: as the scales were divided by it
 };
 
 // G: a form of tile
@@ -144,6 +170,13 @@ __global__ __launch_bounds__(G::THREADS) void dw8_kernel(const Dw8Args p) {
     return;
   using CT = std::conditional_t<PARTIAL, float, T>;
   CT* c = (CT*)p.c + (PARTIAL ? (int64_t)sp * p.o.M * p.ldc : 0);
+  if constexpr (!PARTIAL && __is_same(T, _Float16)) {
+    const float unit = *p.unit;
+#pragma unroll
+    for (int i = 0; i < G::TN; ++i)
+#pragma unroll
+      for (int j = 0; j < G::TM; ++j) acc[i][j] *= unit;
+  }
   const bool wide = (p.ldc * sizeof(CT)) % 16 == 0 && ((uintptr_t)p.c & 15) == 0;
   const int M = p.o.M, N = p.o.N, m0 = G::row(mt * G::BM, wave, lane), n0 = G::column(nt * G::BN, wave, lane);
   if constexpr (sizeof(CT) == 2) {
@@ -184,7 +217,7 @@ __global__ __launch_bounds__(G::THREADS) void dw8_kernel(const Dw8Args p) {
 // Adds the ranges' sums in their order: 4 columns a thread; part [splits][N][ldp], ldp a multiple of 4.
 template <typename T>
 __global__ __launch_bounds__(256) void dw8_join_kernel(const float* __restrict__ part, int splits, int64_t ldp, T* __restrict__ c,
-                                                       int64_t ldc, int N, int K) {
+                                                       int64_t ldc, int N, int K, const float* __restrict__ unit) {
   const int k = (blockIdx.x * 256 + threadIdx.x) * 4, n = blockIdx.y;
   if (k >= K) return;
   const float* src = part + n * ldp + k;
@@ -193,14 +226,14 @@ __global__ __launch_bounds__(256) void dw8_join_kernel(const float* __restrict__
     const float4 q = *reinterpret_cast<const float4*>(src + i * N * ldp);
     v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
   }
-  const float o[4] = {v.x, v.y, v.z, v.w};
+  const float u = __is_same(T, _Float16) ? *unit : 1.0f, o[4] = {v.x * u, v.y * u, v.z * u, v.w * u};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (k + e < K) c[n * ldc + k + e] = from_f32<T>(o[e]);
 }
 
 struct DwPlan {
-  int64_t Mp, xt_at, part_at, ldp, bytes;
+  int64_t Mp, xt_at, unit_at, part_at, ldp, bytes;
   int form, splits;
 };
 
@@ -211,7 +244,8 @@ DwPlan make_plan(int dt, int64_t M, int64_t N, int64_t K) {
   const int parts = dt == MLS_F32 ? 3 : 1;
   p.Mp = cdiv(M, 64) * 64;
   p.xt_at = up256(N * parts * p.Mp * 2);
-  p.part_at = p.xt_at + up256(K * p.Mp * 2);
+  p.unit_at = p.xt_at + up256(K * p.Mp * 2);
+  p.part_at = p.unit_at + 256;
   p.bytes = p.part_at;
   nt_choose(N, K, parts * p.Mp * 2, p.form, p.splits);
   if (p.splits > 1) {
@@ -239,11 +273,16 @@ int launch_dw8(Dw8Args a, hipStream_t st) {
 template <typename T>
 int run(const TurnArgs& t, void* dw, int64_t lddw, const DwPlan& p, uint8_t* ws, hipStream_t st) {
   const char* fn = "mlsx_dw_int8";
+  float* unit = (float*)(ws + p.unit_at);
+  if constexpr (__is_same(T, _Float16)) {
+    hipLaunchKernelGGL(dw8_unit_kernel, dim3(1), dim3(1024), 0, st, t.s, t.M, unit);
+    if (const int rc = check_launch(fn)) return rc;
+  }
   hipLaunchKernelGGL(dw8_turn_kernel<T>, dim3((unsigned)std::max(cdiv(t.N, sizeof(T) == 4 ? 32 : 64), cdiv(t.K, 64)), (unsigned)(p.Mp / 64), 2), dim3(64), 0, st, t);
   if (const int rc = check_launch(fn)) return rc;
   const int parts = sizeof(T) == 4 ? 3 : 1, ld = (int)p.Mp * 2;
   using P = std::conditional_t<sizeof(T) == 4, __bf16, T>;
-  Dw8Args a{{ws, ws + p.xt_at, parts * ld, ld, t.N, t.K, parts * ld, parts}, dw, lddw, 0, 0, p.splits};
+  Dw8Args a{{ws, ws + p.xt_at, parts * ld, ld, t.N, t.K, parts * ld, parts}, dw, lddw, 0, 0, p.splits, unit};
   return nt_form<Op16<P>>(p.form, [&](auto form) {
     using G = typename decltype(form)::type;
     if constexpr (G::RANGES) {
@@ -252,7 +291,7 @@ int run(const TurnArgs& t, void* dw, int64_t lddw, const DwPlan& p, uint8_t* ws,
         a.ldc = p.ldp;
         if (const int rc = launch_dw8<T, G, true>(a, st)) return rc;
         hipLaunchKernelGGL(dw8_join_kernel<T>, dim3((unsigned)cdiv(t.K, 1024), (unsigned)t.N), dim3(256), 0, st,
-                           (const float*)(ws + p.part_at), p.splits, p.ldp, (T*)dw, lddw, t.N, t.K);
+                           (const float*)(ws + p.part_at), p.splits, p.ldp, (T*)dw, lddw, t.N, t.K, unit);
         return check_launch(fn);
       }
     }
@@ -285,7 +324,7 @@ extern "C" int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* 
   const DwPlan p = make_plan(dt, M, N, K);
   const hipStream_t st = (hipStream_t)stream;
   uint8_t* w = (uint8_t*)ws;
-  const TurnArgs t{dy, lddy, q, ldq, s, (int)M, (int)N, (int)K, (int)p.Mp, w, w + p.xt_at};
+  const TurnArgs t{dy, lddy, q, ldq, s, (int)M, (int)N, (int)K, (int)p.Mp, (const float*)(w + p.unit_at), w, w + p.xt_at};
   if (dt == MLS_F32) return run<float>(t, dw, lddw, p, w, st);
   if (dt == MLS_F16) return run<_Float16>(t, dw, lddw, p, w, st);
   return run<__bf16>(t, dw, lddw, p, w, st);

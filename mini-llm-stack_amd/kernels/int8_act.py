@@ -210,7 +210,8 @@ def silu_mul_backward(dh: torch.Tensor, kept: tuple[torch.Tensor, torch.Tensor])
 def int8_weight_grad(dy: torch.Tensor, x_q: torch.Tensor, sx: torch.Tensor) -> torch.Tensor:
     """dw [N, K] = dy [M, N]^T (x_q sx[:, None]) [M, K] in dy's dtype, fp32 sums: the gradient of a weight whose
     layer kept its input as quantize_rows' codes and scales. For 16-bit dy the kept values are rounded to
-    dy's dtype on the way to the matrix cores; fp32 rounds dy * sx once, to fp32. Up to 2^20 tokens."""
+    dy's dtype on the way to the matrix cores (fp16: in units of a power of two, so that sx may stand for values outside
+    its range); fp32 rounds dy * sx once, to fp32. Up to 2^20 tokens."""
     fn = "int8_weight_grad"
     dt = dt_code(dy.dtype, fn)
     dy, x_q = _two(dy, "dy", fn), _codes(x_q, "x_q", fn)

@@ -1,0 +1,93 @@
+"""int8_weight_grad and the layers that use it where kept values leave 16-bit types' ranges, against 64 bits.
+
+u = 2^-24 is half a step of fp32 relative to the value; eps / 2 half a step of a type."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from kernels import int8_act as a8
+from train.int8 import Int8SwiGLU
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+U = 2.0 ** -24
+
+
+def cuda_gen(seed):
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def some_codes(M, K, seed=0):
+    return torch.randint(-127, 128, (M, K), device="cuda", dtype=torch.int8, generator=cuda_gen(seed))
+
+
+def check_fp16_dw(dw, dy, q, s):
+    """A kept value is rounded to fp16 with the largest scale's at [2^7, 2^8): off by half a step of 2^-10 relative, or half of 2^-24 of that
+    unit where it is small. Then fp32 sums, and one rounding to fp16."""
+    unit = 2.0 ** (math.floor(math.log2(float(s.max()))) - 7)
+    d, v = dy.double().abs().t(), q.double().abs() * s.double()[:, None]
+    ref = dy.double().t() @ (q.double() * s.double()[:, None])
+    tol = d @ (v * 2.0 ** -11 + 2.0 ** -25 * unit) + (2 * len(dy) + 16) * U * (d @ v) + 2.0 ** -11 * ref.abs() + 2.0 ** -25
+    off = (dw.double() - ref).abs()
+    assert float(ref.abs().max()) < 65000  # (an fp16 result holds it)
+    assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 3, 5), (60, 40, 33), (300, 128, 200)])
+@pytest.mark.parametrize("top,size", [(1.2e5, 1e-3), (3e9, 1e-7), (6e4, 1e-3), (1.27e-6, 100.0), (3e-7, 1000.0), (6.0, 0.1)])
+def test_fp16_weight_grad_of_scales_outside_its_range(M, N, K, top, size):
+    """Kept values up to `top`: past 65504, and down to where fp16 has no bits left. Rows' scales spread over 2^6."""
+    q = some_codes(M, K)
+    s = top / 127 * torch.exp2(-6 * torch.rand(M, device="cuda", generator=cuda_gen(1)))
+    s[M // 2] = top / 127
+    dy = (size * torch.randn(M, N, device="cuda", generator=cuda_gen(2))).to(F16)
+    check_fp16_dw(a8.int8_weight_grad(dy, q, s), dy, q, s)
+
+
+def test_fp16_weight_grad_with_rows_of_zeros_and_one_far_above():
+    """Scales of 1e-8 (rows of zeros) beside ordinary ones, and one row 2^17 above the others."""
+    q, s = some_codes(100, 40), torch.full((100,), 0.05, device="cuda")
+    q[::3], s[::3] = 0, 1e-8
+    dy = (1e-2 * torch.randn(100, 30, device="cuda", generator=cuda_gen(2))).to(F16)
+    check_fp16_dw(a8.int8_weight_grad(dy, q, s), dy, q, s)
+    s[7] = 0.05 * 2 ** 17
+    dy[7] *= 1e-2
+    check_fp16_dw(a8.int8_weight_grad(dy, q, s), dy, q, s)
+    q[:], s[:] = 0, 1e-8
+    assert not bool(a8.int8_weight_grad(dy, q, s).any())
+
+
+def test_fp16_swiglu_past_its_range_trains():
+    """gate 400, up 300: the product is past 65504, the forward is finite, and so is every gradient, as in the torch form. The same codes on
+    both sides (the values are exact), so the down projection's gradient differs by its roundings alone: 2^-11 of the sum of sizes and two
+    to fp16."""
+    D, H, M = 16, 64, 40
+    torch.manual_seed(0)
+    lins = [nn.Linear(D, H, bias=False), nn.Linear(D, H, bias=False), nn.Linear(H, D, bias=False)]
+    with torch.no_grad():
+        for lin, v in zip(lins, (4.0, 3.0)):
+            lin.weight.zero_()
+            lin.weight[:, 0] = v
+            lin.weight[H // 2:, 0] = v / 64
+        lins[2].weight.mul_(1e-2)
+    x = torch.zeros(M, D)
+    x[:, 0] = 100.0
+    dy = 1e-3 * torch.randn(M, D, generator=torch.Generator().manual_seed(1))
+    out = []
+    for k in (True, False):
+        layer = Int8SwiGLU(*(m.to("cuda", F16) for m in lins), use_kernel=k)
+        xk = x.to("cuda", F16).requires_grad_()
+        y = layer(xk)
+        assert bool(torch.isfinite(y).all())
+        out.append(torch.autograd.grad(y, [xk, *layer.parameters()], dy.to("cuda", F16)))
+    assert all(bool(torch.isfinite(g).all()) for g in out[0])
+    a, b = (o[3].double() for o in out)
+    h = torch.full((M, H), 400.0 * 300.0, device="cuda", dtype=torch.float64)
+    size = dy.cuda().double().abs().t() @ h
+    assert float(b.abs().max()) > 100 and bool(((a - b).abs() <= 2.0 ** -10 * size + 2.0 ** -10 * b.abs()).all())
