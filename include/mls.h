@@ -172,9 +172,10 @@ int mls_int8_dgrad(const void* dy, int dy_dt, int64_t lddy,
  * weights on the 16-bit MFMA, fp32 accumulation; fp32 dy with M > 16: ys in fp32 as bf16
  * hi + lo parts (as mls_int8_gemm_ws), both multiplied and added in fp32. Needs a caller
  * workspace of mls_int8_dgrad_workspace(M, N, K, dy_dt) bytes, 256-byte aligned (the scaled
- * dy, the transposed weights and a vector of ones); 0 means this shape takes mls_int8_dgrad's
+ * dy, the transposed weights and a vector of row scales); 0 means this shape takes mls_int8_dgrad's
  * route (fp32 dy with M <= 16), for which workspace may be null. Runs on `stream`, three
- * launches. */
+ * launches; fp16 four: ys is rounded in units of a power of two just above the largest scale, so
+ * that small dy * s keep their bits. */
 int64_t mls_int8_dgrad_workspace(int64_t M, int64_t N, int64_t K, int dy_dt);
 int mls_int8_dgrad_ws(const void* dy, int dy_dt, int64_t lddy,
                       const int8_t* w, int64_t ldw,

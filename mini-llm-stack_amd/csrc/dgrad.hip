@@ -5,12 +5,17 @@
 // Two routes:
 //  - matrix cores (mls_int8_dgrad_ws, 16-bit dy): the reference's own arithmetic, the
 //    product (dy * s) rounded to dy's dtype (dequant_matmul.py:128) times the int8 weights
-//    (exact in bf16 / fp16) on the 16-bit MFMA with fp32 accumulation. Three launches on
+//    (exact in bf16 / fp16) on the 16-bit MFMA with fp32 accumulation. Three launches (fp16: four) on
 //    the caller's stream into a caller workspace: (1) ys = dy * s in dy's dtype, columns
 //    padded with zeros to Np = N rounded up to 64, and a vector of K ones; (2) wt = wq^T
 //    [K][Np] (mls_transpose_u8; its padding columns stay unwritten, and multiply only the
 //    zeros of ys); (3) the INT8 weight-only GEMM dx = ys wt^T with unit row scales
 //    (mls_int8_gemm), whose reduction axis is now contiguous in both operands.
+//    fp16: weights' scales are about 2^-11, so that dy * s of an ordinary gradient would lie among fp16's subnormals (dy of
+//    1e-3: error 3.4e-2 of the norm). A launch in front finds the power of two that brings the largest scale to [1/2, 1); (1) multiplies
+//    the scales by it and writes its reciprocal as the row scales, which the GEMM applies to the fp32 sums. ys is never larger than
+//    dy, and where dy * s is a normal number the results are the same bits. (The launch takes about 3 us: 256 x 2048 x 2048
+//    17.7 -> 20.2, 4096 x 11008 x 4096 348 -> 357.)
 //  - matrix cores with fp32 dy (M > 16): ys = dy * s in fp32, split into bf16 hi and lo rows
 //    (mfma16.h), the same transpose, and the split-row GEMM adding both parts in fp32.
 //  - VALU (mls_int8_dgrad, and fp32 dy with M <= 16): block tile 64 (m) x 64 (k), 256 threads, each
@@ -77,7 +82,25 @@ __global__ __launch_bounds__(256) void int8_dgrad_kernel(const T* __restrict__ d
   }
 }
 
-// ys[m][n] = T(dy[m][n] * s[n]) for n < N, 0 for N <= n < Np; ones[k] = 1 for k < K.
+// ones[0]: the power of two just above the largest finite scale, at least 2^-125, so that it and its reciprocal are normal
+// numbers. One block.
+__global__ __launch_bounds__(1024) void dgrad_unit_kernel(const void* s, int s_dt, int N, float* ones) {
+  __shared__ uint32_t red[16];
+  uint32_t top = 0;
+  for (int n = threadIdx.x; n < N; n += 1024) {
+    const uint32_t b = __float_as_uint(s_dt == MLS_F16 ? (float)((const _Float16*)s)[n] : ((const float*)s)[n]) & 0x7FFFFFFFu;
+    if (b < 0x7F800000u) top = max(top, b);
+  }
+  for (int d = 32; d; d /= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 0; w < 16; ++w) top = max(top, red[w]);
+  ones[0] = __uint_as_float((uint32_t)min(max((int)(top >> 23) + 1, 2), 252) << 23);
+}
+
+// ys[m][n] = T(dy[m][n] * s[n]) for n < N, 0 for N <= n < Np; ones[k] = 1 for k < K. fp16: s over ones[0], which
+// the others become too.
 // One thread per 8 consecutive n of a row, consecutive threads on consecutive 16-byte
 // pieces of a row (VEC: one 16-byte load of dy, 16- or 32-byte loads of the scales).
 template <typename T, bool VEC>
@@ -89,8 +112,10 @@ __global__ __launch_bounds__(256) void dgrad_scale_kernel(const T* __restrict__ 
   // ones, grid-stride), y over rows (grid-stride)
   const int64_t per_row = Np / 8;
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  constexpr bool UNIT = __is_same(T, _Float16);
+  const float unit = UNIT ? ones[0] : 1.0f;
   if (blockIdx.y == 0)
-    for (int64_t i = c; i < K; i += (int64_t)gridDim.x * 256) ones[i] = 1.0f;
+    for (int64_t i = c + (UNIT && c == 0 ? (int64_t)gridDim.x * 256 : 0); i < K; i += (int64_t)gridDim.x * 256) ones[i] = unit;
   if (c >= per_row) return;
   const int n0 = (int)c * 8;
   // this thread's 8 scales (0 past N), once for all its rows
@@ -111,6 +136,11 @@ __global__ __launch_bounds__(256) void dgrad_scale_kernel(const T* __restrict__ 
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       sv[e] = n0 + e < N ? (s_dt == MLS_F16 ? (float)((const _Float16*)s)[n0 + e] : ((const float*)s)[n0 + e]) : 0.0f;
+  }
+  if constexpr (UNIT) {
+    const float inv = 1.0f / unit;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sv[e] *= inv;
   }
   const int64_t ystep = gridDim.y;
   int64_t m = blockIdx.y;
@@ -313,6 +343,8 @@ extern "C" int mls_int8_dgrad_ws(const void* dy, int dy_dt, int64_t lddy, const 
     return check_launch("mls_int8_dgrad_ws (split GEMM)");
   }
   if (dy_dt == MLS_F16) {
+    hipLaunchKernelGGL(dgrad_unit_kernel, dim3(1), dim3(1024), 0, st, s, s_dt, (int)N, ones);
+    if (const int rc = check_launch("mls_int8_dgrad_ws (unit)")) return rc;
     auto k = vec ? dgrad_scale_kernel<_Float16, true> : dgrad_scale_kernel<_Float16, false>;
     hipLaunchKernelGGL(k, grid, dim3(256), 0, st, (const _Float16*)dy, lddy, s, s_dt, (_Float16*)ys, L.Np, ones,
                        (int)M, (int)N, (int)K);

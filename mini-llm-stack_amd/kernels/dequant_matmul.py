@@ -53,7 +53,9 @@ def int8_matmul(a: torch.Tensor, w_q: torch.Tensor, scale: torch.Tensor):
 
 
 def int8_dgrad(dy: torch.Tensor, w_q: torch.Tensor, scale: torch.Tensor):
-    """dx [M, K] = (dy ∘ scale) [M, N] @ w_q [N, K]  (kernels/dequant_matmul.py:155-167)."""
+    """dx [M, K] = (dy ∘ scale) [M, N] @ w_q [N, K]  (kernels/dequant_matmul.py:155-167). 16-bit dy: the product dy ∘ scale
+    is rounded to dy's dtype, as the reference does, fp16 in units of a power of two just above the largest scale, so that small
+    gradients keep their bits. fp32: as two bf16 parts (2^-16 of it)."""
     dev = require_hip("int8_dgrad", dy, w_q, scale)
     M, N = dy.shape
     K = w_q.shape[1]
