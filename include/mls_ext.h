@@ -167,6 +167,9 @@ int mlsx_silu_mul_backward(const void* dh, int64_t lddh, int dt, const int8_t* q
 int64_t mlsx_dw_int8_workspace(int dt, int64_t M, int64_t N, int64_t K);
 int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw,
                  int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream);
+/* The same with the fp32 sums rounded to dw's own type dw_dt. */
+int mlsx_dw_int8_to(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw, int dw_dt,
+                    int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream);
 
 /* ---------------------------------------------------------------- FP8 training */
 

@@ -150,14 +150,14 @@ __global__ __launch_bounds__(64) void dw8_turn_kernel(const TurnArgs p) {
 
 struct Dw8Args {
   NtOperands o;
-  void* c;  // direct: [N][ldc]; partial: fp32 [splits][N][K]
+  void* c;  // direct: OT [N][ldc]; partial: fp32 [splits][N][K]
   int64_t ldc;
   int m_tiles, n_tiles, splits;
   const float* unit;  // fp16: as the scales were divided by it
 };
 
-// G: a form of tile
-template <typename T, class G, bool PARTIAL>
+// P: the operands' type, OT: the gradient's, G: a form of tile
+template <typename P, typename OT, class G, bool PARTIAL>
 __global__ __launch_bounds__(G::THREADS) void dw8_kernel(const Dw8Args p) {
   extern __shared__ __align__(16) uint8_t lds[];
   int sp, mt, nt;
@@ -168,9 +168,9 @@ __global__ __launch_bounds__(G::THREADS) void dw8_kernel(const Dw8Args p) {
   if (!G::run(p.o, lds, mt * G::BM, nt * G::BN, (int)((int64_t)units * sp / p.splits), (int)((int64_t)units * (sp + 1) / p.splits), wave,
               lane, acc))
     return;
-  using CT = std::conditional_t<PARTIAL, float, T>;
+  using CT = std::conditional_t<PARTIAL, float, OT>;
   CT* c = (CT*)p.c + (PARTIAL ? (int64_t)sp * p.o.M * p.ldc : 0);
-  if constexpr (!PARTIAL && __is_same(T, _Float16)) {
+  if constexpr (!PARTIAL && __is_same(P, _Float16)) {
     const float unit = *p.unit;
 #pragma unroll
     for (int i = 0; i < G::TN; ++i)
@@ -215,8 +215,8 @@ __global__ __launch_bounds__(G::THREADS) void dw8_kernel(const Dw8Args p) {
 }
 
 // Adds the ranges' sums in their order: 4 columns a thread; part [splits][N][ldp], ldp a multiple of 4.
-template <typename T>
-__global__ __launch_bounds__(256) void dw8_join_kernel(const float* __restrict__ part, int splits, int64_t ldp, T* __restrict__ c,
+template <typename P, typename CT>
+__global__ __launch_bounds__(256) void dw8_join_kernel(const float* __restrict__ part, int splits, int64_t ldp, CT* __restrict__ c,
                                                        int64_t ldc, int N, int K, const float* __restrict__ unit) {
   const int k = (blockIdx.x * 256 + threadIdx.x) * 4, n = blockIdx.y;
   if (k >= K) return;
@@ -226,10 +226,10 @@ __global__ __launch_bounds__(256) void dw8_join_kernel(const float* __restrict__
     const float4 q = *reinterpret_cast<const float4*>(src + i * N * ldp);
     v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
   }
-  const float u = __is_same(T, _Float16) ? *unit : 1.0f, o[4] = {v.x * u, v.y * u, v.z * u, v.w * u};
+  const float u = __is_same(P, _Float16) ? *unit : 1.0f, o[4] = {v.x * u, v.y * u, v.z * u, v.w * u};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (k + e < K) c[n * ldc + k + e] = from_f32<T>(o[e]);
+    if (k + e < K) c[n * ldc + k + e] = from_f32<CT>(o[e]);
 }
 
 struct DwPlan {
@@ -255,14 +255,14 @@ DwPlan make_plan(int dt, int64_t M, int64_t N, int64_t K) {
   return p;
 }
 
-template <typename T, class G, bool PARTIAL>
+template <typename P, typename OT, class G, bool PARTIAL>
 int launch_dw8(Dw8Args a, hipStream_t st) {
   const char* fn = "mlsx_dw_int8";
   a.m_tiles = (int)cdiv(a.o.M, G::BM);
   a.n_tiles = (int)cdiv(a.o.N, G::BN);
   const int64_t blocks = (int64_t)a.m_tiles * a.n_tiles * a.splits;
   if (!grid_fits(blocks, G::THREADS)) return fail(MLS_ERR_UNSUPPORTED, "%s: %d x %d", fn, a.o.M, a.o.N);
-  auto kern = dw8_kernel<T, G, PARTIAL>;
+  auto kern = dw8_kernel<P, OT, G, PARTIAL>;
   // (a call a launch: the limit is the function's on the current device)
   if (hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS) != hipSuccess)
     return fail(MLS_ERR_HIP, "%s: cannot reserve %d bytes of LDS", fn, G::LDS);
@@ -270,8 +270,29 @@ int launch_dw8(Dw8Args a, hipStream_t st) {
   return check_launch(fn);
 }
 
+// The product of turned operands.
+template <typename P, typename OT>
+int run_product(Dw8Args a, int64_t ldp, int form, void* part, hipStream_t st) {
+  return nt_form<Op16<P>>(form, [&](auto f) {
+    using G = typename decltype(f)::type;
+    if constexpr (G::RANGES) {
+      if (a.splits > 1) {
+        Dw8Args b = a;
+        b.c = part;
+        b.ldc = ldp;
+        if (const int rc = launch_dw8<P, OT, G, true>(b, st)) return rc;
+        hipLaunchKernelGGL((dw8_join_kernel<P, OT>), dim3((unsigned)cdiv(a.o.N, 1024), (unsigned)a.o.M), dim3(256), 0, st, (const float*)part,
+                           a.splits, ldp, (OT*)a.c, a.ldc, a.o.M, a.o.N, a.unit);
+        return check_launch("mlsx_dw_int8");
+      }
+    }
+    return launch_dw8<P, OT, G, false>(a, st);
+  });
+}
+
+// T: dy's type
 template <typename T>
-int run(const TurnArgs& t, void* dw, int64_t lddw, const DwPlan& p, uint8_t* ws, hipStream_t st) {
+int run(const TurnArgs& t, void* dw, int dw_dt, int64_t lddw, const DwPlan& p, uint8_t* ws, hipStream_t st) {
   const char* fn = "mlsx_dw_int8";
   float* unit = (float*)(ws + p.unit_at);
   if constexpr (__is_same(T, _Float16)) {
@@ -282,21 +303,11 @@ int run(const TurnArgs& t, void* dw, int64_t lddw, const DwPlan& p, uint8_t* ws,
   if (const int rc = check_launch(fn)) return rc;
   const int parts = sizeof(T) == 4 ? 3 : 1, ld = (int)p.Mp * 2;
   using P = std::conditional_t<sizeof(T) == 4, __bf16, T>;
-  Dw8Args a{{ws, ws + p.xt_at, parts * ld, ld, t.N, t.K, parts * ld, parts}, dw, lddw, 0, 0, p.splits, unit};
-  return nt_form<Op16<P>>(p.form, [&](auto form) {
-    using G = typename decltype(form)::type;
-    if constexpr (G::RANGES) {
-      if (p.splits > 1) {
-        a.c = ws + p.part_at;
-        a.ldc = p.ldp;
-        if (const int rc = launch_dw8<T, G, true>(a, st)) return rc;
-        hipLaunchKernelGGL(dw8_join_kernel<T>, dim3((unsigned)cdiv(t.K, 1024), (unsigned)t.N), dim3(256), 0, st,
-                           (const float*)(ws + p.part_at), p.splits, p.ldp, (T*)dw, lddw, t.N, t.K, unit);
-        return check_launch(fn);
-      }
-    }
-    return launch_dw8<T, G, false>(a, st);
-  });
+  const Dw8Args a{{ws, ws + p.xt_at, parts * ld, ld, t.N, t.K, parts * ld, parts}, dw, lddw, 0, 0, p.splits, unit};
+  void* part = ws + p.part_at;
+  if (dw_dt == MLS_F32) return run_product<P, float>(a, p.ldp, p.form, part, st);
+  if (dw_dt == MLS_F16) return run_product<P, _Float16>(a, p.ldp, p.form, part, st);
+  return run_product<P, __bf16>(a, p.ldp, p.form, part, st);
 }
 
 }  // namespace
@@ -310,11 +321,11 @@ extern "C" int64_t mlsx_dw_int8_workspace(int dt, int64_t M, int64_t N, int64_t 
   return make_plan(dt, M, N, K).bytes;
 }
 
-extern "C" int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw,
-                            int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream) {
+extern "C" int mlsx_dw_int8_to(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw, int dw_dt,
+                               int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream) {
   const char* fn = "mlsx_dw_int8";
   if (M < 1 || N < 0 || K < 0) return fail(MLS_ERR_ARG, "%s: bad size", fn);
-  if (!is_float_dt(dt)) return fail(MLS_ERR_ARG, "%s: bad dtype %d", fn, dt);
+  if (!is_float_dt(dt) || !is_float_dt(dw_dt)) return fail(MLS_ERR_ARG, "%s: bad dtype %d, %d", fn, dt, dw_dt);
   if (N == 0 || K == 0) return MLS_OK;
   const int64_t need = mlsx_dw_int8_workspace(dt, M, N, K);
   if (need == 0) return fail(MLS_ERR_UNSUPPORTED, "%s: M=%lld N=%lld K=%lld", fn, (long long)M, (long long)N, (long long)K);
@@ -325,7 +336,12 @@ extern "C" int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* 
   const hipStream_t st = (hipStream_t)stream;
   uint8_t* w = (uint8_t*)ws;
   const TurnArgs t{dy, lddy, q, ldq, s, (int)M, (int)N, (int)K, (int)p.Mp, (const float*)(w + p.unit_at), w, w + p.xt_at};
-  if (dt == MLS_F32) return run<float>(t, dw, lddw, p, w, st);
-  if (dt == MLS_F16) return run<_Float16>(t, dw, lddw, p, w, st);
-  return run<__bf16>(t, dw, lddw, p, w, st);
+  if (dt == MLS_F32) return run<float>(t, dw, dw_dt, lddw, p, w, st);
+  if (dt == MLS_F16) return run<_Float16>(t, dw, dw_dt, lddw, p, w, st);
+  return run<__bf16>(t, dw, dw_dt, lddw, p, w, st);
+}
+
+extern "C" int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw,
+                            int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream) {
+  return mlsx_dw_int8_to(dy, dt, lddy, q, ldq, s, dw, dt, lddw, M, N, K, ws, ws_bytes, stream);
 }

@@ -124,6 +124,7 @@ EXT_SIGNATURES = {
     "mlsx_silu_mul_backward": ([_P, _I64, _I, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P], _I),
     "mlsx_dw_int8_workspace": ([_I, _I64, _I64, _I64], _I64),
     "mlsx_dw_int8": ([_P, _I, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
+    "mlsx_dw_int8_to": ([_P, _I, _I64, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
     "mlsx_fp8_encode_pad": ([_I, _P, _I, _I64, _I64, _I64, _F, _P, _I64, _P, _P, _P], _I),
     "mlsx_absmax_parts": ([_P, _I, _I64, _P, _P], _I),
     "mlsx_absmax_scales": ([_P, _I, _F, _P, _P, _P], _I),

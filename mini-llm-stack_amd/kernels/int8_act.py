@@ -207,13 +207,15 @@ def silu_mul_backward(dh: torch.Tensor, kept: tuple[torch.Tensor, torch.Tensor])
     return dgate, dup
 
 
-def int8_weight_grad(dy: torch.Tensor, x_q: torch.Tensor, sx: torch.Tensor) -> torch.Tensor:
-    """dw [N, K] = dy [M, N]^T (x_q sx[:, None]) [M, K] in dy's dtype, fp32 sums: the gradient of a weight whose
+def int8_weight_grad(dy: torch.Tensor, x_q: torch.Tensor, sx: torch.Tensor, *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """dw [N, K] = dy [M, N]^T (x_q sx[:, None]) [M, K], fp32 sums rounded to out_dtype (None: dy's dtype): the gradient of a weight whose
     layer kept its input as quantize_rows' codes and scales. For 16-bit dy the kept values are rounded to
     dy's dtype on the way to the matrix cores (fp16: in units of a power of two, so that sx may stand for values outside
     its range); fp32 rounds dy * sx once, to fp32. Up to 2^20 tokens."""
     fn = "int8_weight_grad"
     dt = dt_code(dy.dtype, fn)
+    out_dtype = dy.dtype if out_dtype is None else out_dtype
+    out_dt = dt_code(out_dtype, fn)
     dy, x_q = _two(dy, "dy", fn), _codes(x_q, "x_q", fn)
     (M, N), K = dy.shape, x_q.shape[1]
     if x_q.shape[0] != M:
@@ -223,7 +225,7 @@ def int8_weight_grad(dy: torch.Tensor, x_q: torch.Tensor, sx: torch.Tensor) -> t
         sx = sx.to(torch.float32)
     _no_grad(fn, dy, sx)
     dev = one_device(fn, dy, x_q, sx)
-    dw = torch.empty(N, K, dtype=dy.dtype, device=dy.device)
+    dw = torch.empty(N, K, dtype=out_dtype, device=dy.device)
     if M == 0:
         return dw.zero_()
     if N == 0 or K == 0:
@@ -231,6 +233,6 @@ def int8_weight_grad(dy: torch.Tensor, x_q: torch.Tensor, sx: torch.Tensor) -> t
     lib = kernels.lib()
     need = lib.mlsx_dw_int8_workspace(dt, M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
-    kernels.check(_on(dev, lib.mlsx_dw_int8, dy.data_ptr(), dt, max(dy.stride(0), N), x_q.data_ptr(), max(x_q.stride(0), K),
-                      sx.data_ptr(), dw.data_ptr(), K, M, N, K, ws.data_ptr(), need, _raw_stream(dev)), fn)
+    kernels.check(_on(dev, lib.mlsx_dw_int8_to, dy.data_ptr(), dt, max(dy.stride(0), N), x_q.data_ptr(), max(x_q.stride(0), K),
+                      sx.data_ptr(), dw.data_ptr(), out_dt, K, M, N, K, ws.data_ptr(), need, _raw_stream(dev)), fn)
     return dw

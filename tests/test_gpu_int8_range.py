@@ -11,7 +11,7 @@ import torch
 import torch.nn as nn
 
 from kernels import int8_act as a8
-from train.int8 import Int8SwiGLU
+from train.int8 import Int8Linear, Int8SwiGLU
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,34 @@ def test_fp16_swiglu_past_its_range_trains():
     h = torch.full((M, H), 400.0 * 300.0, device="cuda", dtype=torch.float64)
     size = dy.cuda().double().abs().t() @ h
     assert float(b.abs().max()) > 100 and bool(((a - b).abs() <= 2.0 ** -10 * size + 2.0 ** -10 * b.abs()).all())
+
+
+# ---------------------------------------------------------------- parameters of another type than the activations
+
+@pytest.mark.parametrize("act,param", [(BF16, F32), (F16, F32), (F32, BF16), (F32, F16), (BF16, F16), (F16, BF16)])
+@pytest.mark.parametrize("M,N,K", [(1, 33, 64), (300, 130, 65), (2000, 64, 48)])
+def test_gradients_in_the_parameters_type(M, N, K, act, param):
+    """fp32 sums rounded once, to the parameter's type; 16-bit dy meets the kept values rounded to its type, which is
+    the reference here."""
+    torch.manual_seed(0)
+    layer = Int8Linear(nn.Linear(K, N).to("cuda", param))
+    x = torch.randn(M, K, device="cuda", generator=cuda_gen(1)).to(act)
+    dy = (0.1 * torch.randn(M, N, device="cuda", generator=cuda_gen(2))).to(act)
+    dw, db = torch.autograd.grad(layer(x), [layer.weight, layer.bias], dy)
+    assert dw.dtype == db.dtype == param
+    q, s = a8.quantize_rows(x)
+    v = (q.float() * s[:, None]).to(act).double()
+    half, low = torch.finfo(param).eps / 2, {F32: 2.0 ** -149, F16: 2.0 ** -25, BF16: 2.0 ** -133}[param]
+    for got, ref, size in ((dw, dy.double().t() @ v, dy.double().abs().t() @ v.abs()), (db, dy.double().sum(0), dy.double().abs().sum(0))):
+        tol = (3 * M + 16) * U * size + half * (ref.abs() + (3 * M + 16) * U * size) + low
+        off = (got.double() - ref).abs()
+        assert bool((off <= tol).all()), float((off / tol).max())
+
+
+def test_fp16_sums_past_its_range_reach_fp32_parameters():
+    layer = Int8Linear(nn.Linear(16, 8).cuda())
+    x, dy = torch.ones(2000, 16, device="cuda", dtype=F16), torch.full((2000, 8), 100.0, device="cuda", dtype=F16)
+    dw, db = torch.autograd.grad(layer(x), [layer.weight, layer.bias], dy)
+    assert torch.equal(db, torch.full_like(db, 2e5))
+    # (one row's scale is 1 / 127 in fp32, its value 127 times that, rounded to fp16: within 2^-10 of 1)
+    assert bool(((dw - 2e5).abs() <= 2e5 * 2.0 ** -10).all())
