@@ -394,12 +394,13 @@ def _set_submodule(model: nn.Module, name: str, mod: nn.Module) -> None:
 
 def load_quantized(model: nn.Module, path, device=None, use_kernel: bool = True) -> nn.Module:
     """Load a quantized checkpoint into `model` (the fp architecture, e.g. a freshly
-    built Transformer; it is modified in place and returned): every module the header
+    built Transformer, or one converted by train.int8; it is modified in place and returned): every module the header
     lists becomes a QuantLinear holding the stored buffers, then the remaining
     parameters load as a state dict (strict: missing or unexpected keys raise). With
     `device`, tensors are read straight onto it. MoE experts are stacked for the
     grouped kernels as quantize_model does."""
     from safetensors.torch import load_file
+    from train.int8 import Int8Linear  # (which imports this module)
     meta = read_quantized_metadata(path)
     dev = torch.device(device) if device is not None else None
     tensors = load_file(str(path), device=str(dev) if dev is not None else "cpu")
@@ -409,7 +410,7 @@ def load_quantized(model: nn.Module, path, device=None, use_kernel: bool = True)
         name = key[2:]
         bits, group, in_features = (int(x) for x in spec.split(","))
         old = model.get_submodule(name)
-        if not isinstance(old, (nn.Linear, QuantLinear)):
+        if not isinstance(old, (nn.Linear, QuantLinear, Int8Linear)):
             raise ValueError(f"load_quantized: {name} is a {type(old).__name__}, not a linear layer")
         w_q, scale = tensors.pop(f"{name}.w_q"), tensors.pop(f"{name}.scale")
         out_features = old.out_features

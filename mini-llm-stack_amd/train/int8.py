@@ -153,6 +153,14 @@ class Int8Linear(nn.Module):
         self.weight, self.bias = copy(linear.weight), copy(linear.bias)
         self.use_kernel = use_kernel
 
+    @property
+    def out_features(self) -> int:
+        return self.weight.shape[0]
+
+    @property
+    def in_features(self) -> int:
+        return self.weight.shape[1]
+
     def forward(self, x):
         y = _Int8LinearFn.apply(x.reshape(-1, x.shape[-1]), self.weight, self.bias, self.use_kernel)
         return y.reshape(*x.shape[:-1], self.weight.shape[0])
@@ -160,7 +168,8 @@ class Int8Linear(nn.Module):
 
 class Int8SwiGLU(nn.Module):
     """w_down(silu(w_gate(x)) * w_up(x)) for training with INT8 products and 8-bit activations, under the
-    parameter names of the reference's SwiGLU (train/model.py:127-135). No biases."""
+    parameter names of the reference's SwiGLU (train/model.py:127-135). No biases. With other layers put in their places
+    (serve.quantize.quantize_model's) it runs those one after another."""
 
     def __init__(self, w_gate: nn.Linear, w_up: nn.Linear, w_down: nn.Linear, use_kernel: bool = True):
         super().__init__()
@@ -170,6 +179,8 @@ class Int8SwiGLU(nn.Module):
         self.use_kernel = use_kernel
 
     def forward(self, x):
+        if not all(isinstance(m, Int8Linear) for m in (self.w_gate, self.w_up, self.w_down)):
+            return self.w_down(nn.functional.silu(self.w_gate(x)) * self.w_up(x))
         y = _Int8SwiGLUFn.apply(x.reshape(-1, x.shape[-1]), self.w_gate.weight, self.w_up.weight, self.w_down.weight,
                                 self.use_kernel, torch.is_grad_enabled())
         return y.reshape(*x.shape[:-1], self.w_down.weight.shape[0])
