@@ -182,10 +182,16 @@ class QuantLinear(nn.Module):
         return ((x_q.double() @ self.w_q.double().t()) * self.scale.double() * sx.double()[:, None]).to(out_dtype)
 
 
+def has_hooks(*modules: nn.Module) -> bool:
+    """Whether calling one of these runs more than its forward."""
+    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+
+
 class Int8SwiGLU(nn.Module):
     """w_down(silu(w_gate(x)) * w_up(x)) of three QuantLinear(act_bits=8), under the names that the
     reference's SwiGLU gives them (train/model.py:127-135): x is quantized once for gate and up, and the product
-    once more, in fp32, on its way to w_down."""
+    once more, in fp32, on its way to w_down. The three are not called themselves, unless one has hooks: then each is, and the
+    product is rounded to x's dtype in between."""
 
     def __init__(self, w_gate: QuantLinear, w_up: QuantLinear, w_down: QuantLinear):
         super().__init__()
@@ -195,16 +201,19 @@ class Int8SwiGLU(nn.Module):
         self.w_gate, self.w_up, self.w_down = w_gate, w_up, w_down
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if has_hooks(self.w_gate, self.w_up, self.w_down):
+            g, u = self.w_gate(x).float(), self.w_up(x).float()
+            return self.w_down((g * torch.sigmoid(g) * u).to(x.dtype))
         flat = x.reshape(-1, x.shape[-1])
         if not self.w_gate.use_kernel:
             xq = quantize_int8(flat.float())
             g, u = (m.matmul_codes(*xq, flat.dtype).float() for m in (self.w_gate, self.w_up))
             h = quantize_int8(g * torch.sigmoid(g) * u)
         else:
-            from kernels.int8_act import quantize_rows, silu_mul_quantize
+            from kernels.int8_act import int8_dynamic_matmul, quantize_rows, silu_mul_quantize
             # (up to 16 rows the product quantizes them itself: one launch less)
             if flat.shape[0] <= 16:
-                g, u = self.w_gate(flat), self.w_up(flat)
+                g, u = (int8_dynamic_matmul(flat, m.w_q, m.scale) for m in (self.w_gate, self.w_up))
             else:
                 xq = quantize_rows(flat)
                 g, u = (m.matmul_codes(*xq, flat.dtype) for m in (self.w_gate, self.w_up))

@@ -22,7 +22,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from serve.quantize import quantize_int8
+from serve.quantize import has_hooks, quantize_int8
 
 _GROUP = 128
 
@@ -169,7 +169,7 @@ class Int8Linear(nn.Module):
 class Int8SwiGLU(nn.Module):
     """w_down(silu(w_gate(x)) * w_up(x)) for training with INT8 products and 8-bit activations, under the
     parameter names of the reference's SwiGLU (train/model.py:127-135). No biases. With other layers put in their places
-    (serve.quantize.quantize_model's) it runs those one after another."""
+    (serve.quantize.quantize_model's), or hooks on one of its own, it calls the three one after another."""
 
     def __init__(self, w_gate: nn.Linear, w_up: nn.Linear, w_down: nn.Linear, use_kernel: bool = True):
         super().__init__()
@@ -179,7 +179,8 @@ class Int8SwiGLU(nn.Module):
         self.use_kernel = use_kernel
 
     def forward(self, x):
-        if not all(isinstance(m, Int8Linear) for m in (self.w_gate, self.w_up, self.w_down)):
+        lins = self.w_gate, self.w_up, self.w_down
+        if not all(isinstance(m, Int8Linear) for m in lins) or has_hooks(*lins):
             return self.w_down(nn.functional.silu(self.w_gate(x)) * self.w_up(x))
         y = _Int8SwiGLUFn.apply(x.reshape(-1, x.shape[-1]), self.w_gate.weight, self.w_up.weight, self.w_down.weight,
                                 self.use_kernel, torch.is_grad_enabled())

@@ -46,3 +46,42 @@ def test_other_modules_in_a_listed_place_are_refused(tmp_path):
     c = convert_linears_to_int8(_Model(d=32), use_kernel=False)
     with pytest.raises(ValueError, match="stores"):
         load_quantized(c, tmp_path / "q.safetensors", use_kernel=False)
+
+
+# ---------------------------------------------------------------- hooks
+
+def hook_all(mlp, calls):
+    def hook(name):
+        return lambda m, args, out: calls.append((name, args[0].shape[0], out.shape[-1]))
+    return [getattr(mlp, n).register_forward_hook(hook(n)) for n in ("w_gate", "w_up", "w_down")]
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17])
+def test_hooks_on_projections_fire(rows):
+    torch.manual_seed(0)
+    m = _Model()
+    mlp = m.blocks[0].mlp
+    D, H = mlp.w_gate.in_features, mlp.w_gate.out_features
+    x = torch.randn(rows, D)
+    for e in (quantize_model(m, use_kernel=False, act_bits=8).blocks[0].mlp, convert_linears_to_int8(m, use_kernel=False).blocks[0].mlp):
+        fused, calls = e(x), []
+        handles = hook_all(e, calls)
+        y = e(x)
+        assert calls == [("w_gate", rows, H), ("w_up", rows, H), ("w_down", rows, D)]
+        # (a code may be another where the product is rounded in between: 1 / 127 of the largest, once a weight's size)
+        assert float((y - fused).detach().abs().max()) <= 0.02 * float(fused.detach().abs().max())
+        for h in handles:
+            h.remove()
+        assert torch.equal(e(x), fused) and len(calls) == 3
+
+
+def test_gradients_pass_hooked_projections():
+    torch.manual_seed(0)
+    e = convert_linears_to_int8(_Model(), use_kernel=False).blocks[0].mlp
+    x, seen = torch.randn(9, e.w_gate.in_features, requires_grad=True), []
+    want = torch.autograd.grad(e(x).sum(), [x, *e.parameters()])
+    e.w_up.register_full_backward_hook(lambda m, gi, go: seen.append(go[0].shape))
+    got = torch.autograd.grad(e(x).sum(), [x, *e.parameters()])
+    assert seen == [(9, e.w_up.out_features)]
+    # (here silu's own derivative meets gate and up in full width, there 8 bits of each group of 128)
+    assert all(float((a - b).norm()) <= 0.05 * float(b.norm()) for a, b in zip(got, want))
