@@ -18,7 +18,7 @@ use_kernel=False keeps the reference's dequantize-then-matmul path.
 
 act_bits=8 (no reference counterpart): the input is quantized too, per token as it comes, and INT8 weights meet it
 on the 8-bit matrix cores (kernels.int8_act), at about twice the 16-bit rate for prompts. quantize_model(act_bits=8) also makes
-every SwiGLU an Int8SwiGLU, whose product with the down projection's codes is one kernel. Such layers serve: they have
+every SwiGLU (computes_swiglu) an Int8SwiGLU, whose product with the down projection's codes is one kernel. Such layers serve: they have
 no gradient and refuse inputs that ask for one.
 
 Unlike the reference, this module does not import the model package (the
@@ -225,11 +225,37 @@ _ATTN_SLOTS = ("wq", "wk", "wv", "wo")
 _MLP_SLOTS = ("w_gate", "w_up", "w_down")
 
 
+def computes_swiglu(m: nn.Module) -> bool:
+    """Whether a module with a SwiGLU's slots computes w_down(silu(w_gate(x)) * w_up(x)) and nothing else, so that one that does may take
+    its place. It is asked, not its name: its forward runs in both modes on small numbers in 64 bits, with layers of the probe's in the slots.
+    A module with state of its own or hooks is not replaced, one without a forward says nothing against it."""
+    import copy
+    others = [c for n, c in m.named_children() if n not in _MLP_SLOTS]
+    if has_hooks(m) or m._parameters or m._buffers or any(c.state_dict() for c in others):
+        return False
+    if type(m).forward is nn.Module.forward and "forward" not in m.__dict__:
+        return True
+    D, H, kw = 8, 64, dict(dtype=torch.float64, device="cpu")
+    g = torch.Generator("cpu").manual_seed(0)
+    with torch.no_grad(), torch.random.fork_rng(devices=[]):
+        slots = {n: nn.Linear(a, b, bias=False, **kw) for n, a, b in zip(_MLP_SLOTS, (D, D, H), (H, H, D))}
+        for lin in slots.values():
+            lin.weight.copy_(torch.randn(lin.weight.shape, generator=g, **kw))
+        x = 2 * torch.randn(64, D, generator=g, **kw)
+        want = slots["w_down"](nn.functional.silu(slots["w_gate"](x)) * slots["w_up"](x))
+        probe = copy.copy(m)
+        probe._modules = {n: slots[n] if n in slots else copy.deepcopy(c) for n, c in m._modules.items()}
+        try:
+            return all(torch.allclose(probe.train(mode)(x), want, rtol=1e-9, atol=1e-9) for mode in (True, False))
+        except Exception:  # (another shape, type or argument: not this function)
+            return False
+
+
 def _fuse_int8_mlps(model: nn.Module) -> None:
     """Every SwiGLU of the blocks whose three projections have act_bits=8 becomes an Int8SwiGLU."""
     def fused(m):
         lins = [getattr(m, n, None) for n in _MLP_SLOTS]
-        ok = not isinstance(m, Int8SwiGLU) and all(isinstance(q, QuantLinear) and q.act_bits == 8 for q in lins)
+        ok = not isinstance(m, Int8SwiGLU) and all(isinstance(q, QuantLinear) and q.act_bits == 8 for q in lins) and computes_swiglu(m)
         return Int8SwiGLU(*lins).train(m.training) if ok else m
     for blk in getattr(model, "blocks", []):
         if getattr(blk, "is_moe", False):
@@ -245,7 +271,7 @@ def quantize_model(model: nn.Module, bits: int = 8, group_size: int = 32,
     (serve/quantize.py:98-115). Walks model.blocks; each block's .attn holds
     wq/wk/wv/wo and its .mlp holds w_gate/w_up/w_down, or, when blk.is_moe,
     .mlp.experts is a list of such MLPs. act_bits=8 (with bits=8): their inputs are
-    quantized per token too, and the MLPs become Int8SwiGLU."""
+    quantized per token too, and the MLPs that compute a SwiGLU become Int8SwiGLU."""
     import copy
     _act_bits(act_bits, bits)
     model = copy.deepcopy(model)

@@ -22,7 +22,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
-from serve.quantize import has_hooks, quantize_int8
+from serve.quantize import computes_swiglu, has_hooks, quantize_int8
 
 _GROUP = 128
 
@@ -190,9 +190,20 @@ class Int8SwiGLU(nn.Module):
 def convert_linears_to_int8(model: nn.Module, use_kernel: bool = True) -> nn.Module:
     """A copy of the model whose attention projections (wq/wk/wv/wo) are Int8Linear and whose SwiGLU MLPs (modules with
     w_gate/w_up/w_down) are Int8SwiGLU; embeddings, head, router and norms stay as they are. Modules are recognised by their slot names, as
-    train.fp8.convert_linears_to_fp8 does; the state dict keeps its names."""
+    train.fp8.convert_linears_to_fp8 does, and an MLP that computes something else (serve.quantize.computes_swiglu) keeps its forward, over
+    three Int8Linear. The state dict keeps its names."""
     import copy
     model = copy.deepcopy(model)
+
+    def fused(m):
+        lins = slots(m, ("w_gate", "w_up", "w_down"))
+        if not linears(lins):
+            return m
+        if computes_swiglu(m):
+            return Int8SwiGLU(*lins, use_kernel=use_kernel).train(m.training)
+        for n, lin in zip(("w_gate", "w_up", "w_down"), lins):
+            setattr(m, n, Int8Linear(lin, use_kernel))
+        return m
     slots = lambda m, names: [getattr(m, n, None) for n in names]
     linears = lambda ms: all(isinstance(m, nn.Linear) for m in ms)
     for m in list(model.modules()):
@@ -201,8 +212,7 @@ def convert_linears_to_int8(model: nn.Module, use_kernel: bool = True) -> nn.Mod
             for n, lin in zip(("wq", "wk", "wv", "wo"), attn):
                 setattr(m, n, Int8Linear(lin, use_kernel))
         for name, child in list(m.named_children()):
-            mlp = slots(child, ("w_gate", "w_up", "w_down"))
-            if linears(mlp):
-                setattr(m, name, Int8SwiGLU(*mlp, use_kernel=use_kernel).train(child.training))
-    mlp = slots(model, ("w_gate", "w_up", "w_down"))
-    return Int8SwiGLU(*mlp, use_kernel=use_kernel).train(model.training) if linears(mlp) else model
+            new = fused(child)
+            if new is not child:
+                setattr(m, name, new)
+    return fused(model)

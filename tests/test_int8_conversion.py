@@ -85,3 +85,118 @@ def test_gradients_pass_hooked_projections():
     assert seen == [(9, e.w_up.out_features)]
     # (here silu's own derivative meets gate and up in full width, there 8 bits of each group of 128)
     assert all(float((a - b).norm()) <= 0.05 * float(b.norm()) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------- modules with a SwiGLU's names that compute something else
+
+class _Gated(nn.Module):
+    def __init__(self, d=24, h=40, act=F.silu, drop=0.0):
+        super().__init__()
+        self.w_gate, self.w_up, self.w_down = nn.Linear(d, h, bias=False), nn.Linear(d, h, bias=False), nn.Linear(h, d, bias=False)
+        self.act, self.drop = act, drop
+
+    def forward(self, x):
+        return self.w_down(F.dropout(self.act(self.w_gate(x)) * self.w_up(x), self.drop, self.training))
+
+
+class _Swapped(_Gated):
+    def forward(self, x):
+        return self.w_down(F.silu(self.w_up(x)) * self.w_gate(x))
+
+
+class _Scaled(_Gated):
+    def __init__(self):
+        super().__init__()
+        self.scale = nn.Parameter(torch.full((), 2.0))
+
+    def forward(self, x):
+        return super().forward(x) * self.scale
+
+
+class _Clipped(_Gated):
+    def forward(self, x):
+        return super().forward(x.clamp(-1, 1))
+
+
+class _Rows(_Gated):
+    """Its own way of writing it, with a module for the activation and rows flattened."""
+
+    def __init__(self):
+        super().__init__()
+        self.fn = nn.SiLU()
+
+    def forward(self, x):
+        f = x.reshape(-1, x.shape[-1])
+        up = self.w_up(f)
+        return self.w_down(up * self.fn(self.w_gate(f))).reshape(x.shape)
+
+
+class _Hook(_Gated):
+    def __init__(self):
+        super().__init__()
+        self.register_forward_hook(lambda m, a, out: 3 * out)
+
+
+class _Shell(nn.Module):
+    def __init__(self, mlp):
+        super().__init__()
+        self.mlp = mlp
+
+    def forward(self, x):
+        return self.mlp(x)
+
+
+class _Attn(nn.Module):
+    def __init__(self, d):
+        super().__init__()
+        self.wq, self.wk, self.wv, self.wo = (nn.Linear(d, d, bias=False) for _ in range(4))
+
+
+class _Blocks(nn.Module):
+    def __init__(self, mlp):
+        super().__init__()
+        self.blocks = nn.ModuleList([_Shell(mlp)])
+        self.blocks[0].attn = _Attn(24)
+
+
+OTHERS = [lambda: _Gated(act=F.gelu), lambda: _Gated(act=torch.sigmoid), lambda: _Gated(drop=0.1), _Swapped, _Scaled, _Clipped, _Hook]
+
+
+@pytest.mark.parametrize("make", OTHERS)
+def test_conversion_keeps_what_other_mlps_compute(make):
+    """Their linears are swapped, their forward is their own: the 8-bit operands are all that differs (a SwiGLU in their place is off by
+    a tenth of the outputs and more)."""
+    torch.manual_seed(0)
+    m = _Blocks(make())
+    x = 3 * torch.randn(50, 24)
+    for c in (convert_linears_to_int8(m, use_kernel=False), quantize_model(m, use_kernel=False, act_bits=8)):
+        mlp = c.blocks[0].mlp
+        assert type(mlp) is type(m.blocks[0].mlp) and not isinstance(mlp.w_up, nn.Linear)
+        torch.manual_seed(1)  # (dropout's)
+        want = m.train().blocks[0](x)
+        torch.manual_seed(1)
+        got = c.train().blocks[0](x)
+        assert float((got - want).detach().norm()) <= 0.03 * float(want.detach().norm())
+    assert type(convert_linears_to_int8(make(), use_kernel=False)) is type(make())
+
+
+def test_a_swiglu_by_another_name_is_fused(tmp_path):
+    torch.manual_seed(0)
+    state = torch.get_rng_state()
+    for make in (_Rows, _Gated):
+        m = _Blocks(make()).eval()
+        state = torch.get_rng_state()
+        c, q = convert_linears_to_int8(m, use_kernel=False), quantize_model(m, use_kernel=False, act_bits=8)
+        assert torch.equal(torch.get_rng_state(), state)  # (nothing drawn from the program's own generator)
+        assert type(c.blocks[0].mlp).__name__ == type(q.blocks[0].mlp).__name__ == "Int8SwiGLU"
+        assert not m.blocks[0].mlp.training and not c.blocks[0].mlp.training
+
+
+def test_a_checkpoint_of_another_mlp_loads_as_it_was(tmp_path):
+    torch.manual_seed(0)
+    m = _Blocks(_Gated(act=F.gelu))
+    q = quantize_model(m, use_kernel=False, act_bits=8)
+    save_quantized(q, tmp_path / "q.safetensors")
+    back = load_quantized(_Blocks(_Gated(act=F.gelu)), tmp_path / "q.safetensors", use_kernel=False)
+    x = torch.randn(7, 24)
+    assert type(back.blocks[0].mlp) is _Gated and torch.equal(back.blocks[0](x), q.blocks[0](x))
