@@ -190,8 +190,8 @@ class Int8SwiGLU(nn.Module):
 def convert_linears_to_int8(model: nn.Module, use_kernel: bool = True) -> nn.Module:
     """A copy of the model whose attention projections (wq/wk/wv/wo) are Int8Linear and whose SwiGLU MLPs (modules with
     w_gate/w_up/w_down) are Int8SwiGLU; embeddings, head, router and norms stay as they are. Modules are recognised by their slot names, as
-    train.fp8.convert_linears_to_fp8 does, and an MLP that computes something else (serve.quantize.computes_swiglu) keeps its forward, over
-    three Int8Linear. The state dict keeps its names."""
+    train.fp8.convert_linears_to_fp8 does, and an MLP with biases or that computes something else (serve.quantize.computes_swiglu) keeps its forward,
+    over three Int8Linear. The state dict keeps its names."""
     import copy
     model = copy.deepcopy(model)
 
@@ -199,7 +199,7 @@ def convert_linears_to_int8(model: nn.Module, use_kernel: bool = True) -> nn.Mod
         lins = slots(m, ("w_gate", "w_up", "w_down"))
         if not linears(lins):
             return m
-        if computes_swiglu(m):
+        if all(lin.bias is None for lin in lins) and computes_swiglu(m):
             return Int8SwiGLU(*lins, use_kernel=use_kernel).train(m.training)
         for n, lin in zip(("w_gate", "w_up", "w_down"), lins):
             setattr(m, n, Int8Linear(lin, use_kernel))

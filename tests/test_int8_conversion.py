@@ -200,3 +200,22 @@ def test_a_checkpoint_of_another_mlp_loads_as_it_was(tmp_path):
     back = load_quantized(_Blocks(_Gated(act=F.gelu)), tmp_path / "q.safetensors", use_kernel=False)
     x = torch.randn(7, 24)
     assert type(back.blocks[0].mlp) is _Gated and torch.equal(back.blocks[0](x), q.blocks[0](x))
+
+
+# ---------------------------------------------------------------- biases and ties
+
+class _Biased(_Gated):
+    def __init__(self):
+        super().__init__()
+        self.w_gate, self.w_up, self.w_down = nn.Linear(24, 40), nn.Linear(24, 40, bias=False), nn.Linear(40, 24)
+
+
+def test_an_mlp_with_biases_becomes_three_linears():
+    torch.manual_seed(0)
+    m = _Blocks(_Biased())
+    c = convert_linears_to_int8(m, use_kernel=False)
+    mlp = c.blocks[0].mlp
+    assert type(mlp) is _Biased and all(type(t).__name__ == "Int8Linear" for t in (mlp.w_gate, mlp.w_up, mlp.w_down))
+    assert list(c.state_dict()) == list(m.state_dict()) and type(c.blocks[0].attn.wq).__name__ == "Int8Linear"
+    x = torch.randn(50, 24)
+    assert float((mlp(x) - m.blocks[0].mlp(x)).detach().norm()) <= 0.03 * float(m.blocks[0].mlp(x).detach().norm())
