@@ -25,6 +25,7 @@ from torch.autograd.function import once_differentiable
 from serve.quantize import computes_swiglu, has_hooks, quantize_int8
 
 _GROUP = 128
+_ATTN, _MLP = ("wq", "wk", "wv", "wo"), ("w_gate", "w_up", "w_down")
 
 
 def _rows(x, use_kernel):
@@ -175,7 +176,8 @@ class Int8SwiGLU(nn.Module):
         super().__init__()
         if any(m.bias is not None for m in (w_gate, w_up, w_down)):
             raise ValueError("Int8SwiGLU: projections with biases")
-        self.w_gate, self.w_up, self.w_down = (Int8Linear(m, use_kernel) for m in (w_gate, w_up, w_down))
+        own = lambda m: m if isinstance(m, Int8Linear) else Int8Linear(m, use_kernel)
+        self.w_gate, self.w_up, self.w_down = own(w_gate), own(w_up), own(w_down)
         self.use_kernel = use_kernel
 
     def forward(self, x):
@@ -191,28 +193,41 @@ def convert_linears_to_int8(model: nn.Module, use_kernel: bool = True) -> nn.Mod
     """A copy of the model whose attention projections (wq/wk/wv/wo) are Int8Linear and whose SwiGLU MLPs (modules with
     w_gate/w_up/w_down) are Int8SwiGLU; embeddings, head, router and norms stay as they are. Modules are recognised by their slot names, as
     train.fp8.convert_linears_to_fp8 does, and an MLP with biases or that computes something else (serve.quantize.computes_swiglu) keeps its forward,
-    over three Int8Linear. The state dict keeps its names."""
+    over three Int8Linear. The state dict keeps its names, and what is shared in the model is in the copy."""
     import copy
     model = copy.deepcopy(model)
+    made = {}  # id of a layer or MLP of the copy -> itself and what takes its place, the same in all of its places
+
+    def once(m, make):
+        if id(m) not in made:
+            made[id(m)] = m, make().train(m.training)
+        return made[id(m)][1]
+
+    def linear(lin):
+        def make():
+            new = Int8Linear(lin, use_kernel)
+            new.weight, new.bias = lin.weight, lin.bias  # (the copy's own, which others may share)
+            return new
+        return once(lin, make)
+
+    def linears(m, names):
+        lins = [getattr(m, n, None) for n in names]
+        return lins if all(isinstance(lin, nn.Linear) for lin in lins) else None
 
     def fused(m):
-        lins = slots(m, ("w_gate", "w_up", "w_down"))
-        if not linears(lins):
+        lins = linears(m, _MLP)
+        if lins is None:
             return m
         if all(lin.bias is None for lin in lins) and computes_swiglu(m):
-            return Int8SwiGLU(*lins, use_kernel=use_kernel).train(m.training)
-        for n, lin in zip(("w_gate", "w_up", "w_down"), lins):
-            setattr(m, n, Int8Linear(lin, use_kernel))
+            return once(m, lambda: Int8SwiGLU(*(linear(lin) for lin in lins), use_kernel=use_kernel))
+        for n, lin in zip(_MLP, lins):
+            setattr(m, n, linear(lin))
         return m
-    slots = lambda m, names: [getattr(m, n, None) for n in names]
-    linears = lambda ms: all(isinstance(m, nn.Linear) for m in ms)
+
     for m in list(model.modules()):
-        attn = slots(m, ("wq", "wk", "wv", "wo"))
-        if linears(attn):
-            for n, lin in zip(("wq", "wk", "wv", "wo"), attn):
-                setattr(m, n, Int8Linear(lin, use_kernel))
-        for name, child in list(m.named_children()):
-            new = fused(child)
-            if new is not child:
+        for n, lin in zip(_ATTN, linears(m, _ATTN) or ()):
+            setattr(m, n, linear(lin))
+        for name, child in list(m._modules.items()):  # (named_children names a child that stands twice once)
+            if child is not None and (new := fused(child)) is not child:
                 setattr(m, name, new)
     return fused(model)

@@ -219,3 +219,37 @@ def test_an_mlp_with_biases_becomes_three_linears():
     assert list(c.state_dict()) == list(m.state_dict()) and type(c.blocks[0].attn.wq).__name__ == "Int8Linear"
     x = torch.randn(50, 24)
     assert float((mlp(x) - m.blocks[0].mlp(x)).detach().norm()) <= 0.03 * float(m.blocks[0].mlp(x).detach().norm())
+
+
+def test_ties_stay():
+    """One layer in two places, one parameter in two layers, one MLP in two blocks and under two names: as in the model, so that
+    gradients of all uses meet and an update reaches all."""
+    torch.manual_seed(0)
+    m = nn.Module()
+    mlp = _Gated()
+    m.a, m.b = _Blocks(mlp), _Blocks(mlp)
+    m.a.blocks[0].again = mlp
+    attn = m.a.blocks[0].attn
+    attn.wk = attn.wq
+    attn.wo.weight = attn.wv.weight
+    m.embed = nn.Embedding(24, 24)
+    m.b.blocks[0].attn.wq.weight = m.embed.weight
+    m.out = nn.Linear(24, 24, bias=False)
+    m.out.weight = m.embed.weight
+    other = _Gated(act=F.gelu)
+    other.w_up = other.w_gate
+    m.other = other
+    c = convert_linears_to_int8(m, use_kernel=False)
+    blk, far = c.a.blocks[0], c.b.blocks[0]
+    assert type(blk.mlp).__name__ == "Int8SwiGLU" and blk.mlp is far.mlp and blk.mlp is blk.again
+    assert type(blk.attn.wq).__name__ == "Int8Linear" and blk.attn.wk is blk.attn.wq and blk.attn.wo.weight is blk.attn.wv.weight
+    assert far.attn.wq.weight is c.embed.weight and c.out.weight is c.embed.weight
+    assert c.other.w_up is c.other.w_gate and type(c.other.w_up).__name__ == "Int8Linear"
+    assert len(list(c.parameters())) == len(list(m.parameters())) and list(c.state_dict()) == list(m.state_dict())
+    assert not {id(p) for p in c.parameters()} & {id(p) for p in m.parameters()}
+    x = torch.randn(5, 24)
+    (blk.mlp(x) + far.mlp(x)).sum().backward()
+    got = c.a.blocks[0].mlp.w_up.weight.grad
+    c.zero_grad()
+    far.mlp(x).sum().backward()
+    assert torch.allclose(got, 2 * blk.mlp.w_up.weight.grad)
