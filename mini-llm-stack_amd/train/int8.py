@@ -8,7 +8,8 @@ each operand the one that the forward used.
 
 Int8SwiGLU is a whole MLP, w_down(silu(w_gate(x)) * w_up(x)): the product goes to w_down as codes made in the
 kernel that computes it, and gate and up are kept in 8 bits with a scale for every 128 columns. For a batch of M
-tokens it keeps M (dim + 3 hidden) bytes and scales, where the plain layers keep M (dim + 3 hidden) values and silu's own.
+tokens it keeps M (dim + 3 hidden) bytes and scales, where the plain layers keep M (dim + 3 hidden) values and silu's own; and until the
+backward the weights' codes, 3 dim hidden bytes, where the plain layers have the parameters themselves. What no wanted gradient reads is not kept.
 
 In a captured graph take gradients with torch.autograd.grad, or capture before any eager backward of the same
 parameters: torch's accumulation into .grad stays on the stream where a parameter was first used.
@@ -118,14 +119,16 @@ class _Int8SwiGLUFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, use_kernel, grad):
         # (grad: the caller's grad mode; needs_input_grad does not know of it)
-        grad = grad and any(ctx.needs_input_grad[:4])
+        need_x, need_g, need_u, need_d = (grad and n for n in ctx.needs_input_grad[:4])
+        below = need_x or need_g or need_u  # a gradient that comes through down's
         weights = [_rows(w, use_kernel) for w in (w_gate, w_up, w_down)]
         x_q, sx = _rows(x, use_kernel)
         g, u = (_matmul(x_q, sx, *w, None, x.dtype, use_kernel) for w in weights[:2])
-        h_q, sh, kept = _silu_mul(g, u, use_kernel, grad)
+        h_q, sh, kept = _silu_mul(g, u, use_kernel, below)
         ctx.use_kernel, ctx.dtypes = use_kernel, (w_gate.dtype, w_up.dtype, w_down.dtype)
-        if grad:
-            ctx.save_for_backward(x_q, sx, h_q, sh, *kept, *(t for w in weights for t in w))
+        none = None, None
+        ctx.save_for_backward(*((x_q, sx) if need_g or need_u else none), *((h_q, sh) if need_d else none), *(kept if below else none),
+                              *(weights[0] + weights[1] if need_x else none + none), *(weights[2] if below else none))
         return _matmul(h_q, sh, *weights[2], None, x.dtype, use_kernel)
 
     @staticmethod
@@ -140,6 +143,7 @@ class _Int8SwiGLUFn(torch.autograd.Function):
         dg, du = _silu_mul_grad(_input_grad(dy, dq, ds, k), (kq, ks), k)
         dwg = _weight_grad(dg, x_q, sx, k, tg) if need_g else None
         dwu = _weight_grad(du, x_q, sx, k, tu) if need_u else None
+        # (each product rounded to x's type, then their sum: as autograd adds what two layers give)
         dx = _input_grad(dg, gq, gs, k).add_(_input_grad(du, uq, us, k)) if need_x else None
         return dx, dwg, dwu, dwd, None, None
 
