@@ -101,6 +101,12 @@ def _act_bits(act_bits: int | None, bits: int) -> int | None:
     return act_bits
 
 
+def _no_grad_of(fn: str, *tensors) -> None:
+    """The kernels' refusal of inputs that ask for a gradient, for their torch form (whose scales would carry one)."""
+    from kernels.paged_kv import no_grad_of
+    no_grad_of(fn, *tensors)
+
+
 class QuantLinear(nn.Module):
     """Drop-in nn.Linear replacement holding quantized weights (serve/quantize.py:50-95).
 
@@ -163,6 +169,7 @@ class QuantLinear(nn.Module):
                 from kernels.int8_act import int8_dynamic_matmul
                 y = int8_dynamic_matmul(flat, self.w_q, self.scale)
             else:
+                _no_grad_of("QuantLinear(act_bits=8)", flat)
                 y = self.matmul_codes(*quantize_int8(flat.float()), flat.dtype)
         elif self.use_kernel:
             from kernels.dequant_matmul import int4_matmul, int8_matmul
@@ -179,6 +186,7 @@ class QuantLinear(nn.Module):
         if self.use_kernel:
             from kernels.int8_act import int8_scaled_matmul
             return int8_scaled_matmul(x_q, sx, self.w_q, self.scale, out_dtype=out_dtype)
+        _no_grad_of("QuantLinear.matmul_codes", sx, self.scale)
         return ((x_q.double() @ self.w_q.double().t()) * self.scale.double() * sx.double()[:, None]).to(out_dtype)
 
 
@@ -206,6 +214,7 @@ class Int8SwiGLU(nn.Module):
             return self.w_down((g * torch.sigmoid(g) * u).to(x.dtype))
         flat = x.reshape(-1, x.shape[-1])
         if not self.w_gate.use_kernel:
+            _no_grad_of("Int8SwiGLU", flat)
             xq = quantize_int8(flat.float())
             g, u = (m.matmul_codes(*xq, flat.dtype).float() for m in (self.w_gate, self.w_up))
             h = quantize_int8(g * torch.sigmoid(g) * u)

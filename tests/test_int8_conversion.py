@@ -253,3 +253,25 @@ def test_ties_stay():
     c.zero_grad()
     far.mlp(x).sum().backward()
     assert torch.allclose(got, 2 * blk.mlp.w_up.weight.grad)
+
+
+# ---------------------------------------------------------------- layers that serve have no gradient
+
+def test_serving_layers_refuse_gradients_on_the_host():
+    """Their scales carry a gradient in torch ops, which is no gradient of the layer."""
+    torch.manual_seed(0)
+    lin = QuantLinear(nn.Linear(24, 40, bias=False), use_kernel=False, act_bits=8)
+    mlp = quantize_model(_Blocks(_Gated()), use_kernel=False, act_bits=8).blocks[0].mlp
+    x = torch.randn(3, 24)
+    for layer in (lin, mlp):
+        with pytest.raises(ValueError):
+            layer(x.clone().requires_grad_())
+        with pytest.raises(ValueError):
+            layer((2 * x.clone().requires_grad_()).reshape(1, 3, 24))
+        with pytest.raises(ValueError), torch.autograd.forward_ad.dual_level():
+            layer(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+        y = layer(x)
+        with torch.no_grad():
+            assert torch.equal(layer(x.clone().requires_grad_()), y)
+    with pytest.raises(ValueError):
+        lin.matmul_codes(torch.zeros(3, 24, dtype=torch.int8), torch.ones(3, requires_grad=True), torch.float32)
