@@ -122,8 +122,9 @@ def _product(fn, x, sx, x_dt, w_q, sw, bias, out_dtype):
     y = torch.empty(M, N, dtype=out_dtype, device=x.device)
     if M == 0 or N == 0:
         return y
-    if K == 0:  # (no products: an empty sum, or a scale that is no number times it)
-        return y.zero_() if bias is None else y.copy_(bias.expand(M, N))
+    if K == 0:  # (no products: a sum of zero, times scales that may be no numbers)
+        z = sw.float() * 0 if sx is None else sx[:, None] * 0 + sw.float() * 0
+        return y.copy_((z if bias is None else z + bias.float()).expand(M, N))
     args = _ARGS.pack(x.data_ptr(), 0 if sx is None else sx.data_ptr(), w_q.data_ptr(), sw.data_ptr(), b_at, y.data_ptr(), x_dt,
                       _DT[sw.dtype], b_dt, c_dt, x.stride(0) if M > 1 else K, w_q.stride(0) if N > 1 else K, N, M, N, K)
     entry = kernels.lib().mlsx_a8w8

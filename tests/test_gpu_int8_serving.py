@@ -6,6 +6,7 @@ import pytest
 import torch
 import torch.nn as nn
 
+from kernels.int8_act import int8_scaled_matmul
 from serve.quantize import Int8SwiGLU, QuantLinear
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +28,18 @@ def test_hooks_fire_at_every_batch_size(rows):
     for h in handles:
         h.remove()
     assert torch.equal(e(x), fused) and len(calls) == 3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_sums_of_no_products_meet_their_scales(dtype):
+    """K = 0: zero times the scales, so NaN where one is no finite number, as for any other sum of zero."""
+    sx = torch.tensor([1.0, float("nan"), 2.0, float("inf")], device="cuda")
+    sw = torch.tensor([0.5, float("-inf"), 3.0], device="cuda")
+    bias = torch.tensor([1.5, 2.0, -4.0], device="cuda").to(dtype)
+    for K in (0, 16):
+        q, w = torch.zeros(4, K, dtype=torch.int8, device="cuda"), torch.zeros(3, K, dtype=torch.int8, device="cuda")
+        for b in (None, bias):
+            y = int8_scaled_matmul(q, sx, w, sw, b, out_dtype=dtype)
+            bad = ~torch.isfinite(sx)[:, None] | ~torch.isfinite(sw)
+            want = torch.zeros(4, 3, device="cuda") if b is None else b.float().expand(4, 3)
+            assert y.dtype == dtype and torch.equal(torch.isnan(y), bad) and torch.equal(y[~bad].float(), want[~bad])
