@@ -148,6 +148,9 @@ typedef struct mlsx_a8w8_args {
 } mlsx_a8w8_args;
 int64_t mlsx_a8w8_ws(const mlsx_a8w8_args* args);
 int64_t mlsx_a8w8(const mlsx_a8w8_args* args, void* ws, int64_t ws_bytes, mls_stream_t stream);
+/* What such a call runs: 0 the kernel for few rows, 1 the same with x quantized on the way, 16 (f + 1) + r tiles of form f (0: 64 x 64, 1: 128 x 64,
+ * 2: 128 x 128, 3: 128 x 128 in phases, 4: 256 x 256) in r ranges of K; -1 sizes that it does not take. Tests ask it. */
+int mlsx_a8w8_form(const mlsx_a8w8_args* args);
 
 /* Codes and scales, as mlsx_quantize_rows, of silu(gate) * up (fp32; gate, up: dt, [M][ld]). kept_q, kept_s (both or
  * neither null): codes int8 [2][M][H] and scales fp32 [2][M][ceil(H / 128)] of gate and up by groups of 128
@@ -167,6 +170,8 @@ int mlsx_silu_mul_backward(const void* dh, int64_t lddh, int dt, const int8_t* q
 int64_t mlsx_dw_int8_workspace(int dt, int64_t M, int64_t N, int64_t K);
 int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw,
                  int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream);
+/* The product's tiles, as mlsx_a8w8_form. */
+int mlsx_dw_int8_form(int dt, int64_t M, int64_t N, int64_t K);
 /* The same with the fp32 sums rounded to dw's own type dw_dt. */
 int mlsx_dw_int8_to(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw, int dw_dt,
                     int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream);

@@ -459,6 +459,12 @@ extern "C" int64_t mlsx_a8w8_ws(const mlsx_a8w8_args* args) {
   return make_plan(*args).bytes;
 }
 
+extern "C" int mlsx_a8w8_form(const mlsx_a8w8_args* args) {
+  if (!args || args->M <= 0 || args->N <= 0 || args->K < 1 || args->K > 131071 || args->M > (1 << 22) || args->N > (1 << 22)) return -1;
+  const Plan p = make_plan(*args);
+  return p.few ? (p.fused ? 1 : 0) : 16 * (p.form + 1) + p.splits;
+}
+
 extern "C" int64_t mlsx_a8w8(const mlsx_a8w8_args* args, void* ws, int64_t ws_bytes, mls_stream_t stream) {
   const char* fn = "mlsx_a8w8";
   if (!args) return fail(MLS_ERR_ARG, "%s: null pointer", fn);

@@ -321,6 +321,12 @@ extern "C" int64_t mlsx_dw_int8_workspace(int dt, int64_t M, int64_t N, int64_t 
   return make_plan(dt, M, N, K).bytes;
 }
 
+extern "C" int mlsx_dw_int8_form(int dt, int64_t M, int64_t N, int64_t K) {
+  if (!is_float_dt(dt) || mlsx_dw_int8_workspace(dt, M, N, K) == 0) return -1;
+  const DwPlan p = make_plan(dt, M, N, K);
+  return 16 * (p.form + 1) + p.splits;
+}
+
 extern "C" int mlsx_dw_int8_to(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw, int dw_dt,
                                int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream) {
   const char* fn = "mlsx_dw_int8";

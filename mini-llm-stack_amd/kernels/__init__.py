@@ -120,9 +120,11 @@ EXT_SIGNATURES = {
     "mlsx_quantize_rows": ([_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P], _I),
     "mlsx_a8w8_ws": ([ctypes.c_char_p], _I64),  # (an argument struct, packed)
     "mlsx_a8w8": ([ctypes.c_char_p, _P, _I64, _P], _I64),
+    "mlsx_a8w8_form": ([ctypes.c_char_p], _I),
     "mlsx_silu_mul_quantize": ([_P, _I64, _P, _I64, _I, _I64, _I64, _P, _I64, _P, _P, _P, _P], _I),
     "mlsx_silu_mul_backward": ([_P, _I64, _I, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P], _I),
     "mlsx_dw_int8_workspace": ([_I, _I64, _I64, _I64], _I64),
+    "mlsx_dw_int8_form": ([_I, _I64, _I64, _I64], _I),
     "mlsx_dw_int8": ([_P, _I, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
     "mlsx_dw_int8_to": ([_P, _I, _I64, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
     "mlsx_fp8_encode_pad": ([_I, _P, _I, _I64, _I64, _I64, _F, _P, _I64, _P, _P, _P], _I),
