@@ -37,7 +37,8 @@ __device__ __forceinline__ void store_codes(int8_t* dst, const uint2& c, int64_t
 
 // The same of two chunks of a lane at columns ka and kb, the lanes' neighbours 8 columns on, n a multiple of 16: lanes 2 i and
 // 2 i + 1 trade a chunk, so that each stores 16 bytes of one. Against stores of 8 bytes and no form of three chunks, with the checkpoint:
-// 4096 x 11008 76.8 -> 64.2 us, 2048 x 5632 21.3 -> 20.5, 4096 x 8192 equal; one row of 11008 5.7 -> 6.2, the price of the trade.
+// 4096 x 11008 76.8 -> 64.2 us, 2048 x 5632 21.3 -> 20.5, 4096 x 8192 equal; alone, in replayed graphs, one row of
+// 11008 5.7 -> 5.8 with the checkpoint and 3.6 either way without, 512 rows 13.1 -> 12.6.
 __device__ __forceinline__ void store_two(int8_t* row, const uint2& a, const uint2& b, int64_t ka, int64_t kb, int64_t n, int t) {
   auto neighbour = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false); };
   const bool odd = t & 1;

@@ -4,7 +4,9 @@
 // 16-bit dy: the kept value q s is rounded to dy's type (off by half a step of it, as dy itself is) and the product runs on
 // the 16-bit matrix cores with fp32 sums. fp16: the scales may stand for values past 65504 or below 2^-14 (a product of two
 // activations is quantized from fp32), so a power of two that brings the largest scale to [2^7, 2^8) is taken out of all and put back
-// into the sums: values stay below 2^15, and those of rows with 2^-22 of the largest scale still have all 11 bits. fp32: dy s, rounded once, becomes three bf16 parts that add up to it
+// into the sums: values stay below 2^15, and those of rows with 2^-22 of the largest scale still have all 11 bits. What that rounding
+// costs (2100 tokens, 11008 x 4096, bf16): 2.3e-3 of the norm off, where rounding the result alone is 1.7e-3; without it, dy widened
+// to fp32 and the result rounded to bf16, 1.7e-3 and 449 us instead of 187 on one box. fp32: dy s, rounded once, becomes three bf16 parts that add up to it
 // (8 significant bits each), and each meets the codes, which bf16 holds exactly: three products where two fp32
 // operands would take six. Parts of values under 2^-110 lose bits below 2^-133, bf16's smallest.
 //

@@ -220,7 +220,8 @@ class Int8SwiGLU(nn.Module):
             h = quantize_int8(g * torch.sigmoid(g) * u)
         else:
             from kernels.int8_act import int8_dynamic_matmul, quantize_rows, silu_mul_quantize
-            # (up to 16 rows the product quantizes them itself: one launch less)
+            # (up to 16 rows both products take x: where they quantize it on the way that is a launch less, and where they do not, from 5 rows
+            # of 4096 -> 11008, one more)
             if flat.shape[0] <= 16:
                 g, u = (int8_dynamic_matmul(flat, m.w_q, m.scale) for m in (self.w_gate, self.w_up))
             else:

@@ -4,7 +4,8 @@ INT8 estimator, kernels/autograd_ops.py:95-134, quantizes the weight alone and k
 Forward: the weight (per output row) and the input (per token) are quantized, and their codes meet on the 8-bit
 matrix cores. What a layer keeps for its backward is those codes: a quarter of fp32's bytes, half of 16-bit types'.
 Backward, straight through both quantizers: dx = dy times the quantized weight, dw = dy^T times the kept codes,
-each operand the one that the forward used.
+each operand the one that the forward used, with fp32 sums; dw in the parameter's type. On the kernels one factor of a product is
+rounded for the matrix cores: 16-bit dx and dw to dy's type (dy times a weight's scale, a code times a token's), fp32 dx to two bf16 parts (2^-16).
 
 Int8SwiGLU is a whole MLP, w_down(silu(w_gate(x)) * w_up(x)): the product goes to w_down as codes made in the
 kernel that computes it, and gate and up are kept in 8 bits with a scale for every 128 columns. For a batch of M
@@ -14,7 +15,7 @@ backward the weights' codes, 3 dim hidden bytes, where the plain layers have the
 In a captured graph take gradients with torch.autograd.grad, or capture before any eager backward of the same
 parameters: torch's accumulation into .grad stays on the stream where a parameter was first used.
 
-use_kernel=False runs the same arithmetic in torch ops, on the host or a device.
+use_kernel=False computes the same in torch ops, on the host or a device, with those factors in fp32.
 """
 
 from __future__ import annotations
@@ -62,7 +63,7 @@ def _weight_grad(dy, x_q, sx, use_kernel, dtype):
 def _bias_grad(dy, use_kernel, dtype):
     """dy's sums over tokens, in fp32: on a device as the weight gradient of an input of ones,
     since torch's sum over many rows clears memory with a memset, which a captured graph must not hold.
-    (bf16: 4096 x 11008 47 us, torch's sum 197; 2048 x 4096 26 and 18; 64 x 4096 25 and 10.)"""
+    (bf16: 4096 x 11008 47 us, torch's sum 196; 2048 x 4096 25 and 16; 64 x 4096 24 and 6.)"""
     if use_kernel:
         ones = torch.ones(dy.shape[0], 1, dtype=torch.int8, device=dy.device)
         return _weight_grad(dy, ones, torch.ones(dy.shape[0], device=dy.device), True, dtype).reshape(-1)

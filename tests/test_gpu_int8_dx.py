@@ -94,3 +94,26 @@ def test_fp16_swiglu_gradients_are_their_torch_form():
     for a, b in zip(*out):
         a, b = a.double(), b.double()
         assert float((a - b).norm()) <= 12 * 2.0 ** -11 * float(b.norm())
+
+
+def test_replayed_over_scales_of_other_sizes():
+    """The unit is found in the captured run: scales of other sizes, with eager calls and synchronizations between the replays."""
+    q = torch.randint(-127, 128, (70, 130), device="cuda", dtype=torch.int8, generator=cuda_gen(1))
+    dy, s = torch.zeros(33, 70, device="cuda", dtype=F16), torch.ones(70, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        int8_dgrad(dy, q, s)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = int8_dgrad(dy, q, s)
+    for i, top in enumerate((1e-3, 5.0, 1e-8, 30.0)):
+        d = (1e-2 * torch.randn(33, 70, device="cuda", generator=cuda_gen(i))).to(F16)
+        t = top * (0.1 + torch.rand(70, device="cuda", generator=cuda_gen(9 + i)))
+        dy.copy_(d)
+        s.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, int8_dgrad(d, q, t))
+        check_dx(out, d, q, t)

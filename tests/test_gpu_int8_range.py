@@ -122,3 +122,38 @@ def test_fp16_sums_past_its_range_reach_fp32_parameters():
     assert torch.equal(db, torch.full_like(db, 2e5))
     # (one row's scale is 1 / 127 in fp32, its value 127 times that, rounded to fp16: within 2^-10 of 1)
     assert bool(((dw - 2e5).abs() <= 2e5 * 2.0 ** -10).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N,K", [(1, 3, 5), (300, 130, 65), (2100, 200, 333)])
+def test_full_width_factors_on_request(M, N, K, dtype):
+    """dy in fp32 with a 16-bit output: dy sx is rounded once, to fp32, and the result once."""
+    q, s = some_codes(M, K), torch.rand(M, device="cuda", generator=cuda_gen(1)) + 0.1
+    dy = (0.1 * torch.randn(M, N, device="cuda", generator=cuda_gen(2))).to(dtype)
+    ref = dy.double().t() @ (q.double() * s.double()[:, None])
+    size = dy.double().abs().t() @ (q.double().abs() * s.double()[:, None])
+    tol = (3 * M + 16) * U * size * (1 + torch.finfo(dtype).eps) + torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -25
+    dw = a8.int8_weight_grad(dy.float(), q, s, out_dtype=dtype)
+    assert dw.dtype == dtype and bool(((dw.double() - ref).abs() <= tol).all())
+
+
+def test_weight_grad_replayed_over_scales_of_other_sizes():
+    q, s = some_codes(100, 40), torch.ones(100, device="cuda")
+    dy = torch.zeros(100, 30, device="cuda", dtype=F16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a8.int8_weight_grad(dy, q, s)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = a8.int8_weight_grad(dy, q, s)
+    for i, (top, size) in enumerate(((1e-3, 1.0), (900.0, 1e-3), (1e-8, 100.0), (5e6, 1e-6))):
+        d = (size * torch.randn(100, 30, device="cuda", generator=cuda_gen(i))).to(F16)
+        t = top * (0.1 + torch.rand(100, device="cuda", generator=cuda_gen(9 + i)))
+        dy.copy_(d)
+        s.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, a8.int8_weight_grad(d, q, t))
+        check_fp16_dw(out, d, q, t)
