@@ -13,7 +13,9 @@
 // A stage is two steps: 128 bytes of every row, whole cache lines (64 bytes a row and load: twice the requests, and L2 gives half as
 // much). LDS holds NB stages, filled by loads that write it directly, group 0 a's rows, group 1 b's. Stage t + NB - 1 is asked for
 // from phase 4 t on, when the last read of stage t - 1 is over, and waited for at the end of phase 4 (t + NB - 1) - 1, the last
-// before it is read. (Measured, int8 4096 x 8192 x 8192: 212 us, 2.6 POP/s, matrix cores busy 67%; all wavefronts in step with two buffers 277.)
+// before it is read. (Measured, int8 4096 x 8192 x 8192, single launches traced: 198 to
+// 212 us by box, 2.6 to 2.8 POP/s, matrix cores busy 67%; call upon call, at the clock that is left then, 226 to 231; all wavefronts in step with
+// two buffers 277 where this took 248.)
 //
 // Row r's chunk c of a stage lies in slot r * 8 + (c ^ (r & 7)): the 16 rows of an operand cover all banks. Loads write
 // lane l's chunk to slot base + l, so each lane loads the chunk that belongs there.
@@ -314,7 +316,8 @@ struct NtSmall {
 };
 
 // The forms of tile, and what they take: us a stage of 128 bytes on a CU, with few CUs at work (alone) and with all (busy),
-// from timed calls of 48 to 4096 rows whose weights no cache holds. A CU takes its blocks one after another or side by side; either
+// fitted to timed calls of 48 to 4096 rows whose weights no cache holds (a traced launch alone is quicker: 333 x 4096 x 11008 on 192 CUs, 128 x 64,
+// 86 stages of 0.35). A CU takes its blocks one after another or side by side; either
 // way their stages add up. Bounds: what a CU's loads to LDS bring (86 to 91 bytes a ns; 64 x 64 reads four times as
 // much a product as 256 x 256), a barrier a stage, and at 256 x 256 the matrix cores at the clock that they leave themselves.
 struct NtForm {
