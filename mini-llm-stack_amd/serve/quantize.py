@@ -256,7 +256,8 @@ def computes_swiglu(m: nn.Module) -> bool:
         probe = copy.copy(m)
         probe._modules = {n: slots[n] if n in slots else copy.deepcopy(c) for n, c in m._modules.items()}
         try:
-            return all(torch.allclose(probe.train(mode)(x), want, rtol=1e-9, atol=1e-9) for mode in (True, False))
+            # (1e-5 of the norm: a forward may go through fp32, and one value dropped of the 4096 between the layers is 1e-2)
+            return all(float((probe.train(mode)(x) - want).norm()) <= 1e-5 * float(want.norm()) for mode in (True, False))
         except Exception:  # (another shape, type or argument: not this function)
             return False
 

@@ -131,6 +131,11 @@ class _Rows(_Gated):
         return self.w_down(up * self.fn(self.w_gate(f))).reshape(x.shape)
 
 
+class _Fp32Inside(_Gated):
+    def forward(self, x):
+        return self.w_down((F.silu(self.w_gate(x).float()) * self.w_up(x).float()).to(x.dtype))
+
+
 class _Hook(_Gated):
     def __init__(self):
         super().__init__()
@@ -183,7 +188,7 @@ def test_conversion_keeps_what_other_mlps_compute(make):
 def test_a_swiglu_by_another_name_is_fused(tmp_path):
     torch.manual_seed(0)
     state = torch.get_rng_state()
-    for make in (_Rows, _Gated):
+    for make in (_Rows, _Gated, _Fp32Inside):
         m = _Blocks(make()).eval()
         state = torch.get_rng_state()
         c, q = convert_linears_to_int8(m, use_kernel=False), quantize_model(m, use_kernel=False, act_bits=8)
