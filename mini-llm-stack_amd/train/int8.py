@@ -12,6 +12,8 @@ kernel that computes it, and gate and up are kept in 8 bits with a scale for eve
 tokens it keeps M (dim + 3 hidden) bytes and scales, where the plain layers keep M (dim + 3 hidden) values and silu's own; and until the
 backward the weights' codes, 3 dim hidden bytes, where the plain layers have the parameters themselves. What no wanted gradient reads is not kept.
 
+A backward takes up to 2^20 tokens at a time (int8_weight_grad).
+
 In a captured graph take gradients with torch.autograd.grad, or capture before any eager backward of the same
 parameters: torch's accumulation into .grad stays on the stream where a parameter was first used.
 

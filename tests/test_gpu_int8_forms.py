@@ -119,3 +119,18 @@ def test_few_rows_say_what_they_run():
     values = lambda m, n, k: kernels.lib().mlsx_a8w8_form(a8._ARGS.pack(1 << 20, 0, 1 << 20, 1 << 20, 0, 1 << 20, 2, 0, 0, 2, k, k, n, m, n, k))
     assert values(1, 4096, 4096) == 1 and values(16, 11008, 4096) == 0
     assert kernels.lib().mlsx_a8w8_form(None) == -1 and kernels.lib().mlsx_dw_int8_form(9, 64, 64, 64) == -1 and kernels.lib().mlsx_dw_int8_form(0, 0, 64, 64) == -1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weight_grad_of_the_most_tokens(dtype):
+    """2^20 tokens, 300 columns against 270: rows of turned operands up to 6 MiB apart. Sums of whole numbers below 2^24."""
+    M, N, K = 2 ** 20, 300, 270
+    q, dy = ints(-1, 1, M, K, seed=1, dtype=torch.int8), ints(-2, 2, M, N, seed=2, dtype=dtype)
+    s = torch.exp2(ints(-1, 1, M, seed=3, dtype=F32))
+    want = torch.zeros(N, K, dtype=torch.float64, device="cuda")
+    for m in range(0, M, 2 ** 17):
+        part = slice(m, m + 2 ** 17)
+        want += dy[part].double().t() @ (q[part].double() * s[part].double()[:, None])
+    assert torch.equal(a8.int8_weight_grad(dy, q, s, out_dtype=F32), want.float())
+    with pytest.raises(NotImplementedError):
+        a8.int8_weight_grad(dy[:1].expand(M + 1, N), q[:1].expand(M + 1, K), s[:1].expand(M + 1))
