@@ -164,8 +164,8 @@ int mlsx_silu_mul_backward(const void* dh, int64_t lddh, int dt, const int8_t* q
                            const float* s, int64_t lds, int64_t s_step, int64_t M, int64_t H, void* dgate, void* dup,
                            int64_t ldo, mls_stream_t stream);
 
-/* dw[n][k] = sum_m dy[m][n] s[m] q[m][k] (dy and dw: dt; fp32 sums; 16-bit dt: s q rounded to it, fp16
- * in units of a power of two that suits the largest scale). M >= 1. The
+/* dw[n][k] = sum_m dy[m][n] s[m] q[m][k] (dy and dw: dt; fp32 sums; 16-bit dt: s q rounded to 11 bits, dy exact but for
+ * numbers under 2^-32, fp16 2^-28, of its column's largest dy s). M >= 1. The
  * 16-byte aligned workspace holds mlsx_dw_int8_workspace bytes (0: sizes it does not take). */
 int64_t mlsx_dw_int8_workspace(int dt, int64_t M, int64_t N, int64_t K);
 int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw,

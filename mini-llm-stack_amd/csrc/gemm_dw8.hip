@@ -1,18 +1,18 @@
 // dw[n][k] = sum_m dy[m][n] s[m] q[m][k]: the gradient of a weight whose layer kept its input as 8-bit codes
 // with a scale a token.
 //
-// 16-bit dy: the kept value q s is rounded to dy's type (off by half a step of it, as dy itself is) and the product runs on
-// the 16-bit matrix cores with fp32 sums. fp16: the scales may stand for values past 65504 or below 2^-14 (a product of two
-// activations is quantized from fp32), so a power of two that brings the largest scale to [2^7, 2^8) is taken out of all and put back
-// into the sums: values stay below 2^15, and those of rows with 2^-22 of the largest scale still have all 11 bits. What that rounding
-// costs (2100 tokens, 11008 x 4096, bf16): 2.3e-3 of the norm off, where rounding the result alone is 1.7e-3; without it, dy widened
-// to fp32 and the result rounded to bf16, 1.7e-3 and 449 us instead of 187 on one box. fp32: dy s, rounded once, becomes three bf16 parts that add up to it
+// 16-bit dy: on the fp16 matrix cores, with fp32 sums. A token's scale is f 2^e, f in [1/2, 1): f goes to the codes, rounded to fp16's 11
+// bits (which a code and a scale need 32 of), and 2^e to dy, whose bits stay as they are. So that dy 2^e fits fp16's range, it is held in units of a power of
+// two a column, found first: the column's largest at [2^14, 2^15). Numbers of 2^-32 of that (fp16: 2^-28) are still exact, smaller ones
+// are on a grid of 2^-39. The power is put back into the sums. (2100 tokens, 11008 x 4096, bf16: 1.67e-3 of the norm off, as the rounding of
+// the result alone, 190 us; with the kept value rounded to bf16 instead, which needs no pass over dy's columns, 2.36e-3 and 175; with three parts as fp32, 450.)
+// fp32: dy s, rounded once, becomes three bf16 parts that add up to it
 // (8 significant bits each), and each meets the codes, which bf16 holds exactly: three products where two fp32
 // operands would take six. Parts of values under 2^-110 lose bits below 2^-133, bf16's smallest.
 //
-// Both operands are turned first, so that their rows run along the tokens (dw8_turn_kernel; the rows' ends are padded with zeros to
-// 64 tokens), then multiplied tile by tile (nt_tile.h). 2100 tokens, 11008 x 4096, bf16: turn 22 us (bytes at a copy's rate 23.6), product 155
-// (1.2 PFLOP/s); the library's product of full-width operands 244. fp32, 1000 tokens, 2048 x 1024: 11 and 21, the library's 37.
+// Both operands are turned first, so that their rows run along the tokens (the rows' ends are padded with zeros to
+// 64 tokens), then multiplied tile by tile (nt_tile.h). The same call: exponents and the codes' turn 15 us, dy's 19 (92 MB, 4.9 TB/s), product 160
+// (1.2 PFLOP/s); the library's product of full-width operands 244. fp32, 1000 tokens, 2048 x 1024: 11 and 22, the library's 37.
 #include <algorithm>
 #include <type_traits>
 
@@ -39,9 +39,11 @@ struct TurnArgs {
   int64_t ldq;
   const float* s;
   int M, N, K, Mp;
-  const float* unit;  // fp16: the power of two that the scales are divided by
-  void* dyt;  // [N][Mp]; fp32: bf16 [N][3][Mp]
+  void* dyt;  // fp16 [N][Mp]; fp32: bf16 [N][3][Mp]
   void* xt;   // [K][Mp]
+  // 16-bit dy: columns' exponents, rows of N8 (N rounded up to 8): of each of `chunks` parts of the tokens, and of all
+  int16_t *some, *exps;
+  int chunks, N8;
 };
 
 // n <= W consecutive values of a row, zeros past them
@@ -58,21 +60,70 @@ __device__ __forceinline__ void load_some(const T* src, int64_t n, float (&v)[W]
   }
 }
 
-// unit: the power of two that divides the largest finite scale to [2^7, 2^8). One block.
-__global__ __launch_bounds__(1024) void dw8_unit_kernel(const float* s, int M, float* unit) {
-  __shared__ uint32_t red[16];
-  uint32_t top = 0;
-  for (int m = threadIdx.x; m < M; m += 1024) {
-    const uint32_t b = abs_bits(s[m]);
-    top = max(top, b < 0x7F800000u ? b : 0u);
+typedef int16_t i16x8 __attribute__((ext_vector_type(8)));
+
+// Over the 8 lanes of a wavefront that hold the same columns.
+__device__ __forceinline__ i16x8 max_of_tokens(i16x8 v) {
+  uint4 w = __builtin_bit_cast(uint4, v);
+#pragma unroll
+  for (int d = 8; d < 64; d *= 2) {
+    const uint4 o = make_uint4(__shfl_xor(w.x, d, 64), __shfl_xor(w.y, d, 64), __shfl_xor(w.z, d, 64), __shfl_xor(w.w, d, 64));
+    v = __builtin_elementwise_max(v, __builtin_bit_cast(i16x8, o));
+    w = __builtin_bit_cast(uint4, v);
   }
-  top = group_max_bits<64>(top);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int w = 0; w < 16; ++w) top = max(top, red[w]);
-  // (an exponent of 1 at least: its reciprocal is a normal number too)
-  *unit = __uint_as_float((uint32_t)max((int)(top >> 23) - 7, 1) << 23);
+  return v;
+}
+
+constexpr int16_t kNoExponent = -16384;  // of a column of zeros
+
+// The largest e of |dy 2^(a scale's exponent)| < 2^e over a part of the tokens, of 64 columns a wavefront, 8 a lane. Zeros and
+// what is no finite number do not count. A number's bits and the scale's exponent in the place of its own add up: the largest of
+// these sums has the exponent that is looked for, over a bias.
+template <typename T>
+__device__ __forceinline__ void column_exponents(const TurnArgs& p) {
+  constexpr int SHIFT = __is_same(T, _Float16) ? 10 : 7, ALL = 0x7FFF >> SHIFT, BIAS = ALL / 2 - 1;
+  constexpr int NONE = (kNoExponent + BIAS) * (1 << SHIFT);
+  const int c0 = blockIdx.x * 64 + (threadIdx.x & 7) * 8, r = threadIdx.x >> 3;
+  if ((int)blockIdx.y >= p.chunks || (int)blockIdx.x * 64 >= p.N) return;
+  const int lo = (int)((int64_t)p.M * blockIdx.y / p.chunks), hi = (int)((int64_t)p.M * (blockIdx.y + 1) / p.chunks);
+  const bool whole = c0 + 8 <= p.N;
+  int top[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top[e] = NONE;
+  for (int m0 = lo + r; m0 < hi + r; m0 += 64) {
+    uint4 raw[8];
+    float s[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t m = min(m0 + 8 * u, hi - 1);  // (some twice: a maximum)
+      const uint16_t* src = (const uint16_t*)p.dy + m * p.lddy + c0;
+      s[u] = p.s[m];
+      if (whole) {
+        __builtin_memcpy(&raw[u], src, 16);
+      } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c0 + e < p.N) w[e / 2] |= (uint32_t)src[e] << (16 * (e % 2));
+        raw[u] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+      const int x = __builtin_amdgcn_frexp_expf(s[u]) * (1 << SHIFT);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t b = (w[e / 2] >> (16 * (e % 2))) & 0x7FFFu;
+        top[e] = max(top[e], b - 1u < (uint32_t)(ALL << SHIFT) - 1u ? (int)b + x : NONE);
+      }
+    }
+  }
+  i16x8 all;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) all[e] = (int16_t)((top[e] >> SHIFT) - BIAS);
+  all = max_of_tokens(all);
+  if (r == 0 && c0 < p.N) *reinterpret_cast<i16x8*>(p.some + (int64_t)blockIdx.y * p.N8 + c0) = all;
 }
 
 // 8 tokens x W columns a lane, turned in registers, 8 x 8 lanes a wavefront: loads take 128 bytes (codes: 64) of each of 8
@@ -80,16 +131,20 @@ __global__ __launch_bounds__(1024) void dw8_unit_kernel(const float* s, int M, f
 template <typename T, typename P, int W, int PARTS, bool CODES>
 __device__ __forceinline__ void turn(const TurnArgs& p, int C, P* dst) {
   const int c0 = blockIdx.x * 8 * W + (threadIdx.x & 7) * W, m0 = blockIdx.y * 64 + (threadIdx.x >> 3) * 8;
+  i16x8 unit;  // 16-bit dy: the columns' powers of two
+  if constexpr (sizeof(T) == 2 && !CODES) {
+    unit = kNoExponent;
+    if (c0 < C)
+      for (int i = threadIdx.x >> 3; i < p.chunks; i += 8)
+        unit = __builtin_elementwise_max(unit, *reinterpret_cast<const i16x8*>(p.some + (int64_t)i * p.N8 + c0));
+    unit = max_of_tokens(unit) - (int16_t)15;
+    if (c0 < C && m0 == 0) *reinterpret_cast<i16x8*>(p.exps + c0) = unit;
+  }
   if (c0 >= C) return;
   float v[8][W];  // [token][column]
   float scale[8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) scale[r] = p.s[min(m0 + r, p.M - 1)];
-  if constexpr (CODES && __is_same(T, _Float16)) {
-    const float inv = 1.0f / *p.unit;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) scale[r] *= inv;
-  }
   if ((int)(blockIdx.x + 1) * 8 * W <= C) {
     // without branches, so that all rows are on their way at once
     using Raw = std::conditional_t<CODES, int8_t, T>;
@@ -113,12 +168,13 @@ __device__ __forceinline__ void turn(const TurnArgs& p, int C, P* dst) {
       else load_some<W>((const T*)p.dy + m * p.lddy + c0, C - c0, v[r]);
     }
   }
-  // 16-bit: codes become values here; fp32: the scale goes to dy
 #pragma unroll
   for (int r = 0; r < 8; ++r)
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      if constexpr (CODES != (sizeof(T) == 4)) v[r][e] *= scale[r];
+      if constexpr (sizeof(T) == 2 && CODES) v[r][e] *= __builtin_amdgcn_frexp_mantf(scale[r]);
+      if constexpr (sizeof(T) == 2 && !CODES) v[r][e] = __builtin_amdgcn_ldexpf(v[r][e], __builtin_amdgcn_frexp_expf(scale[r]) - unit[e]);
+      if constexpr (sizeof(T) == 4 && !CODES) v[r][e] *= scale[r];
       if (m0 + r >= p.M) v[r][e] = 0.0f;
     }
 #pragma unroll
@@ -138,16 +194,21 @@ __device__ __forceinline__ void turn(const TurnArgs& p, int C, P* dst) {
   }
 }
 
-// blockIdx.z: 0 dy, 1 the kept input
-template <typename T>
+// fp32. blockIdx.z: 0 dy, 1 the kept input
 __global__ __launch_bounds__(64) void dw8_turn_kernel(const TurnArgs p) {
-  if constexpr (sizeof(T) == 4) {
-    if (blockIdx.z == 0) turn<T, __bf16, 4, 3, false>(p, p.N, (__bf16*)p.dyt);
-    else turn<T, __bf16, 8, 1, true>(p, p.K, (__bf16*)p.xt);
-  } else {
-    if (blockIdx.z == 0) turn<T, T, 8, 1, false>(p, p.N, (T*)p.dyt);
-    else turn<T, T, 8, 1, true>(p, p.K, (T*)p.xt);
-  }
+  if (blockIdx.z == 0) turn<float, __bf16, 4, 3, false>(p, p.N, (__bf16*)p.dyt);
+  else turn<float, __bf16, 8, 1, true>(p, p.K, (__bf16*)p.xt);
+}
+
+// 16-bit: the columns' exponents beside the kept input's turn, then dy's.
+template <typename T>
+__global__ __launch_bounds__(64) void dw8_prepare_kernel(const TurnArgs p) {
+  if (blockIdx.z == 0) column_exponents<T>(p);
+  else turn<T, _Float16, 8, 1, true>(p, p.K, (_Float16*)p.xt);
+}
+template <typename T>
+__global__ __launch_bounds__(64) void dw8_turn_dy_kernel(const TurnArgs p) {
+  turn<T, _Float16, 8, 1, false>(p, p.N, (_Float16*)p.dyt);
 }
 
 struct Dw8Args {
@@ -155,7 +216,7 @@ struct Dw8Args {
   void* c;  // direct: OT [N][ldc]; partial: fp32 [splits][N][K]
   int64_t ldc;
   int m_tiles, n_tiles, splits;
-  const float* unit;  // fp16: as the scales were divided by it
+  const int16_t* exps;  // fp16 operands: the powers of two that a's rows are in units of
 };
 
 // P: the operands' type, OT: the gradient's, G: a form of tile
@@ -172,15 +233,19 @@ __global__ __launch_bounds__(G::THREADS) void dw8_kernel(const Dw8Args p) {
     return;
   using CT = std::conditional_t<PARTIAL, float, OT>;
   CT* c = (CT*)p.c + (PARTIAL ? (int64_t)sp * p.o.M * p.ldc : 0);
+  const bool wide = (p.ldc * sizeof(CT)) % 16 == 0 && ((uintptr_t)p.c & 15) == 0;
+  const int M = p.o.M, N = p.o.N, m0 = G::row(mt * G::BM, wave, lane), n0 = G::column(nt * G::BN, wave, lane);
   if constexpr (!PARTIAL && __is_same(P, _Float16)) {
-    const float unit = *p.unit;
+    int x[G::TM];
+#pragma unroll
+    for (int j = 0; j < G::TM; ++j) x[j] = p.exps[min(m0 + 16 * j, M - 1)];
 #pragma unroll
     for (int i = 0; i < G::TN; ++i)
 #pragma unroll
-      for (int j = 0; j < G::TM; ++j) acc[i][j] *= unit;
+      for (int j = 0; j < G::TM; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_ldexpf(acc[i][j][e], x[j]);
   }
-  const bool wide = (p.ldc * sizeof(CT)) % 16 == 0 && ((uintptr_t)p.c & 15) == 0;
-  const int M = p.o.M, N = p.o.N, m0 = G::row(mt * G::BM, wave, lane), n0 = G::column(nt * G::BN, wave, lane);
   if constexpr (sizeof(CT) == 2) {
     const int lk = lane >> 4, nt0 = n0 - 4 * lk;
 #pragma unroll
@@ -219,7 +284,7 @@ __global__ __launch_bounds__(G::THREADS) void dw8_kernel(const Dw8Args p) {
 // Adds the ranges' sums in their order: 4 columns a thread; part [splits][N][ldp], ldp a multiple of 4.
 template <typename P, typename CT>
 __global__ __launch_bounds__(256) void dw8_join_kernel(const float* __restrict__ part, int splits, int64_t ldp, CT* __restrict__ c,
-                                                       int64_t ldc, int N, int K, const float* __restrict__ unit) {
+                                                       int64_t ldc, int N, int K, const int16_t* __restrict__ exps) {
   const int k = (blockIdx.x * 256 + threadIdx.x) * 4, n = blockIdx.y;
   if (k >= K) return;
   const float* src = part + n * ldp + k;
@@ -228,15 +293,16 @@ __global__ __launch_bounds__(256) void dw8_join_kernel(const float* __restrict__
     const float4 q = *reinterpret_cast<const float4*>(src + i * N * ldp);
     v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
   }
-  const float u = __is_same(P, _Float16) ? *unit : 1.0f, o[4] = {v.x * u, v.y * u, v.z * u, v.w * u};
+  const int x = __is_same(P, _Float16) ? exps[n] : 0;
+  const float o[4] = {__builtin_amdgcn_ldexpf(v.x, x), __builtin_amdgcn_ldexpf(v.y, x), __builtin_amdgcn_ldexpf(v.z, x), __builtin_amdgcn_ldexpf(v.w, x)};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (k + e < K) c[n * ldc + k + e] = from_f32<CT>(o[e]);
 }
 
 struct DwPlan {
-  int64_t Mp, xt_at, unit_at, part_at, ldp, bytes;
-  int form, splits;
+  int64_t Mp, xt_at, some_at, exps_at, part_at, ldp, N8, bytes;
+  int form, splits, chunks;
 };
 
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -246,8 +312,15 @@ DwPlan make_plan(int dt, int64_t M, int64_t N, int64_t K) {
   const int parts = dt == MLS_F32 ? 3 : 1;
   p.Mp = cdiv(M, 64) * 64;
   p.xt_at = up256(N * parts * p.Mp * 2);
-  p.unit_at = p.xt_at + up256(K * p.Mp * 2);
-  p.part_at = p.unit_at + 256;
+  p.some_at = p.xt_at + up256(K * p.Mp * 2);
+  p.exps_at = p.part_at = p.some_at;
+  if (dt != MLS_F32) {
+    // parts of the tokens, a wavefront each and 64 columns: 64 tokens, or what makes 64 parts, which cost a lane of the turn 8 loads
+    p.N8 = cdiv(N, 8) * 8;
+    p.chunks = (int)std::min<int64_t>(cdiv(M, 64), 64);
+    p.exps_at = p.some_at + up256(p.chunks * p.N8 * 2);
+    p.part_at = p.exps_at + up256(p.N8 * 2);
+  }
   p.bytes = p.part_at;
   nt_choose(N, K, parts * p.Mp * 2, p.form, p.splits);
   if (p.splits > 1) {
@@ -284,7 +357,7 @@ int run_product(Dw8Args a, int64_t ldp, int form, void* part, hipStream_t st) {
         b.ldc = ldp;
         if (const int rc = launch_dw8<P, OT, G, true>(b, st)) return rc;
         hipLaunchKernelGGL((dw8_join_kernel<P, OT>), dim3((unsigned)cdiv(a.o.N, 1024), (unsigned)a.o.M), dim3(256), 0, st, (const float*)part,
-                           a.splits, ldp, (OT*)a.c, a.ldc, a.o.M, a.o.N, a.unit);
+                           a.splits, ldp, (OT*)a.c, a.ldc, a.o.M, a.o.N, a.exps);
         return check_launch("mlsx_dw_int8");
       }
     }
@@ -296,16 +369,18 @@ int run_product(Dw8Args a, int64_t ldp, int form, void* part, hipStream_t st) {
 template <typename T>
 int run(const TurnArgs& t, void* dw, int dw_dt, int64_t lddw, const DwPlan& p, uint8_t* ws, hipStream_t st) {
   const char* fn = "mlsx_dw_int8";
-  float* unit = (float*)(ws + p.unit_at);
-  if constexpr (__is_same(T, _Float16)) {
-    hipLaunchKernelGGL(dw8_unit_kernel, dim3(1), dim3(1024), 0, st, t.s, t.M, unit);
+  const unsigned across = (unsigned)std::max(cdiv(t.N, sizeof(T) == 4 ? 32 : 64), cdiv(t.K, 64)), down = (unsigned)(p.Mp / 64);
+  if constexpr (sizeof(T) == 4) {
+    hipLaunchKernelGGL(dw8_turn_kernel, dim3(across, down, 2), dim3(64), 0, st, t);
+  } else {
+    hipLaunchKernelGGL(dw8_prepare_kernel<T>, dim3(across, down, 2), dim3(64), 0, st, t);
     if (const int rc = check_launch(fn)) return rc;
+    hipLaunchKernelGGL(dw8_turn_dy_kernel<T>, dim3((unsigned)cdiv(t.N, 64), down), dim3(64), 0, st, t);
   }
-  hipLaunchKernelGGL(dw8_turn_kernel<T>, dim3((unsigned)std::max(cdiv(t.N, sizeof(T) == 4 ? 32 : 64), cdiv(t.K, 64)), (unsigned)(p.Mp / 64), 2), dim3(64), 0, st, t);
   if (const int rc = check_launch(fn)) return rc;
   const int parts = sizeof(T) == 4 ? 3 : 1, ld = (int)p.Mp * 2;
-  using P = std::conditional_t<sizeof(T) == 4, __bf16, T>;
-  const Dw8Args a{{ws, ws + p.xt_at, parts * ld, ld, t.N, t.K, parts * ld, parts}, dw, lddw, 0, 0, p.splits, unit};
+  using P = std::conditional_t<sizeof(T) == 4, __bf16, _Float16>;
+  const Dw8Args a{{ws, ws + p.xt_at, parts * ld, ld, t.N, t.K, parts * ld, parts}, dw, lddw, 0, 0, p.splits, t.exps};
   void* part = ws + p.part_at;
   if (dw_dt == MLS_F32) return run_product<P, float>(a, p.ldp, p.form, part, st);
   if (dw_dt == MLS_F16) return run_product<P, _Float16>(a, p.ldp, p.form, part, st);
@@ -343,7 +418,8 @@ extern "C" int mlsx_dw_int8_to(const void* dy, int dt, int64_t lddy, const int8_
   const DwPlan p = make_plan(dt, M, N, K);
   const hipStream_t st = (hipStream_t)stream;
   uint8_t* w = (uint8_t*)ws;
-  const TurnArgs t{dy, lddy, q, ldq, s, (int)M, (int)N, (int)K, (int)p.Mp, (const float*)(w + p.unit_at), w, w + p.xt_at};
+  const TurnArgs t{dy, lddy, q, ldq, s, (int)M, (int)N, (int)K, (int)p.Mp, w, w + p.xt_at, (int16_t*)(w + p.some_at), (int16_t*)(w + p.exps_at),
+                   p.chunks, (int)p.N8};
   if (dt == MLS_F32) return run<float>(t, dw, dw_dt, lddw, p, w, st);
   if (dt == MLS_F16) return run<_Float16>(t, dw, dw_dt, lddw, p, w, st);
   return run<__bf16>(t, dw, dw_dt, lddw, p, w, st);

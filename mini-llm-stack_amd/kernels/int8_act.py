@@ -210,11 +210,11 @@ def silu_mul_backward(dh: torch.Tensor, kept: tuple[torch.Tensor, torch.Tensor])
 
 def int8_weight_grad(dy: torch.Tensor, x_q: torch.Tensor, sx: torch.Tensor, *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """dw [N, K] = dy [M, N]^T (x_q sx[:, None]) [M, K], fp32 sums rounded to out_dtype (None: dy's dtype): the gradient of a weight whose
-    layer kept its input as quantize_rows' codes and scales. For 16-bit dy the kept values are rounded to
-    dy's dtype on the way to the matrix cores (fp16: in units of a power of two, so that sx may stand for values outside
-    its range); fp32 rounds dy * sx once, to fp32. Up to 2^20 tokens.
+    layer kept its input as quantize_rows' codes and scales. For 16-bit dy a kept value is rounded to 11 bits
+    on the way to the matrix cores, and dy is not (but for numbers under 2^-32, fp16 2^-28, of its column's largest dy sx, which are on a grid of
+    2^-39 of that); fp32 rounds dy * sx once, to fp32. Up to 2^20 tokens.
 
-    So int8_weight_grad(dy.float(), x_q, sx, out_dtype=dy.dtype) rounds the result alone to 16 bits, at three times the products."""
+    int8_weight_grad(dy.float(), x_q, sx, out_dtype=dy.dtype) rounds the result alone to 16 bits, at three times the products."""
     fn = "int8_weight_grad"
     dt = dt_code(dy.dtype, fn)
     out_dtype = dy.dtype if out_dtype is None else out_dtype

@@ -5,7 +5,8 @@ Forward: the weight (per output row) and the input (per token) are quantized, an
 matrix cores. What a layer keeps for its backward is those codes: a quarter of fp32's bytes, half of 16-bit types'.
 Backward, straight through both quantizers: dx = dy times the quantized weight, dw = dy^T times the kept codes,
 each operand the one that the forward used, with fp32 sums; dw in the parameter's type. On the kernels one factor of a product is
-rounded for the matrix cores: 16-bit dx and dw to dy's type (dy times a weight's scale, a code times a token's), fp32 dx to two bf16 parts (2^-16).
+rounded for the matrix cores: 16-bit dx to dy's type (dy times a weight's scale), 16-bit dw to 11 bits (a code times a token's), fp32 dx to two bf16
+parts (2^-16).
 
 Int8SwiGLU is a whole MLP, w_down(silu(w_gate(x)) * w_up(x)): the product goes to w_down as codes made in the
 kernel that computes it, and gate and up are kept in 8 bits with a scale for every 128 columns. For a batch of M
