@@ -170,6 +170,11 @@ int mlsx_silu_mul_backward(const void* dh, int64_t lddh, int dt, const int8_t* q
 int64_t mlsx_dw_int8_workspace(int dt, int64_t M, int64_t N, int64_t K);
 int mlsx_dw_int8(const void* dy, int dt, int64_t lddy, const int8_t* q, int64_t ldq, const float* s, void* dw,
                  int64_t lddw, int64_t M, int64_t N, int64_t K, void* ws, int64_t ws_bytes, mls_stream_t stream);
+/* db[n] = sum_m dy[m][n] (dy: dt, [M][lddy]; fp32 sums, rounded to db_dt), a bias's gradient. M >= 1. The 16-byte aligned workspace holds
+ * mlsx_bias_grad_workspace bytes (0: none). */
+int64_t mlsx_bias_grad_workspace(int64_t M, int64_t N);
+int mlsx_bias_grad(const void* dy, int dt, int64_t lddy, void* db, int db_dt, int64_t M, int64_t N, void* ws, int64_t ws_bytes,
+                   mls_stream_t stream);
 /* The product's tiles, as mlsx_a8w8_form. */
 int mlsx_dw_int8_form(int dt, int64_t M, int64_t N, int64_t K);
 /* The same with the fp32 sums rounded to dw's own type dw_dt. */

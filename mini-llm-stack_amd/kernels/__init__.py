@@ -124,6 +124,8 @@ EXT_SIGNATURES = {
     "mlsx_silu_mul_quantize": ([_P, _I64, _P, _I64, _I, _I64, _I64, _P, _I64, _P, _P, _P, _P], _I),
     "mlsx_silu_mul_backward": ([_P, _I64, _I, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P], _I),
     "mlsx_dw_int8_workspace": ([_I, _I64, _I64, _I64], _I64),
+    "mlsx_bias_grad_workspace": ([_I64, _I64], _I64),
+    "mlsx_bias_grad": ([_P, _I, _I64, _P, _I, _I64, _I64, _P, _I64, _P], _I),
     "mlsx_dw_int8_form": ([_I, _I64, _I64, _I64], _I),
     "mlsx_dw_int8": ([_P, _I, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
     "mlsx_dw_int8_to": ([_P, _I, _I64, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),

@@ -15,6 +15,7 @@ has that as its scale and zeros as codes: its outputs are NaN, other rows are no
     silu_mul_quantize    gate, up -> codes of silu(gate) * up, and gate and up in 8 bits for the backward
     silu_mul_backward    gradients of gate and up from those
     int8_weight_grad     a weight's gradient from dy and the codes that its layer kept
+    bias_grad            a bias's gradient
 
 serve.quantize.QuantLinear(act_bits=8) serves with these, train.int8 trains with them. They have no
 gradient of their own: inputs that ask for one are refused. The kernels are csrc/act8.hip, csrc/gemm_a8.hip and
@@ -239,3 +240,25 @@ def int8_weight_grad(dy: torch.Tensor, x_q: torch.Tensor, sx: torch.Tensor, *, o
     kernels.check(_on(dev, lib.mlsx_dw_int8_to, dy.data_ptr(), dt, max(dy.stride(0), N), x_q.data_ptr(), max(x_q.stride(0), K),
                       sx.data_ptr(), dw.data_ptr(), out_dt, K, M, N, K, ws.data_ptr(), need, _raw_stream(dev)), fn)
     return dw
+
+
+def bias_grad(dy: torch.Tensor, *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """db [N] = dy [M, N] summed over its rows, fp32 sums rounded to out_dtype (None: dy's dtype), in an order that the sizes alone decide. torch's
+    own sum over many rows clears memory with a memset, which a captured graph must not hold."""
+    fn = "bias_grad"
+    dt = dt_code(dy.dtype, fn)
+    out_dtype = dy.dtype if out_dtype is None else out_dtype
+    out_dt = dt_code(out_dtype, fn)
+    dy = _two(dy, "dy", fn)
+    _no_grad(fn, dy)
+    dev = one_device(fn, dy)
+    M, N = dy.shape
+    db = torch.empty(N, dtype=out_dtype, device=dy.device)
+    if M == 0:
+        return db.zero_()
+    lib = kernels.lib()
+    need = lib.mlsx_bias_grad_workspace(M, N)
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
+    kernels.check(_on(dev, lib.mlsx_bias_grad, dy.data_ptr(), dt, max(dy.stride(0), N), db.data_ptr(), out_dt, M, N, ws.data_ptr(), need,
+                      _raw_stream(dev)), fn)
+    return db

@@ -64,12 +64,9 @@ def _weight_grad(dy, x_q, sx, use_kernel, dtype):
 
 
 def _bias_grad(dy, use_kernel, dtype):
-    """dy's sums over tokens, in fp32: on a device as the weight gradient of an input of ones,
-    since torch's sum over many rows clears memory with a memset, which a captured graph must not hold.
-    (bf16: 4096 x 11008 47 us, torch's sum 196; 2048 x 4096 25 and 16; 64 x 4096 24 and 6.)"""
     if use_kernel:
-        ones = torch.ones(dy.shape[0], 1, dtype=torch.int8, device=dy.device)
-        return _weight_grad(dy, ones, torch.ones(dy.shape[0], device=dy.device), True, dtype).reshape(-1)
+        from kernels.int8_act import bias_grad
+        return bias_grad(dy, out_dtype=dtype)
     return dy.sum(0, dtype=torch.float32).to(dtype)
 
 
