@@ -28,6 +28,8 @@ finds the Linear slots by attribute name.
 
 from __future__ import annotations
 
+import sys
+
 import torch
 import torch.nn as nn
 
@@ -253,9 +255,9 @@ def computes_swiglu(m: nn.Module) -> bool:
             lin.weight.copy_(torch.randn(lin.weight.shape, generator=g, **kw))
         x = 2 * torch.randn(64, D, generator=g, **kw)
         want = slots["w_down"](nn.functional.silu(slots["w_gate"](x)) * slots["w_up"](x))
-        probe = copy.copy(m)
-        probe._modules = {n: slots[n] if n in slots else copy.deepcopy(c) for n, c in m._modules.items()}
         try:
+            probe = copy.copy(m)
+            probe._modules = {n: slots[n] if n in slots else copy.deepcopy(c) for n, c in m._modules.items()}
             # (1e-5 of the norm: a forward may go through fp32, and one value dropped of the 4096 between the layers is 1e-2)
             return all(float((probe.train(mode)(x) - want).norm()) <= 1e-5 * float(want.norm()) for mode in (True, False))
         except Exception:  # (another shape, type or argument: not this function)
@@ -446,9 +448,10 @@ def load_quantized(model: nn.Module, path, device=None, use_kernel: bool = True)
     `device`, tensors are read straight onto it. MoE experts are stacked for the
     grouped kernels as quantize_model does."""
     from safetensors.torch import load_file
-    from train.int8 import Int8Linear  # (which imports this module)
     meta = read_quantized_metadata(path)
     dev = torch.device(device) if device is not None else None
+    # (a model that holds an Int8Linear has imported its module)
+    linears = nn.Linear, QuantLinear, getattr(sys.modules.get("train.int8"), "Int8Linear", QuantLinear)
     tensors = load_file(str(path), device=str(dev) if dev is not None else "cpu")
     for key, spec in meta.items():
         if not key.startswith("q:"):
@@ -456,7 +459,7 @@ def load_quantized(model: nn.Module, path, device=None, use_kernel: bool = True)
         name = key[2:]
         bits, group, in_features = (int(x) for x in spec.split(","))
         old = model.get_submodule(name)
-        if not isinstance(old, (nn.Linear, QuantLinear, Int8Linear)):
+        if not isinstance(old, linears):
             raise ValueError(f"load_quantized: {name} is a {type(old).__name__}, not a linear layer")
         w_q, scale = tensors.pop(f"{name}.w_q"), tensors.pop(f"{name}.scale")
         out_features = old.out_features
