@@ -426,7 +426,7 @@ int run_product(Dw8Args a, int64_t ldp, int form, void* part, hipStream_t st) {
         Dw8Args b = a;
         b.c = part;
         b.ldc = ldp;
-        if (const int rc = launch_dw8<P, OT, G, true>(b, st)) return rc;
+        if (const int rc = launch_dw8<P, float, G, true>(b, st)) return rc;
         hipLaunchKernelGGL((dw8_join_kernel<P, OT>), dim3((unsigned)cdiv(a.o.N, 1024), (unsigned)a.o.M), dim3(256), 0, st, (const float*)part,
                            a.splits, ldp, (OT*)a.c, a.ldc, a.o.M, a.o.N, a.exps);
         return check_launch("mlsx_dw_int8");
